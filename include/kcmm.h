@@ -506,6 +506,99 @@ int kcmm_fused_norm_rope_append_bf16_on_stream(
     uint64_t valid_blocks_ptr, uint32_t block_offsets_f16_len,
     uint32_t num_tokens, uint64_t status_ptr, uint64_t stream_ptr);
 
+/* --- 4-bit KV cache (no reference counterpart) --- */
+
+/*
+ * A 4-bit cache holds K and V as codes of 4 bits with one scale per 32 values along
+ * head_dim, 4.5 bits a value:
+ *   s = bf16(max|x| / 7),  code = round-half-even(x / s) in [-7, 7],  value = code * s;
+ * where s is 0 the codes are, and a group that holds an infinity or NaN reads as NaN.
+ * It lives in an ordinary pool made with head_dim = kcmm_kv4_row_elems(head_dim), so blocks,
+ * tables, sharing, copy-on-write, swap and step tables work on it as they are; only the
+ * calls below read or write its pages (their inner layout is private to them).
+ * head_dim is a multiple of 32 up to 256 and block_size a multiple of 16; -1 otherwise.
+ */
+
+/** The pool head_dim of a 4-bit cache of head_dim values a row: 9/32 of it; 0 unsupported. */
+uint32_t kcmm_kv4_row_elems(uint32_t head_dim);
+/**
+ * Quantise num_tokens rows of K and V ([kv_heads][head_dim], row strides in elements, 0 =
+ * dense) into the slots slot_mapping[i] (device int64, block * block_size + offset; < 0
+ * skips the row).  Offsets, valid flags (0 = none) and the status word (0 = none) as for
+ * kcmm_append_kv_device_slots_on_stream.  Slots within a call must differ.
+ */
+int kcmm_kv4_append_bf16_on_stream(
+    kcmm_pool_t *pool, uint32_t layer_idx, uint64_t slot_mapping_ptr,
+    uint64_t block_offsets_f16_ptr, uint64_t valid_blocks_ptr, uint32_t block_offsets_f16_len,
+    uint32_t num_tokens, uint32_t head_dim, uint64_t k_src_ptr, int64_t k_row_stride,
+    uint64_t v_src_ptr, int64_t v_row_stride, uint64_t status_ptr, uint64_t stream_ptr);
+int kcmm_kv4_append_f16_on_stream(
+    kcmm_pool_t *pool, uint32_t layer_idx, uint64_t slot_mapping_ptr,
+    uint64_t block_offsets_f16_ptr, uint64_t valid_blocks_ptr, uint32_t block_offsets_f16_len,
+    uint32_t num_tokens, uint32_t head_dim, uint64_t k_src_ptr, int64_t k_row_stride,
+    uint64_t v_src_ptr, int64_t v_row_stride, uint64_t status_ptr, uint64_t stream_ptr);
+/**
+ * The values of the slots' rows, rounded once to 16 bits, into k_dst / v_dst (rows of
+ * skipped slots are left untouched): what the decode below attends to, for example to run a
+ * chunked prefill over a cached prefix.
+ */
+int kcmm_kv4_read_bf16_on_stream(
+    kcmm_pool_t *pool, uint32_t layer_idx, uint64_t slot_mapping_ptr,
+    uint64_t block_offsets_f16_ptr, uint64_t valid_blocks_ptr, uint32_t block_offsets_f16_len,
+    uint32_t num_tokens, uint32_t head_dim, uint64_t k_dst_ptr, int64_t k_row_stride,
+    uint64_t v_dst_ptr, int64_t v_row_stride, uint64_t status_ptr, uint64_t stream_ptr);
+int kcmm_kv4_read_f16_on_stream(
+    kcmm_pool_t *pool, uint32_t layer_idx, uint64_t slot_mapping_ptr,
+    uint64_t block_offsets_f16_ptr, uint64_t valid_blocks_ptr, uint32_t block_offsets_f16_len,
+    uint32_t num_tokens, uint32_t head_dim, uint64_t k_dst_ptr, int64_t k_row_stride,
+    uint64_t v_dst_ptr, int64_t v_row_stride, uint64_t status_ptr, uint64_t stream_ptr);
+
+/*
+ * Decode attention over a 4-bit cache, and over the 16-bit cache with accumulated weights.
+ * Tensors as for kcmm_paged_attn_decode_bf16_strided_on_stream (strides 0 = dense);
+ * seq_lens[b] <= 0 leaves row b of every output untouched.  With weights_out_ptr set,
+ *   weights_out[b][g][t] = weights_in[b][g][t] + sum of the softmax weights of token t over
+ *                          the query heads of kv head g,  t < seq_lens[b],
+ * float32, [batch][kv_heads] rows of weights_row_stride entries (tokens past the stride get
+ * none; entries t >= seq_lens[b] are neither read nor written).  in and out may be the same
+ * array.  The 4-bit decode takes weights pointers of 0 for none.  The scratch holds the
+ * scores, 4 bytes for each query head and token of batch x max_blocks_per_seq x block_size.
+ */
+int kcmm_kv4_paged_attn_decode_bf16_on_stream(
+    kcmm_pool_t *pool, uint32_t layer_idx, uint64_t query_ptr, int64_t q_stride_token,
+    int64_t q_stride_head, uint64_t out_ptr, int64_t out_stride_token, int64_t out_stride_head,
+    uint64_t block_tables_ptr, int64_t block_tables_row_stride, uint64_t seq_lens_ptr,
+    uint64_t block_offsets_f16_ptr, uint32_t batch, uint32_t num_q_heads, uint32_t kv_heads,
+    uint32_t head_dim, uint32_t block_size, uint32_t max_blocks_per_seq, float scale,
+    uint64_t weights_in_ptr, uint64_t weights_out_ptr, int64_t weights_row_stride,
+    uint64_t stream_ptr);
+int kcmm_kv4_paged_attn_decode_f16_on_stream(
+    kcmm_pool_t *pool, uint32_t layer_idx, uint64_t query_ptr, int64_t q_stride_token,
+    int64_t q_stride_head, uint64_t out_ptr, int64_t out_stride_token, int64_t out_stride_head,
+    uint64_t block_tables_ptr, int64_t block_tables_row_stride, uint64_t seq_lens_ptr,
+    uint64_t block_offsets_f16_ptr, uint32_t batch, uint32_t num_q_heads, uint32_t kv_heads,
+    uint32_t head_dim, uint32_t block_size, uint32_t max_blocks_per_seq, float scale,
+    uint64_t weights_in_ptr, uint64_t weights_out_ptr, int64_t weights_row_stride,
+    uint64_t stream_ptr);
+/** The 16-bit cache; head_dim 32, 64, 80, 96, 112, 128, 160, 192 or 256, block_size a
+ *  multiple of 16, at most 256 query heads per kv head; weights required. */
+int kcmm_paged_attn_decode_weights_bf16_on_stream(
+    kcmm_pool_t *pool, uint32_t layer_idx, uint64_t query_ptr, int64_t q_stride_token,
+    int64_t q_stride_head, uint64_t out_ptr, int64_t out_stride_token, int64_t out_stride_head,
+    uint64_t block_tables_ptr, int64_t block_tables_row_stride, uint64_t seq_lens_ptr,
+    uint64_t block_offsets_f16_ptr, uint32_t batch, uint32_t num_q_heads, uint32_t kv_heads,
+    uint32_t head_dim, uint32_t block_size, uint32_t max_blocks_per_seq, float scale,
+    uint64_t weights_in_ptr, uint64_t weights_out_ptr, int64_t weights_row_stride,
+    uint64_t stream_ptr);
+int kcmm_paged_attn_decode_weights_f16_on_stream(
+    kcmm_pool_t *pool, uint32_t layer_idx, uint64_t query_ptr, int64_t q_stride_token,
+    int64_t q_stride_head, uint64_t out_ptr, int64_t out_stride_token, int64_t out_stride_head,
+    uint64_t block_tables_ptr, int64_t block_tables_row_stride, uint64_t seq_lens_ptr,
+    uint64_t block_offsets_f16_ptr, uint32_t batch, uint32_t num_q_heads, uint32_t kv_heads,
+    uint32_t head_dim, uint32_t block_size, uint32_t max_blocks_per_seq, float scale,
+    uint64_t weights_in_ptr, uint64_t weights_out_ptr, int64_t weights_row_stride,
+    uint64_t stream_ptr);
+
 /* --- reference counting and copy-on-write (refcount seam of
        ref scripts/kcmm/shadow_allocator.py:22-110, skeleton ref
        src/kcmm/sharing.rs:61-101) --- */

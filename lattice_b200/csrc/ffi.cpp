@@ -770,6 +770,232 @@ int kcmm_paged_attn_decode_bf16_noalloc_on_stream(
 }
 
 // ---------------------------------------------------------------------------
+// 4-bit KV cache
+// ---------------------------------------------------------------------------
+
+uint32_t kcmm_kv4_row_elems(uint32_t head_dim) {
+  return head_dim != 0 && head_dim % 32 == 0 && head_dim <= 256 ? head_dim * 9 / 32 : 0;
+}
+
+// The pool holds a 4-bit cache of head_dim: its row size says so.
+static bool check_kv4_pool(kcmm_pool_t *h, const char *op, uint32_t layer, uint32_t hd) {
+  Pool *p = P(h);
+  if (layer >= p->num_layers) {
+    set_error(h, std::string(op) + ": layer_idx " + std::to_string(layer) + " out of bounds");
+    return false;
+  }
+  const uint32_t row = kcmm_kv4_row_elems(hd);
+  if (row == 0) {
+    set_error(h, std::string(op) + ": head_dim " + std::to_string(hd) +
+                     " unsupported (the 4-bit cache takes multiples of 32 up to 256)");
+    return false;
+  }
+  if (p->cfg_.head_dim != row) {
+    set_error(h, std::string(op) + ": the pool's head_dim is " + std::to_string(p->cfg_.head_dim) +
+                     ", a 4-bit cache of head_dim " + std::to_string(hd) + " needs " +
+                     std::to_string(row) + " (kcmm_kv4_row_elems)");
+    return false;
+  }
+  if (p->block_size % 16 != 0) {
+    set_error(h, std::string(op) + ": block_size " + std::to_string(p->block_size) +
+                     " unsupported (the 4-bit cache takes multiples of 16)");
+    return false;
+  }
+  return true;
+}
+
+static int kv4_rows(kcmm_pool_t *h, const char *op, kcmm::dev::Dtype dtype, bool append,
+                    uint32_t layer, uint64_t slots, uint64_t offsets, uint64_t valid,
+                    uint32_t offsets_len, uint32_t num_tokens, uint32_t hd, uint64_t k,
+                    int64_t k_stride, uint64_t v, int64_t v_stride, uint64_t status,
+                    uint64_t stream) {
+  if (!h || !slots || !offsets || !k || !v) {
+    set_error(h, std::string(op) + ": null pointer argument");
+    return -1;
+  }
+  if (num_tokens == 0 || num_tokens > 0x7fffffffu || offsets_len == 0 ||
+      offsets_len > 0x7fffffffu) {
+    set_error(h, std::string(op) + ": num_tokens and offset table length must be positive");
+    return -1;
+  }
+  if (!check_kv4_pool(h, op, layer, hd)) return -1;
+  Pool *p = P(h);
+  const int64_t row = int64_t(p->cfg_.kv_heads) * hd;
+  if (k_stride < 0 || v_stride < 0 || (k_stride && k_stride < row) ||
+      (v_stride && v_stride < row)) {
+    set_error(h, std::string(op) + ": row strides must be 0 (dense) or >= kv_heads * head_dim");
+    return -1;
+  }
+  if (((k | v) & 1) != 0) {
+    set_error(h, std::string(op) + ": k and v must be aligned to their 16-bit elements");
+    return -1;
+  }
+  if (guarded(h, op, [&] { p->require_device(op); })) return -1;
+  kcmm::dev::Kv4RowsArgs a = {};
+  a.dtype = dtype;
+  a.va_k = reinterpret_cast<void *>(p->va_k[layer]);
+  a.va_v = reinterpret_cast<void *>(p->va_v[layer]);
+  a.region_bytes = p->region_bytes;
+  a.slot_mapping = reinterpret_cast<const int64_t *>(slots);
+  a.block_offsets = reinterpret_cast<const uint64_t *>(offsets);
+  a.valid = reinterpret_cast<const uint8_t *>(valid);
+  a.offsets_len = int(offsets_len);
+  a.num_tokens = int(num_tokens);
+  a.kv_heads = int(p->cfg_.kv_heads);
+  a.head_dim = int(hd);
+  a.block_size = int(p->block_size);
+  a.k = reinterpret_cast<void *>(k);
+  a.v = reinterpret_cast<void *>(v);
+  a.k_stride = k_stride ? k_stride : row;
+  a.v_stride = v_stride ? v_stride : row;
+  a.status = reinterpret_cast<int32_t *>(status);
+  a.vec = ((k | v) & 7) == 0 && a.k_stride % 4 == 0 && a.v_stride % 4 == 0;
+  p->use_device();
+  return check_launch(h, op, append ? kcmm::dev::kv4_append(a, S(stream))
+                                    : kcmm::dev::kv4_read(a, S(stream)));
+}
+
+#define KCMM_KV4_ROWS(name, dt, append)                                                        \
+  int name(kcmm_pool_t *h, uint32_t layer, uint64_t slots, uint64_t offsets, uint64_t valid,   \
+           uint32_t offsets_len, uint32_t num_tokens, uint32_t hd, uint64_t k,                 \
+           int64_t k_stride, uint64_t v, int64_t v_stride, uint64_t status, uint64_t stream) { \
+    return kv4_rows(h, #name, kcmm::dev::Dtype::dt, append, layer, slots, offsets, valid,      \
+                    offsets_len, num_tokens, hd, k, k_stride, v, v_stride, status, stream);    \
+  }
+KCMM_KV4_ROWS(kcmm_kv4_append_bf16_on_stream, BF16, true)
+KCMM_KV4_ROWS(kcmm_kv4_append_f16_on_stream, F16, true)
+KCMM_KV4_ROWS(kcmm_kv4_read_bf16_on_stream, BF16, false)
+KCMM_KV4_ROWS(kcmm_kv4_read_f16_on_stream, F16, false)
+#undef KCMM_KV4_ROWS
+
+// ---------------------------------------------------------------------------
+// Decode over the 4-bit cache, and decode with accumulated attention weights
+// ---------------------------------------------------------------------------
+
+static int decode_weights_impl(kcmm_pool_t *h, const char *op, kcmm::dev::Dtype dtype, bool kv4,
+                               uint32_t layer, uint64_t q, int64_t q_token, int64_t q_head,
+                               uint64_t out, int64_t out_token, int64_t out_head,
+                               uint64_t tables, int64_t tables_row, uint64_t seq_lens,
+                               uint64_t offsets, uint32_t batch, uint32_t hq, uint32_t hkv,
+                               uint32_t hd, uint32_t bs, uint32_t max_bps, float scale,
+                               uint64_t w_in, uint64_t w_out, int64_t w_row, uint64_t stream) {
+  if (!h || !q || !out || !tables || !seq_lens || !offsets) {
+    set_error(h, std::string(op) + ": null pointer argument");
+    return -1;
+  }
+  if (batch == 0 || hq == 0 || hkv == 0 || hd == 0 || bs == 0 || max_bps == 0) {
+    set_error(h, std::string(op) + ": shape arguments must be positive");
+    return -1;
+  }
+  if (hq > 0xFFFF || hkv > 0xFFFF || bs > 0xFFFF || max_bps > 0xFFFF || batch > 0xFFFF ||
+      uint64_t(bs) * max_bps > 0x7fffffffull) {
+    set_error(h, std::string(op) + ": packed shape argument exceeds 65535");
+    return -1;
+  }
+  if (hq < hkv) {
+    set_error(h, std::string(op) + ": num_q_heads must be at least kv_heads");
+    return -1;
+  }
+  if (q_token < 0 || out_token < 0 || (q_head && q_head < int64_t(hd)) ||
+      (out_head && out_head < int64_t(hd)) || (tables_row && tables_row < int64_t(max_bps))) {
+    set_error(h, std::string(op) +
+                     ": strides must be 0 (dense) or positive, head strides >= head_dim and the "
+                     "block-table row stride >= max_blocks_per_seq");
+    return -1;
+  }
+  Pool *p = P(h);
+  if (kv4) {
+    if (!check_kv4_pool(h, op, layer, hd)) return -1;
+    if (bs != p->block_size || hkv != p->cfg_.kv_heads) {
+      set_error(h, std::string(op) + ": kv_heads and block_size must be the pool's");
+      return -1;
+    }
+  } else {
+    if (layer >= p->num_layers) {
+      set_error(h, std::string(op) + ": layer_idx " + std::to_string(layer) + " out of bounds");
+      return -1;
+    }
+    if (bs % 16 != 0) {
+      set_error(h, std::string(op) + ": block_size " + std::to_string(bs) +
+                       " unsupported (attention weights need pages of a multiple of 16 tokens)");
+      return -1;
+    }
+  }
+  if (w_out ? (!w_in || w_row <= 0) : (!kv4 || w_in != 0)) {
+    set_error(h, std::string(op) +
+                     ": weights_in, weights_out and a positive weights row stride go together");
+    return -1;
+  }
+  if (w_out) {
+    if (((w_in | w_out) & 3) != 0) {
+      set_error(h, std::string(op) + ": weights must be 4-byte aligned");
+      return -1;
+    }
+    if ((hq + hkv - 1) / hkv > 256) {
+      set_error(h, std::string(op) + ": attention weights take at most 256 query heads per kv head");
+      return -1;
+    }
+  }
+  if (guarded(h, op, [&] { p->require_device(op); })) return -1;
+  p->use_device();
+  kcmm::dev::DecodeArgs a = {};
+  a.q_stride_token = q_token;
+  a.q_stride_head = q_head;
+  a.out_stride_token = out_token;
+  a.out_stride_head = out_head;
+  a.tables_stride = tables_row;
+  a.dtype = dtype;
+  a.q = reinterpret_cast<const void *>(q);
+  a.out = reinterpret_cast<void *>(out);
+  a.block_tables = reinterpret_cast<const int32_t *>(tables);
+  a.seq_lens = reinterpret_cast<const int32_t *>(seq_lens);
+  a.block_offsets = reinterpret_cast<const uint64_t *>(offsets);
+  a.va_k = reinterpret_cast<const void *>(p->va_k[layer]);
+  a.va_v = reinterpret_cast<const void *>(p->va_v[layer]);
+  a.region_elems = p->region_bytes / 2;
+  a.batch = int(batch);
+  a.num_q_heads = int(hq);
+  a.kv_heads = int(hkv);
+  a.head_dim = int(hd);
+  a.block_size = int(bs);
+  a.max_blocks_per_seq = int(max_bps);
+  a.scale = scale;
+  a.diag = p->diag_word();
+  kcmm::dev::DecodeWeights w;
+  w.w_in = reinterpret_cast<const float *>(w_in);
+  w.w_out = reinterpret_cast<float *>(w_out);
+  w.w_stride = w_row;
+  cudaError_t e = kv4 ? kcmm::dev::kv4_decode_attention(a, w, S(stream))
+                      : kcmm::dev::decode_attention_weights(a, w, S(stream));
+  if (e == cudaErrorNotSupported) {
+    set_error(h, std::string(op) + ": head_dim " + std::to_string(hd) +
+                     " unsupported (attention weights take 32, 64, 80, 96, 112, 128, 160, 192 "
+                     "or 256)");
+    return -1;
+  }
+  return check_launch(h, op, e);
+}
+
+#define KCMM_DECODE_WEIGHTS(name, dt, kv4)                                                      \
+  int name(kcmm_pool_t *h, uint32_t layer, uint64_t q, int64_t q_stride_token,                  \
+           int64_t q_stride_head, uint64_t out, int64_t out_stride_token,                       \
+           int64_t out_stride_head, uint64_t tables, int64_t tables_row_stride,                 \
+           uint64_t seq_lens, uint64_t offsets, uint32_t batch, uint32_t hq, uint32_t hkv,      \
+           uint32_t hd, uint32_t bs, uint32_t max_bps, float scale, uint64_t weights_in,        \
+           uint64_t weights_out, int64_t weights_row_stride, uint64_t stream) {                 \
+    return decode_weights_impl(h, #name, kcmm::dev::Dtype::dt, kv4, layer, q, q_stride_token,   \
+                               q_stride_head, out, out_stride_token, out_stride_head, tables,   \
+                               tables_row_stride, seq_lens, offsets, batch, hq, hkv, hd, bs,    \
+                               max_bps, scale, weights_in, weights_out, weights_row_stride,     \
+                               stream);                                                         \
+  }
+KCMM_DECODE_WEIGHTS(kcmm_kv4_paged_attn_decode_bf16_on_stream, BF16, true)
+KCMM_DECODE_WEIGHTS(kcmm_kv4_paged_attn_decode_f16_on_stream, F16, true)
+KCMM_DECODE_WEIGHTS(kcmm_paged_attn_decode_weights_bf16_on_stream, BF16, false)
+KCMM_DECODE_WEIGHTS(kcmm_paged_attn_decode_weights_f16_on_stream, F16, false)
+#undef KCMM_DECODE_WEIGHTS
+
+// ---------------------------------------------------------------------------
 // Chunked prefill (tcgen05)
 // ---------------------------------------------------------------------------
 

@@ -35,6 +35,7 @@
 #include <mutex>
 
 #include "../launch.hpp"
+#include "finish.cuh"
 #include "pdl.cuh"
 #include "ptx.cuh"
 
@@ -67,6 +68,10 @@ struct DecodeParams {
   // block-table rows tables + b*bt_stride.  Dense: (hq*D, D), (hq*D, D), max_bps.
   int64_t q_sb, q_sh, o_sb, o_sh;
   int64_t bt_stride;
+  // Scores of every (row, token), log2 units, for the accumulated weights (SCORES only):
+  // [b * hq + h][score_stride]; a whole number of units a row.
+  float *scores;
+  int64_t score_stride;
 };
 
 __device__ __forceinline__ int ceil_div_dev(int a, int b) { return (a + b - 1) / b; }
@@ -265,7 +270,9 @@ struct Cfg {
 // and initialises its barriers here.  Returns false when a wait ran out (the CTA
 // has reported it and must stop).
 // TWO (MODE 0 only): 8-token pages, a unit's rows 8-15 read from the next page.
-template <typename T, int D, int W, int NS, int MODE, bool TWO = false>
+// SCORES (MODE 0 only): the scores go to p.scores too, and the result is always a partial
+// (finish.cuh adds up the weights and merges).
+template <typename T, int D, int W, int NS, int MODE, bool TWO = false, bool SCORES = false>
 __device__ __forceinline__ bool decode_body(const DecodeParams &p, const int item,
                                             const int split, int &rb, const int4 ea = int4{},
                                             const int4 ec = int4{}, const int kvh_in = 0) {
@@ -545,6 +552,13 @@ __device__ __forceinline__ bool decode_body(const DecodeParams &p, const int ite
         }
         mx0 = fmaxf(mx0, fmaxf(s[nt][0], s[nt][1]));
         mx1 = fmaxf(mx1, fmaxf(s[nt][2], s[nt][3]));
+        if constexpr (SCORES) {
+          float *sc = p.scores + (int64_t(b) * p.hq + lo + g) * p.score_stride +
+                      (u_begin + warp + k * W) * kUnit + nt * 8 + 2 * t;
+          if (g < G) *reinterpret_cast<float2 *>(sc) = make_float2(s[nt][0], s[nt][1]);
+          if (g + 8 < G)
+            *reinterpret_cast<float2 *>(sc + 8 * p.score_stride) = make_float2(s[nt][2], s[nt][3]);
+        }
       }
       mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
       mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
@@ -599,6 +613,10 @@ __device__ __forceinline__ bool decode_body(const DecodeParams &p, const int ite
           MMA::run(o[2 * j + 1], pl, b2, b3);
         }
       }
+    } else if constexpr (SCORES) {  // a page that could not be read: its tokens weigh nothing
+      for (int i = lane; i < G * kUnit; i += 32)
+        p.scores[(int64_t(b) * p.hq + lo + i / kUnit) * p.score_stride +
+                 (u_begin + warp + k * W) * kUnit + i % kUnit] = -INFINITY;
     }
     __syncwarp();
     if (k + NS < n_w) issue(k + NS);
@@ -665,7 +683,7 @@ __device__ __forceinline__ bool decode_body(const DecodeParams &p, const int ite
       x1 += cO[(w * 16 + h) * D + d + 1] * sc;
     }
     const float inv = 1.f / L;
-    if (n_splits_b == 1) {
+    if (n_splits_b == 1 && !SCORES) {
       T *dst = static_cast<T *>(p.out) + int64_t(b) * p.o_sb + int64_t(lo + h) * p.o_sh + d;
       dst[0] = ptx::from_f32<T>(x0 * inv);
       dst[1] = ptx::from_f32<T>(x1 * inv);
@@ -686,10 +704,10 @@ __device__ __forceinline__ bool decode_body(const DecodeParams &p, const int ite
   return true;
 }
 
-template <typename T, int D, int W, int NS, bool TWO = false>
+template <typename T, int D, int W, int NS, bool TWO = false, bool SCORES = false>
 __global__ void __launch_bounds__(W * 32, 2) decode_kernel(const DecodeParams p) {
   int rb = 0;
-  decode_body<T, D, W, NS, 0, TWO>(p, blockIdx.z, blockIdx.x, rb);
+  decode_body<T, D, W, NS, 0, TWO, SCORES>(p, blockIdx.z, blockIdx.x, rb);
 }
 
 // Shared-prefix decode: persistent CTAs (at most 2 per SM) take items
@@ -1163,7 +1181,26 @@ void *stream_scratch(cudaStream_t stream, size_t bytes) {
   return fresh;
 }
 
-cudaError_t decode_attention(const DecodeArgs &a, cudaStream_t stream) {
+cudaError_t CallScratch::acquire(cudaStream_t stream, size_t bytes) {
+  if ((ptr = stream_scratch(stream, bytes)) != nullptr) return cudaSuccess;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaMemPool_t mp = scratch_pool(dev);
+  if (!mp) return cudaErrorMemoryAllocation;
+  const cudaError_t e = cudaMallocFromPoolAsync(&ptr, bytes, mp, stream);
+  owned = e == cudaSuccess;
+  return e;
+}
+
+cudaError_t CallScratch::release(cudaStream_t stream) {
+  if (!owned) return cudaSuccess;
+  owned = false;
+  return cudaFreeAsync(ptr, stream);
+}
+
+int device_sm_count() { return sm_count(); }
+
+static DecodeParams decode_params(const DecodeArgs &a) {
   DecodeParams p = {};
   p.q = a.q;
   p.out = a.out;
@@ -1186,7 +1223,11 @@ cudaError_t decode_attention(const DecodeArgs &a, cudaStream_t stream) {
   p.o_sb = a.out_stride_token ? a.out_stride_token : dense_row;
   p.o_sh = a.out_stride_head ? a.out_stride_head : a.head_dim;
   p.bt_stride = a.tables_stride ? a.tables_stride : a.max_blocks_per_seq;
+  return p;
+}
 
+cudaError_t decode_attention(const DecodeArgs &a, cudaStream_t stream) {
+  DecodeParams p = decode_params(a);
   Plan pl = make_plan(a);
   if (!pl.fast && a.peer_world > 0) return cudaErrorNotSupported;  // tensor-core path only
   if (!pl.fast) {
@@ -1264,6 +1305,81 @@ cudaError_t decode_attention(const DecodeArgs &a, cudaStream_t stream) {
     if (e == cudaSuccess) e = f;
   }
   return e;
+}
+
+namespace {
+
+template <typename T>
+KernelFn weights_kernel(int D) {
+  switch (D) {
+#define KCMM_CASE(DD) \
+  case DD: return decode_kernel<T, DD, kWarps, kStages, false, true>;
+    KCMM_CASE(32)
+    KCMM_CASE(64)
+    KCMM_CASE(80)
+    KCMM_CASE(96)
+    KCMM_CASE(112)
+    KCMM_CASE(128)
+    KCMM_CASE(160)
+    KCMM_CASE(192)
+    KCMM_CASE(256)
+#undef KCMM_CASE
+    default: return nullptr;
+  }
+}
+
+}  // namespace
+
+cudaError_t decode_attention_weights(const DecodeArgs &a, const DecodeWeights &w,
+                                     cudaStream_t stream) {
+  const Plan pl = make_plan(a);
+  if (!pl.fast || a.block_size % kUnit != 0) return cudaErrorNotSupported;
+  const KernelFn fn = a.dtype == Dtype::BF16 ? weights_kernel<__nv_bfloat16>(a.head_dim)
+                                             : weights_kernel<__half>(a.head_dim);
+  DecodeParams p = decode_params(a);
+  p.units_per_split = pl.units_per_split;
+  p.num_splits = pl.num_splits;
+  p.n_head_tiles = pl.n_head_tiles;
+  const size_t rows = size_t(a.batch) * a.num_q_heads;
+  const int max_tokens = a.max_blocks_per_seq * a.block_size;
+  p.score_stride = max_tokens;
+  const size_t scores_at =
+      (rows * p.num_splits * (size_t(a.head_dim) + 1) * 4 + 15) & ~size_t(15);
+  CallScratch scratch;
+  cudaError_t e = scratch.acquire(stream, scores_at + rows * size_t(p.score_stride) * 4);
+  if (e != cudaSuccess) return e;
+  p.part_o = static_cast<float *>(scratch.ptr);
+  p.part_lse = p.part_o + rows * p.num_splits * a.head_dim;
+  p.scores = reinterpret_cast<float *>(static_cast<char *>(scratch.ptr) + scores_at);
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(pl.smem));
+  if (e == cudaSuccess)
+    e = launch_pdl(fn, dim3(pl.num_splits, a.kv_heads * pl.n_head_tiles, a.batch),
+                   dim3(kWarps * 32), pl.smem, stream, p);
+  if (e == cudaSuccess) {
+    FinishParams f = {};
+    f.seq_lens = a.seq_lens;
+    f.max_tokens = max_tokens;
+    f.hq = a.num_q_heads;
+    f.hkv = a.kv_heads;
+    f.head_dim = a.head_dim;
+    f.num_splits = p.num_splits;
+    f.tokens_per_split = p.units_per_split * kUnit;
+    f.part_o = p.part_o;
+    f.part_lse = p.part_lse;
+    f.out = a.out;
+    f.o_sb = p.o_sb;
+    f.o_sh = p.o_sh;
+    f.scores = p.scores;
+    f.score_stride = p.score_stride;
+    f.w_in = w.w_in;
+    f.w_out = w.w_out;
+    f.w_stride = w.w_stride;
+    const dim3 grid((max_tokens + kFinishTokens - 1) / kFinishTokens, a.kv_heads, a.batch);
+    e = launch_pdl(a.dtype == Dtype::BF16 ? finish_kernel<__nv_bfloat16> : finish_kernel<__half>,
+                   grid, dim3(kFinishThreads), 0, stream, f);
+  }
+  const cudaError_t r = scratch.release(stream);
+  return e != cudaSuccess ? e : r;
 }
 
 namespace {

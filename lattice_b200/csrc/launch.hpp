@@ -96,6 +96,56 @@ struct PrefillArgs {
 // (kernels/prefill.cu).  head_dim 128; num_q_heads / kv_heads must divide 128.
 cudaError_t paged_prefill(const PrefillArgs &a, cudaStream_t stream);
 
+// --- 4-bit KV cache (kernels/kv4.cu) ---
+// Rows of K and V to (append) or from (read) the slots of a 4-bit cache.
+struct Kv4RowsArgs {
+  Dtype dtype;
+  void *va_k;
+  void *va_v;
+  uint64_t region_bytes;
+  const int64_t *slot_mapping;
+  const uint64_t *block_offsets;  // 2-byte units
+  const uint8_t *valid;           // may be null
+  int offsets_len;
+  int num_tokens;
+  int kv_heads, head_dim, block_size;
+  void *k;  // [num_tokens] rows of kv_heads * head_dim values, strides in elements
+  void *v;
+  int64_t k_stride, v_stride;
+  int32_t *status;  // may be null
+  bool vec;         // every row starts on 8 bytes
+};
+cudaError_t kv4_append(const Kv4RowsArgs &a, cudaStream_t stream);
+cudaError_t kv4_read(const Kv4RowsArgs &a, cudaStream_t stream);
+
+// Accumulated attention weights of a decode: w_out = w_in + this step's weights, rows
+// (b * kv_heads + kv head) * w_stride; w_out null for none.
+struct DecodeWeights {
+  const float *w_in = nullptr;
+  float *w_out = nullptr;
+  int64_t w_stride = 0;
+};
+// Decode over the 4-bit cache.  DecodeArgs as for decode_attention (head_dim is the model's;
+// scratch, splits and peer fields unused); head_dim a multiple of 32 up to 256 and
+// block_size a multiple of 16, else cudaErrorNotSupported.
+cudaError_t kv4_decode_attention(const DecodeArgs &a, const DecodeWeights &w,
+                                 cudaStream_t stream);
+// decode_attention with accumulated weights.  Tensor-core shapes with pages of whole
+// 16-token units only, else cudaErrorNotSupported.
+cudaError_t decode_attention_weights(const DecodeArgs &a, const DecodeWeights &w,
+                                     cudaStream_t stream);
+
+// Scratch of one call: the stream's kept buffer where there is one (stream_scratch), else
+// a stream-ordered allocation that release() frees in stream order.
+struct CallScratch {
+  void *ptr = nullptr;
+  bool owned = false;
+  cudaError_t acquire(cudaStream_t stream, size_t bytes);
+  cudaError_t release(cudaStream_t stream);
+};
+// Multiprocessors of the current device (cached).
+int device_sm_count();
+
 // Device scratch kept per (device, stream) between calls (kernels/decode.cu), used by the
 // decode split merge and the prefill tail split.  Calls on one stream share it in stream
 // order.  Null while the stream is being captured or once the per-process stream cache is

@@ -238,6 +238,14 @@ SIGNATURES: dict[str, tuple] = {
     "kcmm_fused_norm_rope_append_bf16_on_stream":
         (i32, [P, u32, u64, u64, u64, u32, f32, u64, u32, u64, u64, u64, f32, u32,
                u64, u64, u64, u32, u32, u64, u64]),
+    "kcmm_kv4_row_elems": (u32, [u32]),
+    **{f"kcmm_kv4_{op}_{dt}_on_stream":
+       (i32, [P, u32, u64, u64, u64, u32, u32, u32, u64, i64, u64, i64, u64, u64])
+       for op in ("append", "read") for dt in ("bf16", "f16")},
+    **{f"kcmm_{op}_{dt}_on_stream":
+       (i32, [P, u32, u64, i64, i64, u64, i64, i64, u64, i64, u64, u64, u32, u32, u32, u32, u32,
+              u32, f32, u64, u64, i64, u64])
+       for op in ("kv4_paged_attn_decode", "paged_attn_decode_weights") for dt in ("bf16", "f16")},
     "kcmm_block_incref": (i32, [P, u32]),
     "kcmm_block_decref": (i32, [P, u32]),
     "kcmm_block_refcount": (u32, [P, u32]),
@@ -338,6 +346,14 @@ class StepTables:
 def _u32_array(values):
     values = [int(v) for v in values]
     return (ctypes.c_uint32 * max(1, len(values)))(*values)
+
+
+def kv4_row_elems(head_dim: int) -> int:
+    """The pool head_dim of a 4-bit cache of `head_dim` (`kcmm_kv4_row_elems`)."""
+    if head_dim <= 0 or head_dim % 32 != 0 or head_dim > 256:
+        raise ValueError(f"the 4-bit cache takes head dims that are multiples of 32 up to 256, "
+                         f"not {head_dim}")
+    return head_dim * 9 // 32
 
 
 class KcmmLibrary:
@@ -589,6 +605,56 @@ class KcmmPool:
             k_ptr, v_ptr, positions_ptr, rope_theta, rope_mode, slot_mapping_ptr,
             block_offsets_f16_ptr, valid_blocks_ptr, block_offsets_f16_len, num_tokens,
             status_ptr, stream_ptr), "kcmm_fused_norm_rope_append_bf16_on_stream")
+
+    # --- 4-bit cache ---------------------------------------------------------
+    def kv4_append(self, layer: int, *, slot_mapping_ptr: int, block_offsets_f16_ptr: int,
+                   block_offsets_f16_len: int, num_tokens: int, head_dim: int, k_src_ptr: int,
+                   v_src_ptr: int, k_row_stride: int = 0, v_row_stride: int = 0,
+                   valid_blocks_ptr: int = 0, status_ptr: int = 0, dtype: str = "bf16",
+                   stream_ptr: int = 0) -> None:
+        """Quantise rows of K and V into the slots of a 4-bit cache."""
+        op = f"kcmm_kv4_append_{dtype}_on_stream"
+        self._check(getattr(self.lib, op)(
+            self.handle, layer, slot_mapping_ptr, block_offsets_f16_ptr, valid_blocks_ptr,
+            block_offsets_f16_len, num_tokens, head_dim, k_src_ptr, k_row_stride, v_src_ptr,
+            v_row_stride, status_ptr, stream_ptr), op)
+
+    def kv4_read(self, layer: int, *, slot_mapping_ptr: int, block_offsets_f16_ptr: int,
+                 block_offsets_f16_len: int, num_tokens: int, head_dim: int, k_dst_ptr: int,
+                 v_dst_ptr: int, k_row_stride: int = 0, v_row_stride: int = 0,
+                 valid_blocks_ptr: int = 0, status_ptr: int = 0, dtype: str = "bf16",
+                 stream_ptr: int = 0) -> None:
+        """The 16-bit values of a 4-bit cache's slots."""
+        op = f"kcmm_kv4_read_{dtype}_on_stream"
+        self._check(getattr(self.lib, op)(
+            self.handle, layer, slot_mapping_ptr, block_offsets_f16_ptr, valid_blocks_ptr,
+            block_offsets_f16_len, num_tokens, head_dim, k_dst_ptr, k_row_stride, v_dst_ptr,
+            v_row_stride, status_ptr, stream_ptr), op)
+
+    def _decode_weights(self, kind, layer, query_ptr, out_ptr, block_tables_ptr, seq_lens_ptr,
+                        block_offsets_f16_ptr, batch, num_q_heads, kv_heads, head_dim, block_size,
+                        max_blocks_per_seq, scale, q_stride_token=0, q_stride_head=0,
+                        out_stride_token=0, out_stride_head=0, block_tables_row_stride=0,
+                        weights_in_ptr=0, weights_out_ptr=0, weights_row_stride=0, dtype="bf16",
+                        stream_ptr=0):
+        op = f"kcmm_{kind}_{dtype}_on_stream"
+        self._check(getattr(self.lib, op)(
+            self.handle, layer, query_ptr, q_stride_token, q_stride_head, out_ptr,
+            out_stride_token, out_stride_head, block_tables_ptr, block_tables_row_stride,
+            seq_lens_ptr, block_offsets_f16_ptr, batch, num_q_heads, kv_heads, head_dim,
+            block_size, max_blocks_per_seq, scale, weights_in_ptr, weights_out_ptr,
+            weights_row_stride, stream_ptr), op)
+
+    def kv4_paged_attn_decode(self, layer: int, **kw) -> None:
+        """Decode attention over a 4-bit cache.  Keywords as `paged_attn_decode` (without
+        `noalloc` / `current_context`), optional strides `q_stride_token`, `q_stride_head`,
+        `out_stride_token`, `out_stride_head`, `block_tables_row_stride` (0 = dense), and
+        optional `weights_in_ptr`, `weights_out_ptr`, `weights_row_stride`."""
+        self._decode_weights("kv4_paged_attn_decode", layer, **kw)
+
+    def paged_attn_decode_weights(self, layer: int, **kw) -> None:
+        """`kv4_paged_attn_decode` over the 16-bit cache, the weights required."""
+        self._decode_weights("paged_attn_decode_weights", layer, **kw)
 
     # --- decode attention --------------------------------------------------
     def paged_attn_decode(self, layer: int, *, query_ptr: int, out_ptr: int,
