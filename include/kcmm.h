@@ -599,6 +599,93 @@ int kcmm_paged_attn_decode_weights_f16_on_stream(
     uint64_t weights_in_ptr, uint64_t weights_out_ptr, int64_t weights_row_stride,
     uint64_t stream_ptr);
 
+/* --- eviction by accumulated attention weight (no reference counterpart) --- */
+
+/** What a pool's pages hold, where a call has to know it. */
+typedef enum {
+    KCMM_CACHE_16BIT = 0, /* f16 or bf16 rows */
+    KCMM_CACHE_KV4   = 1, /* a 4-bit cache (kcmm_kv4_*) */
+} kcmm_cache_format_t;
+
+/**
+ * Cut every sequence's cached tokens of one layer to `budget`, per kv head.  With n =
+ * seq_lens[b] > budget, slot i < n of position
+ *   positions_in[b][g][i] for i < kept_lens[b], else i + next_positions[b] - n,
+ * stays if its position is below `sinks` or at least next_positions[b] - recent; the rest of
+ * the budget goes to the slots of largest weights_in[b][g][i] (ties: the lowest slot; NaN
+ * counts as -inf).  Kept slots >= budget move, in order, into the freed slots below it, K and
+ * V rows bit for bit.  weights_out / positions_out [0, budget) are the kept slots' values,
+ * weights_out [budget, n) is set to 0 for the tokens to come.  Sequences of at most budget
+ * tokens keep their slots (weights and positions copied out).  new_lens[b] = min(n, budget).
+ *   weights, positions   float32 / int32 [batch][kv_heads] rows of row_stride entries; each
+ *                        out may be the same array as its in
+ *   next_positions       int32 [batch]: the position the next token will have
+ *   kept_lens            int32 [batch]: slots with a stored position (new_lens of the last
+ *                        eviction; 0 before the first)
+ * All arrays are device arrays.  Blocks shared with other sequences must be made private
+ * first (kcmm_cow_blocks_on_stream): their rows are overwritten.  After the last layer,
+ * kcmm_truncate_sequence returns the blocks past the budget.  seq_lens[b] above row_stride
+ * or the table's tokens leaves the sequence untouched and sets bit 2 of
+ * kcmm_get_kernel_status.  head_dim is the model's (a multiple of 8 for the 16-bit cache).
+ */
+int kcmm_evict_tokens_on_stream(
+    kcmm_pool_t *pool, uint32_t layer_idx, uint32_t cache_format, uint32_t head_dim,
+    uint64_t block_tables_ptr, int64_t block_tables_row_stride, uint64_t seq_lens_ptr,
+    uint64_t block_offsets_f16_ptr, uint32_t batch, uint32_t max_blocks_per_seq,
+    uint32_t budget, uint32_t sinks, uint32_t recent, uint64_t weights_in_ptr,
+    uint64_t weights_out_ptr, uint64_t positions_in_ptr, uint64_t positions_out_ptr,
+    int64_t row_stride, uint64_t next_positions_ptr, uint64_t kept_lens_ptr,
+    uint64_t new_lens_ptr, uint64_t stream_ptr);
+/** Cut a sequence to its first len tokens (at most its length); the blocks past them are
+ *  released as kcmm_free_blocks does. */
+int kcmm_truncate_sequence(kcmm_pool_t *pool, uint32_t seq_idx, uint32_t len);
+
+/* --- beam search (no reference counterpart) --- */
+
+/** Element types of the logits. */
+typedef enum {
+    KCMM_DTYPE_F16  = 0,
+    KCMM_DTYPE_BF16 = 1,
+    KCMM_DTYPE_F32  = 2,
+} kcmm_dtype_t;
+
+/**
+ * The n_select best of each request's beams x vocab continuations by
+ *   score(k, v) = scores_in[k] + log_softmax(logits[k])[v]
+ * (32 bits), best first, ties to the lowest (k, v): scores_out float32, parents int32 (k) and
+ * tokens int32 (v), each [batch][n_select].  logits [batch][beams] rows of vocab values,
+ * row_stride elements apart (0 = dense), of dtype kcmm_dtype_t.  A NaN logit or score counts
+ * as -inf, a +inf logit as the largest finite value.  finished (uint8 [batch][beams], 0 =
+ * none): a finished beam's only continuation is eos_token at its own score.  n_select <= 64
+ * and <= beams * vocab; beams <= 1024; batch * beams, batch * n_select <= 65535.
+ */
+int kcmm_beam_select_on_stream(kcmm_pool_t *pool, uint64_t logits_ptr, uint32_t dtype,
+                               int64_t row_stride, uint64_t scores_in_ptr,
+                               uint64_t finished_ptr, uint32_t eos_token, uint32_t batch,
+                               uint32_t beams, uint32_t vocab, uint32_t n_select,
+                               uint64_t scores_out_ptr, uint64_t parents_ptr,
+                               uint64_t tokens_ptr, uint64_t stream_ptr);
+/**
+ * Gather per-beam state by parent: dst row (b, j) = src row (b, parents[b][j]), rows of
+ * row_bytes bytes (a multiple of 4), src [batch][beams], dst [batch][n_select], not
+ * overlapping.  With tokens_ptr set, the 32-bit entry token_index of dst row (b, j) becomes
+ * tokens[b][j] (a token history grows by one).  A parent out of range leaves its row and
+ * sets bit 2 of kcmm_get_kernel_status.
+ */
+int kcmm_beam_gather_on_stream(kcmm_pool_t *pool, uint64_t src_ptr, uint64_t dst_ptr,
+                               uint64_t row_bytes, uint64_t parents_ptr, uint32_t batch,
+                               uint32_t beams, uint32_t n_select, uint64_t tokens_ptr,
+                               uint64_t token_index, uint64_t stream_ptr);
+/**
+ * Reorder sequences after a beam step: seq_indices[i] takes the table and length that
+ * seq_indices[parents[i]] has now (host arrays of n).  Blocks move by reference counts alone;
+ * only blocks past a sequence's last whole one, which its next tokens are written to, are
+ * made private where several sequences would share them (fresh blocks, pages copied on
+ * stream_ptr).  On -1 no sequence has changed.
+ */
+int kcmm_reorder_sequences_on_stream(kcmm_pool_t *pool, const uint32_t *seq_indices,
+                                     const uint32_t *parents, uint32_t n, uint64_t stream_ptr);
+
 /* --- reference counting and copy-on-write (refcount seam of
        ref scripts/kcmm/shadow_allocator.py:22-110, skeleton ref
        src/kcmm/sharing.rs:61-101) --- */

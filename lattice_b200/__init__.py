@@ -6,6 +6,7 @@ The product is the native library `libkcmm.so` behind the C ABI in
 """
 from .kcmm import (  # noqa: F401
     BlockLocation,
+    CacheFormat,
     KcmmConfig,
     KcmmError,
     KcmmLibrary,
@@ -14,5 +15,6 @@ from .kcmm import (  # noqa: F401
     KcmmPoolStats,
     RopeMode,
     assert_layout,
+    kv4_row_elems,
     make_config,
 )

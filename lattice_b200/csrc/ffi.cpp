@@ -996,6 +996,220 @@ KCMM_DECODE_WEIGHTS(kcmm_paged_attn_decode_weights_f16_on_stream, F16, false)
 #undef KCMM_DECODE_WEIGHTS
 
 // ---------------------------------------------------------------------------
+// Eviction by accumulated attention weight, beam search
+// ---------------------------------------------------------------------------
+
+int kcmm_evict_tokens_on_stream(kcmm_pool_t *h, uint32_t layer, uint32_t cache_format,
+                                uint32_t hd, uint64_t tables, int64_t tables_row,
+                                uint64_t seq_lens, uint64_t offsets, uint32_t batch,
+                                uint32_t max_bps, uint32_t budget, uint32_t sinks,
+                                uint32_t recent, uint64_t w_in, uint64_t w_out, uint64_t p_in,
+                                uint64_t p_out, int64_t row_stride, uint64_t next_positions,
+                                uint64_t kept_lens, uint64_t new_lens, uint64_t stream) {
+  const char *op = "kcmm_evict_tokens_on_stream";
+  if (!h || !tables || !seq_lens || !offsets || !w_in || !w_out || !p_in || !p_out ||
+      !next_positions || !kept_lens || !new_lens) {
+    set_error(h, std::string(op) + ": null pointer argument");
+    return -1;
+  }
+  if (((tables | seq_lens | w_in | w_out | p_in | p_out | next_positions | kept_lens | new_lens) &
+       3) != 0) {
+    set_error(h, std::string(op) + ": arrays must be 4-byte aligned");
+    return -1;
+  }
+  if (batch == 0 || hd == 0 || max_bps == 0 || budget == 0 || row_stride <= 0) {
+    set_error(h, std::string(op) + ": shape arguments, budget and row stride must be positive");
+    return -1;
+  }
+  Pool *p = P(h);
+  if (batch > 0xFFFF || max_bps > 0xFFFF || p->cfg_.kv_heads > 0xFFFF ||
+      uint64_t(p->block_size) * max_bps > 0x7fffffffull || budget > 0x7fffffffu) {
+    set_error(h, std::string(op) + ": packed shape argument exceeds its limit");
+    return -1;
+  }
+  if (tables_row && tables_row < int64_t(max_bps)) {
+    set_error(h, std::string(op) + ": the block-table row stride must be 0 (dense) or >= "
+                                   "max_blocks_per_seq");
+    return -1;
+  }
+  if (uint64_t(sinks) + recent > budget) {
+    set_error(h, std::string(op) + ": sinks + recent must not exceed budget");
+    return -1;
+  }
+  if (cache_format > 1) {
+    set_error(h, std::string(op) + ": unknown cache_format " + std::to_string(cache_format));
+    return -1;
+  }
+  const bool kv4 = cache_format == KCMM_CACHE_KV4;
+  if (kv4) {
+    if (!check_kv4_pool(h, op, layer, hd)) return -1;
+  } else {
+    if (layer >= p->num_layers) {
+      set_error(h, std::string(op) + ": layer_idx " + std::to_string(layer) + " out of bounds");
+      return -1;
+    }
+    if (hd != p->cfg_.head_dim || hd % 8 != 0) {
+      set_error(h, std::string(op) + ": head_dim must be the pool's and a multiple of 8");
+      return -1;
+    }
+  }
+  if (guarded(h, op, [&] { p->require_device(op); })) return -1;
+  kcmm::dev::EvictArgs a = {};
+  a.kv4 = kv4;
+  a.va_k = reinterpret_cast<uint8_t *>(p->va_k[layer]);
+  a.va_v = reinterpret_cast<uint8_t *>(p->va_v[layer]);
+  a.region_bytes = p->region_bytes;
+  a.tables = reinterpret_cast<const int32_t *>(tables);
+  a.bt_stride = tables_row ? tables_row : int64_t(max_bps);
+  a.seq_lens = reinterpret_cast<const int32_t *>(seq_lens);
+  a.offsets = reinterpret_cast<const uint64_t *>(offsets);
+  a.batch = int(batch);
+  a.kv_heads = int(p->cfg_.kv_heads);
+  a.head_dim = int(hd);
+  a.block_size = int(p->block_size);
+  a.max_tokens = int(max_bps * p->block_size);
+  a.budget = int(budget);
+  a.sinks = int(sinks);
+  a.recent = int(recent);
+  a.w_in = reinterpret_cast<const float *>(w_in);
+  a.w_out = reinterpret_cast<float *>(w_out);
+  a.p_in = reinterpret_cast<const int32_t *>(p_in);
+  a.p_out = reinterpret_cast<int32_t *>(p_out);
+  a.w_stride = row_stride;
+  a.next_positions = reinterpret_cast<const int32_t *>(next_positions);
+  a.kept_lens = reinterpret_cast<const int32_t *>(kept_lens);
+  a.new_lens = reinterpret_cast<int32_t *>(new_lens);
+  a.diag = p->diag_word();
+  p->use_device();
+  return check_launch(h, op, kcmm::dev::evict_tokens(a, S(stream)));
+}
+
+int kcmm_truncate_sequence(kcmm_pool_t *h, uint32_t seq, uint32_t len) {
+  if (!h) return -1;
+  return guarded(h, "kcmm_truncate_sequence", [&] { P(h)->truncate_sequence(seq, len); });
+}
+
+int kcmm_beam_select_on_stream(kcmm_pool_t *h, uint64_t logits, uint32_t dtype,
+                               int64_t row_stride, uint64_t scores_in, uint64_t finished,
+                               uint32_t eos, uint32_t batch, uint32_t beams, uint32_t vocab,
+                               uint32_t n, uint64_t scores_out, uint64_t parents,
+                               uint64_t tokens, uint64_t stream) {
+  const char *op = "kcmm_beam_select_on_stream";
+  if (!h || !logits || !scores_in || !scores_out || !parents || !tokens) {
+    set_error(h, std::string(op) + ": null pointer argument");
+    return -1;
+  }
+  if (batch == 0 || beams == 0 || vocab == 0 || n == 0) {
+    set_error(h, std::string(op) + ": shape arguments must be positive");
+    return -1;
+  }
+  if (dtype > KCMM_DTYPE_F32) {
+    set_error(h, std::string(op) + ": unknown dtype " + std::to_string(dtype));
+    return -1;
+  }
+  if (n > uint32_t(kcmm::dev::kBeamMaxSelect) || beams > 1024 ||
+      uint64_t(batch) * std::max(beams, n) > 0xFFFF || uint64_t(beams) * vocab > 0x7fffffffull ||
+      n > uint64_t(beams) * vocab) {
+    set_error(h, std::string(op) + ": need n_select <= " +
+                     std::to_string(kcmm::dev::kBeamMaxSelect) +
+                     " and <= beams * vocab, beams <= 1024, batch * beams and batch * n_select "
+                     "<= 65535 and beams * vocab < 2^31");
+    return -1;
+  }
+  if (row_stride && row_stride < int64_t(vocab)) {
+    set_error(h, std::string(op) + ": the row stride must be 0 (dense) or >= vocab");
+    return -1;
+  }
+  const uint64_t elem = dtype == KCMM_DTYPE_F32 ? 4 : 2;
+  if (logits % elem || ((scores_in | scores_out | parents | tokens) & 3) != 0) {
+    set_error(h, std::string(op) + ": arrays must be aligned to their elements");
+    return -1;
+  }
+  if (finished && eos >= vocab) {
+    set_error(h, std::string(op) + ": eos_token must be below vocab where finished is given");
+    return -1;
+  }
+  Pool *p = P(h);
+  if (guarded(h, op, [&] { p->require_device(op); })) return -1;
+  kcmm::dev::BeamArgs a = {};
+  a.logits = reinterpret_cast<const void *>(logits);
+  a.type = int(dtype);
+  a.row_stride = row_stride ? row_stride : int64_t(vocab);
+  a.scores_in = reinterpret_cast<const float *>(scores_in);
+  a.finished = reinterpret_cast<const uint8_t *>(finished);
+  a.eos = eos;
+  a.batch = int(batch);
+  a.beams = int(beams);
+  a.vocab = int(vocab);
+  a.n = int(n);
+  a.scores_out = reinterpret_cast<float *>(scores_out);
+  a.parents = reinterpret_cast<int32_t *>(parents);
+  a.tokens = reinterpret_cast<int32_t *>(tokens);
+  p->use_device();
+  return check_launch(h, op, kcmm::dev::beam_select(a, S(stream)));
+}
+
+int kcmm_beam_gather_on_stream(kcmm_pool_t *h, uint64_t src, uint64_t dst, uint64_t row_bytes,
+                               uint64_t parents, uint32_t batch, uint32_t beams, uint32_t n,
+                               uint64_t tokens, uint64_t token_index, uint64_t stream) {
+  const char *op = "kcmm_beam_gather_on_stream";
+  if (!h || !src || !dst || !parents) {
+    set_error(h, std::string(op) + ": null pointer argument");
+    return -1;
+  }
+  if (batch == 0 || beams == 0 || n == 0 || row_bytes == 0) {
+    set_error(h, std::string(op) + ": shape arguments must be positive");
+    return -1;
+  }
+  if (uint64_t(batch) * n > 0xFFFF || beams > 0x7fffffffu || row_bytes > (1ull << 40)) {
+    set_error(h, std::string(op) + ": batch * n_select must be at most 65535");
+    return -1;
+  }
+  if ((row_bytes & 3) || ((src | dst | parents | tokens) & 3)) {
+    set_error(h, std::string(op) + ": rows and arrays must be multiples of 4 bytes");
+    return -1;
+  }
+  if (tokens && token_index >= row_bytes / 4) {
+    set_error(h, std::string(op) + ": token_index lies past the row");
+    return -1;
+  }
+  const uint64_t src_bytes = uint64_t(batch) * beams * row_bytes;
+  const uint64_t dst_bytes = uint64_t(batch) * n * row_bytes;
+  if (src < dst + dst_bytes && dst < src + src_bytes) {
+    set_error(h, std::string(op) + ": src and dst must not overlap");
+    return -1;
+  }
+  Pool *p = P(h);
+  if (guarded(h, op, [&] { p->require_device(op); })) return -1;
+  kcmm::dev::BeamGatherArgs a = {};
+  a.src = reinterpret_cast<const uint8_t *>(src);
+  a.dst = reinterpret_cast<uint8_t *>(dst);
+  a.row_bytes = int64_t(row_bytes);
+  a.parents = reinterpret_cast<const int32_t *>(parents);
+  a.tokens = reinterpret_cast<const int32_t *>(tokens);
+  a.token_index = int64_t(token_index);
+  a.batch = int(batch);
+  a.beams = int(beams);
+  a.n = int(n);
+  a.vec = ((src | dst | row_bytes) & 15) == 0;
+  a.diag = p->diag_word();
+  p->use_device();
+  return check_launch(h, op, kcmm::dev::beam_gather(a, S(stream)));
+}
+
+int kcmm_reorder_sequences_on_stream(kcmm_pool_t *h, const uint32_t *seqs,
+                                     const uint32_t *parents, uint32_t n, uint64_t stream) {
+  const char *op = "kcmm_reorder_sequences_on_stream";
+  if (!h || !seqs || !parents || n == 0) {
+    set_error(h, std::string(op) + ": null arguments or no sequences");
+    return -1;
+  }
+  return guarded(h, op, [&] {
+    P(h)->reorder_sequences(seqs, parents, n, reinterpret_cast<void *>(stream));
+  });
+}
+
+// ---------------------------------------------------------------------------
 // Chunked prefill (tcgen05)
 // ---------------------------------------------------------------------------
 

@@ -252,6 +252,12 @@ class Pool {
   // pages are copied on `stream` before the table entry moves.
   std::vector<uint32_t> cow_blocks(const uint32_t *seqs, const uint32_t *logical,
                                    size_t n, void *stream);
+  // Cut a sequence to its first `len` tokens; blocks past them are released.
+  void truncate_sequence(size_t seq, size_t len);
+  // seqs[i] takes the table and length that seqs[parents[i]] has now (beam search).  Blocks
+  // past a sequence's last whole one are made private: shared ones get a fresh block with
+  // the pages copied on `stream`.  All or nothing: an error changes no sequence.
+  void reorder_sequences(const uint32_t *seqs, const uint32_t *parents, size_t n, void *stream);
   // --- tiering (ref src/kcmm/tiering.rs) ---
   bool tiering_enabled() const { return cfg_.tiering; }
   std::string policy_name();
@@ -302,6 +308,7 @@ class Pool {
 
  private:
   void ensure_capacity_locked();
+  void free_blocks_locked(const uint32_t *ids, size_t n);
   uint32_t install_locked(BlockHandle h);
   void release_block_locked(uint32_t blk, std::vector<BlockHandle> *gpu,
                             std::vector<uint64_t> *cpu_slots);

@@ -22,6 +22,7 @@
 
 #include "../launch.hpp"
 #include "finish.cuh"
+#include "kv4_layout.cuh"
 #include "pdl.cuh"
 #include "ptx.cuh"
 
@@ -29,19 +30,8 @@ namespace kcmm {
 namespace dev {
 namespace {
 
-constexpr int kUnit = 16;   // tokens of a chunk
-constexpr int kGroup = 32;  // values of a scale
-
-// Byte offset, inside a chunk, of lane `lane`'s word w of group j.  Groups lie in pairs
-// where their number is even, so that a lane's load is 16 bytes instead of 8.
-__host__ __device__ constexpr int code_offset(int groups, int j, int lane, int w) {
-  return groups % 2 == 0 ? ((j >> 1) * 32 + lane) * 16 + (j & 1) * 8 + w * 4
-                         : (j * 32 + lane) * 8 + w * 4;
-}
-// Byte offset of the scale of token t (of 16), group j: a lane's tokens g and g+8 adjoin.
-__host__ __device__ constexpr int scale_offset(int groups, int t, int j) {
-  return groups * 256 + (((t & 7) * 2 + (t >> 3)) * groups + j) * 2;
-}
+constexpr int kUnit = kKv4Unit;
+constexpr int kGroup = kKv4Group;
 
 // --- append and read -----------------------------------------------------------------
 
@@ -128,14 +118,14 @@ __global__ void kv4_append_kernel(const Kv4RowsArgs a) {
     if (!live) continue;
     if (is_v) {
       const int lane = in * 4 + (t & 7) / 2;
-      *reinterpret_cast<uint16_t *>(chunk + code_offset(groups, j, lane, t >> 3) + (t & 1) * 2) =
+      *reinterpret_cast<uint16_t *>(chunk + kv4_code_offset(groups, j, lane, t >> 3) + (t & 1) * 2) =
           uint16_t(n[0] | (n[1] << 4) | (n[2] << 8) | (n[3] << 12));
     } else if ((in & 1) == 0) {
       const int lane = (t & 7) * 4 + in / 2;
-      *reinterpret_cast<uint32_t *>(chunk + code_offset(groups, j, lane, t >> 3)) =
+      *reinterpret_cast<uint32_t *>(chunk + kv4_code_offset(groups, j, lane, t >> 3)) =
           half | (other << 8);
     }
-    if (in == 0) *reinterpret_cast<__nv_bfloat16 *>(chunk + scale_offset(groups, t, j)) = s;
+    if (in == 0) *reinterpret_cast<__nv_bfloat16 *>(chunk + kv4_scale_offset(groups, t, j)) = s;
   }
 }
 
@@ -161,13 +151,13 @@ __global__ void kv4_read_kernel(const Kv4RowsArgs a) {
     if (is_v) {
       const int lane = in * 4 + (t & 7) / 2;
       const uint32_t w = *reinterpret_cast<const uint16_t *>(
-          chunk + code_offset(groups, j, lane, t >> 3) + (t & 1) * 2);
+          chunk + kv4_code_offset(groups, j, lane, t >> 3) + (t & 1) * 2);
 #pragma unroll
       for (int k = 0; k < 4; ++k) n[k] = (w >> (4 * k)) & 15u;
     } else {
       const int lane = (t & 7) * 4 + in / 2;
       const uint32_t w =
-          *reinterpret_cast<const uint32_t *>(chunk + code_offset(groups, j, lane, t >> 3)) >>
+          *reinterpret_cast<const uint32_t *>(chunk + kv4_code_offset(groups, j, lane, t >> 3)) >>
           ((in & 1) * 8);
       n[0] = w & 15u;
       n[2] = (w >> 4) & 15u;
@@ -175,7 +165,7 @@ __global__ void kv4_read_kernel(const Kv4RowsArgs a) {
       n[3] = (w >> 20) & 15u;
     }
     const float s = __bfloat162float(
-        *reinterpret_cast<const __nv_bfloat16 *>(chunk + scale_offset(groups, t, j)));
+        *reinterpret_cast<const __nv_bfloat16 *>(chunk + kv4_scale_offset(groups, t, j)));
     T *dst = static_cast<T *>(is_v ? a.v : a.k) +
              int64_t(row) * (is_v ? a.v_stride : a.k_stride) + e;
     __align__(8) T y[4];

@@ -135,6 +135,63 @@ cudaError_t kv4_decode_attention(const DecodeArgs &a, const DecodeWeights &w,
 cudaError_t decode_attention_weights(const DecodeArgs &a, const DecodeWeights &w,
                                      cudaStream_t stream);
 
+// --- eviction by accumulated attention weight (kernels/evict.cu) ---
+struct EvictArgs {
+  bool kv4;
+  uint8_t *va_k;
+  uint8_t *va_v;
+  uint64_t region_bytes;
+  const int32_t *tables;
+  int64_t bt_stride;
+  const int32_t *seq_lens;
+  const uint64_t *offsets;  // 2-byte units
+  int batch, kv_heads, head_dim, block_size;
+  int max_tokens;  // of a table row
+  int budget, sinks, recent;
+  const float *w_in;  // [batch][kv_heads][w_stride], positions alike
+  float *w_out;
+  const int32_t *p_in;
+  int32_t *p_out;
+  int64_t w_stride;
+  const int32_t *next_positions;  // [batch]
+  const int32_t *kept_lens;       // [batch]
+  int32_t *new_lens;              // [batch]
+  int32_t *diag;
+  int32_t *scratch;  // filled by the launcher
+};
+cudaError_t evict_tokens(const EvictArgs &a, cudaStream_t stream);
+
+// --- beam search (kernels/beam.cu) ---
+constexpr int kBeamMaxSelect = 64;
+struct BeamArgs {
+  const void *logits;  // [batch * beams] rows of row_stride
+  int type;            // 0 f16, 1 bf16, 2 f32
+  int64_t row_stride;
+  const float *scores_in;   // [batch * beams]
+  const uint8_t *finished;  // [batch * beams] or null
+  uint32_t eos;
+  int batch, beams, vocab, n;
+  float *scores_out;  // [batch * n]
+  int32_t *parents;
+  int32_t *tokens;
+  int chunks;  // filled by the launcher, as the scratch arrays
+  unsigned long long *cand;
+  float2 *part;
+};
+cudaError_t beam_select(const BeamArgs &a, cudaStream_t stream);
+struct BeamGatherArgs {
+  const uint8_t *src;  // [batch][beams] rows
+  uint8_t *dst;        // [batch][n] rows
+  int64_t row_bytes;
+  const int32_t *parents;  // [batch * n]
+  const int32_t *tokens;   // [batch * n] or null
+  int64_t token_index;     // 32-bit entry of a dst row that takes tokens
+  int batch, beams, n;
+  bool vec;  // rows start on 16 bytes and are a multiple of 16 long
+  int32_t *diag;
+};
+cudaError_t beam_gather(const BeamGatherArgs &a, cudaStream_t stream);
+
 // Scratch of one call: the stream's kept buffer where there is one (stream_scratch), else
 // a stream-ordered allocation that release() frees in stream order.
 struct CallScratch {

@@ -399,6 +399,10 @@ void Pool::finish_release_locked(const std::vector<BlockHandle> &gpu,
 
 void Pool::free_blocks(const uint32_t *ids, size_t n) {
   std::lock_guard<std::mutex> g(mu_);
+  free_blocks_locked(ids, n);
+}
+
+void Pool::free_blocks_locked(const uint32_t *ids, size_t n) {
   std::vector<BlockHandle> gpu;
   std::vector<uint64_t> cpu;
   std::vector<uint32_t> recycled;
@@ -738,6 +742,122 @@ std::vector<uint32_t> Pool::cow_blocks(const uint32_t *seqs, const uint32_t *log
     if (e != cudaSuccess) throw Error(std::string("block copy launch failed: ") + cudaGetErrorString(e));
   }
   return out;
+}
+
+void Pool::truncate_sequence(size_t seq, size_t len) {
+  std::lock_guard<std::mutex> g(mu_);
+  if (seq >= seqs_.size()) throw Error("seq_idx " + std::to_string(seq) + " out of bounds");
+  Sequence &s = seqs_[seq];
+  if (len > s.seq_len) {
+    throw Error("len " + std::to_string(len) + " exceeds the sequence's " +
+                std::to_string(s.seq_len) + " tokens");
+  }
+  const size_t keep = (len + block_size - 1) / block_size;
+  s.seq_len = len;
+  if (keep >= s.table.size()) return;
+  const std::vector<uint32_t> gone(s.table.begin() + long(keep), s.table.end());
+  s.table.resize(keep);
+  touch_table_locked(s, true);
+  free_blocks_locked(gone.data(), gone.size());
+}
+
+void Pool::reorder_sequences(const uint32_t *seqs, const uint32_t *parents, size_t n,
+                             void *stream) {
+  std::lock_guard<std::mutex> g(mu_);
+  std::vector<char> seen(seqs_.size(), 0);
+  for (size_t i = 0; i < n; ++i) {
+    if (seqs[i] >= seqs_.size())
+      throw Error("seq_idx " + std::to_string(seqs[i]) + " out of bounds");
+    if (seen[seqs[i]]++) throw Error("seq_idx " + std::to_string(seqs[i]) + " is listed twice");
+    if (parents[i] >= n) throw Error("parent " + std::to_string(parents[i]) + " out of bounds");
+    for (uint32_t b : seqs_[seqs[i]].table) {
+      if (b >= blocks_.size() || !blocks_[b].in_use)
+        throw Error("block_idx " + std::to_string(b) + " is not in use");
+    }
+  }
+  // The new state, and how many owners each touched block has in it.
+  struct State {
+    std::vector<uint32_t> table;
+    size_t seq_len = 0;
+  };
+  std::vector<State> next(n);
+  std::map<uint32_t, int64_t> owners;
+  auto owner = [&](uint32_t b) -> int64_t & {
+    return owners.emplace(b, int64_t(blocks_[b].refcount)).first->second;
+  };
+  for (size_t i = 0; i < n; ++i) {
+    const Sequence &p = seqs_[seqs[parents[i]]];
+    next[i].table = p.table;
+    next[i].seq_len = p.seq_len;
+    for (uint32_t b : p.table) owner(b) += 1;
+    for (uint32_t b : seqs_[seqs[i]].table) owner(b) -= 1;
+  }
+  // Blocks that later tokens are written to: past the last whole one.
+  struct Copy {
+    size_t seq, logical;
+    uint32_t from;
+    BlockHandle to;
+  };
+  std::vector<Copy> copies;
+  for (size_t i = 0; i < n; ++i) {
+    for (size_t l = next[i].seq_len / block_size; l < next[i].table.size(); ++l) {
+      const uint32_t b = next[i].table[l];
+      if (owner(b) <= 1) continue;
+      if (blocks_[b].loc != Loc::Gpu)
+        throw Error("block_idx " + std::to_string(b) + " is not a GPU-resident live block");
+      owner(b) -= 1;
+      copies.push_back({i, l, b, {}});
+    }
+  }
+  if (!copies.empty()) require_device("kcmm_reorder_sequences_on_stream");
+  size_t got = 0;
+  try {
+    for (; got < copies.size(); ++got) {
+      ensure_capacity_locked();
+      if (!alloc_.try_allocate(&copies[got].to))
+        throw Error("no free block after ensure_capacity");
+    }
+  } catch (...) {
+    while (got > 0) alloc_.free(copies[--got].to);
+    throw;
+  }
+  if (!copies.empty()) {
+    std::vector<uint64_t> src, dst;
+    for (const Copy &c : copies) {
+      src.push_back(blocks_[c.from].va_offset);
+      dst.push_back(offset_of(c.to));
+    }
+    use_device();
+    const cudaError_t e = dev::copy_blocks(d_layer_bases, int(num_layers), src.data(), dst.data(),
+                                           int(src.size()), block_bytes,
+                                           static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) {
+      for (const Copy &c : copies) alloc_.free(c.to);
+      throw Error(std::string("block copy launch failed: ") + cudaGetErrorString(e));
+    }
+  }
+  // Nothing below fails: new owners first, then the old ones go.
+  for (const State &s : next)
+    for (uint32_t b : s.table) blocks_[b].refcount += 1;
+  std::vector<uint32_t> gone;
+  for (size_t i = 0; i < n; ++i) {
+    const auto &t = seqs_[seqs[i]].table;
+    gone.insert(gone.end(), t.begin(), t.end());
+  }
+  for (const Copy &c : copies) {
+    next[c.seq].table[c.logical] = install_locked(c.to);
+    gone.push_back(c.from);
+  }
+  for (size_t i = 0; i < n; ++i) {
+    Sequence &s = seqs_[seqs[i]];
+    if (s.table != next[i].table) {
+      s.table = std::move(next[i].table);
+      touch_table_locked(s, true);
+      register_positions_locked(seqs[i], 0);
+    }
+    s.seq_len = next[i].seq_len;
+  }
+  free_blocks_locked(gone.data(), gone.size());
 }
 
 // --- append destinations ---------------------------------------------------

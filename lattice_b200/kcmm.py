@@ -116,6 +116,15 @@ class BlockLocation:
         return cls._NAMES.get(value, f"unknown({value})")
 
 
+class CacheFormat:
+    """What a pool's pages hold (`kcmm_cache_format_t`)."""
+    BITS16 = 0
+    KV4 = 1
+
+
+_DTYPES = {"f16": 0, "bf16": 1, "f32": 2}  # kcmm_dtype_t
+
+
 class RopeMode:
     REFERENCE = 0
     GPTJ = 1
@@ -246,6 +255,15 @@ SIGNATURES: dict[str, tuple] = {
        (i32, [P, u32, u64, i64, i64, u64, i64, i64, u64, i64, u64, u64, u32, u32, u32, u32, u32,
               u32, f32, u64, u64, i64, u64])
        for op in ("kv4_paged_attn_decode", "paged_attn_decode_weights") for dt in ("bf16", "f16")},
+    "kcmm_evict_tokens_on_stream":
+        (i32, [P, u32, u32, u32, u64, i64, u64, u64, u32, u32, u32, u32, u32, u64, u64, u64, u64,
+               i64, u64, u64, u64, u64]),
+    "kcmm_truncate_sequence": (i32, [P, u32, u32]),
+    "kcmm_beam_select_on_stream":
+        (i32, [P, u64, u32, i64, u64, u64, u32, u32, u32, u32, u32, u64, u64, u64, u64]),
+    "kcmm_beam_gather_on_stream":
+        (i32, [P, u64, u64, u64, u64, u32, u32, u32, u64, u64, u64]),
+    "kcmm_reorder_sequences_on_stream": (i32, [P, pu32, pu32, u32, u64]),
     "kcmm_block_incref": (i32, [P, u32]),
     "kcmm_block_decref": (i32, [P, u32]),
     "kcmm_block_refcount": (u32, [P, u32]),
@@ -655,6 +673,53 @@ class KcmmPool:
     def paged_attn_decode_weights(self, layer: int, **kw) -> None:
         """`kv4_paged_attn_decode` over the 16-bit cache, the weights required."""
         self._decode_weights("paged_attn_decode_weights", layer, **kw)
+
+    # --- eviction by accumulated attention weight -----------------------------
+    def evict_tokens(self, layer: int, *, head_dim: int, block_tables_ptr: int,
+                     seq_lens_ptr: int, block_offsets_f16_ptr: int, batch: int,
+                     max_blocks_per_seq: int, budget: int, sinks: int, recent: int,
+                     weights_in_ptr: int, weights_out_ptr: int, weights_row_stride: int,
+                     positions_in_ptr: int, positions_out_ptr: int, next_positions_ptr: int,
+                     kept_lens_ptr: int, new_lens_ptr: int,
+                     cache_format: int = CacheFormat.BITS16, block_tables_row_stride: int = 0,
+                     stream_ptr: int = 0) -> None:
+        """Cut one layer's cached tokens to `budget` per kv head; `weights_row_stride` is the
+        row stride of the positions too.  `truncate_sequence` afterwards."""
+        self._check(self.lib.kcmm_evict_tokens_on_stream(
+            self.handle, layer, cache_format, head_dim, block_tables_ptr,
+            block_tables_row_stride, seq_lens_ptr, block_offsets_f16_ptr, batch,
+            max_blocks_per_seq, budget, sinks, recent, weights_in_ptr, weights_out_ptr,
+            positions_in_ptr, positions_out_ptr, weights_row_stride, next_positions_ptr,
+            kept_lens_ptr, new_lens_ptr, stream_ptr), "kcmm_evict_tokens_on_stream")
+
+    def truncate_sequence(self, seq_idx: int, length: int) -> None:
+        self._check(self.lib.kcmm_truncate_sequence(self.handle, seq_idx, length),
+                    "kcmm_truncate_sequence")
+
+    # --- beam search -----------------------------------------------------------
+    def beam_select(self, *, logits_ptr: int, dtype: str, scores_in_ptr: int, batch: int,
+                    beams: int, vocab: int, n_select: int, scores_out_ptr: int,
+                    parents_out_ptr: int, tokens_out_ptr: int, row_stride: int = 0, finished_ptr: int = 0, eos_token: int = 0,
+                    stream_ptr: int = 0) -> None:
+        """The `n_select` best continuations of each request's beams."""
+        self._check(self.lib.kcmm_beam_select_on_stream(
+            self.handle, logits_ptr, _DTYPES[dtype], row_stride, scores_in_ptr, finished_ptr,
+            eos_token, batch, beams, vocab, n_select, scores_out_ptr, parents_out_ptr,
+            tokens_out_ptr, stream_ptr), "kcmm_beam_select_on_stream")
+
+    def beam_gather(self, *, src_ptr: int, dst_ptr: int, row_bytes: int, parents_ptr: int,
+                    batch: int, beams: int, n_select: int, tokens_ptr: int = 0,
+                    token_index: int = 0, stream_ptr: int = 0) -> None:
+        """dst row (b, j) = src row (b, parents[b][j])."""
+        self._check(self.lib.kcmm_beam_gather_on_stream(
+            self.handle, src_ptr, dst_ptr, row_bytes, parents_ptr, batch, beams, n_select,
+            tokens_ptr, token_index, stream_ptr), "kcmm_beam_gather_on_stream")
+
+    def reorder_sequences(self, seq_indices, parents, stream_ptr: int = 0) -> None:
+        """seq_indices[i] continues what seq_indices[parents[i]] holds now."""
+        self._check(self.lib.kcmm_reorder_sequences_on_stream(
+            self.handle, _u32_array(seq_indices), _u32_array(parents), len(seq_indices),
+            stream_ptr), "kcmm_reorder_sequences_on_stream")
 
     # --- decode attention --------------------------------------------------
     def paged_attn_decode(self, layer: int, *, query_ptr: int, out_ptr: int,

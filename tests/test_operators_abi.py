@@ -84,3 +84,109 @@ def test_decode_weights_pool_shape_checks(host_pool_factory):
         plain.paged_attn_decode_weights(0, **DECODE)
     with pytest.raises(KcmmError, match="multiple of 16"):
         plain.paged_attn_decode_weights(0, **{**DECODE, **WEIGHTS, "block_size": 8})
+
+
+EVICT = dict(head_dim=64, block_tables_ptr=16, seq_lens_ptr=16, block_offsets_f16_ptr=16, batch=2,
+             max_blocks_per_seq=4, budget=32, sinks=2, recent=8, weights_in_ptr=16,
+             weights_out_ptr=16, weights_row_stride=64, positions_in_ptr=16, positions_out_ptr=16,
+             next_positions_ptr=16, kept_lens_ptr=16, new_lens_ptr=16)
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(kept_lens_ptr=0), "null pointer"), (dict(positions_in_ptr=18), "4-byte aligned"),
+    (dict(budget=0), "must be positive"), (dict(weights_row_stride=0), "must be positive"),
+    (dict(batch=65536), "limit"), (dict(block_tables_row_stride=3), "row stride"),
+    (dict(sinks=30), "must not exceed budget"), (dict(cache_format=2), "unknown cache_format"),
+    (dict(head_dim=32), "the pool's"), (dict(cache_format=1), "needs 18"),
+    (dict(layer=2), "out of bounds"), ({}, "no device memory")])
+def test_evict_checks(host_pool_factory, kw, msg):
+    pool = host_pool_factory(kv_heads=2, head_dim=64, max_batch=2, max_seq_len=64)
+    args = {**EVICT, **kw}
+    layer = args.pop("layer", 0)
+    with pytest.raises(KcmmError, match=msg):
+        pool.evict_tokens(layer, **args)
+
+
+SELECT = dict(logits_ptr=16, dtype="bf16", scores_in_ptr=16, batch=2, beams=4, vocab=1000,
+              n_select=8, scores_out_ptr=16, parents_out_ptr=16, tokens_out_ptr=16)
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(logits_ptr=0), "null pointer"), (dict(vocab=0), "must be positive"),
+    (dict(n_select=65), "n_select <= 64"), (dict(beams=1, vocab=5), "beams \\* vocab"),
+    (dict(batch=20000), "65535"), (dict(vocab=1 << 30), "2\\^31"), (dict(row_stride=999), "stride"),
+    (dict(logits_ptr=17), "aligned"), (dict(finished_ptr=16, eos_token=1000), "eos_token"),
+    ({}, "no device memory")])
+def test_beam_select_checks(host_pool_factory, kw, msg):
+    pool = host_pool_factory(kv_heads=2, head_dim=64, max_batch=2, max_seq_len=64)
+    with pytest.raises(KcmmError, match=msg):
+        pool.beam_select(**{**SELECT, **kw})
+
+
+def test_beam_select_unknown_dtype(kcmm_lib, host_pool_factory):
+    pool = host_pool_factory(kv_heads=2, head_dim=64, max_batch=2, max_seq_len=64)
+    assert kcmm_lib.lib.kcmm_beam_select_on_stream(pool.handle, 16, 3, 0, 16, 0, 0, 1, 1, 8, 1, 16,
+                                                   16, 16, 0) == -1
+    assert "unknown dtype" in pool.last_error()
+
+
+GATHER = dict(src_ptr=1024, dst_ptr=65536, row_bytes=64, parents_ptr=16, batch=2, beams=4,
+              n_select=4)
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(parents_ptr=0), "null pointer"), (dict(row_bytes=0), "must be positive"),
+    (dict(row_bytes=66), "multiples of 4"), (dict(dst_ptr=1024 + 256), "overlap"),
+    (dict(batch=65535), "65535"), (dict(tokens_ptr=16, token_index=16), "past the row"),
+    ({}, "no device memory")])
+def test_beam_gather_checks(host_pool_factory, kw, msg):
+    pool = host_pool_factory(kv_heads=2, head_dim=64, max_batch=2, max_seq_len=64)
+    with pytest.raises(KcmmError, match=msg):
+        pool.beam_gather(**{**GATHER, **kw})
+
+
+def test_truncate_sequence(host_pool_factory):
+    pool = host_pool_factory(kv_heads=2, head_dim=64, max_batch=4, max_seq_len=64)
+    blocks = pool.alloc_blocks(4)
+    seq = pool.register_sequence(blocks)
+    pool.update_seq_len(seq, 60)
+    fork = pool.fork_sequence(seq)
+    pool.truncate_sequence(seq, 33)
+    assert pool.block_table(seq) == blocks[:3] and pool.seq_len(seq) == 33
+    assert pool.blocks_in_use() == 4 and pool.refcount(blocks[3]) == 1  # the fork's
+    pool.truncate_sequence(fork, 32)
+    assert pool.block_table(fork) == blocks[:2] and pool.blocks_in_use() == 3
+    pool.truncate_sequence(seq, 33)
+    pool.truncate_sequence(seq, 0)
+    assert pool.block_table(seq) == [] and pool.blocks_in_use() == 2
+    with pytest.raises(KcmmError, match="exceeds"):
+        pool.truncate_sequence(fork, 33)
+    with pytest.raises(KcmmError, match="out of bounds"):
+        pool.truncate_sequence(9, 0)
+
+
+def test_reorder_sequences(host_pool_factory):
+    """Whole blocks move by reference counts alone; nothing changes on an error."""
+    pool = host_pool_factory(kv_heads=2, head_dim=64, max_batch=4, max_seq_len=64)
+    tables = [pool.alloc_blocks(2) for _ in range(3)]
+    seqs = [pool.register_sequence(t) for t in tables]
+    for s, n in zip(seqs, (32, 32, 16)):
+        pool.update_seq_len(s, n)
+
+    def state():
+        return ([pool.block_table(s) for s in seqs], [pool.seq_len(s) for s in seqs],
+                pool.blocks_in_use(), [pool.refcount(b) for t in tables for b in t])
+
+    before = state()
+    for bad, msg in (((seqs, [0, 1, 3]), "out of bounds"), (([0, 1, 7], [0, 1, 2]), "out of bounds"),
+                     (([0, 1, 0], [0, 1, 2]), "twice"),
+                     ((seqs, [2, 2, 2]), "no device memory")):  # a spare block of 2 is shared
+        with pytest.raises(KcmmError, match=msg):
+            pool.reorder_sequences(*bad)
+        assert state() == before
+    pool.reorder_sequences(seqs, [0, 1, 2])
+    assert state() == before
+    pool.reorder_sequences(seqs, [1, 0, 2])  # a swap frees nothing
+    assert state() == ([tables[1], tables[0], tables[2]], [32, 32, 16], 6, [1] * 6)
+    pool.reorder_sequences(seqs, [1, 1, 2])  # table 1 is dropped, table 0 has two owners
+    assert state() == ([tables[0], tables[0], tables[2]], [32, 32, 16], 4, [2, 2, 0, 0, 1, 1])
