@@ -892,6 +892,10 @@ static int decode_weights_impl(kcmm_pool_t *h, const char *op, kcmm::dev::Dtype 
     set_error(h, std::string(op) + ": packed shape argument exceeds 65535");
     return -1;
   }
+  if (uint64_t(batch) * max_bps * bs > 16ull * 0x3fffffff) {
+    set_error(h, std::string(op) + ": batch * max_blocks_per_seq * block_size overflow");
+    return -1;
+  }
   if (hq < hkv) {
     set_error(h, std::string(op) + ": num_q_heads must be at least kv_heads");
     return -1;

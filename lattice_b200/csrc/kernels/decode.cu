@@ -1140,6 +1140,9 @@ size_t decode_scratch_bytes(const DecodeArgs &a) { return make_plan(a).scratch_b
 // caller then allocates for the call alone.
 constexpr size_t kMaxCachedStreams = 16;
 
+// Every buffer starts with kZeroedCounters zeroed words that the bytes asked for follow.
+constexpr size_t kCounterBytes = size_t(kZeroedCounters) * sizeof(int32_t);
+
 void *stream_scratch(cudaStream_t stream, size_t bytes) {
   cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(stream, &cs) != cudaSuccess) {
@@ -1166,36 +1169,56 @@ void *stream_scratch(cudaStream_t stream, size_t bytes) {
     it = cache.emplace(std::make_pair(dev, id), Entry{}).first;
   }
   Entry &en = it->second;
-  if (en.bytes >= bytes) return en.ptr;
+  if (en.bytes >= bytes) return static_cast<char *>(en.ptr) + kCounterBytes;
   cudaMemPool_t mp = scratch_pool(dev);
   if (!mp) return nullptr;
   void *fresh = nullptr;
   const size_t want = std::max(bytes, en.bytes + en.bytes / 2);
-  if (cudaMallocFromPoolAsync(&fresh, want, mp, stream) != cudaSuccess) {
+  if (cudaMallocFromPoolAsync(&fresh, kCounterBytes + want, mp, stream) != cudaSuccess) {
     cudaGetLastError();
+    return nullptr;
+  }
+  if (cudaMemsetAsync(fresh, 0, kCounterBytes, stream) != cudaSuccess) {
+    cudaGetLastError();
+    cudaFreeAsync(fresh, stream);
     return nullptr;
   }
   if (en.ptr) cudaFreeAsync(en.ptr, stream);
   en.ptr = fresh;
   en.bytes = want;
-  return fresh;
+  return static_cast<char *>(fresh) + kCounterBytes;
 }
 
 cudaError_t CallScratch::acquire(cudaStream_t stream, size_t bytes) {
-  if ((ptr = stream_scratch(stream, bytes)) != nullptr) return cudaSuccess;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  cudaMemPool_t mp = scratch_pool(dev);
-  if (!mp) return cudaErrorMemoryAllocation;
-  const cudaError_t e = cudaMallocFromPoolAsync(&ptr, bytes, mp, stream);
-  owned = e == cudaSuccess;
-  return e;
+  char *base = static_cast<char *>(stream_scratch(stream, bytes));
+  if (base) {
+    base -= kCounterBytes;
+  } else {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaMemPool_t mp = scratch_pool(dev);
+    if (!mp) return cudaErrorMemoryAllocation;
+    void *fresh = nullptr;
+    cudaError_t e = cudaMallocFromPoolAsync(&fresh, kCounterBytes + bytes, mp, stream);
+    if (e != cudaSuccess) return e;
+    owned = true;
+    base = static_cast<char *>(fresh);
+    counters = reinterpret_cast<int32_t *>(base);
+    e = cudaMemsetAsync(base, 0, kCounterBytes, stream);
+    if (e != cudaSuccess) {
+      release(stream);
+      return e;
+    }
+  }
+  counters = reinterpret_cast<int32_t *>(base);
+  ptr = base + kCounterBytes;
+  return cudaSuccess;
 }
 
 cudaError_t CallScratch::release(cudaStream_t stream) {
   if (!owned) return cudaSuccess;
   owned = false;
-  return cudaFreeAsync(ptr, stream);
+  return cudaFreeAsync(counters, stream);
 }
 
 int device_sm_count() { return sm_count(); }
@@ -1374,9 +1397,7 @@ cudaError_t decode_attention_weights(const DecodeArgs &a, const DecodeWeights &w
     f.w_in = w.w_in;
     f.w_out = w.w_out;
     f.w_stride = w.w_stride;
-    const dim3 grid((max_tokens + kFinishTokens - 1) / kFinishTokens, a.kv_heads, a.batch);
-    e = launch_pdl(a.dtype == Dtype::BF16 ? finish_kernel<__nv_bfloat16> : finish_kernel<__half>,
-                   grid, dim3(kFinishThreads), 0, stream, f);
+    e = launch_finish(a.dtype, f, a.batch, stream);
   }
   const cudaError_t r = scratch.release(stream);
   return e != cudaSuccess ? e : r;

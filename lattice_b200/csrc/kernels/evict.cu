@@ -305,8 +305,8 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
       for (int i = lane; i < 2 * groups; i += 32) {
         uint8_t *base = i < groups ? a.va_k : a.va_v;
         const int jg = i % groups;
-        *reinterpret_cast<uint16_t *>(base + d + kv4_scale_offset(groups, td, jg)) =
-            *reinterpret_cast<const uint16_t *>(base + s + kv4_scale_offset(groups, ts, jg));
+        *reinterpret_cast<uint16_t *>(base + d + kv4_scale_offset(i >= groups, groups, td, jg)) =
+            *reinterpret_cast<const uint16_t *>(base + s + kv4_scale_offset(i >= groups, groups, ts, jg));
       }
     }
   }

@@ -12,6 +12,8 @@
 
 #include <cstdint>
 
+#include "../launch.hpp"
+#include "pdl.cuh"
 #include "ptx.cuh"
 
 namespace kcmm {
@@ -27,7 +29,8 @@ struct FinishParams {
   int max_tokens;  // seq_lens are capped to this
   int hq, hkv, head_dim;
   int num_splits, tokens_per_split;
-  const float *part_o;    // [b * hq + h][num_splits][head_dim], each split normalised
+  const float *part_o;    // [b * hq + h][num_splits][head_dim], each split normalised; null:
+                          // the output is done, part_lse has the rows' own
   const float *part_lse;  // [b * hq + h][num_splits], log2 units
   void *out;
   int64_t o_sb, o_sh;
@@ -68,7 +71,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const FinishPara
     if (lane == 0) s_lse[h] = total;
   }
   __syncthreads();
-  if (blockIdx.x == 0) {
+  if (blockIdx.x == 0 && p.part_o) {
     const int D = p.head_dim, quads = D / 4;
     for (int i = threadIdx.x; i < G * quads; i += kFinishThreads) {
       const int h = i / quads, d = (i - h * quads) * 4;
@@ -102,6 +105,13 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const FinishPara
     for (int h = 0; h < G; ++h) sum += ptx::fast_exp2(sc[h * p.score_stride + t] - s_lse[h]);
     p.w_out[wrow + t] = w + sum;
   }
+}
+
+inline cudaError_t launch_finish(Dtype dtype, const FinishParams &f, int batch,
+                                 cudaStream_t stream) {
+  const int chunks = f.scores ? (f.max_tokens + kFinishTokens - 1) / kFinishTokens : 1;
+  return launch_pdl(dtype == Dtype::BF16 ? finish_kernel<__nv_bfloat16> : finish_kernel<__half>,
+                    dim3(chunks, f.hkv, batch), dim3(kFinishThreads), 0, stream, f);
 }
 
 }  // namespace

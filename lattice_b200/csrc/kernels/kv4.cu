@@ -7,12 +7,14 @@
 //
 // Layout.  A page holds [kv head][16-token unit] chunks of 9 D bytes: 8 D of codes, then
 // 16 D/32 scales.  Inside a chunk the codes lie in the order in which the lanes of a warp
-// hold the operands of mma.m16n8k16, so a decode warp loads them straight from global
-// memory into its operand registers, 16 bytes a lane, without shared memory or shuffles:
+// hold the operands of the decode's mma, so that it reads them 16 bytes a lane and unpacks
+// them in place, without shuffles or transposes:
 //   K (A operand, rows = tokens): lane (g, c) holds words of tokens g and g+8;
 //     the word of group j has dims 32j+8c+{0..7}, dim 2i in nibble i and 2i+1 in nibble i+4;
 //   V (A operand transposed, rows = dims): the lane's words are tokens (2c, 2c+1) and
 //     (2c+8, 2c+9), the even token in the low half; nibble i is dim 32j+4g+i.
+// The scales lie in the order of the accumulators they meet: K's by token (g, g+8), V's by
+// token pair as the codes.
 // No byte holds two tokens, so appends need no read-modify-write.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -125,7 +127,8 @@ __global__ void kv4_append_kernel(const Kv4RowsArgs a) {
       *reinterpret_cast<uint32_t *>(chunk + kv4_code_offset(groups, j, lane, t >> 3)) =
           half | (other << 8);
     }
-    if (in == 0) *reinterpret_cast<__nv_bfloat16 *>(chunk + kv4_scale_offset(groups, t, j)) = s;
+    if (in == 0)
+      *reinterpret_cast<__nv_bfloat16 *>(chunk + kv4_scale_offset(is_v, groups, t, j)) = s;
   }
 }
 
@@ -165,7 +168,7 @@ __global__ void kv4_read_kernel(const Kv4RowsArgs a) {
       n[3] = (w >> 20) & 15u;
     }
     const float s = __bfloat162float(
-        *reinterpret_cast<const __nv_bfloat16 *>(chunk + kv4_scale_offset(groups, t, j)));
+        *reinterpret_cast<const __nv_bfloat16 *>(chunk + kv4_scale_offset(is_v, groups, t, j)));
     T *dst = static_cast<T *>(is_v ? a.v : a.k) +
              int64_t(row) * (is_v ? a.v_stride : a.k_stride) + e;
     __align__(8) T y[4];
@@ -183,6 +186,11 @@ __global__ void kv4_read_kernel(const Kv4RowsArgs a) {
 // --- decode ----------------------------------------------------------------------------
 
 constexpr int kWarps = 4;
+constexpr int kMinRange = 16;       // units of a CTA
+constexpr int kMaxPieces = 32;      // of a sequence, about: what its last CTA merges
+constexpr int kStages = 3;            // steps of a warp's ring
+constexpr uint64_t kWaitLimitNs = 1000000000ull;  // a chunk that has not landed in 1 s is
+                                                  // reported, never waited on forever
 
 struct Kv4Params {
   const void *q;
@@ -195,9 +203,11 @@ struct Kv4Params {
   uint64_t region_bytes;
   int batch, hq, hkv, bs, max_bps;
   float scale_log2;
-  int units_per_split, num_splits, n_head_tiles, heads_per_tile;
-  float *part_o, *part_lse;
-  float *scores;
+  int n_head_tiles;
+  float *part_o, *part_lse;  // two slots a CTA: [CTA][2][heads of a tile] rows
+  int32_t *counters;         // a zero per CTA: pieces of a shared sequence that are done
+  float *scores;             // SCORES: [batch * hq][score_stride], log2 units
+  float *lse;                // SCORES: [batch * hq], log2 units
   int64_t score_stride;
   int32_t *diag;
   int64_t q_sb, q_sh, o_sb, o_sh, bt_stride;
@@ -206,97 +216,265 @@ struct Kv4Params {
 
 // Two codes of a word to f16: 0x6400 is 1024 with a unit of 1 in its last place, so a
 // nibble or-ed into bits 0-3 (4-7) adds n (16 n); the subtraction (multiply-add) that
-// leaves n - 8 is exact.
-__device__ __forceinline__ uint32_t low_codes(uint32_t w) {
-  uint32_t x = (w & 0x000f000fu) | 0x64006400u;
+// leaves n - 8 is exact.  `base` is 0x64006400 in a register the compiler cannot see
+// through: with both constants immediate the and-or takes two instructions instead of one.
+__device__ __forceinline__ uint32_t low_codes(uint32_t w, uint32_t base) {
+  uint32_t x;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w), "n"(0x000f000fu), "r"(base));
   asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0x64086408u));
   return x;
 }
-__device__ __forceinline__ uint32_t high_codes(uint32_t w) {
-  uint32_t x = (w & 0x00f000f0u) | 0x64006400u;
+__device__ __forceinline__ uint32_t high_codes(uint32_t w, uint32_t base) {
+  uint32_t x;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w), "n"(0x00f000f0u), "r"(base));
   asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(x) : "r"(0x2c002c00u), "r"(0xd480d480u));
   return x;
 }
+// D = A B (+ D), m16n8k16 f16
+__device__ __forceinline__ void mma_zero(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_add(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ float bf16_lo(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
-// One lane's share of a unit: K and V words and the scales of tokens g and g+8.
-template <int D>
-struct UnitRegs {
-  static constexpr int NG = D / kGroup;  // pages are read through L2 alone, once each
-  alignas(16) uint32_t k[2 * NG];
-  alignas(16) uint32_t v[2 * NG];
-  alignas(16) uint32_t ks[NG];
-  alignas(16) uint32_t vs[NG];  // 2 NG bf16: token g's groups, then token g+8's
+// Units that a warp takes at a time: two give its loads, matrix products and shuffles
+// something to overlap with (see the loop), as long as the registers of both fit.
+__host__ __device__ constexpr int units_at_a_time(int D, int NT) { return D * NT <= 128 ? 2 : 1; }
+__host__ __device__ constexpr int ctas_per_sm(int D, int NT) {
+  return D * NT <= 128 ? 4 : D * NT <= 256 ? 2 : 1;
+}
 
-  __device__ __forceinline__ void load(const uint8_t *kc, const uint8_t *vc, int lane) {
-    if constexpr (NG % 2 == 0) {
-#pragma unroll
-      for (int j = 0; j < NG / 2; ++j) {
-        *reinterpret_cast<uint4 *>(k + 4 * j) =
-            __ldcg(reinterpret_cast<const uint4 *>(kc + (j * 32 + lane) * 16));
-        *reinterpret_cast<uint4 *>(v + 4 * j) =
-            __ldcg(reinterpret_cast<const uint4 *>(vc + (j * 32 + lane) * 16));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        *reinterpret_cast<uint2 *>(k + 2 * j) =
-            __ldcg(reinterpret_cast<const uint2 *>(kc + (j * 32 + lane) * 8));
-        *reinterpret_cast<uint2 *>(v + 2 * j) =
-            __ldcg(reinterpret_cast<const uint2 *>(vc + (j * 32 + lane) * 8));
-      }
-    }
-    const uint8_t *kp = kc + NG * 256 + (lane >> 2) * (NG * 4);
-    const uint8_t *vp = vc + NG * 256 + (lane >> 2) * (NG * 4);
-    if constexpr (NG % 4 == 0) {
-#pragma unroll
-      for (int j = 0; j < NG; j += 4) {
-        *reinterpret_cast<uint4 *>(ks + j) = __ldcg(reinterpret_cast<const uint4 *>(kp + 4 * j));
-        *reinterpret_cast<uint4 *>(vs + j) = __ldcg(reinterpret_cast<const uint4 *>(vp + 4 * j));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        ks[j] = __ldcg(reinterpret_cast<const uint32_t *>(kp) + j);
-        vs[j] = __ldcg(reinterpret_cast<const uint32_t *>(vp) + j);
-      }
-    }
-  }
-  // scale of token g (w = 0) or g + 8 (w = 1), group j
-  __device__ __forceinline__ static float scale(const uint32_t *s, int w, int j) {
-    const int i = w * NG + j;
-    return i & 1 ? bf16_hi(s[i >> 1]) : bf16_lo(s[i >> 1]);
-  }
-};
+// V's scales enter P as f16: two positive bf16 a word, their exponents lowered by a bias
+// common to the warp (in units of bf16's exponent bit), those below f16's range to about 0.
+// The bias keeps the largest scale seen below 2^9 (f16 exponent field 23), so that 64 times
+// it is finite and scales down to 2^-21 of the largest count.
+constexpr int kScaleTop = 23;
+__device__ __forceinline__ uint32_t scales_to_f16(uint32_t s, uint32_t minus_bias) {
+  return __viaddmax_s16x2_relu(s, minus_bias, 0u) << 3;
+}
 
+// K's scale of token g (w = 0) or g + 8 (w = 1), group j, of a lane's 2 NG scales
+template <int NG>
+__device__ __forceinline__ float k_scale(const uint32_t *ks, int w, int j) {
+  const int i = w * NG + j;
+  return i & 1 ? bf16_hi(ks[i >> 1]) : bf16_lo(ks[i >> 1]);
+}
+
+// N words from shared memory in the widest loads that N allows; step: 16-byte vectors (8
+// where N is odd) lie this many bytes apart
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t *r, const unsigned char *p, int step) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+      *reinterpret_cast<uint4 *>(r + 4 * i) = *reinterpret_cast<const uint4 *>(p + i * step);
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+      *reinterpret_cast<uint2 *>(r + 2 * i) = *reinterpret_cast<const uint2 *>(p + i * step);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = *reinterpret_cast<const uint32_t *>(p + i * step);
+  }
+}
+
+// Work split.  The units of all sequences, end to end, are cut into equal ranges, one for each
+// CTA x of a kv head (and head tile) y = blockIdx.y: lengths differ by a factor of 8 within
+// a batch, and CTAs of one (sequence, split) each left the Llama-3-8B decode batch at 60 us
+// where equal shares take 45.  A sequence inside one range is finished there; the pieces of one that
+// several CTAs share go to scratch and the last CTA to finish merges them.
+//
+// A CTA's warps take every kWarps-th step of NU units of its piece.  Each warp runs its own
+// ring of kStages steps: a lane issues a unit's K and V chunks as two bulk copies, the whole
+// warp reads its operands from shared memory.
 template <typename T, int D, int NT, bool SCORES>
-__global__ void __launch_bounds__(kWarps * 32) kv4_decode_kernel(const Kv4Params p) {
+__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
+    kv4_decode_kernel(const Kv4Params p) {
   constexpr int NG = D / kGroup;
+  constexpr int NU = units_at_a_time(D, NT);
   constexpr int HT = 8 * NT;  // heads of a tile
-  extern __shared__ __align__(16) float kv4_smem[];
+  constexpr uint32_t kChunk = 9 * D;
+  extern __shared__ __align__(128) unsigned char kv4_smem[];
+  __shared__ uint64_t s_bar[kWarps * kStages];
+  __shared__ int s_fail, s_last;
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-  const int b = blockIdx.z, split = blockIdx.x;
   const int kvh = int(blockIdx.y) / p.n_head_tiles, ht = int(blockIdx.y) % p.n_head_tiles;
-  const int seq_len = min(p.seq_lens[b], p.max_bps * p.bs);
-  if (seq_len <= 0) return;
-  const int n_units = (seq_len + kUnit - 1) / kUnit;
-  const int u_begin = split * p.units_per_split;
-  if (u_begin >= n_units) return;
-  const int u_end = min(u_begin + p.units_per_split, n_units);
-  const int group_lo = int((int64_t(kvh) * p.hq + p.hkv - 1) / p.hkv);
-  const int group_hi = int((int64_t(kvh + 1) * p.hq + p.hkv - 1) / p.hkv);
+  // query heads h with h * hkv / hq == kvh
+  const int group_lo = int((uint32_t(kvh) * uint32_t(p.hq) + p.hkv - 1) / uint32_t(p.hkv));
+  const int group_hi = int((uint32_t(kvh + 1) * uint32_t(p.hq) + p.hkv - 1) / uint32_t(p.hkv));
   const int lo = group_lo + ht * HT;
   const int G = min(group_hi - lo, HT);
   if (G <= 0) return;
+
+  // ---- this CTA's range of units, and the sequence it starts in ---------------------------
+  const int cap = p.max_bps * p.bs;
+  auto units_of = [&](int b) { return (min(max(p.seq_lens[b], 0), cap) + kUnit - 1) / kUnit; };
+  // every warp for itself: lane i sums a run of sequences
+  const int run = (p.batch + 31) / 32;
+  const int b_lo = min(lane * run, p.batch), b_hi = min(b_lo + run, p.batch);
+  int mine = 0;
+#pragma unroll 4
+  for (int i = b_lo; i < b_hi; ++i) mine += units_of(i);
+  int incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += x;
+  }
+  const int total = __shfl_sync(0xffffffffu, incl, 31);
+  // at least a step or two a warp, less only where the sequences themselves are shorter
+  const int range = max((total + int(gridDim.x) - 1) / int(gridDim.x),
+                        min(kMinRange, (total + p.batch - 1) / p.batch));
+  const int r0 = int(blockIdx.x) * range, r1 = min(r0 + range, total);
+  if (r0 >= total) return;
+  int b_first = b_lo, before = incl - mine;  // units of the sequences before b
+  const uint32_t found = __ballot_sync(0xffffffffu, before <= r0 && r0 < incl);
+  if (before <= r0 && r0 < incl) {
+    for (int n = units_of(b_first); before + n <= r0; n = units_of(b_first)) {
+      before += n;
+      ++b_first;
+    }
+  }
+  b_first = __shfl_sync(0xffffffffu, b_first, __ffs(int(found)) - 1);
+  before = __shfl_sync(0xffffffffu, before, __ffs(int(found)) - 1);
+  uint64_t *bars = s_bar + warp * kStages;
+  if (lane < kStages) ptx::mbar_init(ptx::smem_u32(bars + lane), 1);
+  if (threadIdx.x == 0) s_fail = 0;
+  ptx::fence_proxy_async_smem();
+  __syncthreads();
+
+  unsigned char *ring = kv4_smem + warp * kStages * NU * 2 * kChunk;
+  const int units_per_page = p.bs / kUnit;
+  int st = 0;  // stage and phase of the next step
+  uint32_t parity = 0;
+  auto advance = [&] {
+    if (++st == kStages) {
+      st = 0;
+      parity ^= 1;
+    }
+  };
+  // Count a finished piece of the sequence that starts in CTA `first`: true in the CTA that
+  // finished last, which leaves the counter at zero for the next call.
+  auto last_piece = [&](int first, int pieces) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      __threadfence();  // the CTA's pieces, which the barrier ordered before this
+      int32_t *counter = p.counters + int64_t(blockIdx.y) * gridDim.x + first;
+      s_last = atomicAdd(counter, 1) == pieces - 1;
+      if (s_last) *counter = 0;
+      __threadfence();
+    }
+    __syncthreads();
+    return s_last != 0;
+  };
+  bool lost = false;      // a wait ran out: the rest of the range is given up (and reported)
+  for (int b = b_first; before < r1; ++b) {
+  const int n_units = units_of(b);
+  if (n_units == 0) continue;
+  const int seq_len = min(p.seq_lens[b], cap);
+  const int u_begin = max(r0 - before, 0), u_end = min(r1 - before, n_units);
+  const int x_first = before / range, x_last = (before + n_units - 1) / range;
+  const int pieces = x_last - x_first + 1;  // CTAs that share the sequence
+  const int slot = u_begin == 0 && before > r0 ? 1 : 0;
+  const int at_first = before;
+  before += n_units;
+  if (lost) {
+    if (pieces > 1) last_piece(x_first, pieces);
+    continue;
+  }
+
+  // ---- the query rows (used below; loaded first, their latency overlaps the addresses') ----
+  __align__(16) T q_raw[NT][NG][8];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const T *src = static_cast<const T *>(p.q) + int64_t(b) * p.q_sb +
+                   int64_t(lo + min(nt * 8 + g, G - 1)) * p.q_sh + c * 8;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      if (p.q_vec) {
+        *reinterpret_cast<uint4 *>(q_raw[nt][j]) =
+            *reinterpret_cast<const uint4 *>(src + j * kGroup);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q_raw[nt][j][e] = src[j * kGroup + e];
+      }
+    }
+  }
+
+  // ---- the warp's units and their first copies ------------------------------------------
+  // step i of the warp: units first_unit + i * kWarps * NU + {0, .., NU - 1}; the addresses of
+  // 32 units at a time, one a lane
+  const int first_unit = u_begin + warp * NU;
+  const int n_w = max(0, (u_end - first_unit + kWarps * NU - 1) / (kWarps * NU));
+  int64_t my_at = -1;  // byte offset of the chunk of unit lane % NU of step k0 + lane / NU
+  auto resolve = [&](int k0) {
+    my_at = -1;
+    const int i = k0 + lane / NU;
+    const int u = first_unit + i * (kWarps * NU) + lane % NU;
+    if (i < n_w && u < u_end) {
+      const int page = u / units_per_page, in = u - page * units_per_page;
+      const int blk = p.tables[int64_t(b) * p.bt_stride + page];
+      if (blk >= 0) {
+        const uint64_t off = p.offsets[blk] * 2;
+        if ((off & 15) == 0 &&
+            off + uint64_t(units_per_page) * p.hkv * kChunk <= p.region_bytes)
+          my_at = int64_t(off) + (int64_t(kvh) * units_per_page + in) * kChunk;
+      }
+      if (my_at < 0) atomicOr(p.diag, int32_t(kDiagBadOffset));
+    }
+  };
+  constexpr int kBatchSteps = 32 / NU;
+  uint32_t readable = 0;  // bit st * NU + r: unit r of the step in stage st was copied
+  // unit r of a stage: its K chunk, then its V chunk
+  auto issue = [&](int k, int stage) {
+    if (k % kBatchSteps == 0) resolve(k);
+    int64_t at[NU];
+    readable &= ~(((1u << NU) - 1) << (stage * NU));
+#pragma unroll
+    for (int r = 0; r < NU; ++r) {
+      at[r] = __shfl_sync(0xffffffffu, my_at, (k % kBatchSteps) * NU + r);
+      if (at[r] >= 0) readable |= 1u << (stage * NU + r);
+    }
+    if (lane == 0) {
+      const uint32_t bar = ptx::smem_u32(bars + stage);
+      const uint32_t dst = ptx::smem_u32(ring + stage * NU * 2 * kChunk);
+      uint32_t bytes = 0;
+#pragma unroll
+      for (int r = 0; r < NU; ++r) bytes += at[r] >= 0 ? 2 * kChunk : 0u;
+      ptx::mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+      for (int r = 0; r < NU; ++r) {
+        if (at[r] >= 0) {
+          ptx::bulk_g2s(dst + r * 2 * kChunk, p.va_k + at[r], kChunk, bar);
+          ptx::bulk_g2s(dst + r * 2 * kChunk + kChunk, p.va_v + at[r], kChunk, bar);
+        }
+      }
+    }
+  };
+  for (int k = 0; k < kStages && k < n_w; ++k) issue(k, (st + k) % kStages);
 
   // ---- Q as the B operand (columns = heads), scaled per head by a power of two --------
   // f16 for both input types: with the row's largest magnitude brought into [64, 128) every
@@ -310,18 +488,9 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_decode_kernel(const Kv4Params
     float mx = 0.f;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      const T *src = static_cast<const T *>(p.q) + int64_t(b) * p.q_sb +
-                     int64_t(lo + min(h, G - 1)) * p.q_sh + j * kGroup + c * 8;
-      __align__(16) T tmp[8];
-      if (p.q_vec) {
-        *reinterpret_cast<uint4 *>(tmp) = *reinterpret_cast<const uint4 *>(src);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) tmp[e] = src[e];
-      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[j][e] = h < G ? ptx::to_f32(tmp[e]) : 0.f;
+        x[j][e] = h < G ? ptx::to_f32(q_raw[nt][j][e]) : 0.f;
         mx = fmaxf(mx, fabsf(x[j][e]));
       }
     }
@@ -341,12 +510,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_decode_kernel(const Kv4Params
     s_scale[nt][1] = __shfl_sync(0xffffffffu, down, (2 * c + 1) * 4);
   }
 
-  const int n_w = (u_end - u_begin - warp + kWarps - 1) / kWarps;  // this warp's units
-  const int64_t chunk_bytes = 9 * D;
-  const int units_per_page = p.bs / kUnit;
-  const int64_t page_bytes = int64_t(units_per_page) * p.hkv * chunk_bytes;
-
-  float o[NT][2 * NG][4];
+  float o[NT][2 * NG][4];  // O transposed: rows = dims, columns = heads
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -357,177 +521,280 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_decode_kernel(const Kv4Params
     m[nt][0] = m[nt][1] = -INFINITY;
     l[nt][0] = l[nt][1] = 0.f;
   }
-  float v_up = 0.f;  // power of two on the V scales inside P
-
-  int64_t my_at = -1;  // lane i: byte offset of the chunk of unit i of the current 32
-  auto resolve = [&](int k0) {
-    my_at = -1;
-    const int k = k0 + lane;
-    if (k < n_w) {
-      const int u = u_begin + warp + k * kWarps;
-      const int page = u / units_per_page, in = u - page * units_per_page;
-      const int blk = p.tables[int64_t(b) * p.bt_stride + page];
-      if (blk >= 0) {
-        const uint64_t off = p.offsets[blk] * 2;
-        if ((off & 15) == 0 && off + page_bytes <= p.region_bytes)
-          my_at = int64_t(off) + (int64_t(kvh) * units_per_page + in) * chunk_bytes;
-      }
-      if (my_at < 0) atomicOr(p.diag, int32_t(kDiagBadOffset));
-    }
-  };
-
-  UnitRegs<D> cur, nxt;
-  bool cur_ok = false, nxt_ok = false;
-  auto fetch = [&](int k, UnitRegs<D> &r) {
-    if ((k & 31) == 0) resolve(k);
-    const int64_t at = __shfl_sync(0xffffffffu, my_at, k & 31);
-    if (at >= 0) r.load(p.va_k + at, p.va_v + at, lane);
-    return at >= 0;
-  };
-  if (n_w > 0) cur_ok = fetch(0, cur);
+  int bias = -1;               // exponent bias of V's scales inside P; -1 before the first unit
+  uint32_t minus_bias = 0;     // two of -bias << 7, as 16-bit integers
+  uint32_t scale_limit = 0;    // largest scale (bf16 bits) that the bias admits
+  bool failed = false;
+  uint32_t base;
+  asm volatile("mov.u32 %0, 0x64006400;" : "=r"(base));
 
   for (int k = 0; k < n_w; ++k) {
-    nxt_ok = k + 1 < n_w ? fetch(k + 1, nxt) : false;
-    const int u = u_begin + warp + k * kWarps;
-    const int nvalid = cur_ok ? min(kUnit, seq_len - u * kUnit) : 0;
-    const bool in0 = g < nvalid, in1 = g + 8 < nvalid;
-    if (nvalid > 0) {
-      float s[NT][4];
+    const int u = first_unit + k * (kWarps * NU);
+    const bool landed = ptx::mbar_wait_bounded(ptx::smem_u32(bars + st), parity, kWaitLimitNs);
+    if (!__all_sync(0xffffffffu, landed)) {
+      failed = true;
+      break;
+    }
+    const uint32_t units = (readable >> (st * NU)) & ((1u << NU) - 1);
+    if (units == 0) {  // no page could be read: the tokens weigh nothing
+      if constexpr (SCORES) {
+        for (int i = lane; i < G * NU * kUnit; i += 32) {
+          const int h = i / (NU * kUnit), t = u * kUnit + i % (NU * kUnit);
+          if (t < u_end * kUnit)
+            p.scores[(int64_t(b) * p.hq + lo + h) * p.score_stride + t] = -INFINITY;
+        }
+      }
+      if (k + kStages < n_w) issue(k + kStages, st);
+      advance();
+      continue;
+    }
+    const unsigned char *chunk = ring + st * NU * 2 * kChunk;
+    // ---- S = Q K^T, transposed: rows = tokens, columns = heads -----------------------------
+    float s[NU][NT][4];
+#pragma unroll
+    for (int r = 0; r < NU; ++r) {
+      const unsigned char *kc = chunk + r * 2 * kChunk;
+      alignas(16) uint32_t kw[2 * NG];
+      alignas(16) uint32_t ks[NG];
+      if constexpr (NG % 2 == 0) {
+        load_words<2 * NG>(kw, kc + lane * 16, 512);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NG; ++j) load_words<2>(kw + 2 * j, kc + (j * 32 + lane) * 8, 0);
+      }
+      load_words<NG>(ks, kc + NG * 256 + g * (NG * 4), NG % 4 == 0 ? 16 : NG % 2 == 0 ? 8 : 4);
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        const uint32_t w0 = cur.k[2 * j], w1 = cur.k[2 * j + 1];
-        const uint32_t a0[4] = {low_codes(w0), low_codes(w1), high_codes(w0), high_codes(w1)};
-        const uint32_t a1[4] = {low_codes(w0 >> 8), low_codes(w1 >> 8), high_codes(w0 >> 8),
-                                high_codes(w1 >> 8)};
-        const float k0 = UnitRegs<D>::scale(cur.ks, 0, j), k1 = UnitRegs<D>::scale(cur.ks, 1, j);
+        const uint32_t w0 = kw[2 * j], w1 = kw[2 * j + 1];
+        const uint32_t a0[4] = {low_codes(w0, base), low_codes(w1, base), high_codes(w0, base),
+                                high_codes(w1, base)};
+        const uint32_t a1[4] = {low_codes(w0 >> 8, base), low_codes(w1 >> 8, base),
+                                high_codes(w0 >> 8, base), high_codes(w1 >> 8, base)};
+        const float k0 = k_scale<NG>(ks, 0, j), k1 = k_scale<NG>(ks, 1, j);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          ptx::Mma<__half>::run(acc, a0, qb[nt][j][0], qb[nt][j][1]);
-          ptx::Mma<__half>::run(acc, a1, qb[nt][j][2], qb[nt][j][3]);
+          float acc[4];
+          mma_zero(acc, a0, qb[nt][j][0], qb[nt][j][1]);
+          mma_add(acc, a1, qb[nt][j][2], qb[nt][j][3]);
+          float *sr = s[r][nt];
           if (j == 0) {
-            s[nt][0] = acc[0] * k0;
-            s[nt][1] = acc[1] * k0;
-            s[nt][2] = acc[2] * k1;
-            s[nt][3] = acc[3] * k1;
+            sr[0] = acc[0] * k0;
+            sr[1] = acc[1] * k0;
+            sr[2] = acc[2] * k1;
+            sr[3] = acc[3] * k1;
           } else {
-            s[nt][0] = fmaf(acc[0], k0, s[nt][0]);
-            s[nt][1] = fmaf(acc[1], k0, s[nt][1]);
-            s[nt][2] = fmaf(acc[2], k1, s[nt][2]);
-            s[nt][3] = fmaf(acc[3], k1, s[nt][3]);
+            sr[0] = fmaf(acc[0], k0, sr[0]);
+            sr[1] = fmaf(acc[1], k0, sr[1]);
+            sr[2] = fmaf(acc[2], k1, sr[2]);
+            sr[3] = fmaf(acc[3], k1, sr[3]);
           }
         }
       }
-      float v0[NG], v1[NG], vmx = 0.f;
 #pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        // a slot past the context holds anything: its scales count as 0
-        v0[j] = in0 ? UnitRegs<D>::scale(cur.vs, 0, j) : 0.f;
-        v1[j] = in1 ? UnitRegs<D>::scale(cur.vs, 1, j) : 0.f;
-        vmx = fmaxf(vmx, fmaxf(v0[j], v1[j]));
-      }
-      bool raise = vmx * v_up > 64.f || v_up == 0.f;
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+        for (int i = 0; i < 4; ++i) s[r][nt][i] *= s_scale[nt][i & 1];
+    }
+    alignas(16) uint32_t vs[NU][2 * NG];  // V's scales [group][token pair (2c, 2c+1) + 8 i]
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool in = i < 2 ? in0 : in1;
-          s[nt][i] = in ? s[nt][i] * s_scale[nt][i & 1] : -INFINITY;
-          raise |= s[nt][i] > m[nt][i & 1] + 8.f;
+    for (int r = 0; r < NU; ++r)
+      load_words<2 * NG>(vs[r], chunk + r * 2 * kChunk + kChunk + NG * 256 + c * (NG * 8),
+                         NG % 2 == 0 ? 16 : 8);
+
+    // Slots past the context, and units whose page could not be read, hold anything: their
+    // scores become -inf and their scales 0.
+    if (units != (1u << NU) - 1 || seq_len - u * kUnit < NU * kUnit) {
+#pragma unroll
+      for (int r = 0; r < NU; ++r) {
+        const int nvalid = (units >> r) & 1u ? seq_len - (u + r) * kUnit : 0;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (g >= nvalid) s[r][nt][0] = s[r][nt][1] = -INFINITY;
+          if (g + 8 >= nvalid) s[r][nt][2] = s[r][nt][3] = -INFINITY;
         }
-        if constexpr (SCORES) {
+#pragma unroll
+        for (int i = 0; i < 2 * NG; ++i) {
+          const int t = 2 * c + (i & 1) * 8;
+          vs[r][i] &= (t < nvalid ? 0x0000ffffu : 0u) | (t + 1 < nvalid ? 0xffff0000u : 0u);
+        }
+      }
+    }
+    if constexpr (SCORES) {
+#pragma unroll
+      for (int r = 0; r < NU; ++r) {
+        if (u + r >= u_end) continue;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int h = nt * 8 + 2 * c + (i & 1);
             if (h < G)
-              p.scores[(int64_t(b) * p.hq + lo + h) * p.score_stride + u * kUnit + g +
-                       (i >> 1) * 8] = s[nt][i];
+              p.scores[(int64_t(b) * p.hq + lo + h) * p.score_stride + (u + r) * kUnit + g +
+                       (i >> 1) * 8] = s[r][nt][i];
           }
         }
       }
-      // The running maximum is raised only when a score exceeds it by more than 8 (a factor
-      // of 256, which P's f16 range holds), the V normaliser only past a factor of 64: both
-      // are rare after a warp's first unit, so most units skip the rescaling of O.
-      if (__any_sync(0xffffffffu, raise)) {
+    }
+    // The running maximum is raised only when a score exceeds it by more than 6 (a factor of
+    // 64, which P's f16 range holds), the bias only when a scale passes its limit: both are
+    // rare after a warp's first step, so most steps skip the rescaling of O.
+    uint32_t vmx = 0;
 #pragma unroll
-        for (int o2 = 1; o2 < 32; o2 <<= 1) vmx = fmaxf(vmx, __shfl_xor_sync(0xffffffffu, vmx, o2));
-        float vr = 1.f;
-        if (vmx * v_up > 64.f || v_up == 0.f) {
-          const int ex = max(int(__float_as_uint(vmx) >> 23) - 127, -100);
-          const float up = __uint_as_float(uint32_t(127 + 2 - ex) << 23);
-          vr = v_up == 0.f ? 1.f : up / v_up;
-          v_up = up;
-        }
+    for (int r = 0; r < NU; ++r)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+      for (int i = 0; i < 2 * NG; i += 2) vmx = __vimax3_u16x2(vmx, vs[r][i], vs[r][i + 1]);
+    bool raise = (vmx & 0xffffu) > scale_limit || (vmx >> 16) > scale_limit;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float mx = fmaxf(s[nt][i], s[nt][i + 2]);
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            mx = fmaxf(mx, m[nt][i]);
-            const float r = m[nt][i] == -INFINITY ? 0.f : ptx::fast_exp2(m[nt][i] - mx);
-            m[nt][i] = mx;
-            l[nt][i] *= r;
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int d = 0; d < 2 * NG; ++d) {
-              o[nt][d][i] *= r * vr;
-              o[nt][d][i + 2] *= r * vr;
-            }
-          }
-        }
+      for (int i = 0; i < 2; ++i) {
+        float mx = fmaxf(s[0][nt][i], s[0][nt][i + 2]);
+#pragma unroll
+        for (int r = 1; r < NU; ++r) mx = fmaxf(mx, fmaxf(s[r][nt][i], s[r][nt][i + 2]));
+        raise |= mx > m[nt][i] + 6.f;
       }
+    }
+    if (__any_sync(0xffffffffu, raise || bias < 0)) {
+      uint32_t top = 0;
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        v0[j] *= v_up;
-        v1[j] *= v_up;
+        bool nan = false;  // a NaN scale: its group of O is lost, its codes count as 0 here
+#pragma unroll
+        for (int r = 0; r < NU; ++r) {
+#pragma unroll
+          for (int i = 2 * j; i < 2 * j + 2; ++i) {
+            if ((vs[r][i] & 0xffffu) >= 0x7f80u) {
+              nan = true;
+              vs[r][i] &= 0xffff0000u;
+            }
+            if ((vs[r][i] >> 16) >= 0x7f80u) {
+              nan = true;
+              vs[r][i] &= 0x0000ffffu;
+            }
+            top = max(top, max(vs[r][i] & 0xffffu, vs[r][i] >> 16));
+          }
+        }
+        if (__any_sync(0xffffffffu, nan)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              o[nt][2 * j][i] = o[nt][2 * j + 1][i] = __int_as_float(0x7fc00000);
+        }
       }
-      uint32_t pb[NT][NG][2];
+      top = __reduce_max_sync(0xffffffffu, top);
+      float vr = 1.f;
+      if (bias < 0 || top > scale_limit) {
+        const int fresh = max(int(top >> 7) - kScaleTop + 2, 0);
+        if (bias >= 0) vr = exp2f(float(bias - fresh));
+        bias = fresh;
+        minus_bias = (uint32_t(-(bias << 7)) & 0xffffu) * 0x10001u;
+        scale_limit = uint32_t(min((bias + kScaleTop + 1) << 7, 0x7f80)) - 1;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[nt][i] = ptx::fast_exp2(s[nt][i] - m[nt][i & 1]);
-          l[nt][i & 1] += s[nt][i];
-        }
+        for (int i = 0; i < 2; ++i) {
+          float mx = m[nt][i];
 #pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          // P in f16 carries 11 bits beside the scales' and codes' exact products
-          pb[nt][j][0] = transpose8x8(ptx::Mma<__half>::pack(s[nt][0] * v0[j], s[nt][1] * v0[j]));
-          pb[nt][j][1] = transpose8x8(ptx::Mma<__half>::pack(s[nt][2] * v1[j], s[nt][3] * v1[j]));
+          for (int r = 0; r < NU; ++r) mx = fmaxf(mx, fmaxf(s[r][nt][i], s[r][nt][i + 2]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float rr = m[nt][i] == -INFINITY ? 0.f : ptx::fast_exp2(m[nt][i] - mx);
+          m[nt][i] = mx;
+          l[nt][i] *= rr;
+#pragma unroll
+          for (int d = 0; d < 2 * NG; ++d) {
+            o[nt][d][i] *= rr * vr;
+            o[nt][d][i + 2] *= rr * vr;
+          }
         }
+      }
+    }
+    // ---- O += V^T P^T ----------------------------------------------------------------------
+    // P as the B operand (rows = tokens, columns = heads) in 11 bits, rounded to 11 bits once
+    // more by a group's scales
+    uint32_t pb[NU][NT][2];
+#pragma unroll
+    for (int r = 0; r < NU; ++r) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = ptx::fast_exp2(s[r][nt][i] - m[nt][i & 1]);
+          l[nt][i & 1] += x[i];
+        }
+        pb[r][nt][0] = transpose8x8(ptx::Mma<__half>::pack(x[0], x[1]));
+        pb[r][nt][1] = transpose8x8(ptx::Mma<__half>::pack(x[2], x[3]));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < NU; ++r) {
+      const unsigned char *vc = chunk + r * 2 * kChunk + kChunk;
+      alignas(16) uint32_t vw[2 * NG];
+      if constexpr (NG % 2 == 0) {
+        load_words<2 * NG>(vw, vc + lane * 16, 512);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NG; ++j) load_words<2>(vw + 2 * j, vc + (j * 32 + lane) * 8, 0);
       }
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        const uint32_t w0 = cur.v[2 * j], w1 = cur.v[2 * j + 1];
-        const uint32_t a0[4] = {low_codes(w0), high_codes(w0), low_codes(w1), high_codes(w1)};
-        const uint32_t a1[4] = {low_codes(w0 >> 8), high_codes(w0 >> 8), low_codes(w1 >> 8),
-                                high_codes(w1 >> 8)};
+        const uint32_t w0 = vw[2 * j], w1 = vw[2 * j + 1];
+        const uint32_t a0[4] = {low_codes(w0, base), high_codes(w0, base), low_codes(w1, base),
+                                high_codes(w1, base)};
+        const uint32_t a1[4] = {low_codes(w0 >> 8, base), high_codes(w0 >> 8, base),
+                                low_codes(w1 >> 8, base), high_codes(w1 >> 8, base)};
+        const uint32_t v0 = scales_to_f16(vs[r][2 * j], minus_bias);
+        const uint32_t v1 = scales_to_f16(vs[r][2 * j + 1], minus_bias);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          ptx::Mma<__half>::run(o[nt][2 * j], a0, pb[nt][j][0], pb[nt][j][1]);
-          ptx::Mma<__half>::run(o[nt][2 * j + 1], a1, pb[nt][j][0], pb[nt][j][1]);
+          const uint32_t b0 = mul2(pb[r][nt][0], v0), b1 = mul2(pb[r][nt][1], v1);
+          mma_add(o[nt][2 * j], a0, b0, b1);
+          mma_add(o[nt][2 * j + 1], a1, b0, b1);
         }
       }
-    } else if constexpr (SCORES) {
-      // a page that could not be read: its tokens weigh nothing
-#pragma unroll
-      for (int i = 0; i < 4 * NT; ++i) {
-        const int h = (i >> 2) * 8 + 2 * c + (i & 1);
-        if (h < G)
-          p.scores[(int64_t(b) * p.hq + lo + h) * p.score_stride + u * kUnit + g +
-                   ((i >> 1) & 1) * 8] = -INFINITY;
-      }
     }
-    cur = nxt;
-    cur_ok = nxt_ok;
+    __syncwarp();
+    if (k + kStages < n_w) issue(k + kStages, st);
+    advance();
   }
+  if (failed) {
+    // Let copies still in flight land before the shared memory is released (bounded as
+    // well), then report.
+    for (int st = 0; st < kStages; ++st) {
+      ptx::mbar_wait_bounded(ptx::smem_u32(bars + st), 0, 1000000ull);
+      ptx::mbar_wait_bounded(ptx::smem_u32(bars + st), 1, 1000000ull);
+    }
+    if (lane == 0) {
+      atomicOr(p.diag, int32_t(kDiagWaitTimeout));
+      s_fail = 1;
+    }
+  }
+  __syncthreads();
+  lost = s_fail;
+  const bool whole = pieces == 1;
+  float *part_o = p.part_o + (int64_t(blockIdx.y) * gridDim.x * 2) * HT * D;
+  float *part_lse = p.part_lse + (int64_t(blockIdx.y) * gridDim.x * 2) * HT;
+  auto store = [&](int h, int d, float4 x, float lse) {
+    T *dst = static_cast<T *>(p.out) + int64_t(b) * p.o_sb + int64_t(lo + h) * p.o_sh + d;
+    dst[0] = ptx::from_f32<T>(x.x);
+    dst[1] = ptx::from_f32<T>(x.y);
+    dst[2] = ptx::from_f32<T>(x.z);
+    dst[3] = ptx::from_f32<T>(x.w);
+    if constexpr (SCORES) {
+      if (d == 0) p.lse[int64_t(b) * p.hq + lo + h] = lse;
+    }
+  };
 
-  // ---- merge the warps ----------------------------------------------------------------
-  float *cO = kv4_smem;                 // [kWarps][HT][D]
-  float *cm = cO + kWarps * HT * D;     // [kWarps][HT]
-  float *cl = cm + kWarps * HT;         // [kWarps][HT]
+  // ---- merge the warps (the rings are free) -----------------------------------------------
+  float *cO = reinterpret_cast<float *>(kv4_smem);  // [kWarps][HT][D]
+  float *cm = cO + kWarps * HT * D;                 // [kWarps][HT]
+  float *cl = cm + kWarps * HT;                     // [kWarps][HT]
+  // f16 scale = bf16 scale * 2^(112 - bias): both exponents are biased, by 127 and 15
+  const float v_down = bias < 0 ? 0.f : exp2f(float(bias - 112));
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -541,13 +808,12 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_decode_kernel(const Kv4Params
         cm[warp * HT + h] = m[nt][i];
         cl[warp * HT + h] = sum;
       }
-      const float down = v_up == 0.f ? 0.f : 1.f / v_up;
       if (h < G) {
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
           *reinterpret_cast<float4 *>(cO + (warp * HT + h) * D + j * kGroup + g * 4) =
-              make_float4(o[nt][2 * j][i] * down, o[nt][2 * j][i + 2] * down,
-                          o[nt][2 * j + 1][i] * down, o[nt][2 * j + 1][i + 2] * down);
+              make_float4(o[nt][2 * j][i] * v_down, o[nt][2 * j][i + 2] * v_down,
+                          o[nt][2 * j + 1][i] * v_down, o[nt][2 * j + 1][i + 2] * v_down);
         }
       }
     }
@@ -572,19 +838,60 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_decode_kernel(const Kv4Params
       x.z += v.z * sc;
       x.w += v.w * sc;
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    if (p.num_splits == 1 && !SCORES) {
-      T *dst = static_cast<T *>(p.out) + int64_t(b) * p.o_sb + int64_t(lo + h) * p.o_sh + d;
-      dst[0] = ptx::from_f32<T>(x.x * inv);
-      dst[1] = ptx::from_f32<T>(x.y * inv);
-      dst[2] = ptx::from_f32<T>(x.z * inv);
-      dst[3] = ptx::from_f32<T>(x.w * inv);
+    const float inv = L == 0.f ? 0.f : 1.f / L, lse = M + log2f(L);
+    x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    if (whole) {
+      if (!lost) store(h, d, x, lse);
     } else {
-      const int64_t row = (int64_t(b) * p.hq + lo + h) * p.num_splits + split;
-      *reinterpret_cast<float4 *>(p.part_o + row * D + d) =
-          make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-      if (d == 0) p.part_lse[row] = M + log2f(L);
+      const int64_t row = (int64_t(blockIdx.x) * 2 + slot) * HT + h;
+      *reinterpret_cast<float4 *>(part_o + row * D + d) = x;
+      if (d == 0) part_lse[row] = lse;
     }
+  }
+  if (whole) {
+    __syncthreads();  // the rings' memory is free again
+    continue;
+  }
+  // the last CTA of a shared sequence merges its pieces
+  if (!last_piece(x_first, pieces) || lost) continue;
+  // the first piece lies in its CTA's second slot unless it starts that CTA's range
+  const int64_t first_row = (int64_t(x_first) * 2 + (at_first > x_first * range ? 1 : 0)) * HT;
+  auto row_of = [&](int k) { return k == 0 ? first_row : int64_t(x_first + k) * 2 * HT; };
+  float *weight = reinterpret_cast<float *>(kv4_smem);  // [HT][pieces], then [HT] lse
+  float *row_lse = weight + HT * pieces;
+  for (int h = warp; h < G; h += kWarps) {
+    float M = -INFINITY, sum = 0.f;
+    for (int k = lane; k < pieces; k += 32) {
+      const float x = __ldcg(part_lse + row_of(k) + h);
+      weight[h * pieces + k] = x;
+      M = fmaxf(M, x);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    for (int k = lane; k < pieces; k += 32) sum += ptx::fast_exp2(weight[h * pieces + k] - M);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const float all = M + log2f(sum);
+    for (int k = lane; k < pieces; k += 32)
+      weight[h * pieces + k] = ptx::fast_exp2(weight[h * pieces + k] - all);
+    if (lane == 0) row_lse[h] = all;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < G * (D / 4); i += kWarps * 32) {
+    const int h = i / (D / 4), d = (i % (D / 4)) * 4;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int k = 0; k < pieces; ++k) {
+      const float w = weight[h * pieces + k];
+      const float4 v = __ldcg(reinterpret_cast<const float4 *>(part_o + (row_of(k) + h) * D + d));
+      x.x += v.x * w;
+      x.y += v.y * w;
+      x.z += v.z * w;
+      x.w += v.w * w;
+    }
+    store(h, d, x, row_lse[h]);
+  }
+  __syncthreads();  // the rings' memory is free again
   }
 }
 
@@ -665,58 +972,50 @@ cudaError_t kv4_decode_attention(const DecodeArgs &a, const DecodeWeights &w,
   p.q_vec = ((reinterpret_cast<uintptr_t>(a.q) & 15) | (p.q_sb & 7) | (p.q_sh & 7)) == 0;
   p.n_head_tiles = (g_max + 8 * nt - 1) / (8 * nt);
 
-  const int max_units = int((int64_t(a.max_blocks_per_seq) * a.block_size + kUnit - 1) / kUnit);
-  const int64_t items = int64_t(a.batch) * a.kv_heads * p.n_head_tiles;
-  const int64_t target = int64_t(device_sm_count()) * 4 * 4;
-  const int64_t want = std::max<int64_t>(1, (target + items - 1) / items);
-  int ups = int((max_units + want - 1) / want);
-  ups = std::max(ups, 16);
-  p.units_per_split = ups;
-  p.num_splits = (max_units + ups - 1) / ups;
+  // One wave of CTAs, every one with its share of the units of one kv head (head tile); where
+  // there are many of those, about four waves of smaller shares.
+  const int slots = device_sm_count() * ctas_per_sm(D, nt), Y = a.kv_heads * p.n_head_tiles;
+  const int X = Y * 4 <= slots
+                    ? int(std::min<int64_t>(slots / Y, int64_t(kMaxPieces) * a.batch))
+                    : (4 * slots + Y - 1) / Y;
 
-  const size_t rows = size_t(a.batch) * a.num_q_heads;
-  const bool partial = p.num_splits > 1 || scores;
-  p.score_stride = int64_t(max_units) * kUnit;
-  size_t bytes = 0;
-  if (partial) bytes = rows * p.num_splits * (size_t(D) + 1) * 4;
-  bytes = (bytes + 15) & ~size_t(15);
-  const size_t scores_at = bytes;
-  if (scores) bytes += rows * size_t(p.score_stride) * 4;
+  const size_t rows = size_t(a.batch) * a.num_q_heads, slots_used = size_t(X) * Y * 2 * 8 * nt;
+  const int max_tokens = a.max_blocks_per_seq * a.block_size;
+  p.score_stride = max_tokens;
+  // piece outputs, their log-sum-exp, and for the weights the rows' own and the scores
+  const size_t lse_at = slots_used * D * 4, row_at = lse_at + slots_used * 4;
+  const size_t scores_at = (row_at + (scores ? rows * 4 : 0) + 15) & ~size_t(15);
   CallScratch scratch;
-  if (bytes) {
-    cudaError_t e = scratch.acquire(stream, bytes);
-    if (e != cudaSuccess) return e;
-    p.part_o = static_cast<float *>(scratch.ptr);
-    p.part_lse = p.part_o + rows * p.num_splits * D;
-    if (scores) p.scores = reinterpret_cast<float *>(static_cast<char *>(scratch.ptr) + scores_at);
-  }
-  const size_t smem = size_t(kWarps) * 8 * nt * (D + 2) * 4;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-  if (e == cudaSuccess)
-    e = launch_pdl(fn, dim3(p.num_splits, a.kv_heads * p.n_head_tiles, a.batch),
-                   dim3(kWarps * 32), smem, stream, p);
-  if (e == cudaSuccess && partial) {
+  cudaError_t e =
+      scratch.acquire(stream, scores_at + (scores ? rows * size_t(max_tokens) * 4 : 0));
+  if (e != cudaSuccess) return e;
+  char *base = static_cast<char *>(scratch.ptr);
+  p.part_o = reinterpret_cast<float *>(base);
+  p.part_lse = reinterpret_cast<float *>(base + lse_at);
+  p.lse = reinterpret_cast<float *>(base + row_at);
+  p.scores = scores ? reinterpret_cast<float *>(base + scores_at) : nullptr;
+  p.counters = scratch.counters;
+  const int nu = units_at_a_time(D, nt);
+  const size_t smem = std::max({size_t(kWarps) * kStages * nu * 18 * D,  // rings
+                                size_t(kWarps) * 8 * nt * (D + 2) * 4,   // warps' results
+                                size_t(8 * nt) * (X + 1) * 4});          // pieces' weights
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e == cudaSuccess) e = launch_pdl(fn, dim3(X, Y), dim3(kWarps * 32), smem, stream, p);
+  if (e == cudaSuccess && scores) {
     FinishParams f = {};
     f.seq_lens = a.seq_lens;
-    f.max_tokens = a.max_blocks_per_seq * a.block_size;
+    f.max_tokens = max_tokens;
     f.hq = a.num_q_heads;
     f.hkv = a.kv_heads;
-    f.head_dim = D;
-    f.num_splits = p.num_splits;
-    f.tokens_per_split = p.units_per_split * kUnit;
-    f.part_o = p.part_o;
-    f.part_lse = p.part_lse;
-    f.out = a.out;
-    f.o_sb = p.o_sb;
-    f.o_sh = p.o_sh;
+    f.num_splits = 1;
+    f.tokens_per_split = max_tokens;
+    f.part_lse = p.lse;
     f.scores = p.scores;
     f.score_stride = p.score_stride;
     f.w_in = w.w_in;
     f.w_out = w.w_out;
     f.w_stride = w.w_stride;
-    const int chunks = scores ? (f.max_tokens + kFinishTokens - 1) / kFinishTokens : 1;
-    e = launch_pdl(a.dtype == Dtype::BF16 ? finish_kernel<__nv_bfloat16> : finish_kernel<__half>,
-                   dim3(chunks, a.kv_heads, a.batch), dim3(kFinishThreads), 0, stream, f);
+    e = launch_finish(a.dtype, f, a.batch, stream);
   }
   const cudaError_t r = scratch.release(stream);
   return e != cudaSuccess ? e : r;

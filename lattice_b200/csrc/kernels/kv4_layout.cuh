@@ -14,9 +14,11 @@ __host__ __device__ constexpr int kv4_code_offset(int groups, int j, int lane, i
   return groups % 2 == 0 ? ((j >> 1) * 32 + lane) * 16 + (j & 1) * 8 + w * 4
                          : (j * 32 + lane) * 8 + w * 4;
 }
-// Byte offset of the scale of token t (of 16), group j: a lane's tokens g and g+8 adjoin.
-__host__ __device__ constexpr int kv4_scale_offset(int groups, int t, int j) {
-  return groups * 256 + (((t & 7) * 2 + (t >> 3)) * groups + j) * 2;
+// Byte offset of the scale of token t (of 16), group j.  K's: token g's groups, then token
+// g+8's, by g.  V's: by token pair c, then group, then half of the unit, a pair in one word.
+__host__ __device__ constexpr int kv4_scale_offset(bool is_v, int groups, int t, int j) {
+  return groups * 256 + (is_v ? ((t & 7) >> 1) * groups * 8 + j * 8 + (t >> 3) * 4 + (t & 1) * 2
+                              : (((t & 7) * 2 + (t >> 3)) * groups + j) * 2);
 }
 
 }  // namespace dev

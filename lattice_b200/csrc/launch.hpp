@@ -194,8 +194,11 @@ cudaError_t beam_gather(const BeamGatherArgs &a, cudaStream_t stream);
 
 // Scratch of one call: the stream's kept buffer where there is one (stream_scratch), else
 // a stream-ordered allocation that release() frees in stream order.
+// `counters` are kZeroedCounters 32-bit zeros: a kernel that raises some leaves them zero.
+constexpr int kZeroedCounters = 16384;
 struct CallScratch {
   void *ptr = nullptr;
+  int32_t *counters = nullptr;
   bool owned = false;
   cudaError_t acquire(cudaStream_t stream, size_t bytes);
   cudaError_t release(cudaStream_t stream);
