@@ -849,7 +849,7 @@ static int kv4_rows(kcmm_pool_t *h, const char *op, kcmm::dev::Dtype dtype, bool
   a.k_stride = k_stride ? k_stride : row;
   a.v_stride = v_stride ? v_stride : row;
   a.status = reinterpret_cast<int32_t *>(status);
-  a.vec = ((k | v) & 7) == 0 && a.k_stride % 4 == 0 && a.v_stride % 4 == 0;
+  a.vec = ((k | v) & 15) == 0 && a.k_stride % 8 == 0 && a.v_stride % 8 == 0;
   p->use_device();
   return check_launch(h, op, append ? kcmm::dev::kv4_append(a, S(stream))
                                     : kcmm::dev::kv4_read(a, S(stream)));

@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "../launch.hpp"
 #include "finish.cuh"
@@ -36,11 +37,92 @@ constexpr int kUnit = kKv4Unit;
 constexpr int kGroup = kKv4Group;
 
 // --- append and read -----------------------------------------------------------------
+//
+// One warp a head and K or V of a tile of rows.  Where the tile's 16 slots are one unit of a
+// page (a prompt's chunk), lane (g, c) takes exactly the values whose codes it holds in the
+// layout: its source loads are whole 32-byte sectors, its code stores one 16-byte vector a
+// pair of groups, and no byte goes through shared memory.  Other tiles (decode steps, the
+// ends of a chunk) go row by row, 8 values a lane.  Both are bound by HBM for long inputs
+// and by the latency of slot -> offset -> row for short ones.
 
-// First byte of the chunk that holds `slot`, or -1 (a status as for the 16-bit slot write).
+constexpr int kRowsThreads = 128;
+// Rows of a warp's tile below kTileTokens tokens: decode steps, whose rows lie apart.
+constexpr int kFewRows = 2;
+constexpr int kTileTokens = 512;
+
+template <typename T>
+__device__ __forceinline__ float widen16(uint32_t bits) {
+  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
+    return __half2float(__ushort_as_half(uint16_t(bits)));
+  } else {
+    return __uint_as_float(bits << 16);
+  }
+}
+
+// The scale of a group from the largest magnitude bits among its values.
+struct GroupScale {
+  uint32_t bits;  // bf16
+  float s, inv;
+  int kind;  // 0: the codes are 0; 1: quotients through 1/s; 2: s is too small or large for that
+};
+template <typename T>
+__device__ __forceinline__ GroupScale group_scale(uint32_t mag) {
+  constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  GroupScale r;
+  const __nv_bfloat16 s = __float2bfloat16_rn(__fdiv_rn(widen16<T>(mag), 7.f));
+  r.bits = mag >= kInf ? 0x7fc0u : uint32_t(__bfloat16_as_ushort(s));
+  r.s = __bfloat162float(s);
+  const bool plain = r.s > 1e-30f && r.s < 1e30f;
+  r.inv = plain ? __frcp_rn(r.s) : 0.f;
+  r.kind = mag >= kInf || r.s == 0.f ? 0 : plain ? 1 : 2;
+  return r;
+}
+
+// code + 8 of a value, in the low 4 bits of 0x4b400000 + code + 8.  The quotient is corrected
+// once by its exact remainder (Markstein's division step): half-way quotients come out exact,
+// and all others of a value of 11 bits by a scale of 8 lie 2^-14 or more away from half-way,
+// so that rounding to even on adding 1.5 2^23 gives the code of the exact quotient.
+__device__ __forceinline__ uint32_t code_bits(float x, const GroupScale &r) {
+  constexpr float kRound = 12582920.f;  // 1.5 2^23 + 8
+  float q;
+  if (r.kind == 1) {
+    q = x * r.inv;
+    q = fmaf(fmaf(-q, r.s, x), r.inv, q);
+  } else if (r.kind == 2) {
+    q = fminf(fmaxf(__fdiv_rn(x, r.s), -7.f), 7.f);
+  } else {
+    q = 0.f;
+  }
+  return __float_as_uint(q + kRound);
+}
+
+// Nibbles of 4 codes, code i at bit step * i, from code_bits' words.
+template <int STEP>
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  constexpr uint32_t k = 0x4b400000u;
+  return (a - k) + ((b - k) << STEP) + ((c - k) << (2 * STEP)) + ((d - k) << (3 * STEP));
+}
+// A K word: dims 8c + {0..7}, dim 2i in nibble i, 2i + 1 in nibble i + 4.
+__device__ __forceinline__ uint32_t pack_k(const uint32_t *n) {
+  return pack4<4>(n[0], n[2], n[4], n[6]) + (pack4<4>(n[1], n[3], n[5], n[7]) << 16);
+}
+__device__ __forceinline__ float code_value(uint32_t nibble, float s) {
+  return (__uint_as_float(0x4b000000u | nibble) - 8388616.f) * s;  // (n - 8) s
+}
+
+// Byte offset of the first chunk (head 0) of the unit that holds `slot`, or -1 (with a status
+// as for the 16-bit slot write); *t the slot's place in its unit.
 __device__ __forceinline__ int64_t chunk_of(const Kv4RowsArgs &a, int64_t slot, int *t) {
-  const int64_t blk = slot / a.block_size;
-  const int in = int(slot - blk * a.block_size);
+  if (slot < 0) return -1;
+  int64_t blk;
+  int in;
+  if (slot < 0x7fffffff) {
+    blk = uint32_t(slot) / uint32_t(a.block_size);
+    in = int(uint32_t(slot) - uint32_t(blk) * uint32_t(a.block_size));
+  } else {
+    blk = slot / a.block_size;
+    in = int(slot - blk * a.block_size);
+  }
   *t = in % kUnit;
   if (blk >= a.offsets_len) {
     if (a.status) atomicCAS(a.status, 0, 1);
@@ -59,127 +141,292 @@ __device__ __forceinline__ int64_t chunk_of(const Kv4RowsArgs &a, int64_t slot, 
   return int64_t(off) + int64_t(in / kUnit) * 9 * a.head_dim;
 }
 
-// Four consecutive values a thread; the 8 threads of a group share its maximum.
-template <typename T>
-__global__ void kv4_append_kernel(const Kv4RowsArgs a) {
+// The rows of a warp's tile: lane i has row i's chunk; `unit` where they are one whole unit.
+struct Tile {
+  int row0, rows, head;
+  bool is_v, unit;
+  int64_t chunk;  // of row `lane`, at this head
+  int t;
+};
+template <int ROWS>
+__device__ __forceinline__ bool find_tile(const Kv4RowsArgs &a, Tile *tile) {
+  const int lane = threadIdx.x & 31;
+  const int w = int(blockIdx.y) * (kRowsThreads / 32) + int(threadIdx.x >> 5);
+  if (w >= 2 * a.kv_heads) return false;
+  tile->is_v = w >= a.kv_heads;
+  tile->head = tile->is_v ? w - a.kv_heads : w;
+  tile->row0 = int(blockIdx.x) * ROWS;
+  tile->rows = min(ROWS, a.num_tokens - tile->row0);
+  tile->chunk = -1;
+  tile->t = 0;
+  int64_t slot = -1;
+  if (lane < tile->rows) {
+    slot = a.slot_mapping[tile->row0 + lane];
+    tile->chunk = chunk_of(a, slot, &tile->t);
+    if (tile->chunk >= 0)
+      tile->chunk += int64_t(tile->head) * (a.block_size / kUnit) * 9 * a.head_dim;
+  }
+  const int64_t first = __shfl_sync(0xffffffffu, slot, 0);
+  const bool in_order = lane >= kUnit || (slot == first + lane && tile->chunk >= 0);
+  tile->unit = ROWS == kUnit && first % kUnit == 0 && __all_sync(0xffffffffu, in_order);
+  return true;
+}
+
+template <int N>
+__device__ __forceinline__ void load_row(uint32_t *w, const uint16_t *src, bool vec) {
+  if (vec) {
+    if constexpr (N == 4) {
+      *reinterpret_cast<uint4 *>(w) = __ldcs(reinterpret_cast<const uint4 *>(src));
+    } else {
+      *reinterpret_cast<uint2 *>(w) = __ldcs(reinterpret_cast<const uint2 *>(src));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = uint32_t(src[2 * i]) | (uint32_t(src[2 * i + 1]) << 16);
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_row(uint16_t *dst, const uint32_t *w, bool vec) {
+  if (vec) {
+    if constexpr (N == 4) {
+      *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(w);
+    } else {
+      *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(w);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      dst[2 * i] = uint16_t(w[i]);
+      dst[2 * i + 1] = uint16_t(w[i] >> 16);
+    }
+  }
+}
+// Largest magnitude bits of N words' halves, by half.
+template <int N>
+__device__ __forceinline__ uint32_t magnitudes(const uint32_t *w) {
+  uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  return m;
+}
+__device__ __forceinline__ uint32_t larger_half(uint32_t m) { return max(m & 0xffffu, m >> 16); }
+
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kRowsThreads) kv4_append_kernel(const Kv4RowsArgs a) {
+  constexpr int NG = D / kGroup, PAIR = NG % 2 == 0 ? 2 : 1;  // groups of a code vector
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
-  const int row = blockIdx.x;
-  const int64_t slot = a.slot_mapping[row];
-  if (slot < 0) return;
-  int t;
-  const int64_t chunk0 = chunk_of(a, slot, &t);
-  if (chunk0 < 0) return;
-  const int D = a.head_dim, groups = D / kGroup, quads = a.kv_heads * D / 4;
-  const int64_t head_stride = int64_t(a.block_size / kUnit) * 9 * D;
-  // quads is a multiple of 8: the 8 threads of a group run or idle together
-  for (int base = 0; base < 2 * quads; base += blockDim.x) {
-    const int i0 = base + int(threadIdx.x);
-    const bool live = i0 < 2 * quads;
-    const int i = live ? i0 : 0;
-    const bool is_v = i >= quads;
-    const int e = (is_v ? i - quads : i) * 4, head = e / D, d = e - head * D;
-    const T *src = static_cast<const T *>(is_v ? a.v : a.k) +
-                   int64_t(row) * (is_v ? a.v_stride : a.k_stride) + e;
-    __align__(8) T raw[4];
-    if (a.vec) {
-      *reinterpret_cast<uint2 *>(raw) = *reinterpret_cast<const uint2 *>(src);
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  Tile tile;
+  if (!find_tile<ROWS>(a, &tile)) return;
+  const uint16_t *src = static_cast<const uint16_t *>(tile.is_v ? a.v : a.k) + tile.head * D;
+  const int64_t stride = tile.is_v ? a.v_stride : a.k_stride;
+  uint8_t *region = static_cast<uint8_t *>(tile.is_v ? a.va_v : a.va_k);
+  src += int64_t(tile.row0) * stride;
+
+  if (tile.unit) {
+    uint8_t *chunk = region + __shfl_sync(0xffffffffu, tile.chunk, 0);
+    alignas(16) uint32_t scales[2 * NG];
+#pragma unroll
+    for (int j0 = 0; j0 < NG; j0 += PAIR) {
+      alignas(16) uint32_t codes[2 * PAIR];
+#pragma unroll
+      for (int jj = 0; jj < PAIR; ++jj) {
+        const int j = j0 + jj;
+        if (!tile.is_v) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {  // tokens g, g + 8: 8 values
+            alignas(16) uint32_t x[4];
+            load_row<4>(x, src + (g + 8 * w) * stride + j * kGroup + c * 8, a.vec);
+            uint32_t m = magnitudes<4>(x);
+            m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const GroupScale s = group_scale<T>(larger_half(m));
+            uint32_t n[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              n[e] = code_bits(widen16<T>((x[e / 2] >> (16 * (e & 1))) & 0xffffu), s);
+            codes[jj * 2 + w] = pack_k(n);
+            scales[w * NG + j] = s.bits;
+          }
+        } else {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {  // tokens 2c, 2c + 1 (+ 8): 4 values each
+            alignas(8) uint32_t x0[2], x1[2];
+            const uint16_t *at = src + (2 * c + 8 * w) * stride + j * kGroup + g * 4;
+            load_row<2>(x0, at, a.vec);
+            load_row<2>(x1, at + stride, a.vec);
+            uint32_t m = larger_half(magnitudes<2>(x0)) | (larger_half(magnitudes<2>(x1)) << 16);
+            m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            const GroupScale s0 = group_scale<T>(m & 0xffffu), s1 = group_scale<T>(m >> 16);
+            uint32_t n0[4], n1[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              n0[e] = code_bits(widen16<T>((x0[e / 2] >> (16 * (e & 1))) & 0xffffu), s0);
+              n1[e] = code_bits(widen16<T>((x1[e / 2] >> (16 * (e & 1))) & 0xffffu), s1);
+            }
+            codes[jj * 2 + w] = pack4<4>(n0[0], n0[1], n0[2], n0[3]) |
+                                (pack4<4>(n1[0], n1[1], n1[2], n1[3]) << 16);
+            scales[2 * j + w] = s0.bits | (s1.bits << 16);
+          }
+        }
+      }
+      if constexpr (PAIR == 2) {
+        *reinterpret_cast<uint4 *>(chunk + kv4_code_offset(NG, j0, lane, 0)) =
+            *reinterpret_cast<const uint4 *>(codes);
+      } else {
+        *reinterpret_cast<uint2 *>(chunk + kv4_code_offset(NG, j0, lane, 0)) =
+            *reinterpret_cast<const uint2 *>(codes);
+      }
+    }
+    if (!tile.is_v && c == 0) {
+#pragma unroll
+      for (int i = 0; i < NG; ++i)
+        *reinterpret_cast<uint32_t *>(chunk + NG * 256 + (g * NG + i) * 4) =
+            scales[2 * i] | (scales[2 * i + 1] << 16);
+    } else if (tile.is_v && g == 0) {
+#pragma unroll
+      for (int i = 0; i < 2 * NG; ++i)
+        *reinterpret_cast<uint32_t *>(chunk + NG * 256 + (c * 2 * NG + i) * 4) = scales[i];
+    }
+    return;
+  }
+
+  constexpr int P = D / 8;  // lanes of a row
+  for (int base = 0; base < tile.rows * P; base += 32) {
+    const int i = base + lane, r = min(i / P, tile.rows - 1), piece = i % P;
+    const int64_t at = __shfl_sync(0xffffffffu, tile.chunk, r);
+    const int t = __shfl_sync(0xffffffffu, tile.t, r);
+    const bool live = i < tile.rows * P && at >= 0;
+    alignas(16) uint32_t x[4] = {0u, 0u, 0u, 0u};
+    if (live) load_row<4>(x, src + r * stride + piece * 8, a.vec);
+    uint32_t m = magnitudes<4>(x);  // P is a multiple of 4: the lanes of a group are one row's
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    if (!live) continue;
+    const GroupScale s = group_scale<T>(larger_half(m));
+    uint32_t n[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      n[e] = code_bits(widen16<T>((x[e / 2] >> (16 * (e & 1))) & 0xffffu), s);
+    const int j = piece / 4, q = piece % 4;
+    uint8_t *chunk = region + at;
+    if (!tile.is_v) {
+      *reinterpret_cast<uint32_t *>(chunk + kv4_code_offset(NG, j, (t & 7) * 4 + q, t >> 3)) =
+          pack_k(n);
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) raw[k] = src[k];
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<uint16_t *>(
+            chunk + kv4_code_offset(NG, j, (2 * q + h) * 4 + (t & 7) / 2, t >> 3) + (t & 1) * 2) =
+            uint16_t(pack4<4>(n[4 * h], n[4 * h + 1], n[4 * h + 2], n[4 * h + 3]));
     }
-    float x[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = ptx::to_f32(raw[k]);
-    float mx = 0.f;
-    bool bad = false;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      mx = fmaxf(mx, fabsf(x[k]));
-      bad |= !isfinite(x[k]);
-    }
-    if (bad) mx = INFINITY;
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    // The 16-bit inputs and the 8-bit scale make x / s miss every rounding boundary by far
-    // more than a 32-bit quotient's rounding, unless it lies on one: the codes are exact.
-    __nv_bfloat16 s = __float2bfloat16_rn(__fdiv_rn(mx, 7.f));
-    if (mx == INFINITY) s = __ushort_as_bfloat16(0x7fc0);
-    const float sf = __bfloat162float(s);
-    uint32_t n[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float q = sf > 0.f ? rintf(__fdiv_rn(x[k], sf)) : 0.f;
-      q = fminf(fmaxf(q, -7.f), 7.f);
-      n[k] = uint32_t(int(q) + 8);
-    }
-    const int j = d / kGroup, in = (d % kGroup) / 4;  // the thread's place in its group
-    uint8_t *chunk = static_cast<uint8_t *>(is_v ? a.va_v : a.va_k) + chunk0 + head * head_stride;
-    const uint32_t half = n[0] | (n[2] << 4) | (n[1] << 16) | (n[3] << 20);
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, half, 1);
-    if (!live) continue;
-    if (is_v) {
-      const int lane = in * 4 + (t & 7) / 2;
-      *reinterpret_cast<uint16_t *>(chunk + kv4_code_offset(groups, j, lane, t >> 3) + (t & 1) * 2) =
-          uint16_t(n[0] | (n[1] << 4) | (n[2] << 8) | (n[3] << 12));
-    } else if ((in & 1) == 0) {
-      const int lane = (t & 7) * 4 + in / 2;
-      *reinterpret_cast<uint32_t *>(chunk + kv4_code_offset(groups, j, lane, t >> 3)) =
-          half | (other << 8);
-    }
-    if (in == 0)
-      *reinterpret_cast<__nv_bfloat16 *>(chunk + kv4_scale_offset(is_v, groups, t, j)) = s;
+    if (q == 0)
+      *reinterpret_cast<uint16_t *>(chunk + kv4_scale_offset(tile.is_v, NG, t, j)) =
+          uint16_t(s.bits);
   }
 }
 
 template <typename T>
-__global__ void kv4_read_kernel(const Kv4RowsArgs a) {
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  return ptx::Mma<T>::pack(lo, hi);
+}
+
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kRowsThreads) kv4_read_kernel(const Kv4RowsArgs a) {
+  constexpr int NG = D / kGroup, PAIR = NG % 2 == 0 ? 2 : 1;
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
-  const int row = blockIdx.x;
-  const int64_t slot = a.slot_mapping[row];
-  if (slot < 0) return;
-  int t;
-  const int64_t chunk0 = chunk_of(a, slot, &t);
-  if (chunk0 < 0) return;
-  const int D = a.head_dim, groups = D / kGroup, quads = a.kv_heads * D / 4;
-  const int64_t head_stride = int64_t(a.block_size / kUnit) * 9 * D;
-  for (int i = threadIdx.x; i < 2 * quads; i += blockDim.x) {
-    const bool is_v = i >= quads;
-    const int e = (is_v ? i - quads : i) * 4, head = e / D, d = e - head * D;
-    const int j = d / kGroup, in = (d % kGroup) / 4;
-    const uint8_t *chunk =
-        static_cast<const uint8_t *>(is_v ? a.va_v : a.va_k) + chunk0 + head * head_stride;
-    uint32_t n[4];
-    if (is_v) {
-      const int lane = in * 4 + (t & 7) / 2;
-      const uint32_t w = *reinterpret_cast<const uint16_t *>(
-          chunk + kv4_code_offset(groups, j, lane, t >> 3) + (t & 1) * 2);
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  Tile tile;
+  if (!find_tile<ROWS>(a, &tile)) return;
+  uint16_t *dst = static_cast<uint16_t *>(tile.is_v ? a.v : a.k) + tile.head * D;
+  const int64_t stride = tile.is_v ? a.v_stride : a.k_stride;
+  const uint8_t *region = static_cast<const uint8_t *>(tile.is_v ? a.va_v : a.va_k);
+  dst += int64_t(tile.row0) * stride;
+
+  if (tile.unit) {
+    const uint8_t *chunk = region + __shfl_sync(0xffffffffu, tile.chunk, 0);
+    uint32_t scales[2 * NG];  // K: two bf16 a word, token g's then token g + 8's; V: [group][w]
 #pragma unroll
-      for (int k = 0; k < 4; ++k) n[k] = (w >> (4 * k)) & 15u;
-    } else {
-      const int lane = (t & 7) * 4 + in / 2;
-      const uint32_t w =
-          *reinterpret_cast<const uint32_t *>(chunk + kv4_code_offset(groups, j, lane, t >> 3)) >>
-          ((in & 1) * 8);
-      n[0] = w & 15u;
-      n[2] = (w >> 4) & 15u;
-      n[1] = (w >> 16) & 15u;
-      n[3] = (w >> 20) & 15u;
+    for (int i = 0; i < (tile.is_v ? 2 * NG : NG); ++i)
+      scales[i] = *reinterpret_cast<const uint32_t *>(
+          chunk + NG * 256 + (tile.is_v ? c * 2 * NG + i : g * NG + i) * 4);
+#pragma unroll
+    for (int j0 = 0; j0 < NG; j0 += PAIR) {
+      alignas(16) uint32_t codes[2 * PAIR];
+      if constexpr (PAIR == 2) {
+        *reinterpret_cast<uint4 *>(codes) = __ldcs(
+            reinterpret_cast<const uint4 *>(chunk + kv4_code_offset(NG, j0, lane, 0)));
+      } else {
+        *reinterpret_cast<uint2 *>(codes) = __ldcs(
+            reinterpret_cast<const uint2 *>(chunk + kv4_code_offset(NG, j0, lane, 0)));
+      }
+#pragma unroll
+      for (int jj = 0; jj < PAIR; ++jj) {
+        const int j = j0 + jj;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint32_t x = codes[jj * 2 + w];
+          if (!tile.is_v) {
+            const int i = w * NG + j;
+            const float s = __uint_as_float(i & 1 ? scales[i >> 1] & 0xffff0000u
+                                                  : scales[i >> 1] << 16);
+            alignas(16) uint32_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              y[e] = pack16<T>(code_value((x >> (4 * e)) & 15u, s),
+                               code_value((x >> (4 * e + 16)) & 15u, s));
+            store_row<4>(dst + (g + 8 * w) * stride + j * kGroup + c * 8, y, a.vec);
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float s = __uint_as_float(h ? scales[2 * j + w] & 0xffff0000u
+                                                : scales[2 * j + w] << 16);
+              const uint32_t z = x >> (16 * h);
+              alignas(8) uint32_t y[2] = {
+                  pack16<T>(code_value(z & 15u, s), code_value((z >> 4) & 15u, s)),
+                  pack16<T>(code_value((z >> 8) & 15u, s), code_value((z >> 12) & 15u, s))};
+              store_row<2>(dst + (2 * c + h + 8 * w) * stride + j * kGroup + g * 4, y, a.vec);
+            }
+          }
+        }
+      }
     }
-    const float s = __bfloat162float(
-        *reinterpret_cast<const __nv_bfloat16 *>(chunk + kv4_scale_offset(is_v, groups, t, j)));
-    T *dst = static_cast<T *>(is_v ? a.v : a.k) +
-             int64_t(row) * (is_v ? a.v_stride : a.k_stride) + e;
-    __align__(8) T y[4];
+    return;
+  }
+
+  constexpr int P = D / 8;
+  for (int base = 0; base < tile.rows * P; base += 32) {
+    const int i = base + lane, r = min(i / P, tile.rows - 1), piece = i % P;
+    const int64_t at = __shfl_sync(0xffffffffu, tile.chunk, r);
+    const int t = __shfl_sync(0xffffffffu, tile.t, r);
+    if (i >= tile.rows * P || at < 0) continue;
+    const int j = piece / 4, q = piece % 4;
+    const uint8_t *chunk = region + at;
+    const float s = __uint_as_float(
+        uint32_t(*reinterpret_cast<const uint16_t *>(chunk + kv4_scale_offset(tile.is_v, NG, t, j)))
+        << 16);
+    alignas(16) uint32_t y[4];
+    if (!tile.is_v) {
+      const uint32_t x = *reinterpret_cast<const uint32_t *>(
+          chunk + kv4_code_offset(NG, j, (t & 7) * 4 + q, t >> 3));
 #pragma unroll
-    for (int k = 0; k < 4; ++k) y[k] = ptx::from_f32<T>(float(int(n[k]) - 8) * s);
-    if (a.vec) {
-      *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(y);
+      for (int e = 0; e < 4; ++e)
+        y[e] = pack16<T>(code_value((x >> (4 * e)) & 15u, s),
+                         code_value((x >> (4 * e + 16)) & 15u, s));
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) dst[k] = y[k];
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t z = *reinterpret_cast<const uint16_t *>(
+            chunk + kv4_code_offset(NG, j, (2 * q + h) * 4 + (t & 7) / 2, t >> 3) + (t & 1) * 2);
+        y[2 * h] = pack16<T>(code_value(z & 15u, s), code_value((z >> 4) & 15u, s));
+        y[2 * h + 1] = pack16<T>(code_value((z >> 8) & 15u, s), code_value((z >> 12) & 15u, s));
+      }
     }
+    store_row<4>(dst + r * stride + piece * 8, y, a.vec);
   }
 }
 
@@ -922,20 +1169,49 @@ Kv4Fn pick(int D, int nt, bool scores) {
 
 }  // namespace
 
+namespace {
+
+using Kv4RowsFn = void (*)(const Kv4RowsArgs);
+
+template <typename T, int D>
+Kv4RowsFn pick_rows(bool append, bool tiles) {
+  return append ? tiles ? kv4_append_kernel<T, D, kUnit> : kv4_append_kernel<T, D, kFewRows>
+                : tiles ? kv4_read_kernel<T, D, kUnit> : kv4_read_kernel<T, D, kFewRows>;
+}
+template <typename T>
+Kv4RowsFn pick_rows(int D, bool append, bool tiles) {
+  switch (D) {
+    case 32: return pick_rows<T, 32>(append, tiles);
+    case 64: return pick_rows<T, 64>(append, tiles);
+    case 96: return pick_rows<T, 96>(append, tiles);
+    case 128: return pick_rows<T, 128>(append, tiles);
+    case 160: return pick_rows<T, 160>(append, tiles);
+    case 192: return pick_rows<T, 192>(append, tiles);
+    case 224: return pick_rows<T, 224>(append, tiles);
+    case 256: return pick_rows<T, 256>(append, tiles);
+    default: return nullptr;
+  }
+}
+
+cudaError_t launch_rows(const Kv4RowsArgs &a, bool append, cudaStream_t stream) {
+  const bool tiles = a.num_tokens >= kTileTokens;
+  const Kv4RowsFn fn = a.dtype == Dtype::BF16
+                           ? pick_rows<__nv_bfloat16>(a.head_dim, append, tiles)
+                           : pick_rows<__half>(a.head_dim, append, tiles);
+  if (!fn) return cudaErrorNotSupported;
+  const int rows = tiles ? kUnit : kFewRows, per = kRowsThreads / 32;
+  return launch_pdl(fn, dim3((a.num_tokens + rows - 1) / rows, (2 * a.kv_heads + per - 1) / per),
+                    dim3(kRowsThreads), 0, stream, a);
+}
+
+}  // namespace
+
 cudaError_t kv4_append(const Kv4RowsArgs &a, cudaStream_t stream) {
-  const int items = 2 * a.kv_heads * a.head_dim / 4;
-  const int threads = std::min(512, (items + 31) / 32 * 32);
-  return launch_pdl(a.dtype == Dtype::BF16 ? kv4_append_kernel<__nv_bfloat16>
-                                           : kv4_append_kernel<__half>,
-                    dim3(a.num_tokens), dim3(threads), 0, stream, a);
+  return launch_rows(a, true, stream);
 }
 
 cudaError_t kv4_read(const Kv4RowsArgs &a, cudaStream_t stream) {
-  const int items = 2 * a.kv_heads * a.head_dim / 4;
-  const int threads = std::min(512, (items + 31) / 32 * 32);
-  return launch_pdl(a.dtype == Dtype::BF16 ? kv4_read_kernel<__nv_bfloat16>
-                                           : kv4_read_kernel<__half>,
-                    dim3(a.num_tokens), dim3(threads), 0, stream, a);
+  return launch_rows(a, false, stream);
 }
 
 cudaError_t kv4_decode_attention(const DecodeArgs &a, const DecodeWeights &w,

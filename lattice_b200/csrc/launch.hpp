@@ -113,7 +113,7 @@ struct Kv4RowsArgs {
   void *v;
   int64_t k_stride, v_stride;
   int32_t *status;  // may be null
-  bool vec;         // every row starts on 8 bytes
+  bool vec;         // every row starts on 16 bytes
 };
 cudaError_t kv4_append(const Kv4RowsArgs &a, cudaStream_t stream);
 cudaError_t kv4_read(const Kv4RowsArgs &a, cudaStream_t stream);
