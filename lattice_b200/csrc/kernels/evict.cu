@@ -8,9 +8,12 @@
 // (>= budget) is never a destination (< budget): the moves need no order among themselves,
 // and only the rows that have to move are touched.
 //
-// The selection is a radix select (11 + 11 + 10 bits) over 32-bit keys, a cluster of CTAs a
-// row.  It is bound by the latency of its passes over the row's weights, which stay in L1
-// and L2 after the first.  The moves are a copy, bound by HBM.
+// The selection narrows a range of 32-bit keys by histograms of 2048 equal bins, as wide as
+// the range asks for: accumulated weights spread over a few octaves, and bins fixed to their
+// leading bits would put half of them into 4 (measured: 72 us a call at 16,700 tokens, the
+// atomics on one bin serialised, where range bins take a few). A cluster of CTAs shares a long
+// row.  It is bound by the latency of its passes, over keys in shared memory where they fit.
+// The moves are a copy, bound by HBM.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -29,8 +32,11 @@ namespace {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWarps = kSelectThreads / 32;
+static_assert(kSelectWarps == 32, "a warp reduces over the warps");
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
+constexpr int kSliceTokens = 4096;
+constexpr int kKeyCapacity = 49152;  // keys in shared memory: 192 KB
 
 // One row's moves: count, then [budget] each of destination slots, source slots and the
 // weights and positions that move with them.
@@ -63,7 +69,9 @@ struct Counts {
 };
 
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictArgs a) {
-  __shared__ int s_hist[kBins];
+  __shared__ __align__(8) int s_hist[kBins];
+  __shared__ int4 s_range[kSelectWarps], s_total;
+  extern __shared__ uint32_t s_keys[];
   __shared__ Counts s_warp[kSelectWarps];
   __shared__ Counts s_cta;
   __shared__ int s_scan[kSelectWarps];
@@ -105,58 +113,116 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     return;
   }
   const int slice = (n + C - 1) / C, begin = min(rank * slice, n), end = min(begin + slice, n);
-  auto key_of = [&](int i) {
+  auto make_key = [&](int i) {
     const int p = pos_of(i);
     return p < a.sinks || p >= next - a.recent ? kHeldKey : weight_key(w_in[i]);
   };
 
-  // ---- threshold: the budget-th largest key, and how many equal to it stay -------------
-  uint32_t prefix = 0;
-  int want = a.budget;  // keys to take among those that match the prefix
-#pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const int top = pass == 0 ? 32 : pass == 1 ? 21 : 10;  // bits below are undecided
-    const uint32_t mask = pass == 2 ? 1023u : 2047u;
-    for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
-    __syncthreads();
+  // ---- keys, their range, and how many slots are held -----------------------------------------
+  // The keys of this CTA's slice stay in shared memory where it holds them.
+  const bool staged = end - begin <= a.key_capacity;
+  uint32_t kmin = 0xffffffffu, kmax = 0;
+  int held = 0;
 #pragma unroll 4
-    for (int i = begin + tid; i < end; i += kSelectThreads) {
-      const uint32_t k = key_of(i);
-      if (pass == 0 || (k >> top) == prefix) atomicAdd(&s_hist[(k >> shift) & mask], 1);
+  for (int i = begin + tid; i < end; i += kSelectThreads) {
+    const uint32_t k = make_key(i);
+    if (staged) s_keys[i - begin] = k;
+    held += k == kHeldKey;
+    if (k != kHeldKey) {
+      kmin = min(kmin, k);
+      kmax = max(kmax, k);
     }
-    cluster.sync();
-    // Bins from the top: thread t has bins 2047 - 2t and 2046 - 2t, all CTAs' sums.
-    const int hi = kBins - 1 - 2 * tid;
-    int c0 = 0, c1 = 0;
-    for (int r = 0; r < C; ++r) {
-      const int *h = cluster.map_shared_rank(s_hist, r);
-      c0 += h[hi];
-      c1 += h[hi - 1];
-    }
-    int sum = c0 + c1;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
-    }
-    if (lane == 31) s_scan[warp] = sum;
-    __syncthreads();
-    int before = 0;
-    for (int w = 0; w < warp; ++w) before += s_scan[w];
-    before += sum - c0 - c1;  // keys above this thread's bins
-    if (before < want && before + c0 >= want) {
-      s_digit = hi;
-      s_above = before;
-    } else if (before + c0 < want && before + c0 + c1 >= want) {
-      s_digit = hi - 1;
-      s_above = before + c0;
-    }
-    cluster.sync();  // every CTA has read this one's histogram
-    prefix = (prefix << (pass == 2 ? 10 : 11)) | uint32_t(s_digit);
-    want -= s_above;
   }
-  const uint32_t threshold = prefix;  // `want` keys equal to it stay: the lowest slots
+  kmin = __reduce_min_sync(0xffffffffu, kmin);
+  kmax = __reduce_max_sync(0xffffffffu, kmax);
+  held = __reduce_add_sync(0xffffffffu, held);
+  if (lane == 0) s_range[warp] = make_int4(int(kmin), int(kmax), held, 0);
+  for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
+  __syncthreads();
+  if (warp == 0) {
+    const int4 r = s_range[lane];
+    kmin = __reduce_min_sync(0xffffffffu, uint32_t(r.x));
+    kmax = __reduce_max_sync(0xffffffffu, uint32_t(r.y));
+    held = __reduce_add_sync(0xffffffffu, r.z);
+    if (lane == 0) s_total = make_int4(int(kmin), int(kmax), held, 0);
+  }
+  cluster.sync();
+  kmin = 0xffffffffu;
+  kmax = 0;
+  held = 0;
+  for (int r = 0; r < C; ++r) {
+    const int4 t = *cluster.map_shared_rank(&s_total, r);
+    kmin = min(kmin, uint32_t(t.x));
+    kmax = max(kmax, uint32_t(t.y));
+    held += t.z;
+  }
+  auto key_of = [&](int i) { return staged ? s_keys[i - begin] : make_key(i); };
+
+  // ---- threshold: the budget-th largest key, and how many equal to it stay -------------
+  uint32_t threshold = kHeldKey;
+  int want = a.budget;  // keys at or below kmax to take, when the held ones are taken
+  if (held < a.budget) {
+    want -= held;
+    uint32_t lo = kmin, hi = kmax;  // the wanted key lies in [lo, hi]; keys above hi are taken
+#pragma unroll 1
+    while (lo != hi) {
+      const int bits = 32 - __clz(int(hi - lo));  // of the range
+      const int shift = max(bits - 11, 0);
+#pragma unroll 4
+      for (int base = begin; base < end; base += kSelectThreads) {
+        const int i = base + tid;
+        const uint32_t k = i < end ? key_of(i) : 0;
+        const bool in = i < end && k >= lo && k <= hi;
+        const int bin = in ? int((k - lo) >> shift) : -1;
+        // lanes that share the first live lane's bin count as one (equal weights would
+        // otherwise serialise)
+        const uint32_t live = __ballot_sync(0xffffffffu, in);
+        if (live == 0) continue;
+        const int first = __shfl_sync(0xffffffffu, bin, __ffs(int(live)) - 1);
+        const uint32_t same = __ballot_sync(0xffffffffu, bin == first);
+        if (bin == first) {
+          if (lane == __ffs(int(same)) - 1) atomicAdd(&s_hist[bin], __popc(same));
+        } else if (in) {
+          atomicAdd(&s_hist[bin], 1);
+        }
+      }
+      cluster.sync();
+      // Bins from the top: thread t has bins 2047 - 2t and 2046 - 2t, all CTAs' sums.
+      const int top = kBins - 1 - 2 * tid;
+      int c0 = 0, c1 = 0;
+      for (int r = 0; r < C; ++r) {
+        const int2 h = *reinterpret_cast<const int2 *>(cluster.map_shared_rank(s_hist, r) + top - 1);
+        c0 += h.y;
+        c1 += h.x;
+      }
+      int sum = c0 + c1;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+      }
+      if (lane == 31) s_scan[warp] = sum;
+      cluster.sync();  // every CTA has read this one's histogram
+      const int other = s_scan[lane];  // of the kSelectWarps = 32 warps
+      int above = lane < warp ? other : 0;
+      above = __reduce_add_sync(0xffffffffu, above) + sum - c0 - c1;  // keys above these bins
+      if (above < want && above + c0 >= want) {
+        s_digit = top;
+        s_above = above;
+      } else if (above + c0 < want && above + c0 + c1 >= want) {
+        s_digit = top - 1;
+        s_above = above + c0;
+      }
+      for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
+      __syncthreads();
+      want -= s_above;
+      const uint32_t base = lo + (uint32_t(s_digit) << shift);
+      hi = min(hi, base + ((1u << shift) - 1));
+      lo = base;
+    }
+    threshold = lo;
+  }
+  // `want` keys equal to the threshold stay: the lowest slots
 
   // ---- counts per warp segment, then over the CTA and the cluster ------------------------
   const int seg = (end - begin + kSelectWarps - 1) / kSelectWarps;
@@ -176,15 +242,12 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   c.eq_lo = __reduce_add_sync(0xffffffffu, c.eq_lo);
   if (lane == 0) s_warp[warp] = c;
   __syncthreads();
-  if (tid == 0) {
-    Counts t = {0, 0, 0, 0};
-    for (int w = 0; w < kSelectWarps; ++w) {
-      t.gt += s_warp[w].gt;
-      t.eq += s_warp[w].eq;
-      t.gt_lo += s_warp[w].gt_lo;
-      t.eq_lo += s_warp[w].eq_lo;
-    }
-    s_cta = t;
+  if (warp == 0) {
+    const Counts w = s_warp[lane];
+    const Counts t = {__reduce_add_sync(0xffffffffu, w.gt), __reduce_add_sync(0xffffffffu, w.eq),
+                      __reduce_add_sync(0xffffffffu, w.gt_lo),
+                      __reduce_add_sync(0xffffffffu, w.eq_lo)};
+    if (lane == 0) s_cta = t;
   }
   cluster.sync();
   int gt = 0, eq = 0, gt_lo = 0, eq_lo = 0;  // gt, eq: before this warp's segment
@@ -197,10 +260,8 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     gt_lo += t.gt_lo;
     eq_lo += t.eq_lo;
   }
-  for (int w = 0; w < warp; ++w) {
-    gt += s_warp[w].gt;
-    eq += s_warp[w].eq;
-  }
+  gt += __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[lane].gt : 0);
+  eq += __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[lane].eq : 0);
   const int kept_lo = gt_lo + min(eq_lo, want);  // slots below the budget that stay
   const int moves = a.budget - kept_lo;
 
@@ -265,7 +326,10 @@ __device__ __forceinline__ int64_t slot_bytes(const EvictArgs &a, int b, int g, 
   return int64_t(off) + (int64_t(in) * a.kv_heads + g) * row;
 }
 
-// One warp a move.
+// 32 moves a warp: each lane resolves one (slot -> page -> offset, three loads deep), then the
+// warp copies them, 8 vectors a lane
+// in flight before their stores.
+constexpr int kMovesInFlight = 8;
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArgs a) {
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
@@ -273,40 +337,69 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
   const RowMoves mv = row_moves(a, b * a.kv_heads + g);
   const int moves = mv.count[0];
   const int warps = int(gridDim.x) * (kMoveThreads / 32);
-  for (int j = int(blockIdx.x) * (kMoveThreads / 32) + (threadIdx.x >> 5); j < moves; j += warps) {
-    int ts, td;
-    const int64_t s = slot_bytes(a, b, g, mv.src[j], &ts), d = slot_bytes(a, b, g, mv.dst[j], &td);
-    if (s < 0 || d < 0) {
-      if (lane == 0) atomicOr(a.diag, int32_t(kDiagBadOffset));
-      continue;
+  for (int j0 = (int(blockIdx.x) * (kMoveThreads / 32) + int(threadIdx.x >> 5)) * 32; j0 < moves;
+       j0 += warps * 32) {
+    const int n = min(32, moves - j0);
+    int64_t s = 0, d = -1;
+    int ts = 0, td = 0;
+    if (lane < n) {
+      s = slot_bytes(a, b, g, mv.src[j0 + lane], &ts);
+      d = slot_bytes(a, b, g, mv.dst[j0 + lane], &td);
+      if (s < 0 || d < 0) {
+        atomicOr(a.diag, int32_t(kDiagBadOffset));
+        d = -1;
+      }
     }
     if (!a.kv4) {
-      const int pieces = a.head_dim / 8;  // 16 bytes each; K's, then V's
-      for (int i = lane; i < 2 * pieces; i += 32) {
-        uint8_t *base = i < pieces ? a.va_k : a.va_v;
-        const int at = (i < pieces ? i : i - pieces) * 16;
-        *reinterpret_cast<uint4 *>(base + d + at) = *reinterpret_cast<const uint4 *>(base + s + at);
+      const int pieces = a.head_dim / 8;  // of a row, 16 bytes each; K's, then V's
+      const int all = 2 * pieces * n;
+      for (int i0 = lane; i0 - lane < all; i0 += 32 * kMovesInFlight) {
+        uint4 x[kMovesInFlight];
+        uint8_t *to[kMovesInFlight];
+#pragma unroll
+        for (int k = 0; k < kMovesInFlight; ++k) {
+          const int i = i0 + 32 * k, m = min(i / (2 * pieces), n - 1);
+          const int64_t sm = __shfl_sync(0xffffffffu, s, m), dm = __shfl_sync(0xffffffffu, d, m);
+          const int e = i - m * 2 * pieces;
+          uint8_t *base = e < pieces ? a.va_k : a.va_v;
+          const int at = (e < pieces ? e : e - pieces) * 16;
+          to[k] = i < all && dm >= 0 ? base + dm + at : nullptr;
+          if (to[k]) x[k] = __ldcs(reinterpret_cast<const uint4 *>(base + sm + at));
+        }
+#pragma unroll
+        for (int k = 0; k < kMovesInFlight; ++k)
+          if (to[k]) *reinterpret_cast<uint4 *>(to[k]) = x[k];
       }
-    } else {
-      const int groups = a.head_dim / 32;
+      continue;
+    }
+    const int groups = a.head_dim / 32;
+    for (int m = 0; m < n; ++m) {
+      const int64_t sm = __shfl_sync(0xffffffffu, s, m), dm = __shfl_sync(0xffffffffu, d, m);
+      const int tsm = __shfl_sync(0xffffffffu, ts, m), tdm = __shfl_sync(0xffffffffu, td, m);
+      if (dm < 0) continue;
       for (int i = lane; i < 4 * groups; i += 32) {  // K: the 4 words of each group
         const int jg = i / 4, c = i % 4;
-        *reinterpret_cast<uint32_t *>(a.va_k + d + kv4_code_offset(groups, jg, (td & 7) * 4 + c, td >> 3)) =
+        *reinterpret_cast<uint32_t *>(
+            a.va_k + dm + kv4_code_offset(groups, jg, (tdm & 7) * 4 + c, tdm >> 3)) =
             *reinterpret_cast<const uint32_t *>(
-                a.va_k + s + kv4_code_offset(groups, jg, (ts & 7) * 4 + c, ts >> 3));
+                a.va_k + sm + kv4_code_offset(groups, jg, (tsm & 7) * 4 + c, tsm >> 3));
       }
       for (int i = lane; i < 8 * groups; i += 32) {  // V: the 8 half words of each group
         const int jg = i / 8, q = i % 8;
-        *reinterpret_cast<uint16_t *>(a.va_v + d + kv4_code_offset(groups, jg, q * 4 + (td & 7) / 2, td >> 3) +
-                                      (td & 1) * 2) =
+        *reinterpret_cast<uint16_t *>(
+            a.va_v + dm + kv4_code_offset(groups, jg, q * 4 + (tdm & 7) / 2, tdm >> 3) +
+            (tdm & 1) * 2) =
             *reinterpret_cast<const uint16_t *>(
-                a.va_v + s + kv4_code_offset(groups, jg, q * 4 + (ts & 7) / 2, ts >> 3) + (ts & 1) * 2);
+                a.va_v + sm + kv4_code_offset(groups, jg, q * 4 + (tsm & 7) / 2, tsm >> 3) +
+                (tsm & 1) * 2);
       }
       for (int i = lane; i < 2 * groups; i += 32) {
         uint8_t *base = i < groups ? a.va_k : a.va_v;
         const int jg = i % groups;
-        *reinterpret_cast<uint16_t *>(base + d + kv4_scale_offset(i >= groups, groups, td, jg)) =
-            *reinterpret_cast<const uint16_t *>(base + s + kv4_scale_offset(i >= groups, groups, ts, jg));
+        *reinterpret_cast<uint16_t *>(base + dm +
+                                      kv4_scale_offset(i >= groups, groups, tdm, jg)) =
+            *reinterpret_cast<const uint16_t *>(base + sm +
+                                                kv4_scale_offset(i >= groups, groups, tsm, jg));
       }
     }
   }
@@ -321,14 +414,22 @@ cudaError_t evict_tokens(const EvictArgs &args, cudaStream_t stream) {
   cudaError_t e = scratch.acquire(stream, (size_t(rows) + size_t(rows) * a.budget * 4) * 4);
   if (e != cudaSuccess) return e;
   a.scratch = static_cast<int32_t *>(scratch.ptr);
-  // CTAs of a row's cluster: as many as leave each 2048 tokens, while they all run at once.
+  // CTAs of a row's cluster: as many as leave each kSliceTokens, while they all run at once.
   int C = 1;
-  while (C < kMaxCluster && a.max_tokens / (2 * C) >= 2048 &&
+  while (C < kMaxCluster && a.max_tokens / (2 * C) >= kSliceTokens &&
          int64_t(rows) * 2 * C <= device_sm_count())
     C *= 2;
+  a.key_capacity = std::min((a.max_tokens + C - 1) / C, kKeyCapacity);
+  const int smem = a.key_capacity * 4;
+  e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) {
+    scratch.release(stream);
+    return e;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(C, a.kv_heads, a.batch);
   cfg.blockDim = dim3(kSelectThreads);
+  cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -341,9 +442,9 @@ cudaError_t evict_tokens(const EvictArgs &args, cudaStream_t stream) {
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   e = cudaLaunchKernelEx(&cfg, evict_select_kernel, a);
   if (e == cudaSuccess) {
-    // a move is 1 to 2 KB each way: enough warps for every SM, none for moves that cannot be
+    // enough warps for every SM, none for moves that cannot be
     const int most = std::min(a.budget, std::max(a.max_tokens - a.budget, 1));
-    const int per = kMoveThreads / 32;
+    const int per = kMoveThreads;  // 32 a warp
     const int want = std::max(1, 8 * device_sm_count() / rows);
     const int grid = std::min((most + per - 1) / per, want);
     e = launch_pdl(evict_move_kernel, dim3(grid, a.kv_heads, a.batch), dim3(kMoveThreads), 0,

@@ -39,6 +39,7 @@ struct FinishParams {
   const float *w_in;  // [b][hkv][w_stride]
   float *w_out;
   int64_t w_stride;
+  bool w_vec;  // rows of weights start on 16 bytes
 };
 
 // Grid (token chunks, hkv, batch).  Every CTA computes the log-sum-exp of its group's
@@ -99,16 +100,40 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const FinishPara
   const int64_t wrow = (int64_t(b) * p.hkv + kvh) * p.w_stride;
   // a weights row of w_stride entries holds the weights of the first w_stride tokens
   const int t1 = int(min(int64_t(min(len, t0 + kFinishTokens)), p.w_stride));
-  for (int t = t0 + threadIdx.x; t < t1; t += kFinishThreads) {
-    float w = p.w_in[wrow + t];
-    float sum = 0.f;
-    for (int h = 0; h < G; ++h) sum += ptx::fast_exp2(sc[h * p.score_stride + t] - s_lse[h]);
-    p.w_out[wrow + t] = w + sum;
+  const int t = t0 + int(threadIdx.x) * 4;
+  if (t >= t1) return;
+  __align__(16) float w[4] = {0.f, 0.f, 0.f, 0.f};
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  const float *w_in = p.w_in + wrow + t;
+  float *w_out = p.w_out + wrow + t;
+  const bool vec = p.w_vec && t + 4 <= t1;
+  if (vec) {
+    *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(w_in);
+  } else {
+    for (int i = 0; i < 4 && t + i < t1; ++i) w[i] = w_in[i];
+  }
+  // rows of scores are whole units long: reading past the last token stays inside
+#pragma unroll 4
+  for (int h = 0; h < G; ++h) {
+    const float4 x = *reinterpret_cast<const float4 *>(sc + h * p.score_stride + t);
+    const float lse = s_lse[h];
+    sum[0] += ptx::fast_exp2(x.x - lse);
+    sum[1] += ptx::fast_exp2(x.y - lse);
+    sum[2] += ptx::fast_exp2(x.z - lse);
+    sum[3] += ptx::fast_exp2(x.w - lse);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] += sum[i];
+  if (vec) {
+    *reinterpret_cast<float4 *>(w_out) = *reinterpret_cast<const float4 *>(w);
+  } else {
+    for (int i = 0; i < 4 && t + i < t1; ++i) w_out[i] = w[i];
   }
 }
 
-inline cudaError_t launch_finish(Dtype dtype, const FinishParams &f, int batch,
-                                 cudaStream_t stream) {
+inline cudaError_t launch_finish(Dtype dtype, FinishParams f, int batch, cudaStream_t stream) {
+  f.w_vec = ((reinterpret_cast<uintptr_t>(f.w_in) | reinterpret_cast<uintptr_t>(f.w_out)) & 15) == 0 &&
+            f.w_stride % 4 == 0;
   const int chunks = f.scores ? (f.max_tokens + kFinishTokens - 1) / kFinishTokens : 1;
   return launch_pdl(dtype == Dtype::BF16 ? finish_kernel<__nv_bfloat16> : finish_kernel<__half>,
                     dim3(chunks, f.hkv, batch), dim3(kFinishThreads), 0, stream, f);

@@ -158,6 +158,7 @@ struct EvictArgs {
   int32_t *new_lens;              // [batch]
   int32_t *diag;
   int32_t *scratch;  // filled by the launcher
+  int key_capacity;  // keys that a CTA holds in shared memory
 };
 cudaError_t evict_tokens(const EvictArgs &a, cudaStream_t stream);
 

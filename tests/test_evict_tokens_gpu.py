@@ -232,3 +232,16 @@ def test_evict_then_decode_and_truncate():
                 assert (err <= 1.25 * 2.0 ** -11 * mass + 2.0 ** -8 * np.abs(ref) + 1e-7).all()
         finally:
             c.close()
+
+
+def test_evict_rows_past_the_keys_that_shared_memory_holds():
+    """50,001 tokens a row, more rows than clusters fit: the keys are computed anew."""
+    c = Cache([50001], 75, 8, seed=15)
+    try:
+        c.fill_rows()
+        e = Evict(c, 50001, seed=16)
+        before = e.snapshot()
+        e.run(2000, 4, 100)
+        e.check(2000, 4, 100, before)
+    finally:
+        c.close()

@@ -284,3 +284,34 @@ def test_bad_block_is_reported():
         assert c.pool.kernel_status() == 0
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hkv,d,bs,first", [(2, 128, 16, 0), (3, 64, 32, 16), (1, 96, 48, 32),
+                                            (2, 256, 16, 5), (1, 32, 16, 0), (5, 160, 64, 1)])
+def test_append_and_read_long_chunks(dtype, hkv, d, bs, first):
+    """Chunks of many rows: whole units, ends that are not, chunks that start inside a unit,
+    skipped rows among them; magnitudes from the smallest to the largest."""
+    torch = torch_cuda()
+    n = 1200
+    c = Cache([n + first], hkv, d, bs, kv4=True, dtype=dtype, seed=d)
+    try:
+        x = c.rng.standard_normal((2, n, hkv, d))
+        x *= np.geomspace(1e-7 if dtype == "f16" else 1e-37, 1e4, n)[None, :, None, None]
+        x[0, 100] = np.round(x[0, 100] / x[0, 100].max() * 14) / 2  # ties
+        x[1, 200, 0, 5], x[0, 300, 0, 7] = np.nan, np.inf
+        tk, tv = (torch.from_numpy(y).cuda().to(c.tdt) for y in x)
+        slots = c.slots(0, first + np.arange(n))
+        skipped = np.array([3, 40, 777])
+        at = slots.copy()
+        at[skipped] = -1
+        c.write(tk, tv, at)
+        got = c.read(slots)
+        keep = np.setdiff1d(np.arange(n), skipped)
+        kt = torch.from_numpy(keep).cuda()
+        for g, y in zip(got, (tk, tv)):
+            assert equal_rows(g[kt], quantised(y.double().cpu().numpy())[keep], dtype)
+            assert bool(torch.isnan(g[torch.from_numpy(skipped).cuda()]).all())  # NaN bits as made
+        assert int(c.status.item()) == 0
+    finally:
+        c.close()
