@@ -1111,7 +1111,7 @@ int kcmm_beam_select_on_stream(kcmm_pool_t *h, uint64_t logits, uint32_t dtype,
     set_error(h, std::string(op) + ": unknown dtype " + std::to_string(dtype));
     return -1;
   }
-  if (n > uint32_t(kcmm::dev::kBeamMaxSelect) || beams > 1024 ||
+  if (n > uint32_t(kcmm::dev::kBeamMaxSelect) || beams > uint32_t(kcmm::dev::kBeamMaxBeams) ||
       uint64_t(batch) * std::max(beams, n) > 0xFFFF || uint64_t(beams) * vocab > 0x7fffffffull ||
       n > uint64_t(beams) * vocab) {
     set_error(h, std::string(op) + ": need n_select <= " +

@@ -6,11 +6,11 @@
 // logit scores -inf everywhere.  A finished beam has the one candidate (k, eos) of its own
 // score; its other tokens score -inf.
 //
-// Pass 1 reads the logits once, 64 bytes a thread, and keeps of each chunk the running
-// maximum and sum of the softmax and the n largest logits: the n-th largest of the threads'
-// own maxima bounds them from below, so that a second look at the registers leaves little
-// more than n to sort.  It is bound by HBM for large vocabularies and by latency for small
-// ones.  Pass 2 scores and ranks a request's beams x chunks x n candidates.
+// A CTA reads 16 KB of a beam's logits once, 64 bytes a thread, and keeps the chunk's
+// maximum, its sum of exponentials and its n largest logits: the n-th largest of the threads'
+// own maxima bounds those from below, so that a second look at the registers leaves little
+// more than n to sort.  The last CTA of a request scores and ranks its beams x chunks x n
+// candidates.  Large vocabularies are bound by HBM, small ones by latency.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -55,7 +55,7 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
 }
 
 struct TopShared {
-  unsigned long long warp_top[kWarps * kMaxSelect];
+  unsigned long long warp_top[kThreads];  // kWarps lists of min(n, 32)
   unsigned long long bound;
   int count;
 };
@@ -69,31 +69,17 @@ __device__ unsigned long long nth_maximum(unsigned long long mine, int n, TopSha
   unsigned long long k = mine;
   for (int r = 0; r < m; ++r) {
     const unsigned long long top = warp_max(k);
-    if (lane == 0) sh->warp_top[warp * kMaxSelect + r] = top;
+    if (lane == 0) sh->warp_top[warp * m + r] = top;
     if (k == top) k = 0;
   }
-  __syncthreads();
-  // rank of every warp's r-th maximum among all: how many are larger
-  const int total = kWarps * m;
   if (threadIdx.x == 0) sh->bound = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < total; i += kThreads) {
-    const unsigned long long x = sh->warp_top[(i / m) * kMaxSelect + i % m];
+  const int total = kWarps * m;
+  if (int(threadIdx.x) < total) {  // the one that n - 1 others exceed
+    const unsigned long long x = sh->warp_top[threadIdx.x];
     int larger = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      // a warp's list descends: count its entries above x
-      const unsigned long long *l = sh->warp_top + w * kMaxSelect;
-      int lo = 0, hi = m;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (l[mid] > x) {
-          lo = mid + 1;
-        } else {
-          hi = mid;
-        }
-      }
-      larger += lo;
-    }
+#pragma unroll 8
+    for (int i = 0; i < total; ++i) larger += sh->warp_top[i] > x;
     if (x != 0 && larger == n - 1) sh->bound = x;
   }
   __syncthreads();
@@ -109,134 +95,30 @@ __device__ __forceinline__ float widen<float>(float x) {
   return x;
 }
 
-// Grid (chunks, rows), a row being one beam of one request.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const BeamArgs a) {
-  constexpr int PER = 16 / sizeof(T);  // logits of a load
-  constexpr int MOST = kVecs * PER;    // of a thread
-  __shared__ TopShared sh;
-  __shared__ unsigned long long s_list[kMaxSelect * MOST];
-  __shared__ float s_red[kWarps];
-  ptx::grid_dependency_wait();
-  ptx::launch_dependents();
-  const int row = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
-  const int warp = tid >> 5, lane = tid & 31;
-  if (a.finished && a.finished[row]) return;  // pass 2 knows its one candidate
-  const T *base = static_cast<const T *>(a.logits) + int64_t(row) * a.row_stride;
-  // 16-byte blocks counted from the one that holds the row's first logit
-  const int lead = int((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
-  const int64_t first = int64_t(chunk) * (kChunkBytes / int(sizeof(T))) - lead;
-  if (first >= a.vocab) {  // an aligned row needs no chunk for its lead
-    if (tid == 0) a.part[int64_t(row) * a.chunks + chunk] = make_float2(-INFINITY, 0.f);
-    if (tid < a.n) a.cand[(int64_t(row) * a.chunks + chunk) * a.n + tid] = 0ull;
-    return;
-  }
-  alignas(16) T x[kVecs][PER];
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int64_t at = first + (int64_t(i) * kThreads + tid) * PER;
-    if (at >= 0 && at + PER <= a.vocab) {
-      *reinterpret_cast<uint4 *>(x[i]) = __ldcs(reinterpret_cast<const uint4 *>(base + at));
-    } else {
-#pragma unroll
-      for (int e = 0; e < PER; ++e)
-        if (at + e >= 0 && at + e < a.vocab) x[i][e] = base[at + e];
-    }
-  }
-  unsigned long long mine = 0;
-  float mx = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int64_t at = first + (int64_t(i) * kThreads + tid) * PER;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      if (at + e < 0 || at + e >= a.vocab) continue;
-      const float v = clean(widen(x[i][e]));
-      mx = fmaxf(mx, v);
-      const unsigned long long k = make_key(v, uint32_t(at + e));
-      mine = k > mine ? k : mine;
-    }
-  }
-  // maximum and sum of the chunk
-  float m = mx;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) s_red[warp] = m;
-  __syncthreads();
-  m = s_red[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_red[w]);
-  float sum = 0.f;
-  if (m != -INFINITY) {
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int64_t at = first + (int64_t(i) * kThreads + tid) * PER;
-#pragma unroll
-      for (int e = 0; e < PER; ++e)
-        if (at + e >= 0 && at + e < a.vocab) sum += __expf(clean(widen(x[i][e])) - m);
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  __syncthreads();
-  if (lane == 0) s_red[warp] = sum;
-  if (tid == 0) sh.count = 0;
-  const unsigned long long bound = nth_maximum(mine, a.n, &sh);  // synchronises
-  if (tid == 0) {
-    float total = 0.f;
-    for (int w = 0; w < kWarps; ++w) total += s_red[w];
-    a.part[int64_t(row) * a.chunks + chunk] = make_float2(m, total);
-  }
-  if (mine != 0 && mine >= bound) {
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int64_t at = first + (int64_t(i) * kThreads + tid) * PER;
-#pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        if (at + e < 0 || at + e >= a.vocab) continue;
-        const unsigned long long k = make_key(clean(widen(x[i][e])), uint32_t(at + e));
-        if (k >= bound) s_list[atomicAdd(&sh.count, 1)] = k;
-      }
-    }
-  }
-  __syncthreads();
-  const int count = sh.count;
-  unsigned long long *cand = a.cand + (int64_t(row) * a.chunks + chunk) * a.n;
-  for (int i = tid; i < max(count, a.n); i += kThreads) {
-    if (i >= count) {
-      cand[i] = 0ull;  // fewer than n logits in the chunk
-      continue;
-    }
-    const unsigned long long k = s_list[i];
-    int larger = 0;
-    for (int j = 0; j < count; ++j) larger += s_list[j] > k;
-    if (larger < a.n) cand[larger] = k;
-  }
-}
-
-constexpr int kBestThreads = 256;
-
-// One CTA a request.
-__global__ void __launch_bounds__(kBestThreads) beam_best_kernel(const BeamArgs a) {
-  __shared__ TopShared sh;
-  extern __shared__ float2 s_norm[];  // [beams]: max, log of the sum
+// One CTA's part of the choice: the last one of request b.
+__device__ void beam_best(const BeamArgs &a, int b, TopShared *sh) {
+  __shared__ float2 s_norm[kBeamMaxBeams];  // max, log of the sum
   __shared__ unsigned long long s_best[kMaxSelect];
-  ptx::grid_dependency_wait();
-  ptx::launch_dependents();
-  const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  for (int k = warp; k < a.beams; k += kBestThreads / 32) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  for (int k = warp; k < a.beams; k += kWarps) {
     const int row = b * a.beams + k;
     if (a.finished && a.finished[row]) continue;
     const float2 *part = a.part + int64_t(row) * a.chunks;
-    float M = -INFINITY;
-    for (int i = lane; i < a.chunks; i += 32) M = fmaxf(M, part[i].x);
+    float M = -INFINITY, sum = 0.f;  // of this lane's chunks
+    for (int i = lane; i < a.chunks; i += 32) {
+      const float2 x = __ldcg(part + i);
+      const float top = fmaxf(M, x.x);
+      if (top != -INFINITY) sum = sum * __expf(M - top) + x.y * __expf(x.x - top);
+      M = top;
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    float sum = 0.f;
-    if (M != -INFINITY)
-      for (int i = lane; i < a.chunks; i += 32) sum += part[i].y * __expf(part[i].x - M);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int o = 16; o > 0; o >>= 1) {
+      const float M2 = __shfl_xor_sync(0xffffffffu, M, o);
+      const float sum2 = __shfl_xor_sync(0xffffffffu, sum, o);
+      const float top = fmaxf(M, M2);
+      if (top != -INFINITY) sum = sum * __expf(M - top) + sum2 * __expf(M2 - top);
+      M = top;
+    }
     if (lane == 0) s_norm[k] = make_float2(M, logf(sum));
   }
   __syncthreads();
@@ -252,7 +134,7 @@ __global__ void __launch_bounds__(kBestThreads) beam_best_kernel(const BeamArgs 
       token = r == 0 ? a.eos : r <= a.eos ? r - 1 : r;
       if (r > 0) score = -INFINITY;
     } else {
-      const unsigned long long c = a.cand[int64_t(row) * a.chunks * a.n + r];
+      const unsigned long long c = __ldcg(a.cand + int64_t(row) * a.chunks * a.n + r);
       if (c == 0ull) return 0ull;
       token = key_index(c);
       const float x = key_value(uint32_t(c >> 32));
@@ -261,53 +143,48 @@ __global__ void __launch_bounds__(kBestThreads) beam_best_kernel(const BeamArgs 
     if (!(score == score)) score = -INFINITY;
     return make_key(score, uint32_t(k) * uint32_t(a.vocab) + token);
   };
-  // repeatedly the n-th largest of the threads' maxima bounds the result from below; the
-  // keys at or above it fit n per thread, and the list is drained in rounds of one key a
-  // thread in descending order
+  // Rounds: the n-th largest of the threads' maxima bounds what is left from below, and the
+  // largest second key of a thread says down to where the maxima are final.
   unsigned long long cut = ~0ull;  // keys below it are left
   int done = 0;
   while (done < a.n) {
-    unsigned long long mine = 0;
-    for (int i = tid; i < total; i += kBestThreads) {
+    unsigned long long mine = 0, second = 0;
+    for (int i = tid; i < total; i += kThreads) {
       const unsigned long long k = candidate(i);
-      if (k < cut && k > mine) mine = k;
+      if (k >= cut) continue;
+      if (k > mine) {
+        second = mine;
+        mine = k;
+      } else if (k > second) {
+        second = k;
+      }
     }
     const int left = a.n - done;
-    if (tid == 0) sh.count = 0;
-    const unsigned long long bound = nth_maximum(mine, left, &sh);
-    // Thread maxima at or above the bound are not yet the result: a thread may hold a second
-    // key above another's maximum.  Those down to the largest second key are final.
-    unsigned long long second = 0;
-    if (mine != 0 && mine >= bound)
-      for (int i = tid; i < total; i += kBestThreads) {
-        const unsigned long long k = candidate(i);
-        if (k < mine && k > second) second = k;
-      }
+    const unsigned long long bound = nth_maximum(mine, left, sh);
+    if (mine < bound) second = 0;
     const unsigned long long top = warp_max(second);
-    __syncthreads();
-    if (lane == 0) sh.warp_top[warp] = top;
+    if (lane == 0) sh->warp_top[warp] = top;
+    if (tid == 0) sh->count = 0;
     __syncthreads();
     unsigned long long floor_key = 0;
-    for (int w = 0; w < kBestThreads / 32; ++w)
-      floor_key = sh.warp_top[w] > floor_key ? sh.warp_top[w] : floor_key;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) floor_key = max(floor_key, sh->warp_top[w]);
     const unsigned long long take = bound > floor_key ? bound : floor_key + 1;
     __syncthreads();
-    unsigned long long *maxima = sh.warp_top;  // [kBestThreads], reused
-    maxima[tid] = mine != 0 && mine >= take ? mine : 0ull;
+    // the final maxima, at most `left`, ranked among themselves
+    if (mine != 0 && mine >= take) sh->warp_top[atomicAdd(&sh->count, 1)] = mine;
     __syncthreads();
-    if (maxima[tid] != 0) {
+    const int count = sh->count;
+    if (count == 0) break;  // no candidate is left
+    if (tid < count) {
+      const unsigned long long x = sh->warp_top[tid];
       int larger = 0;
-      for (int t = 0; t < kBestThreads; ++t) larger += maxima[t] > maxima[tid];
-      if (larger < left) {
-        s_best[done + larger] = maxima[tid];
-        atomicAdd(&sh.count, 1);
-      }
+      for (int i = 0; i < count; ++i) larger += sh->warp_top[i] > x;
+      if (larger < left) s_best[done + larger] = x;
     }
     __syncthreads();
-    if (sh.count == 0) break;  // no candidate is left
-    done += sh.count;
+    done += min(count, left);
     cut = s_best[done - 1];
-    __syncthreads();
   }
   if (tid < done) {
     const unsigned long long k = s_best[tid];
@@ -317,6 +194,117 @@ __global__ void __launch_bounds__(kBestThreads) beam_best_kernel(const BeamArgs 
     a.parents[at] = int32_t(i / uint32_t(a.vocab));
     a.tokens[at] = int32_t(i % uint32_t(a.vocab));
   }
+}
+
+// Grid (chunks, rows), a row being one beam of one request.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) beam_select_kernel(const BeamArgs a) {
+  constexpr int PER = 16 / sizeof(T);  // logits of a load
+  constexpr int MOST = kVecs * PER;    // of a thread
+  __shared__ TopShared sh;
+  __shared__ unsigned long long s_list[kMaxSelect * MOST];
+  __shared__ float s_red[kWarps], s_sum[kWarps];
+  __shared__ int s_last;
+  ptx::grid_dependency_wait();
+  ptx::launch_dependents();
+  const int row = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
+  const int warp = tid >> 5, lane = tid & 31, b = row / a.beams;
+  const bool finished = a.finished && a.finished[row];  // beam_best knows its candidate
+  if (!finished) {
+    const T *base = static_cast<const T *>(a.logits) + int64_t(row) * a.row_stride;
+    // 16-byte blocks counted from the one that holds the row's first logit
+    const int lead = int((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
+    const int64_t first = int64_t(chunk) * (kChunkBytes / int(sizeof(T))) - lead;
+    alignas(16) T x[kVecs][PER];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int64_t at = first + (int64_t(i) * kThreads + tid) * PER;
+      if (at >= 0 && at + PER <= a.vocab) {
+        *reinterpret_cast<uint4 *>(x[i]) = __ldcs(reinterpret_cast<const uint4 *>(base + at));
+      } else {
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          if (at + e >= 0 && at + e < a.vocab) x[i][e] = base[at + e];
+      }
+    }
+    const int64_t at0 = first + int64_t(tid) * PER;  // load i's first logit: + i * kThreads * PER
+    auto each = [&](auto f) {  // f(logit, index) of the thread's logits
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) {
+        const int64_t at = at0 + int64_t(i) * kThreads * PER;
+        if (at >= 0 && at + PER <= a.vocab) {
+#pragma unroll
+          for (int e = 0; e < PER; ++e) f(clean(widen(x[i][e])), int(at) + e);
+        } else {
+#pragma unroll
+          for (int e = 0; e < PER; ++e)
+            if (at + e >= 0 && at + e < a.vocab) f(clean(widen(x[i][e])), int(at + e));
+        }
+      }
+    };
+    // the thread's maximum, the chunk's, and the chunk's sum
+    float mx = -INFINITY;
+    each([&](float v, int) { mx = fmaxf(mx, v); });
+    float m = mx;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) s_red[warp] = m;
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    m = s_red[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_red[w]);
+    float sum = 0.f;
+    int lowest = -1;  // index of the thread's first logit that equals its maximum
+    if (m != -INFINITY) {
+      each([&](float v, int i) {
+        sum += __expf(v - m);
+        if (v == mx && lowest < 0) lowest = i;
+      });
+    } else {
+      each([&](float, int i) {
+        if (lowest < 0) lowest = i;
+      });
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) s_sum[warp] = sum;
+    const unsigned long long mine = lowest >= 0 ? make_key(mx, uint32_t(lowest)) : 0ull;
+    const unsigned long long bound = nth_maximum(mine, a.n, &sh);  // synchronises
+    if (tid == 0) {
+      float total = 0.f;
+      for (int w = 0; w < kWarps; ++w) total += s_sum[w];
+      a.part[int64_t(row) * a.chunks + chunk] = make_float2(m, total);
+    }
+    if (mine != 0 && mine >= bound) {
+      each([&](float v, int i) {
+        const unsigned long long k = make_key(v, uint32_t(i));
+        if (k >= bound) s_list[atomicAdd(&sh.count, 1)] = k;
+      });
+    }
+    __syncthreads();
+    const int count = sh.count;
+    unsigned long long *cand = a.cand + (int64_t(row) * a.chunks + chunk) * a.n;
+    for (int i = tid; i < max(count, a.n); i += kThreads) {
+      if (i >= count) {
+        cand[i] = 0ull;  // fewer than n logits in the chunk
+        continue;
+      }
+      const unsigned long long k = s_list[i];
+      int larger = 0;
+      for (int j = 0; j < count; ++j) larger += s_list[j] > k;
+      if (larger < a.n) cand[larger] = k;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    __threadfence();  // the CTA's candidates, which the barrier ordered before this
+    s_last = atomicAdd(a.counters + b, 1) == a.beams * a.chunks - 1;
+    if (s_last) a.counters[b] = 0;  // for the next call
+    __threadfence();
+  }
+  __syncthreads();
+  if (s_last) beam_best(a, b, &sh);
 }
 
 // dst row (b, j) = src row (b, parents[b, j]); with tokens, its entry token_index = tokens[b, j].
@@ -373,13 +361,11 @@ cudaError_t beam_select(const BeamArgs &args, cudaStream_t stream) {
   a.cand = static_cast<unsigned long long *>(scratch.ptr);
   a.part = reinterpret_cast<float2 *>(static_cast<char *>(scratch.ptr) + cand_bytes);
   const dim3 grid(a.chunks, rows);
-  e = launch_pdl(a.type == 0   ? beam_chunk_kernel<__half>
-                 : a.type == 1 ? beam_chunk_kernel<__nv_bfloat16>
-                               : beam_chunk_kernel<float>,
+  a.counters = scratch.counters;
+  e = launch_pdl(a.type == 0   ? beam_select_kernel<__half>
+                 : a.type == 1 ? beam_select_kernel<__nv_bfloat16>
+                               : beam_select_kernel<float>,
                  grid, dim3(kThreads), 0, stream, a);
-  if (e == cudaSuccess)
-    e = launch_pdl(beam_best_kernel, dim3(a.batch), dim3(kBestThreads),
-                   size_t(a.beams) * sizeof(float2), stream, a);
   const cudaError_t r = scratch.release(stream);
   return e != cudaSuccess ? e : r;
 }

@@ -164,6 +164,7 @@ cudaError_t evict_tokens(const EvictArgs &a, cudaStream_t stream);
 
 // --- beam search (kernels/beam.cu) ---
 constexpr int kBeamMaxSelect = 64;
+constexpr int kBeamMaxBeams = 1024;
 struct BeamArgs {
   const void *logits;  // [batch * beams] rows of row_stride
   int type;            // 0 f16, 1 bf16, 2 f32
@@ -178,6 +179,7 @@ struct BeamArgs {
   int chunks;  // filled by the launcher, as the scratch arrays
   unsigned long long *cand;
   float2 *part;
+  int32_t *counters;  // a zero per request: CTAs that are done
 };
 cudaError_t beam_select(const BeamArgs &a, cudaStream_t stream);
 struct BeamGatherArgs {
@@ -196,7 +198,7 @@ cudaError_t beam_gather(const BeamGatherArgs &a, cudaStream_t stream);
 // Scratch of one call: the stream's kept buffer where there is one (stream_scratch), else
 // a stream-ordered allocation that release() frees in stream order.
 // `counters` are kZeroedCounters 32-bit zeros: a kernel that raises some leaves them zero.
-constexpr int kZeroedCounters = 16384;
+constexpr int kZeroedCounters = 65536;
 struct CallScratch {
   void *ptr = nullptr;
   int32_t *counters = nullptr;
