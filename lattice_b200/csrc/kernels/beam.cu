@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../launch.hpp"
 #include "pdl.cuh"
@@ -43,8 +44,20 @@ __device__ __forceinline__ unsigned long long make_key(float x, uint32_t index) 
 __device__ __forceinline__ uint32_t key_index(unsigned long long k) {
   return 0xffffffffu - uint32_t(k);
 }
-__device__ __forceinline__ float clean(float x) {
-  return x == x ? fminf(x, 3.402823466e38f) : -INFINITY;
+// NaN to -inf, +inf to the largest finite value, in the logits' own type.
+__device__ __forceinline__ uint32_t clean(uint32_t x, float) {
+  const float v = __uint_as_float(x);
+  return __float_as_uint(fminf(fmaxf(v, -INFINITY), 3.402823466e38f));
+}
+__device__ __forceinline__ uint32_t clean(uint32_t x, __half) {
+  asm("max.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0xfc00fc00u));
+  asm("min.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0x7bff7bffu));
+  return x;
+}
+__device__ __forceinline__ uint32_t clean(uint32_t x, __nv_bfloat16) {
+  asm("max.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0xff80ff80u));
+  asm("min.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0x7f7f7f7fu));
+  return x;
 }
 
 // The largest of the warp's keys (0 = none).
@@ -86,13 +99,32 @@ __device__ unsigned long long nth_maximum(unsigned long long mine, int n, TopSha
   return sh->bound;
 }
 
-template <typename T>
-__device__ __forceinline__ float widen(T x) {
-  return ptx::to_f32(x);
-}
-template <>
-__device__ __forceinline__ float widen<float>(float x) {
-  return x;
+// The n-th largest of the CTA's per-thread values, as its value_key (every thread has one,
+// n <= kThreads; equal values count as often as they occur).
+__device__ uint32_t nth_value(uint32_t mine, int n, TopShared *sh) {
+  uint32_t *tops = reinterpret_cast<uint32_t *>(sh->warp_top);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int m = min(n, 32);
+  uint32_t k = mine;
+  for (int r = 0; r < m; ++r) {
+    const uint32_t top = __reduce_max_sync(0xffffffffu, k);
+    if (lane == 0) tops[warp * m + r] = top;
+    if (lane == __ffs(int(__ballot_sync(0xffffffffu, k == top))) - 1) k = 0;
+  }
+  __syncthreads();
+  const int total = kWarps * m;
+  if (int(threadIdx.x) < total) {  // fewer than n larger, n or more not smaller
+    const uint32_t x = tops[threadIdx.x];
+    int larger = 0, equal = 0;
+#pragma unroll 8
+    for (int i = 0; i < total; ++i) {
+      larger += tops[i] > x;
+      equal += tops[i] == x;
+    }
+    if (larger < n && larger + equal >= n) sh->bound = x;  // one value, of equal threads
+  }
+  __syncthreads();
+  return uint32_t(sh->bound);
 }
 
 // One CTA's part of the choice: the last one of request b.
@@ -198,7 +230,7 @@ __device__ void beam_best(const BeamArgs &a, int b, TopShared *sh) {
 
 // Grid (chunks, rows), a row being one beam of one request.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) beam_select_kernel(const BeamArgs a) {
+__global__ void __launch_bounds__(kThreads, 6) beam_select_kernel(const BeamArgs a) {
   constexpr int PER = 16 / sizeof(T);  // logits of a load
   constexpr int MOST = kVecs * PER;    // of a thread
   __shared__ TopShared sh;
@@ -215,70 +247,100 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const BeamArgs a)
     // 16-byte blocks counted from the one that holds the row's first logit
     const int lead = int((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
     const int64_t first = int64_t(chunk) * (kChunkBytes / int(sizeof(T))) - lead;
-    alignas(16) T x[kVecs][PER];
+    uint32_t x[kVecs][4];
+    const int64_t at0 = first + int64_t(tid) * PER;  // load i's first logit: + i * kThreads * PER
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const int64_t at = first + (int64_t(i) * kThreads + tid) * PER;
+      const int64_t at = at0 + int64_t(i) * kThreads * PER;
       if (at >= 0 && at + PER <= a.vocab) {
-        *reinterpret_cast<uint4 *>(x[i]) = __ldcs(reinterpret_cast<const uint4 *>(base + at));
-      } else {
+        const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(base + at));
+        x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
+      } else {  // the row's ends: logits outside it become NaN here, and -inf below
 #pragma unroll
-        for (int e = 0; e < PER; ++e)
-          if (at + e >= 0 && at + e < a.vocab) x[i][e] = base[at + e];
+        for (int w = 0; w < 4; ++w) {
+          constexpr int PW = 4 / sizeof(T);
+          x[i][w] = 0xffffffffu;
+#pragma unroll
+          for (int e = 0; e < PW; ++e) {
+            const int64_t k = at + w * PW + e;
+            if (k < 0 || k >= a.vocab) continue;
+            if constexpr (PW == 1) {
+              x[i][w] = reinterpret_cast<const uint32_t *>(base)[k];
+            } else {
+              const uint32_t bits = reinterpret_cast<const uint16_t *>(base)[k];
+              x[i][w] = e ? (x[i][w] & 0xffffu) | (bits << 16) : (x[i][w] & 0xffff0000u) | bits;
+            }
+          }
+        }
       }
     }
-    const int64_t at0 = first + int64_t(tid) * PER;  // load i's first logit: + i * kThreads * PER
-    auto each = [&](auto f) {  // f(logit, index) of the thread's logits
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i) {
-        const int64_t at = at0 + int64_t(i) * kThreads * PER;
-        if (at >= 0 && at + PER <= a.vocab) {
-#pragma unroll
-          for (int e = 0; e < PER; ++e) f(clean(widen(x[i][e])), int(at) + e);
-        } else {
-#pragma unroll
-          for (int e = 0; e < PER; ++e)
-            if (at + e >= 0 && at + e < a.vocab) f(clean(widen(x[i][e])), int(at + e));
-        }
+    auto value = [&](int i, int e) {  // logit e of load i
+      if constexpr (sizeof(T) == 4) {
+        return __uint_as_float(x[i][e]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        return __half2float(__ushort_as_half(uint16_t(x[i][e / 2] >> (16 * (e & 1)))));
+      } else {
+        return __uint_as_float(e & 1 ? x[i][e / 2] & 0xffff0000u : x[i][e / 2] << 16);
       }
     };
     // the thread's maximum, the chunk's, and the chunk's sum
     float mx = -INFINITY;
-    each([&](float v, int) { mx = fmaxf(mx, v); });
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) x[i][w] = clean(x[i][w], T());
+#pragma unroll
+      for (int e = 0; e < PER; ++e) mx = fmaxf(mx, value(i, e));
+    }
     float m = mx;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) s_red[warp] = m;
     if (tid == 0) sh.count = 0;
-    __syncthreads();
+    const uint32_t limit = nth_value(value_key(mx), a.n, &sh);  // synchronises
     m = s_red[0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_red[w]);
     float sum = 0.f;
-    int lowest = -1;  // index of the thread's first logit that equals its maximum
     if (m != -INFINITY) {
-      each([&](float v, int i) {
-        sum += __expf(v - m);
-        if (v == mx && lowest < 0) lowest = i;
-      });
-    } else {
-      each([&](float, int i) {
-        if (lowest < 0) lowest = i;
-      });
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+        for (int e = 0; e < PER; ++e) sum += __expf(value(i, e) - m);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_sum[warp] = sum;
-    const unsigned long long mine = lowest >= 0 ? make_key(mx, uint32_t(lowest)) : 0ull;
-    const unsigned long long bound = nth_maximum(mine, a.n, &sh);  // synchronises
+    // Threads whose maximum reaches the n-th largest one hold the n largest logits.  Where equal
+    // maxima make them more than n, those of the lowest indexes count.
+    const bool holds = value_key(mx) >= limit;
+    const float floor_value = key_value(limit);
+    auto each = [&](auto f) {  // f(key) of the thread's logits at or above the limit: few
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          const float v = value(i, e);
+          if (v >= floor_value) {
+            const int64_t at = at0 + int64_t(i) * kThreads * PER + e;
+            if (at >= 0 && at < a.vocab) f(make_key(v, uint32_t(at)));
+          }
+        }
+      }
+    };
+    unsigned long long bound = static_cast<unsigned long long>(limit) << 32;
+    if (__syncthreads_count(holds) > a.n) {
+      unsigned long long mine = 0ull;
+      if (holds) each([&](unsigned long long k) { mine = k > mine ? k : mine; });
+      bound = nth_maximum(mine, a.n, &sh);
+    }
     if (tid == 0) {
       float total = 0.f;
       for (int w = 0; w < kWarps; ++w) total += s_sum[w];
       a.part[int64_t(row) * a.chunks + chunk] = make_float2(m, total);
     }
-    if (mine != 0 && mine >= bound) {
-      each([&](float v, int i) {
-        const unsigned long long k = make_key(v, uint32_t(i));
+    if (holds) {
+      each([&](unsigned long long k) {
         if (k >= bound) s_list[atomicAdd(&sh.count, 1)] = k;
       });
     }
