@@ -30,9 +30,7 @@ namespace kcmm {
 namespace dev {
 namespace {
 
-constexpr int kSelectThreads = 1024;
-constexpr int kSelectWarps = kSelectThreads / 32;
-static_assert(kSelectWarps == 32, "a warp reduces over the warps");
+constexpr int kFewKeys = 256;  // ranked one against all instead of by another histogram
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
 constexpr int kSliceTokens = 4096;
@@ -68,18 +66,39 @@ struct Counts {
   int gt_lo, eq_lo;  // those among the slots below the budget
 };
 
+// CLUSTER: several CTAs share a row; a single CTA's barriers cost a third of a cluster's.
+template <int kSelectThreads, bool CLUSTER>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictArgs a) {
+  constexpr int kSelectWarps = kSelectThreads / 32;
+  static_assert(kSelectWarps <= 32 && kBins % (2 * kSelectThreads) == 0, "a warp sums the warps");
+  constexpr int kPairs = kBins / 2 / kSelectThreads;  // bin pairs of a thread
   __shared__ __align__(8) int s_hist[kBins];
   __shared__ int4 s_range[kSelectWarps], s_total;
   extern __shared__ uint32_t s_keys[];
   __shared__ Counts s_warp[kSelectWarps];
   __shared__ Counts s_cta;
   __shared__ int s_scan[kSelectWarps];
-  __shared__ int s_digit, s_above;
+  __shared__ int s_digit, s_above, s_in_bin, s_few;
+  __shared__ uint32_t s_list[kFewKeys], s_threshold;
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+  const int C = CLUSTER ? int(cluster.num_blocks()) : 1;
+  const int rank = CLUSTER ? int(cluster.block_rank()) : 0;
+  auto sync = [&] {
+    if constexpr (CLUSTER) {
+      cluster.sync();
+    } else {
+      __syncthreads();
+    }
+  };
+  auto of_rank = [&](auto *x, int r) {  // CTA r's copy of a shared variable
+    if constexpr (CLUSTER) {
+      return cluster.map_shared_rank(x, r);
+    } else {
+      return x;
+    }
+  };
   const int b = blockIdx.z, g = blockIdx.y, row = b * a.kv_heads + g;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n = max(a.seq_lens[b], 0);
@@ -140,18 +159,18 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
   __syncthreads();
   if (warp == 0) {
-    const int4 r = s_range[lane];
+    const int4 r = lane < kSelectWarps ? s_range[lane] : make_int4(-1, 0, 0, 0);
     kmin = __reduce_min_sync(0xffffffffu, uint32_t(r.x));
     kmax = __reduce_max_sync(0xffffffffu, uint32_t(r.y));
     held = __reduce_add_sync(0xffffffffu, r.z);
     if (lane == 0) s_total = make_int4(int(kmin), int(kmax), held, 0);
   }
-  cluster.sync();
+  sync();
   kmin = 0xffffffffu;
   kmax = 0;
   held = 0;
   for (int r = 0; r < C; ++r) {
-    const int4 t = *cluster.map_shared_rank(&s_total, r);
+    const int4 t = *of_rank(&s_total, r);
     kmin = min(kmin, uint32_t(t.x));
     kmax = max(kmax, uint32_t(t.y));
     held += t.z;
@@ -186,39 +205,75 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
           atomicAdd(&s_hist[bin], 1);
         }
       }
-      cluster.sync();
-      // Bins from the top: thread t has bins 2047 - 2t and 2046 - 2t, all CTAs' sums.
-      const int top = kBins - 1 - 2 * tid;
-      int c0 = 0, c1 = 0;
-      for (int r = 0; r < C; ++r) {
-        const int2 h = *reinterpret_cast<const int2 *>(cluster.map_shared_rank(s_hist, r) + top - 1);
-        c0 += h.y;
-        c1 += h.x;
+      sync();
+      // Bins from the top: thread t has the 2 kPairs bins below kBins - 2 kPairs t, all CTAs' sums.
+      const int top = kBins - 2 * kPairs * tid;
+      int2 c[kPairs];  // c[i]: bins top - 2i - 2 (x) and top - 2i - 1 (y)
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        c[i] = make_int2(0, 0);
+        for (int r = 0; r < C; ++r) {
+          const int2 h = *reinterpret_cast<const int2 *>(of_rank(s_hist, r) + top - 2 * i - 2);
+          c[i].x += h.x;
+          c[i].y += h.y;
+        }
+        mine += c[i].x + c[i].y;
       }
-      int sum = c0 + c1;
+      int sum = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int x = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += x;
       }
       if (lane == 31) s_scan[warp] = sum;
-      cluster.sync();  // every CTA has read this one's histogram
-      const int other = s_scan[lane];  // of the kSelectWarps = 32 warps
-      int above = lane < warp ? other : 0;
-      above = __reduce_add_sync(0xffffffffu, above) + sum - c0 - c1;  // keys above these bins
-      if (above < want && above + c0 >= want) {
-        s_digit = top;
-        s_above = above;
-      } else if (above + c0 < want && above + c0 + c1 >= want) {
-        s_digit = top - 1;
-        s_above = above + c0;
+      sync();  // every CTA has read this one's histogram
+      int above = lane < warp ? s_scan[lane] : 0;
+      above = __reduce_add_sync(0xffffffffu, above) + sum - mine;  // keys above these bins
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int n_bin = e == 0 ? c[i].y : c[i].x;
+          if (above < want && above + n_bin >= want) {
+            s_digit = top - 2 * i - 1 - e;
+            s_above = above;
+            s_in_bin = n_bin;
+          }
+          above += n_bin;
+        }
       }
       for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
+      if (tid == 0) s_few = 0;
       __syncthreads();
       want -= s_above;
       const uint32_t base = lo + (uint32_t(s_digit) << shift);
       hi = min(hi, base + ((1u << shift) - 1));
       lo = base;
+      if (!CLUSTER && lo != hi && s_in_bin <= kFewKeys) {
+        // few keys are left: each is ranked against all
+        for (int i = begin + tid; i < end; i += kSelectThreads) {
+          const uint32_t k = key_of(i);
+          if (k >= lo && k <= hi) s_list[atomicAdd(&s_few, 1)] = k;
+        }
+        __syncthreads();
+        const int few = s_few;
+        if (tid < few) {
+          const uint32_t k = s_list[tid];
+          int larger = 0, equal = 0;
+          for (int i = 0; i < few; ++i) {
+            larger += s_list[i] > k;
+            equal += s_list[i] == k;
+          }
+          if (larger < want && larger + equal >= want) {  // equal keys write the same
+            s_threshold = k;
+            s_above = larger;
+          }
+        }
+        __syncthreads();
+        want -= s_above;
+        lo = hi = s_threshold;
+      }
     }
     threshold = lo;
   }
@@ -243,16 +298,16 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   if (lane == 0) s_warp[warp] = c;
   __syncthreads();
   if (warp == 0) {
-    const Counts w = s_warp[lane];
+    const Counts w = lane < kSelectWarps ? s_warp[lane] : Counts{0, 0, 0, 0};
     const Counts t = {__reduce_add_sync(0xffffffffu, w.gt), __reduce_add_sync(0xffffffffu, w.eq),
                       __reduce_add_sync(0xffffffffu, w.gt_lo),
                       __reduce_add_sync(0xffffffffu, w.eq_lo)};
     if (lane == 0) s_cta = t;
   }
-  cluster.sync();
+  sync();
   int gt = 0, eq = 0, gt_lo = 0, eq_lo = 0;  // gt, eq: before this warp's segment
   for (int r = 0; r < C; ++r) {
-    const Counts t = *cluster.map_shared_rank(&s_cta, r);
+    const Counts t = *of_rank(&s_cta, r);
     if (r < rank) {
       gt += t.gt;
       eq += t.eq;
@@ -287,8 +342,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     eq += __popc(eqs);
   }
   if (rank == 0 && tid == 0) mv.count[0] = moves;
-  __threadfence();
-  cluster.sync();  // the lists are complete, and nothing past the budget is read again
+  sync();  // the lists are complete, and nothing past the budget is read again
 
   // ---- weights and positions of the kept slots; the slots past them weigh 0 --------------
   for (int i = begin + tid; i < end; i += kSelectThreads) {
@@ -301,7 +355,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
       w_out[i] = 0.f;
     }
   }
-  cluster.sync();
+  sync();
   for (int j = rank * kSelectThreads + tid; j < moves; j += C * kSelectThreads) {
     const int d = __ldcg(mv.dst + j);
     w_out[d] = __ldcg(mv.w + j);
@@ -326,9 +380,8 @@ __device__ __forceinline__ int64_t slot_bytes(const EvictArgs &a, int b, int g, 
   return int64_t(off) + (int64_t(in) * a.kv_heads + g) * row;
 }
 
-// 32 moves a warp: each lane resolves one (slot -> page -> offset, three loads deep), then the
-// warp copies them, 8 vectors a lane
-// in flight before their stores.
+// Up to 32 moves a warp: each lane resolves one (slot -> page -> offset, three loads deep), then
+// the warp copies them, 8 vectors a lane in flight before their stores.
 constexpr int kMovesInFlight = 8;
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArgs a) {
   ptx::grid_dependency_wait();
@@ -337,9 +390,9 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
   const RowMoves mv = row_moves(a, b * a.kv_heads + g);
   const int moves = mv.count[0];
   const int warps = int(gridDim.x) * (kMoveThreads / 32);
-  for (int j0 = (int(blockIdx.x) * (kMoveThreads / 32) + int(threadIdx.x >> 5)) * 32; j0 < moves;
-       j0 += warps * 32) {
-    const int n = min(32, moves - j0);
+  for (int j0 = (int(blockIdx.x) * (kMoveThreads / 32) + int(threadIdx.x >> 5)) * a.warp_moves;
+       j0 < moves; j0 += warps * a.warp_moves) {
+    const int n = min(a.warp_moves, moves - j0);
     int64_t s = 0, d = -1;
     int ts = 0, td = 0;
     if (lane < n) {
@@ -421,30 +474,37 @@ cudaError_t evict_tokens(const EvictArgs &args, cudaStream_t stream) {
     C *= 2;
   a.key_capacity = std::min((a.max_tokens + C - 1) / C, kKeyCapacity);
   const int smem = a.key_capacity * 4;
-  e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const bool small = (a.max_tokens + C - 1) / C <= kSliceTokens;
+  const int threads = small ? 512 : 1024;
+  void (*fn)(const EvictArgs) =
+      C > 1 ? small ? evict_select_kernel<512, true> : evict_select_kernel<1024, true>
+            : small ? evict_select_kernel<512, false> : evict_select_kernel<1024, false>;
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
     scratch.release(stream);
     return e;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(C, a.kv_heads, a.batch);
-  cfg.blockDim = dim3(kSelectThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = C;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, evict_select_kernel, a);
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = C;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = pdl_enabled() ? attr : attr + 1;
+  cfg.numAttrs = (pdl_enabled() ? 1 : 0) + (C > 1 ? 1 : 0);
+  e = cudaLaunchKernelEx(&cfg, fn, a);
   if (e == cudaSuccess) {
     // enough warps for every SM, none for moves that cannot be
     const int most = std::min(a.budget, std::max(a.max_tokens - a.budget, 1));
-    const int per = kMoveThreads;  // 32 a warp
+    // 8 a warp while that leaves warps idle
+    a.warp_moves = int64_t(rows) * most <= int64_t(device_sm_count()) * 64 * 8 ? 8 : 32;
+    const int per = kMoveThreads / 32 * a.warp_moves;
     const int want = std::max(1, 8 * device_sm_count() / rows);
     const int grid = std::min((most + per - 1) / per, want);
     e = launch_pdl(evict_move_kernel, dim3(grid, a.kv_heads, a.batch), dim3(kMoveThreads), 0,

@@ -65,42 +65,59 @@ struct GroupScale {
   float s, inv;
   int kind;  // 0: the codes are 0; 1: quotients through 1/s; 2: s is too small or large for that
 };
+// max / 7 by the reciprocal: the product's error is under half a unit of 24 bits, and a value
+// of 11 bits over 7 lies 2^-13 or more from where bf16 rounding turns, unless it lies on it;
+// then the product rounds to it.
 template <typename T>
 __device__ __forceinline__ GroupScale group_scale(uint32_t mag) {
   constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   GroupScale r;
-  const __nv_bfloat16 s = __float2bfloat16_rn(__fdiv_rn(widen16<T>(mag), 7.f));
-  r.bits = mag >= kInf ? 0x7fc0u : uint32_t(__bfloat16_as_ushort(s));
-  r.s = __bfloat162float(s);
-  const bool plain = r.s > 1e-30f && r.s < 1e30f;
-  r.inv = plain ? __frcp_rn(r.s) : 0.f;
+  const float mx = widen16<T>(mag);
+  const bool plain = mx > 1e-28f && mx < 1e30f;
+  float s = mx * (1.f / 7.f);
+  if (!plain) s = __fdiv_rn(mx, 7.f);
+  const __nv_bfloat16 rounded = __float2bfloat16_rn(s);
+  r.bits = mag >= kInf ? 0x7fc0u : uint32_t(__bfloat16_as_ushort(rounded));
+  r.s = __bfloat162float(rounded);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.inv) : "f"(r.s));
   r.kind = mag >= kInf || r.s == 0.f ? 0 : plain ? 1 : 2;
   return r;
 }
 
-// code + 8 of a value, in the low 4 bits of 0x4b400000 + code + 8.  The quotient is corrected
-// once by its exact remainder (Markstein's division step): half-way quotients come out exact,
-// and all others of a value of 11 bits by a scale of 8 lie 2^-14 or more away from half-way,
-// so that rounding to even on adding 1.5 2^23 gives the code of the exact quotient.
-__device__ __forceinline__ uint32_t code_bits(float x, const GroupScale &r) {
+// code + 8 of N values, in the low 4 bits of 0x4b400000 + code + 8.  The quotient by the
+// approximate reciprocal is corrected once by its exact remainder (Markstein's division step):
+// half-way quotients come out exact, and all others of a value of 11 bits by a scale of 8 lie
+// 2^-14 or more away from half-way, so that rounding to even on adding 1.5 2^23 gives the
+// code of the exact quotient.
+template <int N>
+__device__ __forceinline__ void code_bits(const float *x, const GroupScale &r, uint32_t *n) {
   constexpr float kRound = 12582920.f;  // 1.5 2^23 + 8
-  float q;
   if (r.kind == 1) {
-    q = x * r.inv;
-    q = fmaf(fmaf(-q, r.s, x), r.inv, q);
-  } else if (r.kind == 2) {
-    q = fminf(fmaxf(__fdiv_rn(x, r.s), -7.f), 7.f);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float q = x[e] * r.inv;
+      n[e] = __float_as_uint(fmaf(fmaf(-q, r.s, x[e]), r.inv, q) + kRound);
+    }
   } else {
-    q = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float q = r.kind == 0 ? 0.f : fminf(fmaxf(__fdiv_rn(x[e], r.s), -7.f), 7.f);
+      n[e] = __float_as_uint(q + kRound);
+    }
   }
-  return __float_as_uint(q + kRound);
+}
+template <typename T, int N>
+__device__ __forceinline__ void widen_all(const uint32_t *w, float *x) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) x[e] = widen16<T>((w[e / 2] >> (16 * (e & 1))) & 0xffffu);
 }
 
 // Nibbles of 4 codes, code i at bit step * i, from code_bits' words.
 template <int STEP>
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   constexpr uint32_t k = 0x4b400000u;
-  return (a - k) + ((b - k) << STEP) + ((c - k) << (2 * STEP)) + ((d - k) << (3 * STEP));
+  return a + (b << STEP) + (c << (2 * STEP)) + (d << (3 * STEP)) -
+         k * (1u + (1u << STEP) + (1u << (2 * STEP)) + (1u << (3 * STEP)));
 }
 // A K word: dims 8c + {0..7}, dim 2i in nibble i, 2i + 1 in nibble i + 4.
 __device__ __forceinline__ uint32_t pack_k(const uint32_t *n) {
@@ -243,9 +260,9 @@ __global__ void __launch_bounds__(kRowsThreads) kv4_append_kernel(const Kv4RowsA
             m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
             const GroupScale s = group_scale<T>(larger_half(m));
             uint32_t n[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              n[e] = code_bits(widen16<T>((x[e / 2] >> (16 * (e & 1))) & 0xffffu), s);
+            float f[8];
+            widen_all<T, 8>(x, f);
+            code_bits<8>(f, s, n);
             codes[jj * 2 + w] = pack_k(n);
             scales[w * NG + j] = s.bits;
           }
@@ -262,11 +279,11 @@ __global__ void __launch_bounds__(kRowsThreads) kv4_append_kernel(const Kv4RowsA
             m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 16));
             const GroupScale s0 = group_scale<T>(m & 0xffffu), s1 = group_scale<T>(m >> 16);
             uint32_t n0[4], n1[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              n0[e] = code_bits(widen16<T>((x0[e / 2] >> (16 * (e & 1))) & 0xffffu), s0);
-              n1[e] = code_bits(widen16<T>((x1[e / 2] >> (16 * (e & 1))) & 0xffffu), s1);
-            }
+            float f[4];
+            widen_all<T, 4>(x0, f);
+            code_bits<4>(f, s0, n0);
+            widen_all<T, 4>(x1, f);
+            code_bits<4>(f, s1, n1);
             codes[jj * 2 + w] = pack4<4>(n0[0], n0[1], n0[2], n0[3]) |
                                 (pack4<4>(n1[0], n1[1], n1[2], n1[3]) << 16);
             scales[2 * j + w] = s0.bits | (s1.bits << 16);
@@ -308,9 +325,9 @@ __global__ void __launch_bounds__(kRowsThreads) kv4_append_kernel(const Kv4RowsA
     if (!live) continue;
     const GroupScale s = group_scale<T>(larger_half(m));
     uint32_t n[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      n[e] = code_bits(widen16<T>((x[e / 2] >> (16 * (e & 1))) & 0xffffu), s);
+    float f[8];
+    widen_all<T, 8>(x, f);
+    code_bits<8>(f, s, n);
     const int j = piece / 4, q = piece % 4;
     uint8_t *chunk = region + at;
     if (!tile.is_v) {

@@ -159,6 +159,7 @@ struct EvictArgs {
   int32_t *diag;
   int32_t *scratch;  // filled by the launcher
   int key_capacity;  // keys that a CTA holds in shared memory
+  int warp_moves;    // moves of a warp at a time
 };
 cudaError_t evict_tokens(const EvictArgs &a, cudaStream_t stream);
 
