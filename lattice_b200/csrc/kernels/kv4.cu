@@ -43,12 +43,15 @@ constexpr int kGroup = kKv4Group;
 // layout: its source loads are whole 32-byte sectors, its code stores one 16-byte vector a
 // pair of groups, and no byte goes through shared memory.  Other tiles (decode steps, the
 // ends of a chunk) go row by row, 8 values a lane.  Both are bound by HBM for long inputs
-// and by the latency of slot -> offset -> row for short ones.
+// (16,384 tokens of 8 heads of 128: 179 us row by row, 45 by units, 3.8 TB/s) and by the
+// latency of slot -> offset -> row for short ones (64 tokens: 4.4 us).
 
 constexpr int kRowsThreads = 128;
-// Rows of a warp's tile below kTileTokens tokens: decode steps, whose rows lie apart.
+// A tile has a unit's 16 rows where that leaves every SM kTileWarps warps, else kFewRows: at 8
+// heads 16 rows take 9.2, 10.1, 11.1 and 45 us for 512, 1024, 2048 and 16,384 tokens, 2 rows
+// 5.4, 8.1, 12.9 and 81.  1 and 4 rows take 4.5 and 5.6 us for 64 tokens, 2 rows 4.4.
+constexpr int kTileWarps = 10;
 constexpr int kFewRows = 2;
-constexpr int kTileTokens = 512;
 
 template <typename T>
 __device__ __forceinline__ float widen16(uint32_t bits) {
@@ -450,9 +453,19 @@ __global__ void __launch_bounds__(kRowsThreads) kv4_read_kernel(const Kv4RowsArg
 // --- decode ----------------------------------------------------------------------------
 
 constexpr int kWarps = 4;
-constexpr int kMinRange = 16;       // units of a CTA
-constexpr int kMaxPieces = 32;      // of a sequence, about: what its last CTA merges
-constexpr int kStages = 3;            // steps of a warp's ring
+// Query heads of a CTA, the columns of the mma.  More heads of a kv head become more CTAs, that
+// unpack the same codes again, from L2: two tiles of 16 in a CTA's registers instead took
+// 28.4 us against 23.1 for 16 sequences of up to 2000 tokens with 16 heads on 1 (38.0 against
+// 36.6 for 32 of up to 4096 with 64 on 4, 44.8 against 33.3 at heads of 256).
+constexpr int kHeads = 8;
+// Units of a CTA, at least.  8 leave more pieces to merge, 32 fewer CTAs: 17.4 and 16.7 us
+// against 15.8 for 4 sequences of up to 700 tokens, 19.1 and 27.6 against 20.9 for 8 of up to
+// 2000.
+constexpr int kMinRange = 16;
+// Pieces of a sequence, about, which its last CTA merges: 16 and 64 took 26.2 and 22.6 us
+// against 21.2 for one of 32,768 tokens.
+constexpr int kMaxPieces = 32;
+constexpr int kStages = 3;  // steps of a warp's ring; 2 are as fast
 constexpr uint64_t kWaitLimitNs = 1000000000ull;  // a chunk that has not landed in 1 s is
                                                   // reported, never waited on forever
 
@@ -522,11 +535,10 @@ __device__ __forceinline__ float bf16_lo(uint32_t x) { return __uint_as_float(x 
 __device__ __forceinline__ float bf16_hi(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
 // Units that a warp takes at a time: two give its loads, matrix products and shuffles
-// something to overlap with (see the loop), as long as the registers of both fit.
-__host__ __device__ constexpr int units_at_a_time(int D, int NT) { return D * NT <= 128 ? 2 : 1; }
-__host__ __device__ constexpr int ctas_per_sm(int D, int NT) {
-  return D * NT <= 128 ? 4 : D * NT <= 256 ? 2 : 1;
-}
+// something to overlap with (21.2 against 23.3 us for one sequence of 32,768 tokens, 8 kv
+// heads of 128; 58.6 against 59.1 for the batch below), as long as the registers of both fit.
+__host__ __device__ constexpr int units_at_a_time(int D) { return D <= 128 ? 2 : 1; }
+__host__ __device__ constexpr int ctas_per_sm(int D) { return D <= 128 ? 4 : 2; }
 
 // V's scales enter P as f16: two positive bf16 a word, their exponents lowered by a bias
 // common to the warp (in units of bf16's exponent bit), those below f16's range to about 0.
@@ -564,19 +576,23 @@ __device__ __forceinline__ void load_words(uint32_t *r, const unsigned char *p, 
 
 // Work split.  The units of all sequences, end to end, are cut into equal ranges, one for each
 // CTA x of a kv head (and head tile) y = blockIdx.y: lengths differ by a factor of 8 within
-// a batch, and CTAs of one (sequence, split) each left the Llama-3-8B decode batch at 60 us
-// where equal shares take 45.  A sequence inside one range is finished there; the pieces of one that
-// several CTAs share go to scratch and the last CTA to finish merges them.
+// a batch, and CTAs of one (sequence, split) each took 60 us for the Llama-3-8B decode batch
+// (64 sequences of 512 to 4096 tokens, 8 kv heads of 128) where equal shares take 56.  A sequence
+// inside one range is finished there; the pieces of one that several CTAs share go to scratch
+// and the last CTA to finish merges them.
+//
+// That batch is bound by issue slots, at 3.0 TB/s: 16 tokens of a head cost about 330
+// warp instructions, half of them unpacking and scaling codes (matrix products on 8-bit
+// codes instead needed as many), and 4 CTAs an SM leave few slots idle.  Few sequences are bound by latency: lengths -> table -> offset -> chunk -> merge.
 //
 // A CTA's warps take every kWarps-th step of NU units of its piece.  Each warp runs its own
 // ring of kStages steps: a lane issues a unit's K and V chunks as two bulk copies, the whole
 // warp reads its operands from shared memory.
-template <typename T, int D, int NT, bool SCORES>
-__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
+template <typename T, int D, bool SCORES>
+__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
     kv4_decode_kernel(const Kv4Params p) {
   constexpr int NG = D / kGroup;
-  constexpr int NU = units_at_a_time(D, NT);
-  constexpr int HT = 8 * NT;  // heads of a tile
+  constexpr int NU = units_at_a_time(D);
   constexpr uint32_t kChunk = 9 * D;
   extern __shared__ __align__(128) unsigned char kv4_smem[];
   __shared__ uint64_t s_bar[kWarps * kStages];
@@ -589,8 +605,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
   // query heads h with h * hkv / hq == kvh
   const int group_lo = int((uint32_t(kvh) * uint32_t(p.hq) + p.hkv - 1) / uint32_t(p.hkv));
   const int group_hi = int((uint32_t(kvh + 1) * uint32_t(p.hq) + p.hkv - 1) / uint32_t(p.hkv));
-  const int lo = group_lo + ht * HT;
-  const int G = min(group_hi - lo, HT);
+  const int lo = group_lo + ht * kHeads;
+  const int G = min(group_hi - lo, kHeads);
   if (G <= 0) return;
 
   // ---- this CTA's range of units, and the sequence it starts in ---------------------------
@@ -671,20 +687,17 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
   }
 
   // ---- the query rows (used below; loaded first, their latency overlaps the addresses') ----
-  __align__(16) T q_raw[NT][NG][8];
+  __align__(16) T q_raw[NG][8];
+  const T *src = static_cast<const T *>(p.q) + int64_t(b) * p.q_sb +
+                 int64_t(lo + min(g, G - 1)) * p.q_sh + c * 8;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const T *src = static_cast<const T *>(p.q) + int64_t(b) * p.q_sb +
-                   int64_t(lo + min(nt * 8 + g, G - 1)) * p.q_sh + c * 8;
+  for (int j = 0; j < NG; ++j) {
+    if (p.q_vec) {
+      *reinterpret_cast<uint4 *>(q_raw[j]) =
+          *reinterpret_cast<const uint4 *>(src + j * kGroup);
+    } else {
 #pragma unroll
-    for (int j = 0; j < NG; ++j) {
-      if (p.q_vec) {
-        *reinterpret_cast<uint4 *>(q_raw[nt][j]) =
-            *reinterpret_cast<const uint4 *>(src + j * kGroup);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) q_raw[nt][j][e] = src[j * kGroup + e];
-      }
+      for (int e = 0; e < 8; ++e) q_raw[j][e] = src[j * kGroup + e];
     }
   }
 
@@ -743,48 +756,40 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
   // ---- Q as the B operand (columns = heads), scaled per head by a power of two --------
   // f16 for both input types: with the row's largest magnitude brought into [64, 128) every
   // bf16 or f16 value is exact down to 2^-20 of that, and nothing overflows.
-  uint32_t qb[NT][NG][4];
-  float s_scale[NT][2];
+  uint32_t qb[NG][4];
+  float s_scale[2];
+  const int h = g;
+  float x[NG][8];
+  float mx = 0.f;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int h = nt * 8 + g;
-    float x[NG][8];
-    float mx = 0.f;
+  for (int j = 0; j < NG; ++j) {
 #pragma unroll
-    for (int j = 0; j < NG; ++j) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[j][e] = h < G ? ptx::to_f32(q_raw[nt][j][e]) : 0.f;
-        mx = fmaxf(mx, fabsf(x[j][e]));
-      }
+    for (int e = 0; e < 8; ++e) {
+      x[j][e] = h < G ? ptx::to_f32(q_raw[j][e]) : 0.f;
+      mx = fmaxf(mx, fabsf(x[j][e]));
     }
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const int ex = max(int((__float_as_uint(mx) >> 23) & 255u) - 127, -100);
-    const float up = __uint_as_float(uint32_t(127 + 6 - ex) << 23);
-    const float down = __uint_as_float(uint32_t(127 - 6 + ex) << 23) * p.scale_log2;
-#pragma unroll
-    for (int j = 0; j < NG; ++j) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        qb[nt][j][i] = ptx::Mma<__half>::pack(x[j][2 * i] * up, x[j][2 * i + 1] * up);
-    }
-    // this lane's score columns are heads 2c and 2c+1
-    s_scale[nt][0] = __shfl_sync(0xffffffffu, down, (2 * c) * 4);
-    s_scale[nt][1] = __shfl_sync(0xffffffffu, down, (2 * c + 1) * 4);
   }
+  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+  const int ex = max(int((__float_as_uint(mx) >> 23) & 255u) - 127, -100);
+  const float up = __uint_as_float(uint32_t(127 + 6 - ex) << 23);
+  const float down = __uint_as_float(uint32_t(127 - 6 + ex) << 23) * p.scale_log2;
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      qb[j][i] = ptx::Mma<__half>::pack(x[j][2 * i] * up, x[j][2 * i + 1] * up);
+  }
+  // this lane's score columns are heads 2c and 2c+1
+  s_scale[0] = __shfl_sync(0xffffffffu, down, (2 * c) * 4);
+  s_scale[1] = __shfl_sync(0xffffffffu, down, (2 * c + 1) * 4);
 
-  float o[NT][2 * NG][4];  // O transposed: rows = dims, columns = heads
+  float o[2 * NG][4];  // O transposed: rows = dims, columns = heads
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int i = 0; i < 2 * NG; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
-  float m[NT][2], l[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
-  }
+  for (int i = 0; i < 2 * NG; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[2], l[2];
+  m[0] = m[1] = -INFINITY;
+  l[0] = l[1] = 0.f;
   int bias = -1;               // exponent bias of V's scales inside P; -1 before the first unit
   uint32_t minus_bias = 0;     // two of -bias << 7, as 16-bit integers
   uint32_t scale_limit = 0;    // largest scale (bf16 bits) that the bias admits
@@ -814,7 +819,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
     }
     const unsigned char *chunk = ring + st * NU * 2 * kChunk;
     // ---- S = Q K^T, transposed: rows = tokens, columns = heads -----------------------------
-    float s[NU][NT][4];
+    float s[NU][4];
 #pragma unroll
     for (int r = 0; r < NU; ++r) {
       const unsigned char *kc = chunk + r * 2 * kChunk;
@@ -835,29 +840,24 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
         const uint32_t a1[4] = {low_codes(w0 >> 8, base), low_codes(w1 >> 8, base),
                                 high_codes(w0 >> 8, base), high_codes(w1 >> 8, base)};
         const float k0 = k_scale<NG>(ks, 0, j), k1 = k_scale<NG>(ks, 1, j);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float acc[4];
-          mma_zero(acc, a0, qb[nt][j][0], qb[nt][j][1]);
-          mma_add(acc, a1, qb[nt][j][2], qb[nt][j][3]);
-          float *sr = s[r][nt];
-          if (j == 0) {
-            sr[0] = acc[0] * k0;
-            sr[1] = acc[1] * k0;
-            sr[2] = acc[2] * k1;
-            sr[3] = acc[3] * k1;
-          } else {
-            sr[0] = fmaf(acc[0], k0, sr[0]);
-            sr[1] = fmaf(acc[1], k0, sr[1]);
-            sr[2] = fmaf(acc[2], k1, sr[2]);
-            sr[3] = fmaf(acc[3], k1, sr[3]);
-          }
+        float acc[4];
+        mma_zero(acc, a0, qb[j][0], qb[j][1]);
+        mma_add(acc, a1, qb[j][2], qb[j][3]);
+        float *sr = s[r];
+        if (j == 0) {
+          sr[0] = acc[0] * k0;
+          sr[1] = acc[1] * k0;
+          sr[2] = acc[2] * k1;
+          sr[3] = acc[3] * k1;
+        } else {
+          sr[0] = fmaf(acc[0], k0, sr[0]);
+          sr[1] = fmaf(acc[1], k0, sr[1]);
+          sr[2] = fmaf(acc[2], k1, sr[2]);
+          sr[3] = fmaf(acc[3], k1, sr[3]);
         }
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[r][nt][i] *= s_scale[nt][i & 1];
+      for (int i = 0; i < 4; ++i) s[r][i] *= s_scale[i & 1];
     }
     alignas(16) uint32_t vs[NU][2 * NG];  // V's scales [group][token pair (2c, 2c+1) + 8 i]
 #pragma unroll
@@ -871,11 +871,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
 #pragma unroll
       for (int r = 0; r < NU; ++r) {
         const int nvalid = (units >> r) & 1u ? seq_len - (u + r) * kUnit : 0;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (g >= nvalid) s[r][nt][0] = s[r][nt][1] = -INFINITY;
-          if (g + 8 >= nvalid) s[r][nt][2] = s[r][nt][3] = -INFINITY;
-        }
+        if (g >= nvalid) s[r][0] = s[r][1] = -INFINITY;
+        if (g + 8 >= nvalid) s[r][2] = s[r][3] = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 2 * NG; ++i) {
           const int t = 2 * c + (i & 1) * 8;
@@ -888,14 +885,11 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
       for (int r = 0; r < NU; ++r) {
         if (u + r >= u_end) continue;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int h = nt * 8 + 2 * c + (i & 1);
-            if (h < G)
-              p.scores[(int64_t(b) * p.hq + lo + h) * p.score_stride + (u + r) * kUnit + g +
-                       (i >> 1) * 8] = s[r][nt][i];
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int h = 2 * c + (i & 1);
+          if (h < G)
+            p.scores[(int64_t(b) * p.hq + lo + h) * p.score_stride + (u + r) * kUnit + g +
+                     (i >> 1) * 8] = s[r][i];
         }
       }
     }
@@ -909,14 +903,11 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
       for (int i = 0; i < 2 * NG; i += 2) vmx = __vimax3_u16x2(vmx, vs[r][i], vs[r][i + 1]);
     bool raise = (vmx & 0xffffu) > scale_limit || (vmx >> 16) > scale_limit;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int i = 0; i < 2; ++i) {
+      float mx = fmaxf(s[0][i], s[0][i + 2]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float mx = fmaxf(s[0][nt][i], s[0][nt][i + 2]);
-#pragma unroll
-        for (int r = 1; r < NU; ++r) mx = fmaxf(mx, fmaxf(s[r][nt][i], s[r][nt][i + 2]));
-        raise |= mx > m[nt][i] + 6.f;
-      }
+      for (int r = 1; r < NU; ++r) mx = fmaxf(mx, fmaxf(s[r][i], s[r][i + 2]));
+      raise |= mx > m[i] + 6.f;
     }
     if (__any_sync(0xffffffffu, raise || bias < 0)) {
       uint32_t top = 0;
@@ -940,10 +931,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
         }
         if (__any_sync(0xffffffffu, nan)) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              o[nt][2 * j][i] = o[nt][2 * j + 1][i] = __int_as_float(0x7fc00000);
+          for (int i = 0; i < 4; ++i)
+            o[2 * j][i] = o[2 * j + 1][i] = __int_as_float(0x7fc00000);
         }
       }
       top = __reduce_max_sync(0xffffffffu, top);
@@ -956,43 +945,37 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
         scale_limit = uint32_t(min((bias + kScaleTop + 1) << 7, 0x7f80)) - 1;
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int i = 0; i < 2; ++i) {
+        float mx = m[i];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float mx = m[nt][i];
+        for (int r = 0; r < NU; ++r) mx = fmaxf(mx, fmaxf(s[r][i], s[r][i + 2]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float rr = m[i] == -INFINITY ? 0.f : ptx::fast_exp2(m[i] - mx);
+        m[i] = mx;
+        l[i] *= rr;
 #pragma unroll
-          for (int r = 0; r < NU; ++r) mx = fmaxf(mx, fmaxf(s[r][nt][i], s[r][nt][i + 2]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float rr = m[nt][i] == -INFINITY ? 0.f : ptx::fast_exp2(m[nt][i] - mx);
-          m[nt][i] = mx;
-          l[nt][i] *= rr;
-#pragma unroll
-          for (int d = 0; d < 2 * NG; ++d) {
-            o[nt][d][i] *= rr * vr;
-            o[nt][d][i + 2] *= rr * vr;
-          }
+        for (int d = 0; d < 2 * NG; ++d) {
+          o[d][i] *= rr * vr;
+          o[d][i + 2] *= rr * vr;
         }
       }
     }
     // ---- O += V^T P^T ----------------------------------------------------------------------
     // P as the B operand (rows = tokens, columns = heads) in 11 bits, rounded to 11 bits once
     // more by a group's scales
-    uint32_t pb[NU][NT][2];
+    uint32_t pb[NU][2];
 #pragma unroll
     for (int r = 0; r < NU; ++r) {
+      float x[4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = ptx::fast_exp2(s[r][nt][i] - m[nt][i & 1]);
-          l[nt][i & 1] += x[i];
-        }
-        pb[r][nt][0] = transpose8x8(ptx::Mma<__half>::pack(x[0], x[1]));
-        pb[r][nt][1] = transpose8x8(ptx::Mma<__half>::pack(x[2], x[3]));
+      for (int i = 0; i < 4; ++i) {
+        x[i] = ptx::fast_exp2(s[r][i] - m[i & 1]);
+        l[i & 1] += x[i];
       }
+      pb[r][0] = transpose8x8(ptx::Mma<__half>::pack(x[0], x[1]));
+      pb[r][1] = transpose8x8(ptx::Mma<__half>::pack(x[2], x[3]));
     }
 #pragma unroll
     for (int r = 0; r < NU; ++r) {
@@ -1013,12 +996,9 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
                                 low_codes(w1 >> 8, base), high_codes(w1 >> 8, base)};
         const uint32_t v0 = scales_to_f16(vs[r][2 * j], minus_bias);
         const uint32_t v1 = scales_to_f16(vs[r][2 * j + 1], minus_bias);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const uint32_t b0 = mul2(pb[r][nt][0], v0), b1 = mul2(pb[r][nt][1], v1);
-          mma_add(o[nt][2 * j], a0, b0, b1);
-          mma_add(o[nt][2 * j + 1], a1, b0, b1);
-        }
+        const uint32_t b0 = mul2(pb[r][0], v0), b1 = mul2(pb[r][1], v1);
+        mma_add(o[2 * j], a0, b0, b1);
+        mma_add(o[2 * j + 1], a1, b0, b1);
       }
     }
     __syncwarp();
@@ -1040,8 +1020,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
   __syncthreads();
   lost = s_fail;
   const bool whole = pieces == 1;
-  float *part_o = p.part_o + (int64_t(blockIdx.y) * gridDim.x * 2) * HT * D;
-  float *part_lse = p.part_lse + (int64_t(blockIdx.y) * gridDim.x * 2) * HT;
+  float *part_o = p.part_o + (int64_t(blockIdx.y) * gridDim.x * 2) * kHeads * D;
+  float *part_lse = p.part_lse + (int64_t(blockIdx.y) * gridDim.x * 2) * kHeads;
   auto store = [&](int h, int d, float4 x, float lse) {
     T *dst = static_cast<T *>(p.out) + int64_t(b) * p.o_sb + int64_t(lo + h) * p.o_sh + d;
     dst[0] = ptx::from_f32<T>(x.x);
@@ -1054,31 +1034,28 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
   };
 
   // ---- merge the warps (the rings are free) -----------------------------------------------
-  float *cO = reinterpret_cast<float *>(kv4_smem);  // [kWarps][HT][D]
-  float *cm = cO + kWarps * HT * D;                 // [kWarps][HT]
-  float *cl = cm + kWarps * HT;                     // [kWarps][HT]
+  float *cO = reinterpret_cast<float *>(kv4_smem);  // [kWarps][kHeads][D]
+  float *cm = cO + kWarps * kHeads * D;                 // [kWarps][kHeads]
+  float *cl = cm + kWarps * kHeads;                     // [kWarps][kHeads]
   // f16 scale = bf16 scale * 2^(112 - bias): both exponents are biased, by 127 and 15
   const float v_down = bias < 0 ? 0.f : exp2f(float(bias - 112));
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+  for (int i = 0; i < 2; ++i) {
+    float sum = l[i];
+    sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+    const int h = 2 * c + i;
+    if (g == 0) {
+      cm[warp * kHeads + h] = m[i];
+      cl[warp * kHeads + h] = sum;
+    }
+    if (h < G) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float sum = l[nt][i];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-      const int h = nt * 8 + 2 * c + i;
-      if (g == 0) {
-        cm[warp * HT + h] = m[nt][i];
-        cl[warp * HT + h] = sum;
-      }
-      if (h < G) {
-#pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          *reinterpret_cast<float4 *>(cO + (warp * HT + h) * D + j * kGroup + g * 4) =
-              make_float4(o[nt][2 * j][i] * v_down, o[nt][2 * j][i + 2] * v_down,
-                          o[nt][2 * j + 1][i] * v_down, o[nt][2 * j + 1][i + 2] * v_down);
-        }
+      for (int j = 0; j < NG; ++j) {
+        *reinterpret_cast<float4 *>(cO + (warp * kHeads + h) * D + j * kGroup + g * 4) =
+            make_float4(o[2 * j][i] * v_down, o[2 * j][i + 2] * v_down,
+                        o[2 * j + 1][i] * v_down, o[2 * j + 1][i + 2] * v_down);
       }
     }
   }
@@ -1087,15 +1064,15 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
     const int h = i / (D / 4), d = (i % (D / 4)) * 4;
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, cm[w * HT + h]);
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, cm[w * kHeads + h]);
     float L = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float mw = cm[w * HT + h], lw = cl[w * HT + h];
+      const float mw = cm[w * kHeads + h], lw = cl[w * kHeads + h];
       if (mw == -INFINITY && lw == 0.f) continue;  // the warp saw no token
       const float sc = ptx::fast_exp2(mw - M);
-      const float4 v = *reinterpret_cast<const float4 *>(cO + (w * HT + h) * D + d);
+      const float4 v = *reinterpret_cast<const float4 *>(cO + (w * kHeads + h) * D + d);
       L += lw * sc;
       x.x += v.x * sc;
       x.y += v.y * sc;
@@ -1107,7 +1084,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
     if (whole) {
       if (!lost) store(h, d, x, lse);
     } else {
-      const int64_t row = (int64_t(blockIdx.x) * 2 + slot) * HT + h;
+      const int64_t row = (int64_t(blockIdx.x) * 2 + slot) * kHeads + h;
       *reinterpret_cast<float4 *>(part_o + row * D + d) = x;
       if (d == 0) part_lse[row] = lse;
     }
@@ -1119,10 +1096,10 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
   // the last CTA of a shared sequence merges its pieces
   if (!last_piece(x_first, pieces) || lost) continue;
   // the first piece lies in its CTA's second slot unless it starts that CTA's range
-  const int64_t first_row = (int64_t(x_first) * 2 + (at_first > x_first * range ? 1 : 0)) * HT;
-  auto row_of = [&](int k) { return k == 0 ? first_row : int64_t(x_first + k) * 2 * HT; };
-  float *weight = reinterpret_cast<float *>(kv4_smem);  // [HT][pieces], then [HT] lse
-  float *row_lse = weight + HT * pieces;
+  const int64_t first_row = (int64_t(x_first) * 2 + (at_first > x_first * range ? 1 : 0)) * kHeads;
+  auto row_of = [&](int k) { return k == 0 ? first_row : int64_t(x_first + k) * 2 * kHeads; };
+  float *weight = reinterpret_cast<float *>(kv4_smem);  // [kHeads][pieces], then [kHeads] lse
+  float *row_lse = weight + kHeads * pieces;
   for (int h = warp; h < G; h += kWarps) {
     float M = -INFINITY, sum = 0.f;
     for (int k = lane; k < pieces; k += 32) {
@@ -1161,25 +1138,21 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT))
 
 using Kv4Fn = void (*)(const Kv4Params);
 
-template <typename T, int D, int NT>
-Kv4Fn pick_scores(bool scores) {
-  return scores ? kv4_decode_kernel<T, D, NT, true> : kv4_decode_kernel<T, D, NT, false>;
-}
 template <typename T, int D>
-Kv4Fn pick_tiles(int nt, bool scores) {
-  return nt == 1 ? pick_scores<T, D, 1>(scores) : pick_scores<T, D, 2>(scores);
+Kv4Fn pick_scores(bool scores) {
+  return scores ? kv4_decode_kernel<T, D, true> : kv4_decode_kernel<T, D, false>;
 }
 template <typename T>
-Kv4Fn pick(int D, int nt, bool scores) {
+Kv4Fn pick(int D, bool scores) {
   switch (D) {
-    case 32: return pick_tiles<T, 32>(nt, scores);
-    case 64: return pick_tiles<T, 64>(nt, scores);
-    case 96: return pick_tiles<T, 96>(nt, scores);
-    case 128: return pick_tiles<T, 128>(nt, scores);
-    case 160: return pick_tiles<T, 160>(nt, scores);
-    case 192: return pick_tiles<T, 192>(nt, scores);
-    case 224: return pick_tiles<T, 224>(nt, scores);
-    case 256: return pick_tiles<T, 256>(nt, scores);
+    case 32: return pick_scores<T, 32>(scores);
+    case 64: return pick_scores<T, 64>(scores);
+    case 96: return pick_scores<T, 96>(scores);
+    case 128: return pick_scores<T, 128>(scores);
+    case 160: return pick_scores<T, 160>(scores);
+    case 192: return pick_scores<T, 192>(scores);
+    case 224: return pick_scores<T, 224>(scores);
+    case 256: return pick_scores<T, 256>(scores);
     default: return nullptr;
   }
 }
@@ -1211,7 +1184,8 @@ Kv4RowsFn pick_rows(int D, bool append, bool tiles) {
 }
 
 cudaError_t launch_rows(const Kv4RowsArgs &a, bool append, cudaStream_t stream) {
-  const bool tiles = a.num_tokens >= kTileTokens;
+  const bool tiles =
+      int64_t(a.num_tokens / kUnit) * 2 * a.kv_heads >= int64_t(kTileWarps) * device_sm_count();
   const Kv4RowsFn fn = a.dtype == Dtype::BF16
                            ? pick_rows<__nv_bfloat16>(a.head_dim, append, tiles)
                            : pick_rows<__half>(a.head_dim, append, tiles);
@@ -1235,10 +1209,9 @@ cudaError_t kv4_decode_attention(const DecodeArgs &a, const DecodeWeights &w,
                                  cudaStream_t stream) {
   const int D = a.head_dim;
   const int g_max = (a.num_q_heads + a.kv_heads - 1) / a.kv_heads;
-  const int nt = g_max <= 8 ? 1 : 2;
   const bool scores = w.w_out != nullptr;
-  const Kv4Fn fn = a.dtype == Dtype::BF16 ? pick<__nv_bfloat16>(D, nt, scores)
-                                          : pick<__half>(D, nt, scores);
+  const Kv4Fn fn = a.dtype == Dtype::BF16 ? pick<__nv_bfloat16>(D, scores)
+                                          : pick<__half>(D, scores);
   if (!fn) return cudaErrorNotSupported;
   Kv4Params p = {};
   p.q = a.q;
@@ -1263,16 +1236,15 @@ cudaError_t kv4_decode_attention(const DecodeArgs &a, const DecodeWeights &w,
   p.o_sh = a.out_stride_head ? a.out_stride_head : D;
   p.bt_stride = a.tables_stride ? a.tables_stride : a.max_blocks_per_seq;
   p.q_vec = ((reinterpret_cast<uintptr_t>(a.q) & 15) | (p.q_sb & 7) | (p.q_sh & 7)) == 0;
-  p.n_head_tiles = (g_max + 8 * nt - 1) / (8 * nt);
+  p.n_head_tiles = (g_max + kHeads - 1) / kHeads;
 
-  // One wave of CTAs, every one with its share of the units of one kv head (head tile); where
-  // there are many of those, about four waves of smaller shares.
-  const int slots = device_sm_count() * ctas_per_sm(D, nt), Y = a.kv_heads * p.n_head_tiles;
-  const int X = Y * 4 <= slots
-                    ? int(std::min<int64_t>(slots / Y, int64_t(kMaxPieces) * a.batch))
-                    : (4 * slots + Y - 1) / Y;
+  // One wave of CTAs, every one with its share of the units of one kv head's (head tile's)
+  // tokens.  Four waves of smaller shares where those are many lost: 96 kv heads of 256, 4
+  // sequences of 100 to 2000 tokens 73 against 45 us, of 2000 to 6000 155 against 121.
+  const int slots = device_sm_count() * ctas_per_sm(D), Y = a.kv_heads * p.n_head_tiles;
+  const int X = int(std::min<int64_t>(std::max(1, slots / Y), int64_t(kMaxPieces) * a.batch));
 
-  const size_t rows = size_t(a.batch) * a.num_q_heads, slots_used = size_t(X) * Y * 2 * 8 * nt;
+  const size_t rows = size_t(a.batch) * a.num_q_heads, slots_used = size_t(X) * Y * 2 * kHeads;
   const int max_tokens = a.max_blocks_per_seq * a.block_size;
   p.score_stride = max_tokens;
   // piece outputs, their log-sum-exp, and for the weights the rows' own and the scores
@@ -1288,10 +1260,10 @@ cudaError_t kv4_decode_attention(const DecodeArgs &a, const DecodeWeights &w,
   p.lse = reinterpret_cast<float *>(base + row_at);
   p.scores = scores ? reinterpret_cast<float *>(base + scores_at) : nullptr;
   p.counters = scratch.counters;
-  const int nu = units_at_a_time(D, nt);
+  const int nu = units_at_a_time(D);
   const size_t smem = std::max({size_t(kWarps) * kStages * nu * 18 * D,  // rings
-                                size_t(kWarps) * 8 * nt * (D + 2) * 4,   // warps' results
-                                size_t(8 * nt) * (X + 1) * 4});          // pieces' weights
+                                size_t(kWarps) * kHeads * (D + 2) * 4,   // warps' results
+                                size_t(kHeads) * (X + 1) * 4});          // pieces' weights
   e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e == cudaSuccess) e = launch_pdl(fn, dim3(X, Y), dim3(kWarps * 32), smem, stream, p);
   if (e == cudaSuccess && scores) {
