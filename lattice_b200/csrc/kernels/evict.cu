@@ -79,10 +79,12 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   __shared__ Counts s_cta;
   __shared__ int s_scan[kSelectWarps];
   __shared__ int s_digit, s_above, s_in_bin, s_few;
-  __shared__ uint32_t s_list[kFewKeys], s_threshold;
+  __shared__ __align__(16) uint32_t s_list[kFewKeys + 4], s_all[CLUSTER ? kFewKeys + 4 : 4];
+  __shared__ uint32_t s_threshold;
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
+  constexpr int kMostRanks = CLUSTER ? kMaxCluster : 1;
   const int C = CLUSTER ? int(cluster.num_blocks()) : 1;
   const int rank = CLUSTER ? int(cluster.block_rank()) : 0;
   auto sync = [&] {
@@ -169,7 +171,9 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   kmin = 0xffffffffu;
   kmax = 0;
   held = 0;
-  for (int r = 0; r < C; ++r) {
+#pragma unroll
+  for (int r = 0; r < kMostRanks; ++r) {
+    if (r >= C) continue;
     const int4 t = *of_rank(&s_total, r);
     kmin = min(kmin, uint32_t(t.x));
     kmax = max(kmax, uint32_t(t.y));
@@ -213,10 +217,15 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
         c[i] = make_int2(0, 0);
-        for (int r = 0; r < C; ++r) {
-          const int2 h = *reinterpret_cast<const int2 *>(of_rank(s_hist, r) + top - 2 * i - 2);
-          c[i].x += h.x;
-          c[i].y += h.y;
+        int2 h[kMostRanks];  // all in flight together
+#pragma unroll
+        for (int r = 0; r < kMostRanks; ++r)
+          h[r] = r < C ? *reinterpret_cast<const int2 *>(of_rank(s_hist, r) + top - 2 * i - 2)
+                       : make_int2(0, 0);
+#pragma unroll
+        for (int r = 0; r < kMostRanks; ++r) {
+          c[i].x += h[r].x;
+          c[i].y += h[r].y;
         }
         mine += c[i].x + c[i].y;
       }
@@ -250,20 +259,38 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
       const uint32_t base = lo + (uint32_t(s_digit) << shift);
       hi = min(hi, base + ((1u << shift) - 1));
       lo = base;
-      if (!CLUSTER && lo != hi && s_in_bin <= kFewKeys) {
+      if (lo != hi && s_in_bin <= kFewKeys) {
         // few keys are left: each is ranked against all
         for (int i = begin + tid; i < end; i += kSelectThreads) {
           const uint32_t k = key_of(i);
           if (k >= lo && k <= hi) s_list[atomicAdd(&s_few, 1)] = k;
         }
+        sync();
+        // every CTA's keys, then zeros, which are below any key, up to a multiple of 4
+        const uint32_t *list = s_list;
+        int few = s_few;
+        if constexpr (CLUSTER) {
+          few = 0;
+#pragma unroll
+          for (int r = 0; r < kMostRanks; ++r) {
+            if (r >= C) continue;
+            const int some = *of_rank(&s_few, r);
+            if (tid < some) s_all[few + tid] = of_rank(s_list, r)[tid];
+            few += some;
+          }
+          list = s_all;
+          if (tid < 3) s_all[few + tid] = 0;
+        } else {
+          if (tid < 3) s_list[few + tid] = 0;
+        }
         __syncthreads();
-        const int few = s_few;
         if (tid < few) {
-          const uint32_t k = s_list[tid];
+          const uint32_t k = list[tid];
           int larger = 0, equal = 0;
-          for (int i = 0; i < few; ++i) {
-            larger += s_list[i] > k;
-            equal += s_list[i] == k;
+          for (int i = 0; i < few; i += 4) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(list + i);
+            larger += (x.x > k) + (x.y > k) + (x.z > k) + (x.w > k);
+            equal += (x.x == k) + (x.y == k) + (x.z == k) + (x.w == k);
           }
           if (larger < want && larger + equal >= want) {  // equal keys write the same
             s_threshold = k;
@@ -306,7 +333,9 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   }
   sync();
   int gt = 0, eq = 0, gt_lo = 0, eq_lo = 0;  // gt, eq: before this warp's segment
-  for (int r = 0; r < C; ++r) {
+#pragma unroll
+  for (int r = 0; r < kMostRanks; ++r) {
+    if (r >= C) continue;
     const Counts t = *of_rank(&s_cta, r);
     if (r < rank) {
       gt += t.gt;
