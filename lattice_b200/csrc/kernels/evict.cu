@@ -10,10 +10,12 @@
 //
 // The selection narrows a range of 32-bit keys by histograms of 2048 equal bins, as wide as
 // the range asks for: accumulated weights spread over a few octaves, and bins fixed to their
-// leading bits would put half of them into 4 (measured: 72 us a call at 16,700 tokens, the
-// atomics on one bin serialised, where range bins take a few). A cluster of CTAs shares a long
-// row.  It is bound by the latency of its passes, over keys in shared memory where they fit.
-// The moves are a copy, bound by HBM.
+// leading bits would put half of them into 4 (measured: 72 us a call for 16 rows of 16,700
+// tokens, the atomics on one bin serialised, against 25).  The last few keys are ranked one
+// against all: another histogram or two took 2 to 5 us more.  A cluster of CTAs shares a long
+// row.  It is bound by the latency of its passes, over keys in shared memory where they fit
+// (128 rows of 3700 tokens: 11 us).  The moves are a copy of scattered rows, bound by HBM
+// where they are many (105,000 rows of 2 x 256 bytes: 18.5 us, 5.8 TB/s both ways).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -32,15 +34,14 @@ namespace {
 
 constexpr int kFewKeys = 256;  // ranked one against all instead of by another histogram
 constexpr int kBins = 2048;
+constexpr int kCopies = 4;  // slots of a thread in flight
 constexpr int kMaxCluster = 8;
 constexpr int kSliceTokens = 4096;
 constexpr int kKeyCapacity = 49152;  // keys in shared memory: 192 KB
 
-// One row's moves: count, then [budget] each of destination slots, source slots and the
-// weights and positions that move with them.
+// One row's moves: count, then [budget] each of destination and source slots.
 struct RowMoves {
-  int32_t *count, *dst, *src, *pos;
-  float *w;
+  int32_t *count, *dst, *src;
 };
 __device__ __forceinline__ RowMoves row_moves(const EvictArgs &a, int row) {
   const int64_t rows = int64_t(a.batch) * a.kv_heads, at = int64_t(row) * a.budget;
@@ -48,8 +49,6 @@ __device__ __forceinline__ RowMoves row_moves(const EvictArgs &a, int row) {
   r.count = a.scratch + row;
   r.dst = a.scratch + rows + at;
   r.src = r.dst + rows * a.budget;
-  r.pos = r.src + rows * a.budget;
-  r.w = reinterpret_cast<float *>(r.pos + rows * a.budget);
   return r;
 }
 
@@ -78,7 +77,8 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   __shared__ Counts s_warp[kSelectWarps];
   __shared__ Counts s_cta;
   __shared__ int s_scan[kSelectWarps];
-  __shared__ int s_digit, s_above, s_in_bin, s_few;
+  __shared__ __align__(16) int4 s_bin;
+  __shared__ int s_above, s_few;
   __shared__ __align__(16) uint32_t s_list[kFewKeys + 4], s_all[CLUSTER ? kFewKeys + 4 : 4];
   __shared__ uint32_t s_threshold;
   ptx::grid_dependency_wait();
@@ -210,56 +210,62 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
         }
       }
       sync();
-      // Bins from the top: thread t has the 2 kPairs bins below kBins - 2 kPairs t, all CTAs' sums.
-      const int top = kBins - 2 * kPairs * tid;
-      int2 c[kPairs];  // c[i]: bins top - 2i - 2 (x) and top - 2i - 1 (y)
-      int mine = 0;
+      // Bins from the top: thread t has the 2 kPairs bins below kBins - 2 kPairs t.  One CTA
+      // adds up all the CTAs' and tells the others: each reading them all took 2 us longer.
+      if (rank == 0) {
+        const int top = kBins - 2 * kPairs * tid;
+        int2 c[kPairs];  // c[i]: bins top - 2i - 2 (x) and top - 2i - 1 (y)
+        int mine = 0;
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        c[i] = make_int2(0, 0);
-        int2 h[kMostRanks];  // all in flight together
+        for (int i = 0; i < kPairs; ++i) {
+          c[i] = make_int2(0, 0);
+          int2 h[kMostRanks];  // all in flight together
 #pragma unroll
-        for (int r = 0; r < kMostRanks; ++r)
-          h[r] = r < C ? *reinterpret_cast<const int2 *>(of_rank(s_hist, r) + top - 2 * i - 2)
-                       : make_int2(0, 0);
+          for (int r = 0; r < kMostRanks; ++r)
+            h[r] = r < C ? *reinterpret_cast<const int2 *>(of_rank(s_hist, r) + top - 2 * i - 2)
+                         : make_int2(0, 0);
 #pragma unroll
-        for (int r = 0; r < kMostRanks; ++r) {
-          c[i].x += h[r].x;
-          c[i].y += h[r].y;
-        }
-        mine += c[i].x + c[i].y;
-      }
-      int sum = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += x;
-      }
-      if (lane == 31) s_scan[warp] = sum;
-      sync();  // every CTA has read this one's histogram
-      int above = lane < warp ? s_scan[lane] : 0;
-      above = __reduce_add_sync(0xffffffffu, above) + sum - mine;  // keys above these bins
-#pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int n_bin = e == 0 ? c[i].y : c[i].x;
-          if (above < want && above + n_bin >= want) {
-            s_digit = top - 2 * i - 1 - e;
-            s_above = above;
-            s_in_bin = n_bin;
+          for (int r = 0; r < kMostRanks; ++r) {
+            c[i].x += h[r].x;
+            c[i].y += h[r].y;
           }
-          above += n_bin;
+          mine += c[i].x + c[i].y;
+        }
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += x;
+        }
+        if (lane == 31) s_scan[warp] = sum;
+        __syncthreads();
+        int above = lane < warp ? s_scan[lane] : 0;
+        above = __reduce_add_sync(0xffffffffu, above) + sum - mine;  // keys above these bins
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int n_bin = e == 0 ? c[i].y : c[i].x;
+            if (above < want && above + n_bin >= want) {
+              const int4 x = make_int4(top - 2 * i - 1 - e, above, n_bin, 0);
+#pragma unroll
+              for (int r = 0; r < kMostRanks; ++r)
+                if (r < C) *of_rank(&s_bin, r) = x;
+            }
+            above += n_bin;
+          }
         }
       }
-      for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
       if (tid == 0) s_few = 0;
+      sync();
+      for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
+      const int4 wanted = s_bin;  // bin, keys above it, keys in it
       __syncthreads();
-      want -= s_above;
-      const uint32_t base = lo + (uint32_t(s_digit) << shift);
+      want -= wanted.y;
+      const uint32_t base = lo + (uint32_t(wanted.x) << shift);
       hi = min(hi, base + ((1u << shift) - 1));
       lo = base;
-      if (lo != hi && s_in_bin <= kFewKeys) {
+      if (lo != hi && wanted.z <= kFewKeys) {
         // few keys are left: each is ranked against all
         for (int i = begin + tid; i < end; i += kSelectThreads) {
           const uint32_t k = key_of(i);
@@ -361,35 +367,43 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     const int kept_before = gt + __popc(gts & below) + min(eq_before, want);
     const bool keep = in && (k > threshold || (k == threshold && eq_before < want));
     if (in && i < a.budget && !keep) mv.dst[i - kept_before] = i;
-    if (keep && i >= a.budget) {
-      const int j = kept_before - kept_lo;
-      mv.src[j] = i;
-      mv.w[j] = w_in[i];
-      mv.pos[j] = pos_of(i);
-    }
+    if (keep && i >= a.budget) mv.src[kept_before - kept_lo] = i;
     gt += __popc(gts);
     eq += __popc(eqs);
   }
   if (rank == 0 && tid == 0) mv.count[0] = moves;
-  sync();  // the lists are complete, and nothing past the budget is read again
 
-  // ---- weights and positions of the kept slots; the slots past them weigh 0 --------------
-  for (int i = begin + tid; i < end; i += kSelectThreads) {
-    if (i < a.budget) {
-      const float w = w_in[i];
-      const int p = pos_of(i);
-      w_out[i] = w;
-      p_out[i] = p;
-    } else {
-      w_out[i] = 0.f;
+  // ---- weights and positions of the slots below the budget, freed ones included ------------
+  // (inputs and outputs may be the same memory: loads of several slots before their stores)
+  const int low_end = min(end, a.budget);
+  for (int base = begin + tid; base < low_end; base += kCopies * kSelectThreads) {
+    float w[kCopies];
+    int p[kCopies];
+#pragma unroll
+    for (int k = 0; k < kCopies; ++k) {
+      const int i = base + k * kSelectThreads;
+      w[k] = i < low_end ? w_in[i] : 0.f;
+      p[k] = i < low_end ? pos_of(i) : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kCopies; ++k) {
+      const int i = base + k * kSelectThreads;
+      if (i < low_end) {
+        w_out[i] = w[k];
+        p_out[i] = p[k];
+      }
     }
   }
-  sync();
+  sync();  // the lists are complete, and the freed slots may be filled
   for (int j = rank * kSelectThreads + tid; j < moves; j += C * kSelectThreads) {
-    const int d = __ldcg(mv.dst + j);
-    w_out[d] = __ldcg(mv.w + j);
-    p_out[d] = __ldcg(mv.pos + j);
+    const int d = __ldcg(mv.dst + j), i = __ldcg(mv.src + j);
+    const float w = w_in[i];
+    const int p = pos_of(i);
+    w_out[d] = w;
+    p_out[d] = p;
   }
+  sync();  // the moved slots' weights have been read; the slots past the budget weigh 0
+  for (int i = max(begin, a.budget) + tid; i < end; i += kSelectThreads) w_out[i] = 0.f;
 }
 
 constexpr int kMoveThreads = 256;
@@ -493,21 +507,24 @@ cudaError_t evict_tokens(const EvictArgs &args, cudaStream_t stream) {
   EvictArgs a = args;
   const int rows = a.batch * a.kv_heads;
   CallScratch scratch;
-  cudaError_t e = scratch.acquire(stream, (size_t(rows) + size_t(rows) * a.budget * 4) * 4);
+  cudaError_t e = scratch.acquire(stream, (size_t(rows) + size_t(rows) * a.budget * 2) * 4);
   if (e != cudaSuccess) return e;
   a.scratch = static_cast<int32_t *>(scratch.ptr);
   // CTAs of a row's cluster: as many as leave each kSliceTokens, while they all run at once.
+  // 16 rows of up to 16,900 tokens: slices of 2048 tokens (8 CTAs) 41 us, 4096 (4) 24.6, 8192
+  // (2) 31, whole rows 43.  A whole row above it takes 1024 threads (32 rows of 8000 tokens:
+  // 25.5 against 27.9 us), all else 512 (16 rows of 3700 in CTAs of their own 29.3 us both ways,
+  // 512 of 1200 47 against 58; the clusters above 28.3, with registers spilled).
   int C = 1;
   while (C < kMaxCluster && a.max_tokens / (2 * C) >= kSliceTokens &&
          int64_t(rows) * 2 * C <= device_sm_count())
     C *= 2;
   a.key_capacity = std::min((a.max_tokens + C - 1) / C, kKeyCapacity);
   const int smem = a.key_capacity * 4;
-  const bool small = (a.max_tokens + C - 1) / C <= kSliceTokens;
-  const int threads = small ? 512 : 1024;
-  void (*fn)(const EvictArgs) =
-      C > 1 ? small ? evict_select_kernel<512, true> : evict_select_kernel<1024, true>
-            : small ? evict_select_kernel<512, false> : evict_select_kernel<1024, false>;
+  const int threads = C == 1 && a.max_tokens > kSliceTokens ? 1024 : 512;
+  void (*fn)(const EvictArgs) = C > 1            ? evict_select_kernel<512, true>
+                                : threads == 512 ? evict_select_kernel<512, false>
+                                                 : evict_select_kernel<1024, false>;
   e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
     scratch.release(stream);
@@ -531,7 +548,8 @@ cudaError_t evict_tokens(const EvictArgs &args, cudaStream_t stream) {
   if (e == cudaSuccess) {
     // enough warps for every SM, none for moves that cannot be
     const int most = std::min(a.budget, std::max(a.max_tokens - a.budget, 1));
-    // 8 a warp while that leaves warps idle
+    // 8 a warp while that leaves warps idle: 35.2 -> 30.8 us for one row of 16,384 tokens cut to
+    // half; 32 where there are many: 40.3 -> 32.0 us for 128 rows of 3700 cut to 1024
     a.warp_moves = int64_t(rows) * most <= int64_t(device_sm_count()) * 64 * 8 ? 8 : 32;
     const int per = kMoveThreads / 32 * a.warp_moves;
     const int want = std::max(1, 8 * device_sm_count() / rows);
