@@ -7,10 +7,16 @@
 // score; its other tokens score -inf.
 //
 // A CTA reads 16 KB of a beam's logits once, 64 bytes a thread, and keeps the chunk's
-// maximum, its sum of exponentials and its n largest logits: the n-th largest of the threads'
-// own maxima bounds those from below, so that a second look at the registers leaves little
-// more than n to sort.  The last CTA of a request scores and ranks its beams x chunks x n
-// candidates.  Large vocabularies are bound by HBM, small ones by latency.
+// maximum, its sum of exponentials and its n largest logits: the n-th largest of its warps'
+// maxima (its threads', where n is above 8) bounds those from below, so that a second look at
+// the registers leaves little more than n to sort.  The last CTA of a request scores and ranks
+// its beams x chunks x n candidates in the same way.  Bounds from all threads' maxima cost a
+// second pass wherever 16-bit maxima were equal: 24.4 us against 17.1 for 16 requests of 4
+// beams over 128,256 bf16 logits, the gathers of histories and tables included.
+//
+// That call is bound by the latency of a CTA's steps (load, maximum, exponentials, list,
+// counter, then the ranking; 16 MB of logits would take 2.5 us): chunks of 8 and 32 KB took 19.8
+// and 36 us.  So are small vocabularies.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -29,6 +35,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kVecs = 4;                                // 16-byte loads of a thread
 constexpr int kChunkBytes = kThreads * kVecs * 16;      // logits of one CTA of pass 1
 constexpr int kMaxSelect = kBeamMaxSelect;
+constexpr int kFewKeys = kThreads;  // ranked one against all
 
 // (value, index) as one key: larger value first, then lower index.
 __device__ __forceinline__ uint32_t value_key(float x) {
@@ -58,6 +65,35 @@ __device__ __forceinline__ uint32_t clean(uint32_t x, __nv_bfloat16) {
   asm("max.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0xff80ff80u));
   asm("min.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0x7f7f7f7fu));
   return x;
+}
+
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, __half) {
+  asm("max.f16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+  return a;
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, __nv_bfloat16) {
+  asm("max.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+  return a;
+}
+template <typename T>
+__device__ __forceinline__ float half_of(uint32_t x, int e) {  // the low or high 16 bits
+  if constexpr (std::is_same<T, __half>::value) {
+    return __half2float(__ushort_as_half(uint16_t(x >> (16 * e))));
+  } else {
+    return __uint_as_float(e ? x & 0xffff0000u : x << 16);
+  }
+}
+
+// The n-th largest of the kWarps values of `top`, n <= kWarps.
+template <typename K>
+__device__ __forceinline__ K nth_of_warps(const K *top, int n) {
+  const int lane = threadIdx.x & 31, me = lane % kWarps;
+  const K x = top[me];
+  int before = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) before += top[w] > x || (top[w] == x && w < me);
+  const uint32_t is = __ballot_sync(0xffffffffu, before == n - 1);
+  return __shfl_sync(0xffffffffu, x, __ffs(int(is)) - 1);
 }
 
 // The largest of the warp's keys (0 = none).
@@ -128,7 +164,7 @@ __device__ uint32_t nth_value(uint32_t mine, int n, TopShared *sh) {
 }
 
 // One CTA's part of the choice: the last one of request b.
-__device__ void beam_best(const BeamArgs &a, int b, TopShared *sh) {
+__device__ void beam_best(const BeamArgs &a, int b, TopShared *sh, unsigned long long *list) {
   __shared__ float2 s_norm[kBeamMaxBeams];  // max, log of the sum
   __shared__ unsigned long long s_best[kMaxSelect];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -175,11 +211,51 @@ __device__ void beam_best(const BeamArgs &a, int b, TopShared *sh) {
     if (!(score == score)) score = -INFINITY;
     return make_key(score, uint32_t(k) * uint32_t(a.vocab) + token);
   };
-  // Rounds: the n-th largest of the threads' maxima bounds what is left from below, and the
-  // largest second key of a thread says down to where the maxima are final.
-  unsigned long long cut = ~0ull;  // keys below it are left
+  // As for a chunk: the n-th largest of the warps' maxima bounds the n largest from below.
   int done = 0;
-  while (done < a.n) {
+  bool ranked = false;
+  if (a.n <= kWarps) {
+    unsigned long long mine = 0, second = 0;
+    for (int i = tid; i < total; i += kThreads) {
+      const unsigned long long k = candidate(i);
+      second = k > mine ? mine : k > second ? k : second;
+      mine = k > mine ? k : mine;
+    }
+    const unsigned long long top = warp_max(mine);
+    if (lane == 0) sh->warp_top[warp] = top;
+    if (tid == 0) sh->count = 0;
+    __syncthreads();
+    unsigned long long bound = nth_of_warps(sh->warp_top, a.n);
+    bound = bound == 0 ? 1 : bound;  // fewer warps have keys: all keys count
+    auto put = [&](unsigned long long k) {
+      const int at = atomicAdd(&sh->count, 1);
+      if (at < kFewKeys) list[at] = k;
+    };
+    if (mine >= bound) put(mine);
+    if (second >= bound) {
+      for (int i = tid; i < total; i += kThreads) {
+        const unsigned long long k = candidate(i);
+        if (k >= bound && k != mine) put(k);
+      }
+    }
+    __syncthreads();
+    const int count = sh->count;
+    ranked = count <= kFewKeys;
+    if (ranked) {
+      if (tid < count) {
+        const unsigned long long x = list[tid];
+        int larger = 0;
+        for (int i = 0; i < count; ++i) larger += list[i] > x;
+        if (larger < a.n) s_best[larger] = x;
+      }
+      done = min(count, a.n);
+    }
+    __syncthreads();
+  }
+  // Else in rounds: the n-th largest of the threads' maxima bounds what is left from below, and
+  // the largest second key of a thread says down to where the maxima are final.
+  unsigned long long cut = ~0ull;  // keys below it are left
+  while (!ranked && done < a.n) {
     unsigned long long mine = 0, second = 0;
     for (int i = tid; i < total; i += kThreads) {
       const unsigned long long k = candidate(i);
@@ -230,7 +306,7 @@ __device__ void beam_best(const BeamArgs &a, int b, TopShared *sh) {
 
 // Grid (chunks, rows), a row being one beam of one request.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 6) beam_select_kernel(const BeamArgs a) {
+__global__ void __launch_bounds__(kThreads, 5) beam_select_kernel(const BeamArgs a) {
   constexpr int PER = 16 / sizeof(T);  // logits of a load
   constexpr int MOST = kVecs * PER;    // of a thread
   __shared__ TopShared sh;
@@ -277,10 +353,8 @@ __global__ void __launch_bounds__(kThreads, 6) beam_select_kernel(const BeamArgs
     auto value = [&](int i, int e) {  // logit e of load i
       if constexpr (sizeof(T) == 4) {
         return __uint_as_float(x[i][e]);
-      } else if constexpr (std::is_same<T, __half>::value) {
-        return __half2float(__ushort_as_half(uint16_t(x[i][e / 2] >> (16 * (e & 1)))));
       } else {
-        return __uint_as_float(e & 1 ? x[i][e / 2] & 0xffff0000u : x[i][e / 2] << 16);
+        return half_of<T>(x[i][e / 2], e & 1);
       }
     };
     // the thread's maximum, the chunk's, and the chunk's sum
@@ -289,18 +363,68 @@ __global__ void __launch_bounds__(kThreads, 6) beam_select_kernel(const BeamArgs
     for (int i = 0; i < kVecs; ++i) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) x[i][w] = clean(x[i][w], T());
+    }
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int e = 0; e < PER; ++e) mx = fmaxf(mx, value(i, e));
+      for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, value(i, e));
+    } else {
+      uint32_t two = x[0][0];
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) two = max2(two, x[i][w], T());
+      mx = fmaxf(half_of<T>(two, 0), half_of<T>(two, 1));
     }
     float m = mx;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) s_red[warp] = m;
     if (tid == 0) sh.count = 0;
-    const uint32_t limit = nth_value(value_key(mx), a.n, &sh);  // synchronises
+    // a bound of the n largest from below: n warps, or n threads, have a logit that reaches it
+    float floor_value;
+    if (a.n <= kWarps) {
+      __syncthreads();
+      floor_value = nth_of_warps(s_red, a.n);
+    } else {
+      floor_value = key_value(nth_value(value_key(mx), a.n, &sh));  // synchronises
+    }
     m = s_red[0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_red[w]);
+    // The logits that reach it: few, unless many are equal or fewer than n are finite.
+    auto index = [&](int bit) {
+      return at0 + int64_t(bit / PER) * kThreads * PER + bit % PER;
+    };
+    uint32_t reach = 0;  // bit i * PER + e
+    if (mx >= floor_value) {
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          reach |= value(i, e) >= floor_value ? 1u << (i * PER + e) : 0u;
+    }
+    auto each = [&](auto f) {  // f(key) of the thread's logits that reach the bound
+      for (uint32_t left = reach; left != 0; left &= left - 1) {
+        const int bit = __ffs(int(left)) - 1;
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+          for (int e = 0; e < PER; ++e) v = bit == i * PER + e ? value(i, e) : v;
+        const int64_t at = index(bit);
+        if (at >= 0 && at < a.vocab) f(make_key(v, uint32_t(at)));
+      }
+    };
+    if (floor_value == -INFINITY) {
+      if (tid == 0) sh.count = kFewKeys + 1;  // logits outside the row would reach it as well
+    } else if (reach != 0) {
+      each([&](unsigned long long k) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kFewKeys) s_list[at] = k;
+      });
+    }
     float sum = 0.f;
     if (m != -INFINITY) {
 #pragma unroll
@@ -311,41 +435,27 @@ __global__ void __launch_bounds__(kThreads, 6) beam_select_kernel(const BeamArgs
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_sum[warp] = sum;
-    // Threads whose maximum reaches the n-th largest one hold the n largest logits.  Where equal
-    // maxima make them more than n, those of the lowest indexes count.
-    const bool holds = value_key(mx) >= limit;
-    const float floor_value = key_value(limit);
-    auto each = [&](auto f) {  // f(key) of the thread's logits at or above the limit: few
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i) {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) {
-          const float v = value(i, e);
-          if (v >= floor_value) {
-            const int64_t at = at0 + int64_t(i) * kThreads * PER + e;
-            if (at >= 0 && at < a.vocab) f(make_key(v, uint32_t(at)));
-          }
-        }
-      }
-    };
-    unsigned long long bound = static_cast<unsigned long long>(limit) << 32;
-    if (__syncthreads_count(holds) > a.n) {
-      unsigned long long mine = 0ull;
-      if (holds) each([&](unsigned long long k) { mine = k > mine ? k : mine; });
-      bound = nth_maximum(mine, a.n, &sh);
-    }
+    __syncthreads();
     if (tid == 0) {
       float total = 0.f;
       for (int w = 0; w < kWarps; ++w) total += s_sum[w];
       a.part[int64_t(row) * a.chunks + chunk] = make_float2(m, total);
     }
-    if (holds) {
+    int count = sh.count;
+    if (count > kFewKeys) {
+      // the n-th largest of the threads' own largest keys is the bound: at most n threads, all
+      // of whose logits fit, have keys that reach it
+      __syncthreads();
+      if (tid == 0) sh.count = 0;
+      unsigned long long mine = 0ull;
+      each([&](unsigned long long k) { mine = k > mine ? k : mine; });
+      const unsigned long long bound = nth_maximum(mine, a.n, &sh);
       each([&](unsigned long long k) {
         if (k >= bound) s_list[atomicAdd(&sh.count, 1)] = k;
       });
+      __syncthreads();
+      count = sh.count;
     }
-    __syncthreads();
-    const int count = sh.count;
     unsigned long long *cand = a.cand + (int64_t(row) * a.chunks + chunk) * a.n;
     for (int i = tid; i < max(count, a.n); i += kThreads) {
       if (i >= count) {
@@ -366,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 6) beam_select_kernel(const BeamArgs
     __threadfence();
   }
   __syncthreads();
-  if (s_last) beam_best(a, b, &sh);
+  if (s_last) beam_best(a, b, &sh, s_list);
 }
 
 // dst row (b, j) = src row (b, parents[b, j]); with tokens, its entry token_index = tokens[b, j].
