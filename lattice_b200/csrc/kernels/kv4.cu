@@ -42,9 +42,10 @@ constexpr int kGroup = kKv4Group;
 // page (a prompt's chunk), lane (g, c) takes exactly the values whose codes it holds in the
 // layout: its source loads are whole 32-byte sectors, its code stores one 16-byte vector a
 // pair of groups, and no byte goes through shared memory.  Other tiles (decode steps, the
-// ends of a chunk) go row by row, 8 values a lane.  Both are bound by HBM for long inputs
-// (16,384 tokens of 8 heads of 128: 179 us row by row, 45 by units, 3.8 TB/s) and by the
-// latency of slot -> offset -> row for short ones (64 tokens: 4.4 us).
+// ends of a chunk) go row by row, 8 values a lane.  16,384 tokens of 8 heads of 128 took 179 us
+// row by row for both kernels and take 45 by units (3.8 TB/s, 60 to 68 % of the issue slots:
+// HBM and the arithmetic bound them together); short inputs are bound by the latency of
+// slot -> offset -> row (64 tokens: 4.4 us).
 
 constexpr int kRowsThreads = 128;
 // A tile has a unit's 16 rows where that leaves every SM kTileWarps warps, else kFewRows: at 8
@@ -584,11 +585,11 @@ __device__ __forceinline__ void load_words(uint32_t *r, const unsigned char *p, 
 // inside one range is finished there; the pieces of one that several CTAs share go to scratch
 // and the last CTA to finish merges them.
 //
-// That batch is bound by issue slots, at 3.0 TB/s: 16 tokens of a head cost about 330
-// warp instructions, half of them unpacking and scaling codes (matrix products on 8-bit
-// codes instead needed as many), and 4 CTAs an SM leave few slots idle.  Few sequences are
-// bound by latency: lengths -> table -> offset -> chunk -> counter -> merge (14.9 us for 3 of up
-// to 777 tokens).
+// That batch is bound by instructions, at 3.0 TB/s: 16 tokens of a head cost about 330 warp
+// instructions, half of them unpacking and scaling codes (matrix products on 8-bit codes
+// instead needed as many); 58 % of the issue slots are used over the whole call, its start and
+// its merges included.  Few sequences are bound by latency: lengths -> table -> offset -> chunk
+// -> counter -> merge (14.9 us for 3 of up to 777 tokens).
 //
 // A CTA's warps take every kWarps-th step of NU units of its piece.  Each warp runs its own
 // ring of kStages steps: a lane issues a unit's K and V chunks as two bulk copies, the whole
