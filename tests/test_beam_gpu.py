@@ -104,6 +104,30 @@ def test_ties_go_to_the_lowest_index(pool):
         check(pool, logits, torch.full((2, 3), -2.0, device="cuda"), min(64, 3 * V))
 
 
+@pytest.mark.parametrize("n", [1, 4, 8, 9])
+def test_ties_of_few_selected(pool, n):
+    """More equal logits than are ranked one against all, in part of a row, a row, all rows."""
+    torch = torch_cuda()
+    for V in (300, 20000, 70001):
+        for dt, name in ((torch.bfloat16, "bf16"), (torch.float32, "f32")):
+            logits = torch.zeros(3, 2, V, device="cuda", dtype=dt)
+            logits[1, :, V // 2:] = 1.0
+            logits[2, 0, ::2] = -float("inf")
+            logits[2, 1, 5:] = -float("inf")
+            check(pool, logits, torch.full((3, 2), -2.0, device="cuda"), n, dtype=name)
+
+
+def test_beams_whose_candidates_crowd_one_warp(pool):
+    """One warp of the ranking holds more candidates above the others' best than are ranked one
+    against all."""
+    torch = torch_cuda()
+    g = torch.Generator(device="cuda").manual_seed(8)
+    logits = torch.randn(1, 256, 50, device="cuda", generator=g)
+    scores = -100 - torch.rand(1, 256, device="cuda", generator=g)
+    scores[0, torch.arange(256, device="cuda") % 32 < 4] += 99
+    check(pool, logits, scores, 8)
+
+
 def test_masked_rows_and_specials(pool):
     """-inf over parts, whole rows and whole requests; NaN and +inf logits; beams of score
     -inf (the first step, where only beam 0 counts)."""

@@ -147,6 +147,21 @@ def test_evict_long_rows(n, budget):
         c.close()
 
 
+@pytest.mark.parametrize("n,hkv,budget", [(16999, 4, 16384), (33000, 1, 1024), (9001, 3, 4500),
+                                          (8500, 40, 8000)])
+def test_evict_long_rows_of_distinct_weights(n, hkv, budget):
+    """The last few candidates for the threshold differ: they are ranked one against all."""
+    c = Cache([n, n - 700], hkv, 64, seed=n)
+    try:
+        c.fill_rows()
+        e = Evict(c, n, seed=3)
+        before = e.snapshot()
+        e.run(budget, 1, 200)
+        e.check(budget, 1, 200, before)
+    finally:
+        c.close()
+
+
 @pytest.mark.parametrize("kind", ["equal", "zeros", "special", "nan"])
 def test_evict_ties_and_special_weights(kind):
     """All weights equal, signed zeros, infinities, negatives and NaN."""

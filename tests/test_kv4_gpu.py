@@ -286,14 +286,8 @@ def test_bad_block_is_reported():
         c.close()
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
-@pytest.mark.parametrize("hkv,d,bs,first", [(2, 128, 16, 0), (3, 64, 32, 16), (1, 96, 48, 32),
-                                            (2, 256, 16, 5), (1, 32, 16, 0), (5, 160, 64, 1)])
-def test_append_and_read_long_chunks(dtype, hkv, d, bs, first):
-    """Chunks of many rows: whole units, ends that are not, chunks that start inside a unit,
-    skipped rows among them; magnitudes from the smallest to the largest."""
+def append_and_read_long_chunk(dtype, hkv, d, bs, first, n):
     torch = torch_cuda()
-    n = 1200
     c = Cache([n + first], hkv, d, bs, kv4=True, dtype=dtype, seed=d)
     try:
         x = c.rng.standard_normal((2, n, hkv, d))
@@ -313,5 +307,39 @@ def test_append_and_read_long_chunks(dtype, hkv, d, bs, first):
             assert equal_rows(g[kt], quantised(y.double().cpu().numpy())[keep], dtype)
             assert bool(torch.isnan(g[torch.from_numpy(skipped).cuda()]).all())  # NaN bits as made
         assert int(c.status.item()) == 0
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hkv,d,bs,first", [(2, 128, 16, 0), (3, 64, 32, 16), (1, 96, 48, 32),
+                                            (2, 256, 16, 5), (1, 32, 16, 0), (5, 160, 64, 1)])
+def test_append_and_read_long_chunks(dtype, hkv, d, bs, first):
+    """Chunks of many rows: whole units, ends that are not, chunks that start inside a unit,
+    skipped rows among them; magnitudes from the smallest to the largest."""
+    append_and_read_long_chunk(dtype, hkv, d, bs, first, 1200)
+
+
+@pytest.mark.parametrize("hkv,d,bs,first,n", [(8, 128, 16, 5, 1900), (12, 64, 32, 16, 1303),
+                                              (3, 96, 48, 32, 4100), (1, 32, 16, 0, 12001),
+                                              (16, 256, 16, 0, 2 * 777)])
+def test_append_and_read_chunks_of_whole_units(hkv, d, bs, first, n):
+    """The same where the rows are enough for tiles of a whole unit."""
+    for dtype in ("bf16", "f16"):
+        append_and_read_long_chunk(dtype, hkv, d, bs, first, n)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(320, 320, 32), (700, 700, 32), (128, 2, 64), (96, 96, 256)])
+def test_decode_many_heads(hq, hkv, d):
+    """More kv heads, and tiles of a kv head's query heads, than CTAs that run at once."""
+    torch = torch_cuda()
+    c = Cache(LENS, hkv, d, kv4=True, seed=hq + d)
+    try:
+        rows = c.fill_rows(k_amp=1.3)
+        q = torch.from_numpy(c.rng.standard_normal((len(LENS), hq, d))).cuda().to(c.tdt)
+        out = torch.full_like(q, float("nan"))
+        c.decode(q, d ** -0.5, out)
+        check_decode(c, rows, q, out, d ** -0.5, untouched=np.full((len(LENS), hq, d), np.nan))
+        assert c.pool.kernel_status() == 0
     finally:
         c.close()
