@@ -16,7 +16,9 @@ any framework (torch here, in tests and the bench) can own them.
 from __future__ import annotations
 
 import ctypes
+import gc
 import os
+import weakref
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
@@ -415,6 +417,29 @@ def make_config(*, num_layers: int, kv_heads: int, head_dim: int, max_batch: int
     return cfg
 
 
+class _Regions:
+    """Holds a pool's device memory: a pool that was destroyed releases it when neither the
+    pool nor any `RegionAddress` refers to this any more."""
+
+    def __init__(self, lib, handle):
+        self.lib, self.handle, self.closed = lib, handle, False
+
+    def __del__(self):
+        if self.closed:
+            self.lib.kcmm_pool_destroy(self.handle)
+
+
+class RegionAddress(int):
+    """A region's device address.  The region stays mapped while this object lives, so that a
+    tensor over it (`__cuda_array_interface__` with this object in "data") may outlive the
+    pool; what arithmetic makes of it is a plain int and holds nothing."""
+
+    def __new__(cls, address: int, regions: _Regions):
+        self = super().__new__(cls, address)
+        self._regions = regions
+        return self
+
+
 class KcmmPool:
     """One pool handle; every method raises `KcmmError` on a -1 return."""
 
@@ -422,6 +447,7 @@ class KcmmPool:
         self.library = library
         self.lib = library.lib
         self.handle = ctypes.c_void_p(handle)
+        self._regions = _Regions(self.lib, self.handle)
         self._destroyed = False
 
     def __enter__(self) -> "KcmmPool":
@@ -444,9 +470,16 @@ class KcmmPool:
             raise KcmmError(f"{op} failed: {self.last_error() or 'unknown KCMM error'}")
 
     def destroy(self) -> None:
-        if not self._destroyed:
-            self.lib.kcmm_pool_destroy(self.handle)
-            self._destroyed = True
+        """Release everything; the regions only once no address of `va_k` / `va_v`, nor a tensor
+        over one, is left.  No other call on the pool may follow."""
+        if self._destroyed:
+            return
+        self._destroyed = True
+        self._regions.closed = True
+        held = weakref.ref(self._regions)
+        self._regions = None
+        if held() is not None:
+            gc.collect()  # the class that hands an address to a tensor lies in a cycle
 
     # --- blocks and sequences --------------------------------------------
     def alloc_blocks(self, count: int) -> list[int]:
@@ -552,17 +585,21 @@ class KcmmPool:
     def block_state_epoch(self) -> int:
         return self.lib.kcmm_block_state_epoch(self.handle)
 
-    def va_k(self, layer: int) -> int:
-        va = self.lib.kcmm_get_va_k(self.handle, layer)
-        if not va:
-            raise KcmmError(f"kcmm_get_va_k: layer {layer} out of bounds")
-        return va
+    def va_k(self, layer: int) -> RegionAddress:
+        """Base of a layer's K region, which stays mapped while the address is held."""
+        return self._region_address("kcmm_get_va_k", layer)
 
-    def va_v(self, layer: int) -> int:
-        va = self.lib.kcmm_get_va_v(self.handle, layer)
+    def va_v(self, layer: int) -> RegionAddress:
+        """Base of a layer's V region, which stays mapped while the address is held."""
+        return self._region_address("kcmm_get_va_v", layer)
+
+    def _region_address(self, op: str, layer: int) -> RegionAddress:
+        if self._destroyed:
+            raise KcmmError(f"{op}: the pool is destroyed")
+        va = getattr(self.lib, op)(self.handle, layer)
         if not va:
-            raise KcmmError(f"kcmm_get_va_v: layer {layer} out of bounds")
-        return va
+            raise KcmmError(f"{op}: layer {layer} out of bounds")
+        return RegionAddress(va, self._regions)
 
     def stats(self) -> dict:
         s = KcmmPoolStats()
