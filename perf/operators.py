@@ -268,7 +268,6 @@ class _Pool:
         n = pages // per * (_SB_BYTES // 2)
 
         class _View:
-            owner = self  # the tensor keeps the view, and the view the pool, alive
             __cuda_array_interface__ = {"shape": (n,), "typestr": "<i2", "data": (base, False),
                                         "version": 3}
 
