@@ -1095,6 +1095,9 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
       if (d == 0) part_lse[row] = lse;
     }
   }
+  // The next sequence's bulk copies refill what the merge wrote: a proxy of their own, which
+  // only this orders after these threads' accesses (the barrier of either branch follows).
+  ptx::fence_proxy_async_smem();
   if (whole) {
     __syncthreads();  // the rings' memory is free again
     continue;

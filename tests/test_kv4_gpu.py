@@ -343,3 +343,27 @@ def test_decode_many_heads(hq, hkv, d):
         assert c.pool.kernel_status() == 0
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d,n,most", [("bf16", 32, 8, 128, 900, 40),
+                                                   ("f16", 8, 1, 64, 3000, 90),
+                                                   ("bf16", 6, 2, 256, 500, 70)])
+def test_decode_many_sequences_a_cta(dtype, hq, hkv, d, n, most):
+    """CTAs that take several short sequences one after another reuse their copy buffers
+    between them: the same bits each time."""
+    torch = torch_cuda()
+    lens = np.random.default_rng(n).integers(0, most, n)
+    c = Cache(lens, hkv, d, kv4=True, dtype=dtype, seed=n)
+    try:
+        total = len(c.offsets) * c.bs
+        x = [torch.from_numpy(c.rng.standard_normal((total, hkv, d)).astype(np.float32)).cuda().to(
+            c.tdt) for _ in "kv"]
+        c.write(*x, np.arange(total))
+        q = torch.from_numpy(c.rng.standard_normal((n, hq, d))).cuda().to(c.tdt)
+        first = c.decode(q, d ** -0.5, torch.zeros_like(q))
+        assert bool(torch.isfinite(first).all())
+        for _ in range(20):
+            assert torch.equal(c.decode(q, d ** -0.5, torch.zeros_like(q)), first)
+        assert c.pool.kernel_status() == 0
+    finally:
+        c.close()
