@@ -469,6 +469,7 @@ constexpr int kMaxPieces = 32;
 // Pieces that the merge takes at a time.  A first pass over their sums took 30.0 us against 27.8
 // for 8 sequences of 32,768 tokens and 8 heads on 1; 4 and 16 at a time 30.0 and 28.4.
 constexpr int kMergeAtOnce = 8;
+constexpr float kNoMax = -3e38f;  // a row's maximum before its first finite score
 constexpr int kStages = 3;  // steps of a warp's ring; 2 are as fast
 constexpr uint64_t kWaitLimitNs = 1000000000ull;  // a chunk that has not landed in 1 s is
                                                   // reported, never waited on forever
@@ -525,10 +526,13 @@ __device__ __forceinline__ void mma_add(float *d, const uint32_t *a, uint32_t b0
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-  uint32_t y;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
-  return y;
+// The code's value, exactly, as bf16: two of a word's codes at 4 bits in each half (the others
+// masked away).  0x4300 is 128 with a unit of 1 in its last place.
+__device__ __forceinline__ uint32_t bf16_codes(uint32_t w, uint32_t base) {
+  uint32_t x;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w), "n"(0x000f000fu), "r"(base));
+  asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0x43084308u));
+  return x;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -544,13 +548,12 @@ __device__ __forceinline__ float bf16_hi(uint32_t x) { return __uint_as_float(x 
 __host__ __device__ constexpr int units_at_a_time(int D) { return D <= 128 ? 2 : 1; }
 __host__ __device__ constexpr int ctas_per_sm(int D) { return D <= 128 ? 4 : 2; }
 
-// V's scales enter P as f16: two positive bf16 a word, their exponents lowered by a bias
-// common to the warp (in units of bf16's exponent bit), those below f16's range to about 0.
-// The bias keeps the largest scale seen below 2^9 (f16 exponent field 23), so that 64 times
-// it is finite and scales down to 2^-21 of the largest count.
-constexpr int kScaleTop = 23;
-__device__ __forceinline__ uint32_t scales_to_f16(uint32_t s, uint32_t minus_bias) {
-  return __viaddmax_s16x2_relu(s, minus_bias, 0u) << 3;
+// The high halves of two floats, a's low; the low halves.
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
+  return __byte_perm(a, b, 0x7632);
+}
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) {
+  return __byte_perm(a, b, 0x5410);
 }
 
 // K's scale of token g (w = 0) or g + 8 (w = 1), group j, of a lane's 2 NG scales
@@ -794,14 +797,12 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
 #pragma unroll
   for (int i = 0; i < 2 * NG; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[2], l[2];
-  m[0] = m[1] = -INFINITY;
+  m[0] = m[1] = kNoMax;
   l[0] = l[1] = 0.f;
-  int bias = -1;               // exponent bias of V's scales inside P; -1 before the first unit
-  uint32_t minus_bias = 0;     // two of -bias << 7, as 16-bit integers
-  uint32_t scale_limit = 0;    // largest scale (bf16 bits) that the bias admits
   bool failed = false;
-  uint32_t base;
+  uint32_t base, v_base;
   asm volatile("mov.u32 %0, 0x64006400;" : "=r"(base));
+  asm volatile("mov.u32 %0, 0x43004300;" : "=r"(v_base));
 
   for (int k = 0; k < n_w; ++k) {
     const int u = first_unit + k * (kWarps * NU);
@@ -899,15 +900,9 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
         }
       }
     }
-    // The running maximum is raised only when a score exceeds it by more than 6 (a factor of
-    // 64, which P's f16 range holds), the bias only when a scale passes its limit: both are
-    // rare after a warp's first step, so most steps skip the rescaling of O.
-    uint32_t vmx = 0;
-#pragma unroll
-    for (int r = 0; r < NU; ++r)
-#pragma unroll
-      for (int i = 0; i < 2 * NG; i += 2) vmx = __vimax3_u16x2(vmx, vs[r][i], vs[r][i + 1]);
-    bool raise = (vmx & 0xffffu) > scale_limit || (vmx >> 16) > scale_limit;
+    // The running maximum is raised only when a score exceeds it by more than 6: rare after a
+    // warp's first step, so most steps skip the rescaling of O.
+    bool raise = false;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float mx = fmaxf(s[0][i], s[0][i + 2]);
@@ -915,41 +910,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
       for (int r = 1; r < NU; ++r) mx = fmaxf(mx, fmaxf(s[r][i], s[r][i + 2]));
       raise |= mx > m[i] + 6.f;
     }
-    if (__any_sync(0xffffffffu, raise || bias < 0)) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        bool nan = false;  // a NaN scale: its group of O is lost, its codes count as 0 here
-#pragma unroll
-        for (int r = 0; r < NU; ++r) {
-#pragma unroll
-          for (int i = 2 * j; i < 2 * j + 2; ++i) {
-            if ((vs[r][i] & 0xffffu) >= 0x7f80u) {
-              nan = true;
-              vs[r][i] &= 0xffff0000u;
-            }
-            if ((vs[r][i] >> 16) >= 0x7f80u) {
-              nan = true;
-              vs[r][i] &= 0x0000ffffu;
-            }
-            top = max(top, max(vs[r][i] & 0xffffu, vs[r][i] >> 16));
-          }
-        }
-        if (__any_sync(0xffffffffu, nan)) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            o[2 * j][i] = o[2 * j + 1][i] = __int_as_float(0x7fc00000);
-        }
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      float vr = 1.f;
-      if (bias < 0 || top > scale_limit) {
-        const int fresh = max(int(top >> 7) - kScaleTop + 2, 0);
-        if (bias >= 0) vr = exp2f(float(bias - fresh));
-        bias = fresh;
-        minus_bias = (uint32_t(-(bias << 7)) & 0xffffu) * 0x10001u;
-        scale_limit = uint32_t(min((bias + kScaleTop + 1) << 7, 0x7f80)) - 1;
-      }
+    if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float mx = m[i];
@@ -958,30 +919,39 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float rr = m[i] == -INFINITY ? 0.f : ptx::fast_exp2(m[i] - mx);
+        const float rr = ptx::fast_exp2(m[i] - mx);
         m[i] = mx;
         l[i] *= rr;
 #pragma unroll
         for (int d = 0; d < 2 * NG; ++d) {
-          o[d][i] *= rr * vr;
-          o[d][i + 2] *= rr * vr;
+          o[d][i] *= rr;
+          o[d][i + 2] *= rr;
         }
       }
     }
-    // ---- O += V^T P^T ----------------------------------------------------------------------
-    // P as the B operand (rows = tokens, columns = heads) in 11 bits, rounded to 11 bits once
-    // more by a group's scales
-    uint32_t pb[NU][2];
+    // ---- O += V^T (P S)^T, S the scale of a token's group -------------------------------------
+    // The codes are the A operand; the weight of a (token, head, group), the probability times
+    // the scale in 32 bits, is the B operand (rows = tokens, columns = heads) as a pair of bf16,
+    // its leading 8 bits and its remainder's: 16 bits, and the range of 32-bit floats.  Half the
+    // products on f16, 57 us against 61 for the Llama-3-8B batch, round a weight of 11 bits twice
+    // and lose groups and tokens whose scales lie far apart, since one range holds them all.
+    float pt[NU][4];  // P transposed: head g, tokens (2c, 2c+1) + 8 i
 #pragma unroll
     for (int r = 0; r < NU; ++r) {
-      float x[4];
+      uint32_t x[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i] = ptx::fast_exp2(s[r][i] - m[i & 1]);
-        l[i & 1] += x[i];
+        const float p = ptx::fast_exp2(s[r][i] - m[i & 1]);
+        l[i & 1] += p;
+        x[i] = __float_as_uint(p);
       }
-      pb[r][0] = transpose8x8(ptx::Mma<__half>::pack(x[0], x[1]));
-      pb[r][1] = transpose8x8(ptx::Mma<__half>::pack(x[2], x[3]));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t hi = transpose8x8(high_halves(x[2 * i], x[2 * i + 1]));
+        const uint32_t lo = transpose8x8(low_halves(x[2 * i], x[2 * i + 1]));
+        pt[r][2 * i] = __uint_as_float(low_halves(lo, hi));
+        pt[r][2 * i + 1] = __uint_as_float(high_halves(lo, hi));
+      }
     }
 #pragma unroll
     for (int r = 0; r < NU; ++r) {
@@ -996,15 +966,24 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         const uint32_t w0 = vw[2 * j], w1 = vw[2 * j + 1];
-        const uint32_t a0[4] = {low_codes(w0, base), high_codes(w0, base), low_codes(w1, base),
-                                high_codes(w1, base)};
-        const uint32_t a1[4] = {low_codes(w0 >> 8, base), high_codes(w0 >> 8, base),
-                                low_codes(w1 >> 8, base), high_codes(w1 >> 8, base)};
-        const uint32_t v0 = scales_to_f16(vs[r][2 * j], minus_bias);
-        const uint32_t v1 = scales_to_f16(vs[r][2 * j + 1], minus_bias);
-        const uint32_t b0 = mul2(pb[r][0], v0), b1 = mul2(pb[r][1], v1);
-        mma_add(o[2 * j], a0, b0, b1);
-        mma_add(o[2 * j + 1], a1, b0, b1);
+        const uint32_t a0[4] = {bf16_codes(w0, v_base), bf16_codes(w0 >> 4, v_base),
+                                bf16_codes(w1, v_base), bf16_codes(w1 >> 4, v_base)};
+        const uint32_t a1[4] = {bf16_codes(w0 >> 8, v_base), bf16_codes(w0 >> 12, v_base),
+                                bf16_codes(w1 >> 8, v_base), bf16_codes(w1 >> 12, v_base)};
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t sc = vs[r][2 * j + i];
+          const float x0 = pt[r][2 * i] * bf16_lo(sc), x1 = pt[r][2 * i + 1] * bf16_hi(sc);
+          const uint32_t b0 = __float_as_uint(x0), b1 = __float_as_uint(x1);
+          hi[i] = high_halves(b0, b1);
+          lo[i] = ptx::Mma<__nv_bfloat16>::pack(x0 - __uint_as_float(b0 & 0xffff0000u),
+                                                x1 - __uint_as_float(b1 & 0xffff0000u));
+        }
+        ptx::Mma<__nv_bfloat16>::run(o[2 * j], a0, hi[0], hi[1]);
+        ptx::Mma<__nv_bfloat16>::run(o[2 * j + 1], a1, hi[0], hi[1]);
+        ptx::Mma<__nv_bfloat16>::run(o[2 * j], a0, lo[0], lo[1]);
+        ptx::Mma<__nv_bfloat16>::run(o[2 * j + 1], a1, lo[0], lo[1]);
       }
     }
     __syncwarp();
@@ -1043,8 +1022,6 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
   float *cO = reinterpret_cast<float *>(kv4_smem);  // [kWarps][kHeads][D]
   float *cm = cO + kWarps * kHeads * D;                 // [kWarps][kHeads]
   float *cl = cm + kWarps * kHeads;                     // [kWarps][kHeads]
-  // f16 scale = bf16 scale * 2^(112 - bias): both exponents are biased, by 127 and 15
-  const float v_down = bias < 0 ? 0.f : exp2f(float(bias - 112));
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     float sum = l[i];
@@ -1060,15 +1037,14 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         *reinterpret_cast<float4 *>(cO + (warp * kHeads + h) * D + j * kGroup + g * 4) =
-            make_float4(o[2 * j][i] * v_down, o[2 * j][i + 2] * v_down,
-                        o[2 * j + 1][i] * v_down, o[2 * j + 1][i + 2] * v_down);
+            make_float4(o[2 * j][i], o[2 * j][i + 2], o[2 * j + 1][i], o[2 * j + 1][i + 2]);
       }
     }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < G * (D / 4); i += kWarps * 32) {
     const int h = i / (D / 4), d = (i % (D / 4)) * 4;
-    float M = -INFINITY;
+    float M = kNoMax;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) M = fmaxf(M, cm[w * kHeads + h]);
     float L = 0.f;
@@ -1076,7 +1052,6 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float mw = cm[w * kHeads + h], lw = cl[w * kHeads + h];
-      if (mw == -INFINITY && lw == 0.f) continue;  // the warp saw no token
       const float sc = ptx::fast_exp2(mw - M);
       const float4 v = *reinterpret_cast<const float4 *>(cO + (w * kHeads + h) * D + d);
       L += lw * sc;

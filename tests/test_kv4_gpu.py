@@ -350,7 +350,7 @@ def test_decode_many_heads(hq, hkv, d):
                                                    ("bf16", 6, 2, 256, 500, 70)])
 def test_decode_many_sequences_a_cta(dtype, hq, hkv, d, n, most):
     """CTAs that take several short sequences one after another reuse their copy buffers
-    between them: the same bits each time."""
+    between them: every output right, and the same bits each time."""
     torch = torch_cuda()
     lens = np.random.default_rng(n).integers(0, most, n)
     c = Cache(lens, hkv, d, kv4=True, dtype=dtype, seed=n)
@@ -359,11 +359,62 @@ def test_decode_many_sequences_a_cta(dtype, hq, hkv, d, n, most):
         x = [torch.from_numpy(c.rng.standard_normal((total, hkv, d)).astype(np.float32)).cuda().to(
             c.tdt) for _ in "kv"]
         c.write(*x, np.arange(total))
+        hk, hv = (quantised(y.double().cpu().numpy()) for y in x)
+        rows = [(hk[s], hv[s]) for s in (c.slots(b, np.arange(m)) for b, m in enumerate(lens))]
         q = torch.from_numpy(c.rng.standard_normal((n, hq, d))).cuda().to(c.tdt)
         first = c.decode(q, d ** -0.5, torch.zeros_like(q))
-        assert bool(torch.isfinite(first).all())
+        check_decode(c, rows, q, first, d ** -0.5, untouched=np.zeros((n, hq, d)))
         for _ in range(20):
             assert torch.equal(c.decode(q, d ** -0.5, torch.zeros_like(q)), first)
         assert c.pool.kernel_status() == 0
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("dtype,apart", [("bf16", 12), ("bf16", 20), ("bf16", 24), ("bf16", 90),
+                                         ("f16", 12), ("f16", 20), ("f16", 24)])
+def test_decode_groups_far_apart(dtype, apart):
+    """A quiet group of V beside one 2^apart louder: output dims do not depend on each other,
+    so each is held to its own sum of p |v|."""
+    torch = torch_cuda()
+    n, hkv, d = 300, 2, 128
+    c = Cache([n, 40, 1], hkv, d, kv4=True, dtype=dtype, seed=apart)
+    try:
+        rows = []
+        for b, m in enumerate(c.lens):
+            k = c.rng.standard_normal((m, hkv, d))
+            v = np.clip(c.rng.standard_normal((m, hkv, d)), -3, 3)
+            v[..., :32] *= 2.0 ** (apart if dtype == "bf16" else 12)
+            v[..., 96:] *= 2.0 ** (0 if dtype == "bf16" else 12 - apart)
+            tk, tv = (torch.from_numpy(x).cuda().to(c.tdt) for x in (k, v))
+            c.write(tk, tv, c.slots(b, np.arange(m)))
+            rows.append(tuple(quantised(x.double().cpu().numpy()) for x in (tk, tv)))
+        q = torch.from_numpy(c.rng.standard_normal((3, 8, d))).cuda().to(c.tdt)
+        out = c.decode(q, d ** -0.5, torch.zeros_like(q))
+        check_decode(c, rows, q, out, d ** -0.5)
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("at", [0, 150, 299])
+@pytest.mark.parametrize("low,loud", [(20, 12), (40, 24), (60, 50), (30, 30)])
+def test_decode_loud_token_of_little_weight(at, low, loud):
+    """One token of probability near 2^-low whose V is 2^loud times the others': it counts for
+    its share, and the others for theirs."""
+    torch = torch_cuda()
+    n, d = 300, 64
+    c = Cache([n], 1, d, kv4=True, seed=at + low)
+    try:
+        k, v = c.rng.standard_normal((2, n, 1, d))
+        direction = np.where(np.arange(d) % 2, 1.0, -1.0)
+        k[at] = -direction * (low * np.log(2) / d)
+        v[at] *= 2.0 ** loud
+        tk, tv = (torch.from_numpy(x).cuda().to(c.tdt) for x in (k, v))
+        c.write(tk, tv, c.slots(0, np.arange(n)))
+        rows = [tuple(quantised(x.double().cpu().numpy()) for x in (tk, tv))]
+        q = direction + 0.05 * c.rng.standard_normal((1, 6, d))
+        q = torch.from_numpy(q).cuda().to(c.tdt)
+        out = c.decode(q, 1.0, torch.zeros_like(q))
+        check_decode(c, rows, q, out, 1.0)
     finally:
         c.close()
