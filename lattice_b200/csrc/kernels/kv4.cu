@@ -496,42 +496,37 @@ struct Kv4Params {
   bool q_vec;  // every query row starts on 16 bytes
 };
 
-// Two codes of a word to f16: 0x6400 is 1024 with a unit of 1 in its last place, so a
-// nibble or-ed into bits 0-3 (4-7) adds n (16 n); the subtraction (multiply-add) that
-// leaves n - 8 is exact.  `base` is 0x64006400 in a register the compiler cannot see
-// through: with both constants immediate the and-or takes two instructions instead of one.
-__device__ __forceinline__ uint32_t low_codes(uint32_t w, uint32_t base) {
+// The values of two of a word's codes, nibbles I and I + 4, exactly, in T.  f16: 0x6400 is 1024
+// with a unit of 1 in its last place, so a nibble or-ed into bits 0-3 (4-7) adds n (16 n); the
+// subtraction (multiply-add) that leaves n - 8 is exact.  bf16: 0x4300 is 128 alike, for bits 0-3
+// alone.  `base` is that word in a register the compiler cannot see through: with both
+// constants immediate the and-or takes two instructions instead of one.
+template <typename T>
+__device__ __forceinline__ uint32_t code_base() {
+  uint32_t base;
+  if constexpr (std::is_same<T, __half>::value) {
+    asm volatile("mov.u32 %0, 0x64006400;" : "=r"(base));
+  } else {
+    asm volatile("mov.u32 %0, 0x43004300;" : "=r"(base));
+  }
+  return base;
+}
+template <typename T, int I>
+__device__ __forceinline__ uint32_t codes_of(uint32_t w, uint32_t base) {
+  constexpr bool kF16 = std::is_same<T, __half>::value;
+  constexpr int kShift = kF16 ? I / 2 * 8 : I * 4;
   uint32_t x;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w), "n"(0x000f000fu), "r"(base));
-  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0x64086408u));
-  return x;
-}
-__device__ __forceinline__ uint32_t high_codes(uint32_t w, uint32_t base) {
-  uint32_t x;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w), "n"(0x00f000f0u), "r"(base));
-  asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(x) : "r"(0x2c002c00u), "r"(0xd480d480u));
-  return x;
-}
-// D = A B (+ D), m16n8k16 f16
-__device__ __forceinline__ void mma_zero(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
-      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
-__device__ __forceinline__ void mma_add(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
-      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// The code's value, exactly, as bf16: two of a word's codes at 4 bits in each half (the others
-// masked away).  0x4300 is 128 with a unit of 1 in its last place.
-__device__ __forceinline__ uint32_t bf16_codes(uint32_t w, uint32_t base) {
-  uint32_t x;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w), "n"(0x000f000fu), "r"(base));
-  asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0x43084308u));
+  if constexpr (kF16 && I % 2 == 1) {
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w >> kShift), "n"(0x00f000f0u), "r"(base));
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(x) : "r"(0x2c002c00u), "r"(0xd480d480u));
+  } else {
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w >> kShift), "n"(0x000f000fu), "r"(base));
+    if constexpr (kF16) {
+      asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0x64086408u));
+    } else {
+      asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0x43084308u));
+    }
+  }
   return x;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -695,7 +690,10 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
     continue;
   }
 
-  // ---- the query rows (used below; loaded first, their latency overlaps the addresses') ----
+  // ---- Q as the B operand (columns = heads) -------------------------------------------------
+  // In its own type, as it is: brought into f16's range by a power of two a row, as an earlier
+  // form had it for 2.8 us of 63 less, it lost dims 2^-20 below the row's largest, however large
+  // the keys there.  Loaded first: its latency overlaps the addresses'.
   __align__(16) T q_raw[NG][8];
   const T *src = static_cast<const T *>(p.q) + int64_t(b) * p.q_sb +
                  int64_t(lo + min(g, G - 1)) * p.q_sh + c * 8;
@@ -762,36 +760,13 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
   };
   for (int k = 0; k < kStages && k < n_w; ++k) issue(k, (st + k) % kStages);
 
-  // ---- Q as the B operand (columns = heads), scaled per head by a power of two --------
-  // f16 for both input types: with the row's largest magnitude brought into [64, 128) every
-  // bf16 or f16 value is exact down to 2^-20 of that, and nothing overflows.
   uint32_t qb[NG][4];
-  float s_scale[2];
-  const int h = g;
-  float x[NG][8];
-  float mx = 0.f;
-#pragma unroll
-  for (int j = 0; j < NG; ++j) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[j][e] = h < G ? ptx::to_f32(q_raw[j][e]) : 0.f;
-      mx = fmaxf(mx, fabsf(x[j][e]));
-    }
-  }
-  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-  const int ex = max(int((__float_as_uint(mx) >> 23) & 255u) - 127, -100);
-  const float up = __uint_as_float(uint32_t(127 + 6 - ex) << 23);
-  const float down = __uint_as_float(uint32_t(127 - 6 + ex) << 23) * p.scale_log2;
 #pragma unroll
   for (int j = 0; j < NG; ++j) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      qb[j][i] = ptx::Mma<__half>::pack(x[j][2 * i] * up, x[j][2 * i + 1] * up);
+      qb[j][i] = g < G ? reinterpret_cast<const uint32_t *>(q_raw[j])[i] : 0u;
   }
-  // this lane's score columns are heads 2c and 2c+1
-  s_scale[0] = __shfl_sync(0xffffffffu, down, (2 * c) * 4);
-  s_scale[1] = __shfl_sync(0xffffffffu, down, (2 * c + 1) * 4);
 
   float o[2 * NG][4];  // O transposed: rows = dims, columns = heads
 #pragma unroll
@@ -800,9 +775,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
   m[0] = m[1] = kNoMax;
   l[0] = l[1] = 0.f;
   bool failed = false;
-  uint32_t base, v_base;
-  asm volatile("mov.u32 %0, 0x64006400;" : "=r"(base));
-  asm volatile("mov.u32 %0, 0x43004300;" : "=r"(v_base));
+  using B = __nv_bfloat16;  // of the second product
+  const uint32_t k_base = code_base<T>(), v_base = code_base<B>();
 
   for (int k = 0; k < n_w; ++k) {
     const int u = first_unit + k * (kWarps * NU);
@@ -842,14 +816,14 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         const uint32_t w0 = kw[2 * j], w1 = kw[2 * j + 1];
-        const uint32_t a0[4] = {low_codes(w0, base), low_codes(w1, base), high_codes(w0, base),
-                                high_codes(w1, base)};
-        const uint32_t a1[4] = {low_codes(w0 >> 8, base), low_codes(w1 >> 8, base),
-                                high_codes(w0 >> 8, base), high_codes(w1 >> 8, base)};
+        const uint32_t a0[4] = {codes_of<T, 0>(w0, k_base), codes_of<T, 0>(w1, k_base),
+                                codes_of<T, 1>(w0, k_base), codes_of<T, 1>(w1, k_base)};
+        const uint32_t a1[4] = {codes_of<T, 2>(w0, k_base), codes_of<T, 2>(w1, k_base),
+                                codes_of<T, 3>(w0, k_base), codes_of<T, 3>(w1, k_base)};
         const float k0 = k_scale<NG>(ks, 0, j), k1 = k_scale<NG>(ks, 1, j);
-        float acc[4];
-        mma_zero(acc, a0, qb[j][0], qb[j][1]);
-        mma_add(acc, a1, qb[j][2], qb[j][3]);
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        ptx::Mma<T>::run(acc, a0, qb[j][0], qb[j][1]);
+        ptx::Mma<T>::run(acc, a1, qb[j][2], qb[j][3]);
         float *sr = s[r];
         if (j == 0) {
           sr[0] = acc[0] * k0;
@@ -864,7 +838,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[r][i] *= s_scale[i & 1];
+      for (int i = 0; i < 4; ++i) s[r][i] *= p.scale_log2;
     }
     alignas(16) uint32_t vs[NU][2 * NG];  // V's scales [group][token pair (2c, 2c+1) + 8 i]
 #pragma unroll
@@ -966,10 +940,10 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         const uint32_t w0 = vw[2 * j], w1 = vw[2 * j + 1];
-        const uint32_t a0[4] = {bf16_codes(w0, v_base), bf16_codes(w0 >> 4, v_base),
-                                bf16_codes(w1, v_base), bf16_codes(w1 >> 4, v_base)};
-        const uint32_t a1[4] = {bf16_codes(w0 >> 8, v_base), bf16_codes(w0 >> 12, v_base),
-                                bf16_codes(w1 >> 8, v_base), bf16_codes(w1 >> 12, v_base)};
+        const uint32_t a0[4] = {codes_of<B, 0>(w0, v_base), codes_of<B, 1>(w0, v_base),
+                                codes_of<B, 0>(w1, v_base), codes_of<B, 1>(w1, v_base)};
+        const uint32_t a1[4] = {codes_of<B, 2>(w0, v_base), codes_of<B, 3>(w0, v_base),
+                                codes_of<B, 2>(w1, v_base), codes_of<B, 3>(w1, v_base)};
         uint32_t hi[2], lo[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -977,13 +951,13 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
           const float x0 = pt[r][2 * i] * bf16_lo(sc), x1 = pt[r][2 * i + 1] * bf16_hi(sc);
           const uint32_t b0 = __float_as_uint(x0), b1 = __float_as_uint(x1);
           hi[i] = high_halves(b0, b1);
-          lo[i] = ptx::Mma<__nv_bfloat16>::pack(x0 - __uint_as_float(b0 & 0xffff0000u),
-                                                x1 - __uint_as_float(b1 & 0xffff0000u));
+          lo[i] = ptx::Mma<B>::pack(x0 - __uint_as_float(b0 & 0xffff0000u),
+                                    x1 - __uint_as_float(b1 & 0xffff0000u));
         }
-        ptx::Mma<__nv_bfloat16>::run(o[2 * j], a0, hi[0], hi[1]);
-        ptx::Mma<__nv_bfloat16>::run(o[2 * j + 1], a1, hi[0], hi[1]);
-        ptx::Mma<__nv_bfloat16>::run(o[2 * j], a0, lo[0], lo[1]);
-        ptx::Mma<__nv_bfloat16>::run(o[2 * j + 1], a1, lo[0], lo[1]);
+        ptx::Mma<B>::run(o[2 * j], a0, hi[0], hi[1]);
+        ptx::Mma<B>::run(o[2 * j + 1], a1, hi[0], hi[1]);
+        ptx::Mma<B>::run(o[2 * j], a0, lo[0], lo[1]);
+        ptx::Mma<B>::run(o[2 * j + 1], a1, lo[0], lo[1]);
       }
     }
     __syncwarp();

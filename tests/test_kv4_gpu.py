@@ -418,3 +418,26 @@ def test_decode_loud_token_of_little_weight(at, low, loud):
         check_decode(c, rows, q, out, 1.0)
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("dtype,apart", [("bf16", 12), ("bf16", 24), ("bf16", 40), ("f16", 12),
+                                         ("f16", 20)])
+def test_decode_queries_and_keys_far_apart(dtype, apart):
+    """Dims where the query is small and the keys are large count like the others."""
+    torch = torch_cuda()
+    n, hkv, d = 300, 2, 128
+    c = Cache([n, 33], hkv, d, kv4=True, dtype=dtype, seed=apart)
+    try:
+        low = np.where(np.arange(d) < 64, 2.0 ** -apart, 1.0) * (2.0 ** 8 if dtype == "f16" else 1)
+        rows = []
+        for b, m in enumerate(c.lens):
+            k = c.rng.standard_normal((m, hkv, d)) / low
+            v = c.rng.standard_normal((m, hkv, d))
+            tk, tv = (torch.from_numpy(x).cuda().to(c.tdt) for x in (k, v))
+            c.write(tk, tv, c.slots(b, np.arange(m)))
+            rows.append(tuple(quantised(x.double().cpu().numpy()) for x in (tk, tv)))
+        q = torch.from_numpy(c.rng.standard_normal((2, 8, d)) * low).cuda().to(c.tdt)
+        out = c.decode(q, d ** -0.5, torch.zeros_like(q))
+        check_decode(c, rows, q, out, d ** -0.5)
+    finally:
+        c.close()
