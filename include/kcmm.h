@@ -622,6 +622,8 @@ typedef enum {
  *   next_positions       int32 [batch]: the position the next token will have
  *   kept_lens            int32 [batch]: slots with a stored position (new_lens of the last
  *                        eviction; 0 before the first)
+ *   new_lens             int32 [batch]; in the call for the last layer, the same array as
+ *                        kept_lens or seq_lens (the other layers' calls read their old values)
  * All arrays are device arrays.  Blocks shared with other sequences must be made private
  * first (kcmm_cow_blocks_on_stream): their rows are overwritten.  After the last layer,
  * kcmm_truncate_sequence returns the blocks past the budget.  seq_lens[b] above row_stride

@@ -39,15 +39,18 @@ constexpr int kMaxCluster = 8;
 constexpr int kSliceTokens = 4096;
 constexpr int kKeyCapacity = 49152;  // keys in shared memory: 192 KB
 
-// One row's moves: count, then [budget] each of destination and source slots.
+// One row's moves: count, then [budget] each of destination and source slots; and its sequence's
+// new length, which the move kernel passes on: here other CTAs still read the arrays that the
+// caller may have given for it (kept_lens, seq_lens).
 struct RowMoves {
-  int32_t *count, *dst, *src;
+  int32_t *count, *new_len, *dst, *src;
 };
 __device__ __forceinline__ RowMoves row_moves(const EvictArgs &a, int row) {
   const int64_t rows = int64_t(a.batch) * a.kv_heads, at = int64_t(row) * a.budget;
   RowMoves r;
   r.count = a.scratch + row;
-  r.dst = a.scratch + rows + at;
+  r.new_len = a.scratch + rows + row / a.kv_heads;
+  r.dst = a.scratch + rows + a.batch + at;
   r.src = r.dst + rows * a.budget;
   return r;
 }
@@ -115,14 +118,14 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   if (n > a.max_tokens || n > a.w_stride) {  // more tokens than the arguments hold
     if (rank == 0 && tid == 0) {
       mv.count[0] = 0;
-      if (g == 0) a.new_lens[b] = n;
+      if (g == 0) *mv.new_len = n;
       atomicOr(a.diag, int32_t(kDiagBadLaunch));
     }
     return;
   }
   if (rank == 0 && tid == 0) {
     mv.count[0] = 0;
-    if (g == 0) a.new_lens[b] = min(n, a.budget);
+    if (g == 0) *mv.new_len = min(n, a.budget);
   }
   if (n <= a.budget) {  // uniform over the cluster
     for (int i = rank * kSelectThreads + tid; i < n; i += C * kSelectThreads) {
@@ -432,6 +435,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
   const int b = blockIdx.z, g = blockIdx.y, lane = threadIdx.x & 31;
   const RowMoves mv = row_moves(a, b * a.kv_heads + g);
   const int moves = mv.count[0];
+  if (blockIdx.x == 0 && g == 0 && threadIdx.x == 0) a.new_lens[b] = *mv.new_len;
   const int warps = int(gridDim.x) * (kMoveThreads / 32);
   for (int j0 = (int(blockIdx.x) * (kMoveThreads / 32) + int(threadIdx.x >> 5)) * a.warp_moves;
        j0 < moves; j0 += warps * a.warp_moves) {
@@ -507,7 +511,8 @@ cudaError_t evict_tokens(const EvictArgs &args, cudaStream_t stream) {
   EvictArgs a = args;
   const int rows = a.batch * a.kv_heads;
   CallScratch scratch;
-  cudaError_t e = scratch.acquire(stream, (size_t(rows) + size_t(rows) * a.budget * 2) * 4);
+  cudaError_t e = scratch.acquire(
+      stream, (size_t(rows) + a.batch + size_t(rows) * a.budget * 2) * 4);
   if (e != cudaSuccess) return e;
   a.scratch = static_cast<int32_t *>(scratch.ptr);
   // CTAs of a row's cluster: as many as leave each kSliceTokens, while they all run at once.

@@ -260,3 +260,28 @@ def test_evict_rows_past_the_keys_that_shared_memory_holds():
         e.check(2000, 4, 100, before)
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("lens,hkv,budget,kept", [
+    ([90, 100, 57, 20], 16, 60, [60, 90, 57, 0]), ([17003, 16500], 4, 16384, [16384, 100]),
+    ([9000] * 3, 60, 4000, [4000, 0, 9000])])
+@pytest.mark.parametrize("shared", ["kept", "seq_lens", "nxt"])
+def test_evict_new_lens_in_place(lens, hkv, budget, kept, shared):
+    """new_lens in the array of the last eviction's, or of the lengths: every head and every CTA
+    of a row sees the old values."""
+    c = Cache(lens, hkv, 64, seed=21)
+    try:
+        c.fill_rows()
+        e = Evict(c, max(lens), kept=kept, gap=300, seed=22)
+        before = e.snapshot()
+        torch = torch_cuda()
+        array = {"kept": torch.from_numpy(e.kept).cuda(), "nxt": torch.from_numpy(e.nxt).cuda(),
+                 "seq_lens": c.d_lens.clone()}[shared]
+        name = {"kept": "kept_lens_ptr", "nxt": "next_positions_ptr",
+                "seq_lens": "seq_lens_ptr"}[shared]
+        e.run(budget, 3, 16, new_lens_ptr=array.data_ptr(), **{name: array.data_ptr()})
+        assert bool((e.new == -1).all())
+        e.new = array
+        e.check(budget, 3, 16, before)
+    finally:
+        c.close()
