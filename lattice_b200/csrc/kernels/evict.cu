@@ -530,7 +530,9 @@ cudaError_t evict_tokens(const EvictArgs &args, cudaStream_t stream) {
   void (*fn)(const EvictArgs) = C > 1            ? evict_select_kernel<512, true>
                                 : threads == 512 ? evict_select_kernel<512, false>
                                                  : evict_select_kernel<1024, false>;
-  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // The attribute belongs to the kernel, not to the launch: always the largest, so that a call of
+  // another width on another thread does not lower it between here and the launch.
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeyCapacity * 4);
   if (e != cudaSuccess) {
     scratch.release(stream);
     return e;

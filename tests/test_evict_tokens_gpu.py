@@ -285,3 +285,53 @@ def test_evict_new_lens_in_place(lens, hkv, budget, kept, shared):
         e.check(budget, 3, 16, before)
     finally:
         c.close()
+
+
+def test_evict_from_two_threads():
+    """Calls of different widths at the same time, each thread on a stream of its own."""
+    import threading
+
+    torch = torch_cuda()
+    errors = []
+    caches = [Cache([n], 80, 8, seed=n) for n in (4800, 45001)]
+    try:
+        evicts = []
+        for c in caches:
+            c.fill_rows()
+            e = Evict(c, int(c.lens[0]), seed=1)
+            e.run(600, 4, 100)
+            want = [x.clone() for x in (e.w_out, e.p_out, e.new)]
+            evicts.append((c, e, want))
+
+        def work(c, e, want):
+            stream = torch.cuda.Stream()
+            try:
+                for _ in range(1500):
+                    c.pool.evict_tokens(
+                        0, head_dim=8, block_tables_ptr=c.d_tables.data_ptr(),
+                        seq_lens_ptr=c.d_lens.data_ptr(),
+                        block_offsets_f16_ptr=c.d_offsets.data_ptr(), batch=1,
+                        max_blocks_per_seq=c.max_bps, budget=600, sinks=4, recent=100,
+                        weights_in_ptr=e.d["w"].data_ptr(), weights_out_ptr=e.w_out.data_ptr(),
+                        weights_row_stride=e.stride, positions_in_ptr=e.d["p"].data_ptr(),
+                        positions_out_ptr=e.p_out.data_ptr(),
+                        next_positions_ptr=e.d["nxt"].data_ptr(),
+                        kept_lens_ptr=e.d["kept"].data_ptr(), new_lens_ptr=e.new.data_ptr(),
+                        stream_ptr=stream.cuda_stream)
+                stream.synchronize()
+            except Exception as err:  # noqa: BLE001
+                errors.append(str(err))
+
+        threads = [threading.Thread(target=work, args=x) for x in evicts]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not errors
+        for c, e, want in evicts:
+            for got, x in zip((e.w_out, e.p_out, e.new), want):
+                assert torch.equal(got, x)
+            assert c.pool.kernel_status() == 0
+    finally:
+        for c in caches:
+            c.close()
