@@ -1134,7 +1134,8 @@ size_t decode_scratch_bytes(const DecodeArgs &a) { return make_plan(a).scratch_b
 // overlap the previous merge (programmatic dependent launch).  Calls on one
 // stream run in order, and each kernel waits for the previous one before it
 // touches memory, so they can share one buffer; a larger call replaces it in
-// stream order.  Streams are keyed by cudaStreamGetId (never reused in a
+// stream order.  `hold` locks it for the call: the launches of calls that two
+// threads make on one stream do not interleave.  Streams are keyed by cudaStreamGetId (never reused in a
 // process).  Returns null while the stream is being captured (a graph may be
 // replayed on any stream) or once kMaxCachedStreams streams hold a buffer: the
 // caller then allocates for the call alone.
@@ -1143,7 +1144,7 @@ constexpr size_t kMaxCachedStreams = 16;
 // Every buffer starts with kZeroedCounters zeroed words that the bytes asked for follow.
 constexpr size_t kCounterBytes = size_t(kZeroedCounters) * sizeof(int32_t);
 
-void *stream_scratch(cudaStream_t stream, size_t bytes) {
+void *stream_scratch(cudaStream_t stream, size_t bytes, std::unique_lock<std::mutex> *hold) {
   cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(stream, &cs) != cudaSuccess) {
     cudaGetLastError();
@@ -1157,19 +1158,25 @@ void *stream_scratch(cudaStream_t stream, size_t bytes) {
     return nullptr;
   }
   struct Entry {
+    std::mutex busy;
     void *ptr = nullptr;
     size_t bytes = 0;
   };
   static std::mutex mu;
   static std::map<std::pair<int, unsigned long long>, Entry> cache;
-  std::lock_guard<std::mutex> g(mu);
+  std::unique_lock<std::mutex> lookup(mu);
   auto it = cache.find({dev, id});
   if (it == cache.end()) {
     if (cache.size() >= kMaxCachedStreams) return nullptr;
-    it = cache.emplace(std::make_pair(dev, id), Entry{}).first;
+    it = cache.try_emplace(std::make_pair(dev, id)).first;
   }
-  Entry &en = it->second;
-  if (en.bytes >= bytes) return static_cast<char *>(en.ptr) + kCounterBytes;
+  Entry &en = it->second;  // entries stay where they are
+  lookup.unlock();
+  std::unique_lock<std::mutex> busy(en.busy);
+  if (en.bytes >= bytes) {
+    *hold = std::move(busy);
+    return static_cast<char *>(en.ptr) + kCounterBytes;
+  }
   cudaMemPool_t mp = scratch_pool(dev);
   if (!mp) return nullptr;
   void *fresh = nullptr;
@@ -1186,11 +1193,12 @@ void *stream_scratch(cudaStream_t stream, size_t bytes) {
   if (en.ptr) cudaFreeAsync(en.ptr, stream);
   en.ptr = fresh;
   en.bytes = want;
+  *hold = std::move(busy);
   return static_cast<char *>(fresh) + kCounterBytes;
 }
 
 cudaError_t CallScratch::acquire(cudaStream_t stream, size_t bytes) {
-  char *base = static_cast<char *>(stream_scratch(stream, bytes));
+  char *base = static_cast<char *>(stream_scratch(stream, bytes, &hold));
   if (base) {
     base -= kCounterBytes;
   } else {
@@ -1216,6 +1224,7 @@ cudaError_t CallScratch::acquire(cudaStream_t stream, size_t bytes) {
 }
 
 cudaError_t CallScratch::release(cudaStream_t stream) {
+  if (hold) hold.unlock();
   if (!owned) return cudaSuccess;
   owned = false;
   return cudaFreeAsync(counters, stream);
@@ -1270,11 +1279,12 @@ cudaError_t decode_attention(const DecodeArgs &a, cudaStream_t stream) {
 
   void *scratch = nullptr;
   bool owned = false;
+  std::unique_lock<std::mutex> hold;  // of the stream's buffer, until the merge is queued
   if (pl.scratch_bytes) {
     if (a.scratch) {
       if (a.scratch_bytes < pl.scratch_bytes) return cudaErrorInvalidValue;
       scratch = a.scratch;
-    } else if ((scratch = stream_scratch(stream, pl.scratch_bytes)) != nullptr) {
+    } else if ((scratch = stream_scratch(stream, pl.scratch_bytes, &hold)) != nullptr) {
       // kept for the stream
     } else {
       int dev = 0;
@@ -1531,11 +1541,12 @@ cudaError_t decode_attention_shared_prefix(const DecodeArgs &a, const int32_t *g
 
   void *scratch = nullptr;
   bool owned = false;
+  std::unique_lock<std::mutex> hold;  // of the stream's buffer, until the merge is queued
   cudaError_t e = cudaSuccess;
   if (a.scratch) {
     if (a.scratch_bytes < pl.scratch_bytes) return cudaErrorInvalidValue;
     scratch = a.scratch;
-  } else if ((scratch = stream_scratch(stream, pl.scratch_bytes)) == nullptr) {
+  } else if ((scratch = stream_scratch(stream, pl.scratch_bytes, &hold)) == nullptr) {
     e = scratch_acquire(a, pl.scratch_bytes, stream, &scratch, &owned);
     if (e != cudaSuccess) return e;
   }

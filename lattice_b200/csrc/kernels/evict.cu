@@ -412,8 +412,9 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
 constexpr int kMoveThreads = 256;
 
 // First byte of head g's row (16-bit cache) or chunk (4-bit cache) of slot i, and the
-// token's place in its chunk; null where the table or the offset is bad.
+// token's place in its chunk; -1 where the slot, the table or the offset is bad.
 __device__ __forceinline__ int64_t slot_bytes(const EvictArgs &a, int b, int g, int i, int *t) {
+  if (uint32_t(i) >= uint32_t(a.max_tokens)) return -1;
   const int page = i / a.block_size, in = i - page * a.block_size;
   const int blk = a.tables[int64_t(b) * a.bt_stride + page];
   if (blk < 0) return -1;

@@ -1663,9 +1663,10 @@ cudaError_t paged_prefill(const PrefillArgs &a, cudaStream_t stream) {
       int nsplit = 1;
       if (rem > 0 && !(sp && std::strcmp(sp, "0") == 0)) nsplit = std::min(4, sms / rem);
       float *part = nullptr;
+      std::unique_lock<std::mutex> hold;  // of the stream's buffer, until the merge is queued
       if (nsplit > 1) {
         const size_t bytes = size_t(rem) * nsplit * 256 * (kHd + 2) * sizeof(float);
-        part = static_cast<float *>(stream_scratch(stream, bytes));
+        part = static_cast<float *>(stream_scratch(stream, bytes, &hold));
         if (!part) nsplit = 1;  // no per-stream buffer (e.g. under graph capture)
       }
       wp.nqt = nqt;

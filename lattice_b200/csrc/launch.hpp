@@ -6,6 +6,7 @@
 
 #include <cstdint>
 #include <cuda_runtime.h>
+#include <mutex>
 
 namespace kcmm {
 namespace dev {
@@ -197,13 +198,16 @@ struct BeamGatherArgs {
 cudaError_t beam_gather(const BeamGatherArgs &a, cudaStream_t stream);
 
 // Scratch of one call: the stream's kept buffer where there is one (stream_scratch), else
-// a stream-ordered allocation that release() frees in stream order.
+// a stream-ordered allocation that release() frees in stream order.  No other call takes the
+// buffer between acquire() and release() (or this object's end): launches in between may hand
+// results to each other through it, whatever other threads queue on the stream.
 // `counters` are kZeroedCounters 32-bit zeros: a kernel that raises some leaves them zero.
 constexpr int kZeroedCounters = 65536;
 struct CallScratch {
   void *ptr = nullptr;
   int32_t *counters = nullptr;
   bool owned = false;
+  std::unique_lock<std::mutex> hold;
   cudaError_t acquire(cudaStream_t stream, size_t bytes);
   cudaError_t release(cudaStream_t stream);
 };
@@ -214,7 +218,8 @@ int device_sm_count();
 // decode split merge and the prefill tail split.  Calls on one stream share it in stream
 // order.  Null while the stream is being captured or once the per-process stream cache is
 // full; the caller then allocates for the call, or skips the split.
-void *stream_scratch(cudaStream_t stream, size_t bytes);
+// `hold` keeps other calls from the buffer: until it is released, after the call's last launch.
+void *stream_scratch(cudaStream_t stream, size_t bytes, std::unique_lock<std::mutex> *hold);
 
 // All-gather over NVLink peer memory (kernels/peer.cu).  dst[r] is rank r's
 // gathered buffer (two halves of world slices of nbytes, P2P-accessible from
