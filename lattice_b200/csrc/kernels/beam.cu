@@ -10,7 +10,11 @@
 // maximum, its sum of exponentials and its n largest logits: the n-th largest of its warps'
 // maxima (its threads', where n is above 8) bounds those from below, so that a second look at
 // the registers leaves little more than n to sort.  The last CTA of a request scores and ranks
-// its beams x chunks x n candidates in the same way.  Bounds from all threads' maxima cost a
+// its beams x chunks x n candidates in the same way.  Different logits can round to one score
+// (scores of -inf, or large beside the logits' steps), and then the lower token comes first though
+// its logit is the smaller one: each chunk also says how large its largest logit off the list is,
+// and where that one's score equals the n-th best the last CTA looks the ties up in the
+// logits themselves.  Bounds from all threads' maxima cost a
 // second pass wherever 16-bit maxima were equal: 24.4 us against 17.1 for 16 requests of 4
 // beams over 128,256 bf16 logits, the gathers of histories and tables included.
 //
@@ -81,6 +85,22 @@ __device__ __forceinline__ float half_of(uint32_t x, int e) {  // the low or hig
     return __half2float(__ushort_as_half(uint16_t(x >> (16 * e))));
   } else {
     return __uint_as_float(e ? x & 0xffff0000u : x << 16);
+  }
+}
+
+// The value of T next below x (a finite value of T); below the lowest one -inf.
+template <typename T>
+__device__ __forceinline__ float next_below(float x) {
+  if constexpr (sizeof(T) == 4) {
+    return key_value(value_key(x) - 1);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const uint32_t u = __half_as_ushort(__float2half_rn(x));
+    const uint32_t y = (u & 0x7fffu) == 0 ? 0x8001u : u & 0x8000u ? u + 1 : u - 1;
+    return __half2float(__ushort_as_half(uint16_t(y)));
+  } else {
+    const uint32_t u = __float_as_uint(x) >> 16;
+    const uint32_t y = (u & 0x7fffu) == 0 ? 0x8001u : u & 0x8000u ? u + 1 : u - 1;
+    return __uint_as_float(y << 16);
   }
 }
 
@@ -163,11 +183,95 @@ __device__ uint32_t nth_value(uint32_t mine, int n, TopShared *sh) {
   return uint32_t(sh->bound);
 }
 
+// 32-bit score of a logit x of a beam with (maximum, log of the sum) norm.
+__device__ __forceinline__ float score_of(float x, float2 norm, float score_in) {
+  const float s = x == -INFINITY ? -INFINITY : ((x - norm.x) - norm.y) + score_in;
+  return s == s ? s : -INFINITY;
+}
+
+// best[above .. n): the lowest of request b's (beam, token) whose score's key is `want`, looked up
+// in all its logits.  Rare: see the check in beam_best.
+template <typename T>
+__device__ __noinline__ void lowest_ties(const BeamArgs &a, int b, uint32_t want, int above,
+                                         const float2 *norm, unsigned long long *best) {
+  constexpr int kEach = 8;  // tokens of a thread at a time
+  __shared__ int s_found[kWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int found = above;
+  for (int k = 0; k < a.beams && found < a.n; ++k) {
+    const int row = b * a.beams + k;
+    const bool finished = a.finished && a.finished[row];
+    const float score_in = a.scores_in[row];
+    const float2 nrm = norm[k];
+    if (!finished && value_key(score_of(nrm.x, nrm, score_in)) < want) continue;  // all lower
+    const T *x = static_cast<const T *>(a.logits) + int64_t(row) * a.row_stride;
+    for (int base = 0; base < a.vocab && found < a.n; base += kThreads * kEach) {
+      const int v0 = base + tid * kEach;
+      uint32_t hit = 0;
+      for (int e = 0; e < kEach && v0 + e < a.vocab; ++e) {
+        float s;
+        if (finished) {
+          s = uint32_t(v0 + e) == a.eos ? score_in : -INFINITY;
+          s = s == s ? s : -INFINITY;
+        } else {
+          uint32_t bits;
+          if constexpr (sizeof(T) == 4) {
+            bits = reinterpret_cast<const uint32_t *>(x)[v0 + e];
+          } else {
+            bits = reinterpret_cast<const uint16_t *>(x)[v0 + e];
+          }
+          bits = clean(bits, T());
+          float v;
+          if constexpr (sizeof(T) == 4) {
+            v = __uint_as_float(bits);
+          } else {
+            v = half_of<T>(bits, 0);
+          }
+          s = score_of(v, nrm, score_in);
+        }
+        hit |= value_key(s) == want ? 1u << e : 0u;
+      }
+      int sum = __popc(hit);
+      const int mine = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
+      }
+      __syncthreads();  // the last round's reads
+      if (lane == 31) s_found[warp] = sum;
+      __syncthreads();
+      int at = found + sum - mine, all = 0;
+      for (int w = 0; w < kWarps; ++w) {
+        at += w < warp ? s_found[w] : 0;
+        all += s_found[w];
+      }
+      for (; hit != 0 && at < a.n; hit &= hit - 1, ++at)
+        best[at] = (static_cast<unsigned long long>(want) << 32) |
+                   (0xffffffffu - (uint32_t(k) * uint32_t(a.vocab) + v0 + __ffs(int(hit)) - 1));
+      found += all;
+    }
+  }
+  __syncthreads();
+}
+
 // One CTA's part of the choice: the last one of request b.
+template <typename T>
 __device__ void beam_best(const BeamArgs &a, int b, TopShared *sh, unsigned long long *list) {
   __shared__ float2 s_norm[kBeamMaxBeams];  // max, log of the sum
   __shared__ unsigned long long s_best[kMaxSelect];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // the n-th listed and the largest unlisted logit of chunk i, for the check at the end; the
+  // thread's first chunk's are loaded here, ahead of everything that waits
+  const int64_t chunk0 = int64_t(b) * a.beams * a.chunks;
+  auto nth_of = [&](int i) { return __ldcg(a.cand + (chunk0 + i) * a.n + a.n - 1); };
+  auto rest_of = [&](int i) { return __ldcg(a.rest + chunk0 + i); };
+  unsigned long long first_nth = 0;
+  float first_rest = 0.f;
+  if (tid < a.beams * a.chunks) {
+    first_nth = nth_of(tid);
+    first_rest = rest_of(tid);
+  }
   for (int k = warp; k < a.beams; k += kWarps) {
     const int row = b * a.beams + k;
     if (a.finished && a.finished[row]) continue;
@@ -206,7 +310,7 @@ __device__ void beam_best(const BeamArgs &a, int b, TopShared *sh, unsigned long
       if (c == 0ull) return 0ull;
       token = key_index(c);
       const float x = key_value(uint32_t(c >> 32));
-      score = x == -INFINITY ? -INFINITY : ((x - s_norm[k].x) - s_norm[k].y) + score;
+      score = score_of(x, s_norm[k], score);
     }
     if (!(score == score)) score = -INFINITY;
     return make_key(score, uint32_t(k) * uint32_t(a.vocab) + token);
@@ -294,6 +398,40 @@ __device__ void beam_best(const BeamArgs &a, int b, TopShared *sh, unsigned long
     done += min(count, left);
     cut = s_best[done - 1];
   }
+  // A chunk hides ties of the n-th best where its own n-th logit scores as much, and so does a
+  // smaller one off the list; or, where an equal one is off the list (its index is higher than
+  // those of its equals), a larger one on it does.
+  const uint32_t last = uint32_t(s_best[a.n - 1] >> 32);
+  bool hidden = false;
+  for (int i = tid; i < a.beams * a.chunks; i += kThreads) {
+    const int k = i / a.chunks, row = b * a.beams + k;
+    if (a.finished && a.finished[row]) continue;
+    const unsigned long long c = i == tid ? first_nth : nth_of(i);
+    const float rest = i == tid ? first_rest : rest_of(i), score_in = a.scores_in[row];
+    auto scores_last = [&](float x) {
+      return value_key(score_of(x, s_norm[k], score_in)) == last;
+    };
+    if (c == 0ull) continue;  // all of the chunk is on its list
+    const float nth = key_value(uint32_t(c >> 32));
+    if (!scores_last(nth)) continue;
+    if (rest < nth) {
+      hidden |= scores_last(rest);
+    } else {
+      hidden |= nth != -INFINITY && scores_last(next_below<T>(nth));
+      for (int j = a.n - 2; j >= 0; --j) {
+        const float x = key_value(uint32_t(__ldcg(a.cand + (chunk0 + i) * a.n + j) >> 32));
+        if (x == nth) continue;
+        hidden |= scores_last(x);
+        break;
+      }
+    }
+  }
+  if (__syncthreads_or(hidden)) {
+    int above = 0;
+    while (above < a.n && uint32_t(s_best[above] >> 32) != last) ++above;
+    __syncthreads();
+    lowest_ties<T>(a, b, last, above, s_norm, s_best);
+  }
   if (tid < done) {
     const unsigned long long k = s_best[tid];
     const uint32_t i = key_index(k);
@@ -306,12 +444,13 @@ __device__ void beam_best(const BeamArgs &a, int b, TopShared *sh, unsigned long
 
 // Grid (chunks, rows), a row being one beam of one request.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 5) beam_select_kernel(const BeamArgs a) {
+__global__ void __launch_bounds__(kThreads, 5) beam_select_kernel(const __grid_constant__ BeamArgs a) {
   constexpr int PER = 16 / sizeof(T);  // logits of a load
   constexpr int MOST = kVecs * PER;    // of a thread
   __shared__ TopShared sh;
   __shared__ unsigned long long s_list[kMaxSelect * MOST];
   __shared__ float s_red[kWarps], s_sum[kWarps];
+  __shared__ uint32_t s_below[kWarps];
   __shared__ int s_last;
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
@@ -425,6 +564,18 @@ __global__ void __launch_bounds__(kThreads, 5) beam_select_kernel(const BeamArgs
         if (at < kFewKeys) s_list[at] = k;
       });
     }
+    // the largest logit that does not
+    uint32_t below = value_key(mx);
+    if (reach != 0) {
+      below = 0;
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          if (!(reach >> (i * PER + e) & 1u)) below = max(below, value_key(value(i, e)));
+    }
+    below = __reduce_max_sync(0xffffffffu, below);
+    if (lane == 0) s_below[warp] = below;
     float sum = 0.f;
     if (m != -INFINITY) {
 #pragma unroll
@@ -442,7 +593,8 @@ __global__ void __launch_bounds__(kThreads, 5) beam_select_kernel(const BeamArgs
       a.part[int64_t(row) * a.chunks + chunk] = make_float2(m, total);
     }
     int count = sh.count;
-    if (count > kFewKeys) {
+    const bool crowded = count > kFewKeys;
+    if (crowded) {
       // the n-th largest of the threads' own largest keys is the bound: at most n threads, all
       // of whose logits fit, have keys that reach it
       __syncthreads();
@@ -457,6 +609,12 @@ __global__ void __launch_bounds__(kThreads, 5) beam_select_kernel(const BeamArgs
       count = sh.count;
     }
     unsigned long long *cand = a.cand + (int64_t(row) * a.chunks + chunk) * a.n;
+    float *rest = a.rest + int64_t(row) * a.chunks + chunk;  // largest logit off the list, or more
+    if (!crowded && count == a.n && tid == 0) {
+      uint32_t top = s_below[0];
+      for (int w = 1; w < kWarps; ++w) top = max(top, s_below[w]);
+      *rest = key_value(top);
+    }
     for (int i = tid; i < max(count, a.n); i += kThreads) {
       if (i >= count) {
         cand[i] = 0ull;  // fewer than n logits in the chunk
@@ -466,6 +624,7 @@ __global__ void __launch_bounds__(kThreads, 5) beam_select_kernel(const BeamArgs
       int larger = 0;
       for (int j = 0; j < count; ++j) larger += s_list[j] > k;
       if (larger < a.n) cand[larger] = k;
+      if (larger == (crowded ? a.n - 1 : a.n)) *rest = key_value(uint32_t(k >> 32));
     }
   }
   __syncthreads();
@@ -476,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 5) beam_select_kernel(const BeamArgs
     __threadfence();
   }
   __syncthreads();
-  if (s_last) beam_best(a, b, &sh, s_list);
+  if (s_last) beam_best<T>(a, b, &sh, s_list);
 }
 
 // dst row (b, j) = src row (b, parents[b, j]); with tokens, its entry token_index = tokens[b, j].
@@ -528,10 +687,11 @@ cudaError_t beam_select(const BeamArgs &args, cudaStream_t stream) {
   const int rows = a.batch * a.beams;
   const size_t cand_bytes = size_t(rows) * a.chunks * a.n * 8;
   CallScratch scratch;
-  cudaError_t e = scratch.acquire(stream, cand_bytes + size_t(rows) * a.chunks * 8);
+  cudaError_t e = scratch.acquire(stream, cand_bytes + size_t(rows) * a.chunks * 12);
   if (e != cudaSuccess) return e;
   a.cand = static_cast<unsigned long long *>(scratch.ptr);
   a.part = reinterpret_cast<float2 *>(static_cast<char *>(scratch.ptr) + cand_bytes);
+  a.rest = reinterpret_cast<float *>(a.part + size_t(rows) * a.chunks);
   const dim3 grid(a.chunks, rows);
   a.counters = scratch.counters;
   e = launch_pdl(a.type == 0   ? beam_select_kernel<__half>

@@ -181,6 +181,7 @@ struct BeamArgs {
   int chunks;  // filled by the launcher, as the scratch arrays
   unsigned long long *cand;
   float2 *part;
+  float *rest;
   int32_t *counters;  // a zero per request: CTAs that are done
 };
 cudaError_t beam_select(const BeamArgs &a, cudaStream_t stream);

@@ -217,3 +217,67 @@ def test_reorder_copies_shared_tails():
                 assert torch.equal(got, want)
     finally:
         c.close()
+
+
+TYPES = ["f32", "bf16", "f16"]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [40, 900, 20000, 70001])
+@pytest.mark.parametrize("n", [1, 4, 8, 9, 40])
+def test_ties_of_beams_without_a_score(pool, dtype, V, n):
+    """Beams of score -inf or NaN over distinct logits: all their tokens tie, and the lowest come
+    first, after every candidate that has a score."""
+    torch = torch_cuda()
+    g = torch.Generator(device="cuda").manual_seed(V + n)
+    dt = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dtype]
+    logits = (2 * torch.randn(4, 3, V, device="cuda", generator=g)).to(dt)
+    scores = torch.full((4, 3), -float("inf"), device="cuda")
+    scores[1] = float("nan")
+    scores[2, 1] = -3.0  # one beam with 2 finite logits
+    logits[2, 1] = -float("inf")
+    logits[2, 1, [V // 3, V - 1]] = torch.tensor([1.0, 2.0], device="cuda", dtype=dt)
+    scores[3, 1] = -1.0  # a finished beam between two without a score
+    done = torch.zeros(4, 3, dtype=torch.uint8, device="cuda")
+    done[3, 1] = 1
+    check(pool, logits, scores, n, finished=done, eos=V // 2, dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [40, 20000, 70001])
+@pytest.mark.parametrize("n", [1, 4, 8, 33])
+def test_ties_by_rounding_of_the_score(pool, dtype, V, n):
+    """At scores of 1e9 all log-probabilities round away (a unit is 64): every token of the best
+    beams ties.  Units of 2^-10, at 1e4, join some neighbours and not others."""
+    torch = torch_cuda()
+    g = torch.Generator(device="cuda").manual_seed(V * 7 + n)
+    dt = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dtype]
+    for big in (1e9, 1e4):
+        if big == 1e9:
+            logits = (2 * torch.randn(3, 2, V, device="cuda", generator=g)).to(dt)
+            logits[0, 1, V // 2] = float("nan")
+            logits[1, 0, : V // 2] = -float("inf")
+        else:  # levels 1/4 apart, and in 32 bits 4 values within 2^-14 of each: one score
+            steps = torch.randint(0, 40, (3, 2, V), device="cuda", generator=g)
+            logits = (0.25 * steps.float() - 12).to(dt)
+            if dtype == "f32":
+                logits += torch.randint(0, 4, (3, 2, V), device="cuda", generator=g) * 2.0 ** -16
+        scores = torch.full((3, 2), -big, device="cuda")
+        scores[2, 0] = -2 * big
+        s, p, t = select(pool, logits, scores, n, dtype=dtype)
+        for b in range(3):
+            x = logits[b].double().cpu().numpy()
+            x = np.where(np.isnan(x), -np.inf, x)
+            m = x.max(-1, keepdims=True)
+            sc = scores[b].double().cpu().numpy()[:, None]
+            exact = x - (m + np.log(np.exp(x - m).sum(-1, keepdims=True))) + sc
+            unit = np.spacing(np.float32(big)) * (1.0 if b < 2 else 2.0)
+            fin = np.isfinite(exact)
+            if big == 1e4:  # a score this near a rounding boundary says nothing
+                off = np.abs(exact[fin] / unit - np.floor(exact[fin] / unit) - 0.5)
+                if off.min() < 0.02:
+                    continue
+            score = exact.astype(np.float32).reshape(-1)
+            top = np.lexsort((np.arange(score.size), -score))[:n]
+            assert np.array_equal(s[b], score[top])
+            assert np.array_equal(p[b], top // V) and np.array_equal(t[b], top % V)
