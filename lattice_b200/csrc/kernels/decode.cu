@@ -566,8 +566,9 @@ __device__ __forceinline__ bool decode_body(const DecodeParams &p, const int ite
       mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
       const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
       float e0 = mn0, e1 = mn1;  // exponent base
-      if constexpr (MODE == 1) {
-        // a row that has seen only masked keys keeps a zero sum and a max of -inf
+      if constexpr (MODE == 1 || SCORES) {
+        // a row that has seen only masked keys (scores of -inf) keeps a zero sum and a max of
+        // -inf; one that has seen a NaN has a sum of NaN
         if (e0 == -INFINITY) e0 = 0.f;
         if (e1 == -INFINITY) e1 = 0.f;
       }
@@ -676,7 +677,7 @@ __device__ __forceinline__ bool decode_body(const DecodeParams &p, const int ite
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       float mw = cm[w * 16 + h];
-      if (mw == -INFINITY) continue;  // warp saw no unit
+      if (mw == -INFINITY && !(SCORES && cl[w * 16 + h] != 0.f)) continue;  // warp saw no unit
       float sc = ptx::fast_exp2(mw - M);
       L += cl[w * 16 + h] * sc;
       x0 += cO[(w * 16 + h) * D + d] * sc;

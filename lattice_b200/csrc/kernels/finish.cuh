@@ -46,7 +46,9 @@ struct FinishParams {
 
 // Grid (token chunks, hkv, batch).  Every CTA computes the log-sum-exp of its group's
 // heads from the splits' (at most num_splits values a head), the first chunk's CTA merges
-// the outputs.  Sequences of length 0 are left untouched.
+// the outputs.  Sequences of length 0 are left untouched.  A split none of whose pages could be
+// read has log-sum-exp and scores of -inf and weighs nothing; where that is so of all of a row's
+// tokens its output is 0.
 template <typename T>
 __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const FinishParams p) {
   __shared__ float s_lse[kFinishMaxGroup];
@@ -63,14 +65,20 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const FinishPara
   for (int h = warp; h < G; h += kFinishThreads / 32) {
     const float *lse = p.part_lse + (int64_t(b) * p.hq + lo + h) * p.num_splits;
     float M = -INFINITY;
-    for (int s = lane; s < ns; s += 32) M = fmaxf(M, lse[s]);
+    bool nan = false;
+    for (int s = lane; s < ns; s += 32) {
+      M = fmaxf(M, lse[s]);
+      nan |= lse[s] != lse[s];
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    nan = __any_sync(0xffffffffu, nan);
     float sum = 0.f;
     for (int s = lane; s < ns; s += 32) sum += ptx::fast_exp2(lse[s] - M);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float total = M + log2f(sum);
+    // exp2(-inf - (+inf)) = 0
+    const float total = M == -INFINITY && !nan ? INFINITY : M + log2f(sum);
     if (lane == 0) s_lse[h] = total;
   }
   __syncthreads();
@@ -83,8 +91,10 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const FinishPara
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
       for (int s = 0; s < ns; ++s) {
-        const float w = ptx::fast_exp2(p.part_lse[row + s] - total);
-        const float4 v = *reinterpret_cast<const float4 *>(p.part_o + (row + s) * D + d);
+        const float lse = p.part_lse[row + s];
+        const float w = ptx::fast_exp2(lse - total);
+        float4 v = *reinterpret_cast<const float4 *>(p.part_o + (row + s) * D + d);
+        if (lse == -INFINITY) v = make_float4(0.f, 0.f, 0.f, 0.f);  // it normalised no tokens
         acc.x += v.x * w;
         acc.y += v.y * w;
         acc.z += v.z * w;

@@ -77,3 +77,56 @@ def test_long_rows_short_weights_and_a_stream():
         check_decode(c, rows, q, out, 0.125, w_in=before, w_out=w)
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("kv4", [False, True])
+def test_pages_that_cannot_be_read_weigh_nothing(kv4):
+    """Table entries of -1 are reported, and their tokens weigh nothing: all of a sequence's,
+    those of a whole split, single pages."""
+    from kv_cases import attention
+
+    torch = torch_cuda()
+    lens, d = [50, 6000, 50], 64
+    c = Cache(lens, 1, d, kv4=kv4, seed=9)
+    try:
+        rows = c.fill_rows()
+        c.d_tables[0] = -1
+        gone = np.zeros(6000, bool)
+        for first, last in ((1600, 4800), (160, 176), (5984, 6000)):
+            c.d_tables[1, first // 16: last // 16] = -1
+            gone[first:last] = True
+        q = torch.from_numpy(c.rng.standard_normal((3, 4, d))).cuda().to(c.tdt)
+        w_in = torch.rand(3, 1, 6000, device="cuda")
+        w_out = torch.full_like(w_in, -5.0)
+        out = c.decode(q, 0.125, torch.full_like(q, 7.0), w_in=w_in, w_out=w_out)
+        assert c.pool.kernel_status() == 2
+        assert torch.equal(w_out[0, 0, :50], w_in[0, 0, :50]) and bool((out[0] == 0).all())
+        for b, keep in ((1, ~gone), (2, np.ones(50, bool))):
+            k, v = (x[keep] for x in rows[b])
+            ref, mass, w = attention(q[b].double().cpu().numpy(), k, v, 0.125)
+            err = np.abs(out[b].double().cpu().numpy() - ref)
+            assert (err <= 1.25 * 2.0 ** -11 * mass + 2.0 ** -8 * np.abs(ref) + 1e-7).all()
+            step = np.zeros(lens[b])
+            step[keep] = w[0]
+            before, after = (x[b, 0, : lens[b]].double().cpu().numpy() for x in (w_in, w_out))
+            want = before + step
+            assert (np.abs(after - want) <= 2.0 ** -14 * step + 2.0 ** -23 * want + 1e-9).all()
+            assert np.array_equal(after[~keep], before[~keep])
+    finally:
+        c.close()
+
+
+def test_nan_scores_give_nan_weights():
+    torch = torch_cuda()
+    for kv4 in (False, True):
+        c = Cache([40, 40], 1, 64, kv4=kv4, seed=9)
+        try:
+            c.fill_rows()
+            q = torch.from_numpy(c.rng.standard_normal((2, 4, 64))).cuda().to(c.tdt)
+            q[0] = float("nan")
+            w = torch.zeros(2, 1, 40, device="cuda")
+            out = c.decode(q, 0.125, torch.zeros_like(q), w_in=w, w_out=w)
+            assert bool(torch.isnan(w[0]).all()) and bool(torch.isnan(out[0]).all())
+            assert bool(torch.isfinite(w[1]).all()) and bool(torch.isfinite(out[1]).all())
+        finally:
+            c.close()
