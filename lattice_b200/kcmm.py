@@ -754,6 +754,8 @@ class KcmmPool:
 
     def reorder_sequences(self, seq_indices, parents, stream_ptr: int = 0) -> None:
         """seq_indices[i] continues what seq_indices[parents[i]] holds now."""
+        if len(parents) != len(seq_indices):
+            raise ValueError(f"{len(seq_indices)} sequences have {len(parents)} parents")
         self._check(self.lib.kcmm_reorder_sequences_on_stream(
             self.handle, _u32_array(seq_indices), _u32_array(parents), len(seq_indices),
             stream_ptr), "kcmm_reorder_sequences_on_stream")

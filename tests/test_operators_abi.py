@@ -190,3 +190,12 @@ def test_reorder_sequences(host_pool_factory):
     assert state() == ([tables[1], tables[0], tables[2]], [32, 32, 16], 6, [1] * 6)
     pool.reorder_sequences(seqs, [1, 1, 2])  # table 1 is dropped, table 0 has two owners
     assert state() == ([tables[0], tables[0], tables[2]], [32, 32, 16], 4, [2, 2, 0, 0, 1, 1])
+
+
+def test_reorder_sequences_wants_a_parent_for_each(host_pool_factory):
+    """The library reads as many parents as there are sequences."""
+    pool = host_pool_factory(kv_heads=2, head_dim=64, max_batch=4, max_seq_len=64)
+    seqs = [pool.register_sequence(pool.alloc_blocks(1)) for _ in range(3)]
+    for parents in ([0, 1], [], [0, 1, 2, 0]):
+        with pytest.raises(ValueError, match="3 sequences"):
+            pool.reorder_sequences(seqs, parents)
