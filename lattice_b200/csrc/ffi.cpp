@@ -1177,9 +1177,10 @@ int kcmm_beam_gather_on_stream(kcmm_pool_t *h, uint64_t src, uint64_t dst, uint6
     set_error(h, std::string(op) + ": token_index lies past the row");
     return -1;
   }
-  const uint64_t src_bytes = uint64_t(batch) * beams * row_bytes;
-  const uint64_t dst_bytes = uint64_t(batch) * n * row_bytes;
-  if (src < dst + dst_bytes && dst < src + src_bytes) {
+  using Wide = unsigned __int128;  // the ends may lie past 64 bits
+  const Wide src_end = Wide(src) + Wide(batch) * beams * row_bytes;
+  const Wide dst_end = Wide(dst) + Wide(batch) * n * row_bytes;
+  if (src < dst_end && dst < src_end) {
     set_error(h, std::string(op) + ": src and dst must not overlap");
     return -1;
   }

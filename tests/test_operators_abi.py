@@ -199,3 +199,11 @@ def test_reorder_sequences_wants_a_parent_for_each(host_pool_factory):
     for parents in ([0, 1], [], [0, 1, 2, 0]):
         with pytest.raises(ValueError, match="3 sequences"):
             pool.reorder_sequences(seqs, parents)
+
+
+def test_beam_gather_sizes_past_64_bits(host_pool_factory):
+    """The source's 2^64 bytes hold the destination."""
+    pool = host_pool_factory(kv_heads=2, head_dim=64, max_batch=2, max_seq_len=64)
+    with pytest.raises(KcmmError, match="overlap"):
+        pool.beam_gather(**{**GATHER, "batch": 1, "beams": 1 << 30, "row_bytes": 1 << 34,
+                            "n_select": 1, "dst_ptr": 65536})
