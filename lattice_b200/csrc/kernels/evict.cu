@@ -39,19 +39,19 @@ constexpr int kMaxCluster = 8;
 constexpr int kSliceTokens = 4096;
 constexpr int kKeyCapacity = 49152;  // keys in shared memory: 192 KB
 
-// One row's moves: count, then [budget] each of destination and source slots; and its sequence's
+// One row's moves: count, then [most_moves] each of destination and source slots; its sequence's
 // new length, which the move kernel passes on: here other CTAs still read the arrays that the
 // caller may have given for it (kept_lens, seq_lens).
 struct RowMoves {
   int32_t *count, *new_len, *dst, *src;
 };
 __device__ __forceinline__ RowMoves row_moves(const EvictArgs &a, int row) {
-  const int64_t rows = int64_t(a.batch) * a.kv_heads, at = int64_t(row) * a.budget;
+  const int64_t rows = int64_t(a.batch) * a.kv_heads, at = int64_t(row) * a.most_moves;
   RowMoves r;
   r.count = a.scratch + row;
   r.new_len = a.scratch + rows + row / a.kv_heads;
   r.dst = a.scratch + rows + a.batch + at;
-  r.src = r.dst + rows * a.budget;
+  r.src = r.dst + rows * a.most_moves;
   return r;
 }
 
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   gt += __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[lane].gt : 0);
   eq += __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[lane].eq : 0);
   const int kept_lo = gt_lo + min(eq_lo, want);  // slots below the budget that stay
-  const int moves = a.budget - kept_lo;
+  const int moves = min(a.budget - kept_lo, a.most_moves);  // at most budget, and n - budget
 
   // ---- the lists of freed slots and of moving ones, by rank ------------------------------
   const uint32_t below = (1u << lane) - 1;
@@ -369,8 +369,9 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     const int eq_before = eq + __popc(eqs & below);
     const int kept_before = gt + __popc(gts & below) + min(eq_before, want);
     const bool keep = in && (k > threshold || (k == threshold && eq_before < want));
-    if (in && i < a.budget && !keep) mv.dst[i - kept_before] = i;
-    if (keep && i >= a.budget) mv.src[kept_before - kept_lo] = i;
+    const int at = i < a.budget ? i - kept_before : kept_before - kept_lo;
+    if (in && keep == (i >= a.budget) && uint32_t(at) < uint32_t(a.most_moves))
+      (keep ? mv.src : mv.dst)[at] = i;
     gt += __popc(gts);
     eq += __popc(eqs);
   }
@@ -511,9 +512,10 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
 cudaError_t evict_tokens(const EvictArgs &args, cudaStream_t stream) {
   EvictArgs a = args;
   const int rows = a.batch * a.kv_heads;
+  a.most_moves = std::min(a.budget, std::max(a.max_tokens - a.budget, 0));
   CallScratch scratch;
   cudaError_t e = scratch.acquire(
-      stream, (size_t(rows) + a.batch + size_t(rows) * a.budget * 2) * 4);
+      stream, (size_t(rows) + a.batch + size_t(rows) * a.most_moves * 2) * 4);
   if (e != cudaSuccess) return e;
   a.scratch = static_cast<int32_t *>(scratch.ptr);
   // CTAs of a row's cluster: as many as leave each kSliceTokens, while they all run at once.
@@ -555,7 +557,7 @@ cudaError_t evict_tokens(const EvictArgs &args, cudaStream_t stream) {
   e = cudaLaunchKernelEx(&cfg, fn, a);
   if (e == cudaSuccess) {
     // enough warps for every SM, none for moves that cannot be
-    const int most = std::min(a.budget, std::max(a.max_tokens - a.budget, 1));
+    const int most = std::max(a.most_moves, 1);
     // 8 a warp while that leaves warps idle: 35.2 -> 30.8 us for one row of 16,384 tokens cut to
     // half; 32 where there are many: 40.3 -> 32.0 us for 128 rows of 3700 cut to 1024
     a.warp_moves = int64_t(rows) * most <= int64_t(device_sm_count()) * 64 * 8 ? 8 : 32;

@@ -158,7 +158,8 @@ struct EvictArgs {
   const int32_t *kept_lens;       // [batch]
   int32_t *new_lens;              // [batch]
   int32_t *diag;
-  int32_t *scratch;  // filled by the launcher
+  int32_t *scratch;  // filled by the launcher, as what follows
+  int most_moves;    // of a row
   int key_capacity;  // keys that a CTA holds in shared memory
   int warp_moves;    // moves of a warp at a time
 };

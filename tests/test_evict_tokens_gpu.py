@@ -335,3 +335,17 @@ def test_evict_from_two_threads():
     finally:
         for c in caches:
             c.close()
+
+
+@pytest.mark.parametrize("budget", [4096, (1 << 31) - 1])
+def test_evict_budget_past_the_table(budget):
+    """No row can be cut: every sequence keeps its slots, and no lists are made for the budget."""
+    c = Cache([40, 700, 0, 64], 40, 64, seed=31)
+    try:
+        c.fill_rows()
+        e = Evict(c, 700, kept=[40, 12, 0, 0], gap=20, seed=32)
+        before = e.snapshot()
+        e.run(budget, 3, 16)
+        e.check(budget, 3, 16, before)
+    finally:
+        c.close()
