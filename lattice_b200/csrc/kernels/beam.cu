@@ -205,8 +205,8 @@ __device__ __noinline__ void lowest_ties(const BeamArgs &a, int b, uint32_t want
     const float2 nrm = norm[k];
     if (!finished && value_key(score_of(nrm.x, nrm, score_in)) < want) continue;  // all lower
     const T *x = static_cast<const T *>(a.logits) + int64_t(row) * a.row_stride;
-    for (int base = 0; base < a.vocab && found < a.n; base += kThreads * kEach) {
-      const int v0 = base + tid * kEach;
+    for (int64_t base = 0; base < a.vocab && found < a.n; base += kThreads * kEach) {
+      const int64_t v0 = base + tid * kEach;
       uint32_t hit = 0;
       for (int e = 0; e < kEach && v0 + e < a.vocab; ++e) {
         float s;
@@ -248,7 +248,8 @@ __device__ __noinline__ void lowest_ties(const BeamArgs &a, int b, uint32_t want
       }
       for (; hit != 0 && at < a.n; hit &= hit - 1, ++at)
         best[at] = (static_cast<unsigned long long>(want) << 32) |
-                   (0xffffffffu - (uint32_t(k) * uint32_t(a.vocab) + v0 + __ffs(int(hit)) - 1));
+                   (0xffffffffu -
+                    (uint32_t(k) * uint32_t(a.vocab) + uint32_t(v0) + __ffs(int(hit)) - 1));
       found += all;
     }
   }
@@ -683,7 +684,7 @@ cudaError_t beam_select(const BeamArgs &args, cudaStream_t stream) {
   // an unaligned row's first block starts before it
   const bool aligned = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 &&
                        a.row_stride * elem % 16 == 0;
-  a.chunks = int((a.vocab + (aligned ? 0 : 16 / elem - 1) + per - 1) / per);
+  a.chunks = int((int64_t(a.vocab) + (aligned ? 0 : 16 / elem - 1) + per - 1) / per);
   const int rows = a.batch * a.beams;
   const size_t cand_bytes = size_t(rows) * a.chunks * a.n * 8;
   CallScratch scratch;

@@ -281,3 +281,16 @@ def test_ties_by_rounding_of_the_score(pool, dtype, V, n):
             top = np.lexsort((np.arange(score.size), -score))[:n]
             assert np.array_equal(s[b], score[top])
             assert np.array_equal(p[b], top // V) and np.array_equal(t[b], top % V)
+
+
+def test_the_largest_vocabulary(pool):
+    """2^31 - 1 logits: the last few have equal scores in 32 bits and distinct logits."""
+    torch = torch_cuda()
+    V, n = (1 << 31) - 1, 3
+    logits = torch.full((1, 1, V), -float("inf"), device="cuda", dtype=torch.float16)
+    at = torch.tensor([V - 1000, V - 900, V - 30, V - 20, V - 1], device="cuda")
+    logits[0, 0, at] = torch.tensor([0.0, 1.0, 2.0, 3.0, 4.0], device="cuda", dtype=torch.float16)
+    for big, want in ((-1e9, at[:n]), (-3.0, at.flip(0)[:n])):
+        scores = torch.full((1, 1), big, device="cuda")
+        s, p, t = select(pool, logits, scores, n, dtype="f16")
+        assert np.array_equal(t[0], want.cpu().numpy()) and (p == 0).all()
