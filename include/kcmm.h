@@ -562,7 +562,8 @@ int kcmm_kv4_read_f16_on_stream(
  * float32, [batch][kv_heads] rows of weights_row_stride entries (tokens past the stride get
  * none; entries t >= seq_lens[b] are neither read nor written).  in and out may be the same
  * array.  The 4-bit decode takes weights pointers of 0 for none.  The scratch holds the
- * scores, 4 bytes for each query head and token of batch x max_blocks_per_seq x block_size.
+ * scores, 4 bytes for each query head and token of batch x max_blocks_per_seq x block_size, and
+ * is kept for the stream's later calls: tables as wide as the longest sequence keep it small.
  */
 int kcmm_kv4_paged_attn_decode_bf16_on_stream(
     kcmm_pool_t *pool, uint32_t layer_idx, uint64_t query_ptr, int64_t q_stride_token,

@@ -10,17 +10,22 @@
 // maximum, its sum of exponentials and its n largest logits: the n-th largest of its warps'
 // maxima (its threads', where n is above 8) bounds those from below, so that a second look at
 // the registers leaves little more than n to sort.  The last CTA of a request scores and ranks
-// its beams x chunks x n candidates in the same way.  Different logits can round to one score
-// (scores of -inf, or large beside the logits' steps), and then the lower token comes first though
-// its logit is the smaller one: each chunk also says how large its largest logit off the list is,
-// and where that one's score equals the n-th best the last CTA looks the ties up in the
-// logits themselves.  Bounds from all threads' maxima cost a
-// second pass wherever 16-bit maxima were equal: 24.4 us against 17.1 for 16 requests of 4
-// beams over 128,256 bf16 logits, the gathers of histories and tables included.
+// its beams x chunks x n candidates in the same way.  Bounds from all threads' maxima cost a
+// second pass wherever 16-bit maxima were equal: 7 us of the 24 that 16 requests of 4 beams over
+// 128,256 bf16 logits took, the gathers of histories and tables included.
+//
+// Different logits can round to one score (scores of -inf, or large beside the logits' steps), and
+// then the lower token comes first though its logit is the smaller one: each chunk also says how
+// large its largest logit off the list is, and where that one's score equals the n-th best the
+// last CTA looks the ties up in the logits themselves (the check is 2 of that call's 19.2 us).
+//
+// The sum takes __expf: 2 + 1.17 |x| units of 2^-23 off at x = logit - max, which a term's share
+// exp(x) weighs, so that the sum is off by (2 + 1.17 ln vocab) 2^-23 at most, 2^-19, and its
+// logarithm by 2e-6, a unit of a score of 20.
 //
 // That call is bound by the latency of a CTA's steps (load, maximum, exponentials, list,
-// counter, then the ranking; 16 MB of logits would take 2.5 us): chunks of 8 and 32 KB took 19.8
-// and 36 us.  So are small vocabularies.
+// counter, then the ranking; 16 MB of logits would take 2.5 us): chunks of 8 and 32 KB took 3 and
+// 19 us more.  So are small vocabularies.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -565,18 +570,6 @@ __global__ void __launch_bounds__(kThreads, 5) beam_select_kernel(const __grid_c
         if (at < kFewKeys) s_list[at] = k;
       });
     }
-    // the largest logit that does not
-    uint32_t below = value_key(mx);
-    if (reach != 0) {
-      below = 0;
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-        for (int e = 0; e < PER; ++e)
-          if (!(reach >> (i * PER + e) & 1u)) below = max(below, value_key(value(i, e)));
-    }
-    below = __reduce_max_sync(0xffffffffu, below);
-    if (lane == 0) s_below[warp] = below;
     float sum = 0.f;
     if (m != -INFINITY) {
 #pragma unroll
@@ -611,10 +604,20 @@ __global__ void __launch_bounds__(kThreads, 5) beam_select_kernel(const __grid_c
     }
     unsigned long long *cand = a.cand + (int64_t(row) * a.chunks + chunk) * a.n;
     float *rest = a.rest + int64_t(row) * a.chunks + chunk;  // largest logit off the list, or more
-    if (!crowded && count == a.n && tid == 0) {
-      uint32_t top = s_below[0];
-      for (int w = 1; w < kWarps; ++w) top = max(top, s_below[w]);
-      *rest = key_value(top);
+    if (!crowded && count == a.n) {  // all that reach the bound are listed: the largest that does not
+      uint32_t below = 0;
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          if (value(i, e) < floor_value) below = max(below, value_key(value(i, e)));
+      below = __reduce_max_sync(0xffffffffu, below);
+      if (lane == 0) s_below[warp] = below;
+      __syncthreads();
+      if (tid == 0) {
+        for (int w = 0; w < kWarps; ++w) below = max(below, s_below[w]);
+        *rest = key_value(below);
+      }
     }
     for (int i = tid; i < max(count, a.n); i += kThreads) {
       if (i >= count) {

@@ -14,8 +14,9 @@
 // tokens, the atomics on one bin serialised, against 25).  The last few keys are ranked one
 // against all: another histogram or two took 2 to 5 us more.  A cluster of CTAs shares a long
 // row.  It is bound by the latency of its passes, over keys in shared memory where they fit
-// (128 rows of 3700 tokens: 11 us).  The moves are a copy of scattered rows, bound by HBM
-// where they are many (105,000 rows of 2 x 256 bytes: 18.5 us, 5.8 TB/s both ways).
+// (128 rows of 3700 tokens: 11 us).  The moves are a copy of scattered rows:
+// 105,000 of 2 x 256 bytes take 18.5 us, 5.8 TB/s read and written, half of it in L2 (58 MB of
+// HBM traffic, 2.8 TB/s); the loads' latency bounds them, with 30 % of the warps that would fit.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 

@@ -43,8 +43,9 @@ constexpr int kGroup = kKv4Group;
 // layout: its source loads are whole 32-byte sectors, its code stores one 16-byte vector a
 // pair of groups, and no byte goes through shared memory.  Other tiles (decode steps, the
 // ends of a chunk) go row by row, 8 values a lane.  16,384 tokens of 8 heads of 128 took 179 us
-// row by row for both kernels and take 45 by units (3.8 TB/s, 60 to 68 % of the issue slots:
-// HBM and the arithmetic bound them together); short inputs are bound by the latency of
+// row by row for both kernels and take 45 by units.  Neither HBM (1.9 TB/s of its 6.4 in the append)
+// nor the issue slots (61 and 68 %) are full there: a warp waits for the loads of one pair of
+// groups before it asks for the next one's.  Short inputs are bound by the latency of
 // slot -> offset -> row (64 tokens: 4.4 us).
 
 constexpr int kRowsThreads = 128;
@@ -455,19 +456,20 @@ __global__ void __launch_bounds__(kRowsThreads) kv4_read_kernel(const Kv4RowsArg
 
 constexpr int kWarps = 4;
 // Query heads of a CTA, the columns of the mma.  More heads of a kv head become more CTAs, that
-// unpack the same codes again, from L2: two tiles of 16 in a CTA's registers instead took
-// 28.4 us against 23.1 for 16 sequences of up to 2000 tokens with 16 heads on 1 (38.0 against
-// 36.6 for 32 of up to 4096 with 64 on 4, 44.8 against 33.3 at heads of 256).
+// unpack the same codes again, from L2: two tiles of 16 in a CTA's registers instead took a fifth
+// longer for 16 sequences of up to 2000 tokens with 16 heads on 1 (now 19.4 us), 4 % for 32 of up
+// to 4096 with 64 on 4 (38.0), a third at heads of 256 (28.6).
 constexpr int kHeads = 8;
-// Units of a CTA, at least.  8 leave more pieces to merge, 32 fewer CTAs: 17.4 and 16.7 us
-// against 15.8 for 4 sequences of up to 700 tokens, 19.1 and 27.6 against 20.9 for 8 of up to
+// Units of a CTA, at least.  8 leave more pieces to merge, 32 fewer CTAs: 13.2 and 14.6 us
+// against 13.8 for 3 sequences of up to 777 tokens, 16.9 and 26.0 against 19.3 for 8 of up to
 // 2000.
 constexpr int kMinRange = 16;
-// Pieces of a sequence, about, which its last CTA merges: 16 and 64 took 26.2 and 22.6 us
-// against 21.2 for one of 32,768 tokens.
+// Pieces of a sequence, about, which its last CTA merges: 16 and 64 take 26.6 and 24.3 us
+// against 22.1 for one of 32,768 tokens.
 constexpr int kMaxPieces = 32;
-// Pieces that the merge takes at a time.  A first pass over their sums took 30.0 us against 27.8
-// for 8 sequences of 32,768 tokens and 8 heads on 1; 4 and 16 at a time 30.0 and 28.4.
+// Pieces that the merge takes at a time: 4 and 16 take 30.8 and 28.4 us against 28.4 for 8
+// sequences of 32,768 tokens and 8 heads on 1, and 13.6 and 14.2 against 13.8 for 3 of up to 777.  A
+// first pass over their sums cost 2 us more.
 constexpr int kMergeAtOnce = 8;
 constexpr float kNoMax = -3e38f;  // a row's maximum before its first finite score
 constexpr int kStages = 3;  // steps of a warp's ring; 2 are as fast
@@ -538,8 +540,8 @@ __device__ __forceinline__ float bf16_lo(uint32_t x) { return __uint_as_float(x 
 __device__ __forceinline__ float bf16_hi(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
 // Units that a warp takes at a time: two give its loads, matrix products and shuffles
-// something to overlap with (21.2 against 23.3 us for one sequence of 32,768 tokens, 8 kv
-// heads of 128; 58.6 against 59.1 for the batch below), as long as the registers of both fit.
+// something to overlap with (22.1 against 23.9 us for one sequence of 32,768 tokens, 8 kv
+// heads of 128; equal for the batch below), as long as the registers of both fit.
 __host__ __device__ constexpr int units_at_a_time(int D) { return D <= 128 ? 2 : 1; }
 __host__ __device__ constexpr int ctas_per_sm(int D) { return D <= 128 ? 4 : 2; }
 
@@ -578,16 +580,16 @@ __device__ __forceinline__ void load_words(uint32_t *r, const unsigned char *p, 
 
 // Work split.  The units of all sequences, end to end, are cut into equal ranges, one for each
 // CTA x of a kv head (and head tile) y = blockIdx.y: lengths differ by a factor of 8 within
-// a batch, and CTAs of one (sequence, split) each took 60 us for the Llama-3-8B decode batch
-// (64 sequences of 512 to 4096 tokens, 8 kv heads of 128) where equal shares take 56.  A sequence
+// a batch, and CTAs of one (sequence, split) each took 7 % longer for the Llama-3-8B decode batch
+// (64 sequences of 512 to 4096 tokens, 8 kv heads of 128; now 65.9 us).  A sequence
 // inside one range is finished there; the pieces of one that several CTAs share go to scratch
 // and the last CTA to finish merges them.
 //
-// That batch is bound by instructions, at 3.0 TB/s: 16 tokens of a head cost about 330 warp
-// instructions, half of them unpacking and scaling codes (matrix products on 8-bit codes
-// instead needed as many); 58 % of the issue slots are used over the whole call, its start and
-// its merges included.  Few sequences are bound by latency: lengths -> table -> offset -> chunk
-// -> counter -> merge (14.9 us for 3 of up to 777 tokens).
+// That batch fills neither HBM (2.6 TB/s) nor the issue slots (60 %): 16 tokens of a kv head cost
+// about 480 warp instructions, more than half of them unpacking codes and forming their weights,
+// in chains that 3.5 warps a scheduler do not cover (an issue finds 1.0 of them in a fixed
+// latency, 0.85 at a busy pipe, 0.5 at a load).  Few sequences are bound by latency: lengths ->
+// table -> offset -> chunk -> counter -> merge (13.8 us for 3 of up to 777 tokens).
 //
 // A CTA's warps take every kWarps-th step of NU units of its piece.  Each warp runs its own
 // ring of kStages steps: a lane issues a unit's K and V chunks as two bulk copies, the whole
@@ -906,9 +908,9 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
     // ---- O += V^T (P S)^T, S the scale of a token's group -------------------------------------
     // The codes are the A operand; the weight of a (token, head, group), the probability times
     // the scale in 32 bits, is the B operand (rows = tokens, columns = heads) as a pair of bf16,
-    // its leading 8 bits and its remainder's: 16 bits, and the range of 32-bit floats.  Half the
-    // products on f16, 57 us against 61 for the Llama-3-8B batch, round a weight of 11 bits twice
-    // and lose groups and tokens whose scales lie far apart, since one range holds them all.
+    // its leading 8 bits and its remainder's: 16 bits, and the range of 32-bit floats.  One f16,
+    // which took 57 us against 61 for the Llama-3-8B batch, rounds a probability of 11 bits twice
+    // and loses groups and tokens whose scales lie far apart, since one range holds them all.
     float pt[NU][4];  // P transposed: head g, tokens (2c, 2c+1) + 8 i
 #pragma unroll
     for (int r = 0; r < NU; ++r) {
@@ -1196,7 +1198,7 @@ cudaError_t kv4_decode_attention(const DecodeArgs &a, const DecodeWeights &w,
 
   // One wave of CTAs, every one with its share of the units of one kv head's (head tile's)
   // tokens.  Four waves of smaller shares where those are many lost: 96 kv heads of 256, 4
-  // sequences of 100 to 2000 tokens 73 against 45 us, of 2000 to 6000 155 against 121.
+  // sequences of 100 to 2000 tokens took 60 % longer (now 50 us), of 2000 to 6000 28 % (144).
   const int slots = device_sm_count() * ctas_per_sm(D), Y = a.kv_heads * p.n_head_tiles;
   const int X = int(std::min<int64_t>(std::max(1, slots / Y), int64_t(kMaxPieces) * a.batch));
 
