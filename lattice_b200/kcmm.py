@@ -439,6 +439,9 @@ class RegionAddress(int):
         self._regions = regions
         return self
 
+    def __reduce__(self):  # a copy, or what was pickled, is a plain int
+        return int, (int(self),)
+
 
 class KcmmPool:
     """One pool handle; every method raises `KcmmError` on a -1 return."""

@@ -1,7 +1,9 @@
 """A pool's regions stay mapped while an address of theirs, or a tensor over one, is held."""
 from __future__ import annotations
 
+import copy
 import gc
+import pickle
 
 import numpy as np
 import pytest
@@ -23,6 +25,8 @@ def test_destroy_waits_for_the_last_address(host_pool_factory):
     assert mapped(where)
     with pytest.raises(KcmmError, match="destroyed"):
         pool.va_k(0)
+    copies = [copy.deepcopy(k), pickle.loads(pickle.dumps(k))]
+    assert copies == [where, where] and {type(x) for x in copies} == {int}
     del k
     assert mapped(where)  # a region's address holds them all
     del v
