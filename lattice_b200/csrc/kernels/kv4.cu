@@ -472,6 +472,9 @@ constexpr int kMaxPieces = 32;
 // first pass over their sums cost 2 us more.
 constexpr int kMergeAtOnce = 8;
 constexpr float kNoMax = -3e38f;  // a row's maximum before its first finite score
+// The normaliser of a row lies kLift above its maximum (log2 units): probabilities are below
+// 2^(kSlack - kLift), so that the sum of 2^18 values of bf16's largest stays below 32-bit's.
+constexpr float kLift = 24.f, kSlack = 6.f;
 constexpr int kStages = 3;  // steps of a warp's ring; 2 are as fast
 constexpr uint64_t kWaitLimitNs = 1000000000ull;  // a chunk that has not landed in 1 s is
                                                   // reported, never waited on forever
@@ -876,25 +879,26 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
         }
       }
     }
-    // The running maximum is raised only when a score exceeds it by more than 6: rare after a
-    // warp's first step, so most steps skip the rescaling of O.
+    // The normaliser m is raised only when a score exceeds the maximum that it was set for by more
+    // than kSlack: rare after a warp's first step, so most steps skip the rescaling of O.
     bool raise = false;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float mx = fmaxf(s[0][i], s[0][i + 2]);
 #pragma unroll
       for (int r = 1; r < NU; ++r) mx = fmaxf(mx, fmaxf(s[r][i], s[r][i + 2]));
-      raise |= mx > m[i] + 6.f;
+      raise |= mx > m[i] + (kSlack - kLift);
     }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float mx = m[i];
+        float mx = kNoMax;
 #pragma unroll
         for (int r = 0; r < NU; ++r) mx = fmaxf(mx, fmaxf(s[r][i], s[r][i + 2]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        mx = fmaxf(m[i], mx + kLift);
         const float rr = ptx::fast_exp2(m[i] - mx);
         m[i] = mx;
         l[i] *= rr;
@@ -1080,7 +1084,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
       x = make_float4(x.x * r, x.y * r, x.z * r, x.w * r);
 #pragma unroll
       for (int j = 0; j < kMergeAtOnce; ++j) {
-        const float w = lse[j] == -INFINITY ? 0.f : ptx::fast_exp2(lse[j] - M);
+        const float w = lse[j] == -INFINITY ? 0.f : ptx::fast_exp2(lse[j] - (M + kLift));
         L += w;
         x.x += v[j].x * w;
         x.y += v[j].y * w;
@@ -1089,7 +1093,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D))
       }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    store(h, d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), M + log2f(L));
+    store(h, d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv),
+          M + kLift + log2f(L));
   }
   }
 }

@@ -441,3 +441,24 @@ def test_decode_queries_and_keys_far_apart(dtype, apart):
         check_decode(c, rows, q, out, d ** -0.5)
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("n", [1, 2, 300, 5000])
+def test_decode_values_near_the_largest(n):
+    """bf16 values near the type's largest: their weighted mean is finite, their sum is not."""
+    torch = torch_cuda()
+    d = 64
+    c = Cache([n], 1, d, kv4=True, seed=n)
+    try:
+        k, v = c.rng.standard_normal((2, n, 1, d))
+        v[..., :32] = 2e38 * (1 + 0.2 * c.rng.random((n, 1, 32)))
+        v[..., 16:32] *= -1
+        tk, tv = (torch.from_numpy(x).cuda().to(c.tdt) for x in (k, v))
+        c.write(tk, tv, c.slots(0, np.arange(n)))
+        rows = [tuple(quantised(x.double().cpu().numpy()) for x in (tk, tv))]
+        q = torch.from_numpy(0.3 * c.rng.standard_normal((1, 4, d))).cuda().to(c.tdt)
+        out = c.decode(q, d ** -0.5, torch.zeros_like(q))
+        assert bool(torch.isfinite(out).all())
+        check_decode(c, rows, q, out, d ** -0.5)
+    finally:
+        c.close()
