@@ -1561,8 +1561,11 @@ cudaError_t decode_attention_shared_prefix(const DecodeArgs &a, const int32_t *g
   cp.work = reinterpret_cast<int4 *>(res + ((size_t(a.batch) + 2) * 4 + 15) / 16 * 16);
 
   const size_t prep_smem = (size_t(n_groups) * 4 + 1 + size_t(a.batch) * 2) * 4;
+  // The attribute belongs to the kernel, not to the launch: one limit for all batches that it
+  // holds, so that a call on another thread does not lower it between here and the launch.
+  constexpr size_t kPrepSmem = 220 * 1024;
   e = cudaFuncSetAttribute(shared_prefix_prep_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           int(prep_smem));
+                           int(std::max(prep_smem, kPrepSmem)));
   if (e == cudaSuccess)
     e = launch_pdl(shared_prefix_prep_kernel, dim3(1), dim3(1024), prep_smem, stream, p, cp);
   if (e == cudaSuccess)

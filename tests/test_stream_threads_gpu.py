@@ -96,3 +96,56 @@ def test_calls_of_several_threads_on_one_stream():
     finally:
         for c in made:
             c.close()
+
+
+@pytest.mark.parametrize("many", [300, 4000])
+def test_shared_prefix_decodes_of_two_threads(many):
+    """Batches of different sizes, each thread on a stream of its own."""
+    from test_shared_prefix_gpu import _build
+
+    torch = torch_cuda()
+    jobs, errors = [], []
+    try:
+        for batch in (4, many):
+            wl = _build([2] * (batch // 2), [1] * (batch // 2), [20] * batch, hq=4, hkv=1)
+            starts = torch.arange(0, batch + 1, 2, dtype=torch.int32, device="cuda")
+            prefix = torch.full((batch // 2,), 16, dtype=torch.int32, device="cuda")
+            out, stream = torch.zeros_like(wl.q), torch.cuda.Stream()
+
+            def call(wl=wl, starts=starts, prefix=prefix, out=out, stream=stream):
+                rc = wl.pool.lib.kcmm_paged_attn_decode_shared_prefix_bf16_on_stream(
+                    wl.pool.handle, 0, wl.q.data_ptr(), out.data_ptr(), wl.d_tables.data_ptr(),
+                    wl.d_seq_lens.data_ptr(), wl.d_offsets.data_ptr(), wl.batch, 4, 1, 128, 16,
+                    wl.max_blocks_per_seq, wl.scale, starts.data_ptr(), prefix.data_ptr(),
+                    wl.batch // 2, 2, stream.cuda_stream)
+                if rc != 0:
+                    raise RuntimeError(wl.pool.last_error())
+
+            jobs.append((wl, call, out, stream))
+        torch.cuda.synchronize()
+        want = []
+        for _, call, out, stream in jobs:
+            call()
+            stream.synchronize()
+            want.append(out.clone())
+        torch.cuda.synchronize()
+
+        def work(call):
+            try:
+                for _ in range(2000):
+                    call()
+            except RuntimeError as err:
+                errors.append(str(err))
+
+        threads = [threading.Thread(target=work, args=(j[1],)) for j in jobs]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert not errors
+        for (wl, _, out, _), ref in zip(jobs, want):
+            assert torch.equal(out, ref) and wl.pool.kernel_status() == 0
+    finally:
+        for wl, *_ in jobs:
+            wl.close()
