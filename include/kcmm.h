@@ -643,6 +643,95 @@ int kcmm_evict_tokens_on_stream(
  *  released as kcmm_free_blocks does. */
 int kcmm_truncate_sequence(kcmm_pool_t *pool, uint32_t seq_idx, uint32_t len);
 
+/* --- rotary positions with several axes, and the append behind them (no reference
+       counterpart) --- */
+
+/** How a row's pairs are dealt to the axes of their positions. */
+typedef enum {
+    /* the first sections[0] pairs to axis 0, the next sections[1] to axis 1, ... */
+    KCMM_ROPE_SECTIONS    = 0,
+    /* pair i to axis i % axes while i < axes * sections[i % axes], else to axis 0 */
+    KCMM_ROPE_INTERLEAVED = 1,
+} kcmm_rope_layout_t;
+
+/** The rotation of a model's q and k rows. */
+typedef struct {
+    uint32_t mode;                /* KCMM_ROPE_GPTJ or KCMM_ROPE_NEOX; pairs lie within the first
+                                     rotary_dim values, (i, i + rotary_dim / 2) for NEOX */
+    uint32_t rotary_dim;          /* even, 2 .. head_dim; the values past it stay as they are */
+    uint64_t inv_freq_ptr;        /* device float32 [rotary_dim / 2] */
+    uint64_t positions_ptr;       /* device int32 [axes] rows of num_tokens positions */
+    int64_t positions_row_stride; /* entries between the axes' rows, 0 = num_tokens */
+    uint32_t axes;                /* 1 .. 4: text, or time, height and width */
+    uint32_t layout;              /* kcmm_rope_layout_t; not read for one axis */
+    uint32_t sections[4];         /* pairs of each axis, rotary_dim / 2 in all; not read for one */
+} kcmm_rope_t;
+
+/**
+ * Rotate the q and k rows of num_tokens tokens and append k and v to the cache:
+ *   angle = position * inv_freq[i] (64 bits; its cosine and sine rounded to 32),
+ *   x1' = x1 cos - x2 sin,  x2' = x2 cos + x1 sin  (32 bits, rounded once to 16),
+ *   q_out[t] = q[t]',  k_out[t] = k[t]',  cache slot slot_mapping[t] <- k[t]', v[t].
+ * q and q_out [num_tokens][num_q_heads][head_dim] with element strides (0 = dense), q_out may be
+ * q with its strides; num_q_heads 0: neither is touched.  k, v and k_out are rows of kv_heads *
+ * head_dim values (row strides 0 = dense), k_out may be k with its stride, or 0 for none.
+ * cache_format (kcmm_cache_format_t) and head_dim (the model's, even) say what the pool's pages
+ * hold; a 4-bit cache quantises the rounded k' as kcmm_kv4_append_* does.  Slots, offsets, valid
+ * flags and status word as for kcmm_append_kv_device_slots_on_stream: a slot below 0 or with a
+ * status is not written, its q_out and k_out rows are.  Slots within a call must differ.
+ */
+int kcmm_rope_append_bf16_on_stream(
+    kcmm_pool_t *pool, uint32_t layer_idx, uint32_t cache_format, uint32_t head_dim,
+    const kcmm_rope_t *rope, uint64_t q_ptr, int64_t q_stride_token, int64_t q_stride_head,
+    uint64_t q_out_ptr, int64_t q_out_stride_token, int64_t q_out_stride_head,
+    uint32_t num_q_heads, uint64_t k_ptr, int64_t k_row_stride, uint64_t v_ptr,
+    int64_t v_row_stride, uint64_t k_out_ptr, int64_t k_out_row_stride, uint64_t slot_mapping_ptr,
+    uint64_t block_offsets_f16_ptr, uint64_t valid_blocks_ptr, uint32_t block_offsets_f16_len,
+    uint32_t num_tokens, uint64_t status_ptr, uint64_t stream_ptr);
+int kcmm_rope_append_f16_on_stream(
+    kcmm_pool_t *pool, uint32_t layer_idx, uint32_t cache_format, uint32_t head_dim,
+    const kcmm_rope_t *rope, uint64_t q_ptr, int64_t q_stride_token, int64_t q_stride_head,
+    uint64_t q_out_ptr, int64_t q_out_stride_token, int64_t q_out_stride_head,
+    uint32_t num_q_heads, uint64_t k_ptr, int64_t k_row_stride, uint64_t v_ptr,
+    int64_t v_row_stride, uint64_t k_out_ptr, int64_t k_out_row_stride, uint64_t slot_mapping_ptr,
+    uint64_t block_offsets_f16_ptr, uint64_t valid_blocks_ptr, uint32_t block_offsets_f16_len,
+    uint32_t num_tokens, uint64_t status_ptr, uint64_t stream_ptr);
+
+/* --- attention over packed prompts (no reference counterpart) --- */
+
+/**
+ * Attention of packed sequences over K and V rows that lie beside the queries instead of in
+ * pages: a prompt's own rows before or while they are appended (also to a 4-bit cache, whose
+ * prompts need 16-bit rows), or a chunk's rows behind a past that was read back.
+ * Sequence b has the queries [q_start[b], q_start[b+1]) of q [num_q_tokens][num_q_heads]
+ * [head_dim] and the keys [k_start[b], k_start[b+1]) of k and v [num_k_tokens][kv_heads]
+ * [head_dim]; q_start and k_start are ascending device int32 arrays of batch + 1, and may be the
+ * same.  With nq and nk of them, query i attends to the keys j <= i + nk - nq where causal is 1,
+ * to all nk where it is 0:
+ *   out[i] = sum_j softmax_j(scale * q[i].k[j]) v[j],
+ * zeros where a query sees no key (or only scores of -inf).  Any number of queries from 0, any
+ * nk from 0; rows of out that belong to no sequence are left as they were.  Strides are in
+ * elements (0 = dense); pointers and strides are multiples of 16 bytes, head_dim is a multiple
+ * of 8 up to 256, num_q_heads a multiple of kv_heads.  Keys and values past a sequence may hold
+ * anything.  Starts that do not ascend, or pass num_q_tokens or num_k_tokens, set bit 2 of
+ * kcmm_get_kernel_status; what the call writes within out is then undefined.  No page of the
+ * pool is touched: it gives the device and the status word.
+ */
+int kcmm_prompt_attn_bf16_on_stream(
+    kcmm_pool_t *pool, uint64_t query_ptr, int64_t q_stride_token, int64_t q_stride_head,
+    uint64_t key_ptr, int64_t k_stride_token, int64_t k_stride_head, uint64_t value_ptr,
+    int64_t v_stride_token, int64_t v_stride_head, uint64_t out_ptr, int64_t out_stride_token,
+    int64_t out_stride_head, uint64_t q_start_ptr, uint64_t k_start_ptr, uint32_t batch,
+    uint32_t num_q_tokens, uint32_t num_k_tokens, uint32_t num_q_heads, uint32_t kv_heads,
+    uint32_t head_dim, float scale, uint32_t causal, uint64_t stream_ptr);
+int kcmm_prompt_attn_f16_on_stream(
+    kcmm_pool_t *pool, uint64_t query_ptr, int64_t q_stride_token, int64_t q_stride_head,
+    uint64_t key_ptr, int64_t k_stride_token, int64_t k_stride_head, uint64_t value_ptr,
+    int64_t v_stride_token, int64_t v_stride_head, uint64_t out_ptr, int64_t out_stride_token,
+    int64_t out_stride_head, uint64_t q_start_ptr, uint64_t k_start_ptr, uint32_t batch,
+    uint32_t num_q_tokens, uint32_t num_k_tokens, uint32_t num_q_heads, uint32_t kv_heads,
+    uint32_t head_dim, float scale, uint32_t causal, uint64_t stream_ptr);
+
 /* --- beam search (no reference counterpart) --- */
 
 /** Element types of the logits. */

@@ -13,8 +13,10 @@ from .kcmm import (  # noqa: F401
     KcmmMetrics,
     KcmmPool,
     KcmmPoolStats,
+    KcmmRope,
     RopeMode,
     assert_layout,
     kv4_row_elems,
     make_config,
+    make_rope,
 )

@@ -1000,6 +1000,264 @@ KCMM_DECODE_WEIGHTS(kcmm_paged_attn_decode_weights_f16_on_stream, F16, false)
 #undef KCMM_DECODE_WEIGHTS
 
 // ---------------------------------------------------------------------------
+// Rotation and append, attention over packed prompts
+// ---------------------------------------------------------------------------
+
+// nullptr where the rotation is well formed.
+static const char *check_rope(const kcmm_rope_t &r, uint32_t hd, uint32_t num_tokens) {
+  if (!r.inv_freq_ptr || !r.positions_ptr) return "null pointer argument";
+  if (((r.inv_freq_ptr | r.positions_ptr) & 3) != 0)
+    return "frequencies and positions must be 4-byte aligned";
+  if (r.mode != KCMM_ROPE_GPTJ && r.mode != KCMM_ROPE_NEOX)
+    return "rope mode must be KCMM_ROPE_GPTJ or KCMM_ROPE_NEOX";
+  if (r.rotary_dim < 2 || r.rotary_dim % 2 != 0 || r.rotary_dim > hd)
+    return "rotary_dim must be even, 2 to head_dim";
+  if (r.axes < 1 || r.axes > uint32_t(kcmm::dev::kRopeMaxAxes)) return "axes must be 1 to 4";
+  if (r.positions_row_stride < 0 ||
+      (r.positions_row_stride && r.axes > 1 && r.positions_row_stride < int64_t(num_tokens)))
+    return "the positions' row stride must be 0 (dense) or >= num_tokens";
+  if (r.axes == 1) return nullptr;
+  if (r.layout > KCMM_ROPE_INTERLEAVED) return "unknown rope layout";
+  const uint32_t half = r.rotary_dim / 2;
+  uint64_t sum = 0;
+  for (uint32_t x = 0; x < r.axes; ++x) {
+    sum += r.sections[x];
+    if (r.layout == KCMM_ROPE_INTERLEAVED && x > 0 && r.sections[x] > 0 &&
+        x + uint64_t(r.axes) * (r.sections[x] - 1) >= half)
+      return "an interleaved section has more pairs than rotary_dim holds";
+  }
+  if (sum != half) return "sections must add up to rotary_dim / 2";
+  return nullptr;
+}
+
+static int rope_append_impl(kcmm_pool_t *h, const char *op, kcmm::dev::Dtype dtype,
+                            uint32_t layer, uint32_t cache_format, uint32_t hd,
+                            const kcmm_rope_t *rope, uint64_t q, int64_t q_token, int64_t q_head,
+                            uint64_t q_out, int64_t q_out_token, int64_t q_out_head, uint32_t hq,
+                            uint64_t k, int64_t k_stride, uint64_t v, int64_t v_stride,
+                            uint64_t k_out, int64_t k_out_stride, uint64_t slots,
+                            uint64_t offsets, uint64_t valid, uint32_t offsets_len,
+                            uint32_t num_tokens, uint64_t status, uint64_t stream) {
+  if (!h || !rope || !k || !v || !slots || !offsets || (hq && (!q || !q_out))) {
+    set_error(h, std::string(op) + ": null pointer argument");
+    return -1;
+  }
+  if (num_tokens == 0 || num_tokens > 0x7fffffffu || offsets_len == 0 ||
+      offsets_len > 0x7fffffffu) {
+    set_error(h, std::string(op) + ": num_tokens and offset table length must be positive");
+    return -1;
+  }
+  if (hd == 0 || hd > 256 || hd % 2 != 0 || hq > 0xFFFF) {
+    set_error(h, std::string(op) + ": head_dim must be even, at most 256, num_q_heads at most "
+                                   "65535");
+    return -1;
+  }
+  if (const char *msg = check_rope(*rope, hd, num_tokens)) {
+    set_error(h, std::string(op) + ": " + msg);
+    return -1;
+  }
+  if (cache_format > 1) {
+    set_error(h, std::string(op) + ": unknown cache_format " + std::to_string(cache_format));
+    return -1;
+  }
+  Pool *p = P(h);
+  const bool kv4 = cache_format == KCMM_CACHE_KV4;
+  if (kv4) {
+    if (!check_kv4_pool(h, op, layer, hd)) return -1;
+  } else {
+    if (layer >= p->num_layers) {
+      set_error(h, std::string(op) + ": layer_idx " + std::to_string(layer) + " out of bounds");
+      return -1;
+    }
+    if (hd != p->cfg_.head_dim) {
+      set_error(h, std::string(op) + ": head_dim must be the pool's, " +
+                       std::to_string(p->cfg_.head_dim));
+      return -1;
+    }
+  }
+  if (p->cfg_.kv_heads > 0xFFFF) {
+    set_error(h, std::string(op) + ": kv_heads exceeds 65535");
+    return -1;
+  }
+  const int64_t row = int64_t(p->cfg_.kv_heads) * hd;
+  if (q_token < 0 || q_out_token < 0 || (hq && ((q_head && q_head < int64_t(hd)) ||
+                                                (q_out_head && q_out_head < int64_t(hd)))) ||
+      k_stride < 0 || v_stride < 0 || k_out_stride < 0 || (k_stride && k_stride < row) ||
+      (v_stride && v_stride < row) || (k_out && k_out_stride && k_out_stride < row)) {
+    set_error(h, std::string(op) + ": strides must be 0 (dense) or positive, head strides >= "
+                                   "head_dim and row strides >= kv_heads * head_dim");
+    return -1;
+  }
+  if (((k | v | k_out | (hq ? q | q_out : 0)) & 1) != 0) {
+    set_error(h, std::string(op) + ": q, k, v and their outputs must be aligned to their 16-bit "
+                                   "elements");
+    return -1;
+  }
+  if (guarded(h, op, [&] { p->require_device(op); })) return -1;
+  kcmm::dev::RopeAppendArgs a = {};
+  a.dtype = dtype;
+  a.num_q_heads = int(hq);
+  a.q = reinterpret_cast<const void *>(q);
+  a.q_out = reinterpret_cast<void *>(q_out);
+  a.q_stride_head = q_head ? q_head : int64_t(hd);
+  a.q_stride_token = q_token ? q_token : int64_t(hq) * hd;
+  a.q_out_stride_head = q_out_head ? q_out_head : int64_t(hd);
+  a.q_out_stride_token = q_out_token ? q_out_token : int64_t(hq) * hd;
+  a.k = reinterpret_cast<const void *>(k);
+  a.v = reinterpret_cast<const void *>(v);
+  a.k_out = reinterpret_cast<void *>(k_out);
+  a.k_stride = k_stride ? k_stride : row;
+  a.v_stride = v_stride ? v_stride : row;
+  a.k_out_stride = k_out_stride ? k_out_stride : row;
+  a.neox = rope->mode == KCMM_ROPE_NEOX;
+  a.rotary_dim = int(rope->rotary_dim);
+  a.inv_freq = reinterpret_cast<const float *>(rope->inv_freq_ptr);
+  a.positions = reinterpret_cast<const int32_t *>(rope->positions_ptr);
+  a.positions_stride = rope->positions_row_stride ? rope->positions_row_stride
+                                                  : int64_t(num_tokens);
+  a.axes = int(rope->axes);
+  a.interleaved = rope->layout == KCMM_ROPE_INTERLEAVED;
+  for (uint32_t x = 0; x < rope->axes && rope->axes > 1; ++x) a.sections[x] = int(rope->sections[x]);
+  a.va_k = reinterpret_cast<void *>(p->va_k[layer]);
+  a.va_v = reinterpret_cast<void *>(p->va_v[layer]);
+  a.region_elems = p->region_bytes / 2;
+  a.slot_mapping = reinterpret_cast<const int64_t *>(slots);
+  a.block_offsets = reinterpret_cast<const uint64_t *>(offsets);
+  a.valid = reinterpret_cast<const uint8_t *>(valid);
+  a.offsets_len = int(offsets_len);
+  a.num_tokens = int(num_tokens);
+  a.kv_heads = int(p->cfg_.kv_heads);
+  a.head_dim = int(hd);
+  a.block_size = int(p->block_size);
+  a.status = reinterpret_cast<int32_t *>(status);
+  a.kv4 = kv4;
+  p->use_device();
+  return check_launch(h, op, kcmm::dev::rope_append(a, S(stream)));
+}
+
+#define KCMM_ROPE_APPEND(name, dt)                                                               \
+  int name(kcmm_pool_t *h, uint32_t layer, uint32_t cache_format, uint32_t hd,                   \
+           const kcmm_rope_t *rope, uint64_t q, int64_t q_token, int64_t q_head, uint64_t q_out, \
+           int64_t q_out_token, int64_t q_out_head, uint32_t hq, uint64_t k, int64_t k_stride,   \
+           uint64_t v, int64_t v_stride, uint64_t k_out, int64_t k_out_stride, uint64_t slots,   \
+           uint64_t offsets, uint64_t valid, uint32_t offsets_len, uint32_t num_tokens,          \
+           uint64_t status, uint64_t stream) {                                                   \
+    return rope_append_impl(h, #name, kcmm::dev::Dtype::dt, layer, cache_format, hd, rope, q,    \
+                            q_token, q_head, q_out, q_out_token, q_out_head, hq, k, k_stride, v, \
+                            v_stride, k_out, k_out_stride, slots, offsets, valid, offsets_len,   \
+                            num_tokens, status, stream);                                         \
+  }
+KCMM_ROPE_APPEND(kcmm_rope_append_bf16_on_stream, BF16)
+KCMM_ROPE_APPEND(kcmm_rope_append_f16_on_stream, F16)
+#undef KCMM_ROPE_APPEND
+
+static int prompt_attn_impl(kcmm_pool_t *h, const char *op, kcmm::dev::Dtype dtype, uint64_t q,
+                            int64_t q_token, int64_t q_head, uint64_t k, int64_t k_token,
+                            int64_t k_head, uint64_t v, int64_t v_token, int64_t v_head,
+                            uint64_t out, int64_t out_token, int64_t out_head, uint64_t q_start,
+                            uint64_t k_start, uint32_t batch, uint32_t num_q, uint32_t num_k,
+                            uint32_t hq, uint32_t hkv, uint32_t hd, float scale, uint32_t causal,
+                            uint64_t stream) {
+  if (!h || !q || !k || !v || !out || !q_start || !k_start) {
+    set_error(h, std::string(op) + ": null pointer argument");
+    return -1;
+  }
+  if (batch == 0 || num_q == 0 || num_k == 0 || hq == 0 || hkv == 0) {
+    set_error(h, std::string(op) + ": shape arguments must be positive");
+    return -1;
+  }
+  if (batch > 0xFFFF || hq > 0xFFFF || num_q > 0x7fffffffu || num_k > 0x7fffffffu ||
+      (uint64_t(num_q) * hq / 128 + uint64_t(batch) * hkv) > 0x7fffffffull) {
+    set_error(h, std::string(op) + ": shape argument exceeds its limit");
+    return -1;
+  }
+  if (hq % hkv != 0) {
+    set_error(h, std::string(op) + ": num_q_heads must be a multiple of kv_heads");
+    return -1;
+  }
+  if (hd == 0 || hd % 8 != 0 || hd > 256) {
+    set_error(h, std::string(op) + ": head_dim " + std::to_string(hd) +
+                     " unsupported (multiples of 8 up to 256)");
+    return -1;
+  }
+  if (causal > 1) {
+    set_error(h, std::string(op) + ": causal must be 0 or 1");
+    return -1;
+  }
+  for (const int64_t s : {q_head, k_head, v_head, out_head}) {
+    if (s && s < int64_t(hd)) {
+      set_error(h, std::string(op) + ": head strides must be 0 (dense) or >= head_dim");
+      return -1;
+    }
+  }
+  for (const int64_t s : {q_token, k_token, v_token, out_token, q_head, k_head, v_head, out_head}) {
+    if (s < 0 || s % 8 != 0 || s > (int64_t(1) << 38)) {
+      set_error(h, std::string(op) + ": strides must be multiples of 8 elements (16 bytes)");
+      return -1;
+    }
+  }
+  if (((q | k | v | out) & 15) != 0) {
+    set_error(h, std::string(op) + ": q, k, v and out must be 16-byte aligned");
+    return -1;
+  }
+  if (((q_start | k_start) & 3) != 0) {
+    set_error(h, std::string(op) + ": starts must be 4-byte aligned");
+    return -1;
+  }
+  Pool *p = P(h);
+  if (guarded(h, op, [&] { p->require_device(op); })) return -1;
+  p->use_device();
+  alignas(64) unsigned char k_map[128], v_map[128];
+  const int64_t head = int64_t(hd);
+  const int rows = kcmm::dev::prompt_attn_box_rows();
+  if (!kcmm::encode_rows_tensor_map(k_map, k, num_k, int(hkv), int(hd),
+                                    k_token ? k_token : head * hkv, k_head ? k_head : head,
+                                    rows) ||
+      !kcmm::encode_rows_tensor_map(v_map, v, num_k, int(hkv), int(hd),
+                                    v_token ? v_token : head * hkv, v_head ? v_head : head,
+                                    rows)) {
+    set_error(h, std::string(op) + ": k and v cannot be described to the copy engine");
+    return -1;
+  }
+  kcmm::dev::PromptAttnArgs a = {};
+  a.dtype = dtype;
+  a.q = reinterpret_cast<const void *>(q);
+  a.out = reinterpret_cast<void *>(out);
+  a.q_stride_head = q_head ? q_head : head;
+  a.q_stride_token = q_token ? q_token : head * hq;
+  a.out_stride_head = out_head ? out_head : head;
+  a.out_stride_token = out_token ? out_token : head * hq;
+  a.q_start = reinterpret_cast<const int32_t *>(q_start);
+  a.k_start = reinterpret_cast<const int32_t *>(k_start);
+  a.batch = int(batch);
+  a.num_q_tokens = int(num_q);
+  a.num_k_tokens = int(num_k);
+  a.kv_heads = int(hkv);
+  a.group = int(hq / hkv);
+  a.head_dim = int(hd);
+  a.scale = scale;
+  a.causal = causal != 0;
+  a.diag = p->diag_word();
+  a.k_map = k_map;
+  a.v_map = v_map;
+  return check_launch(h, op, kcmm::dev::prompt_attn(a, S(stream)));
+}
+
+#define KCMM_PROMPT_ATTN(name, dt)                                                               \
+  int name(kcmm_pool_t *h, uint64_t q, int64_t q_token, int64_t q_head, uint64_t k,              \
+           int64_t k_token, int64_t k_head, uint64_t v, int64_t v_token, int64_t v_head,         \
+           uint64_t out, int64_t out_token, int64_t out_head, uint64_t q_start,                  \
+           uint64_t k_start, uint32_t batch, uint32_t num_q, uint32_t num_k, uint32_t hq,        \
+           uint32_t hkv, uint32_t hd, float scale, uint32_t causal, uint64_t stream) {           \
+    return prompt_attn_impl(h, #name, kcmm::dev::Dtype::dt, q, q_token, q_head, k, k_token,      \
+                            k_head, v, v_token, v_head, out, out_token, out_head, q_start,       \
+                            k_start, batch, num_q, num_k, hq, hkv, hd, scale, causal, stream);   \
+  }
+KCMM_PROMPT_ATTN(kcmm_prompt_attn_bf16_on_stream, BF16)
+KCMM_PROMPT_ATTN(kcmm_prompt_attn_f16_on_stream, F16)
+#undef KCMM_PROMPT_ATTN
+
+// ---------------------------------------------------------------------------
 // Eviction by accumulated attention weight, beam search
 // ---------------------------------------------------------------------------
 

@@ -97,6 +97,63 @@ struct PrefillArgs {
 // (kernels/prefill.cu).  head_dim 128; num_q_heads / kv_heads must divide 128.
 cudaError_t paged_prefill(const PrefillArgs &a, cudaStream_t stream);
 
+// --- attention over packed prompts (kernels/prompt_attn.cu) ---
+struct PromptAttnArgs {
+  Dtype dtype;
+  const void *q;  // [num_q_tokens][heads][head_dim], strides in elements
+  void *out;
+  int64_t q_stride_token, q_stride_head, out_stride_token, out_stride_head;
+  const int32_t *q_start;  // [batch + 1] first row of each sequence
+  const int32_t *k_start;
+  int batch, num_q_tokens, num_k_tokens;
+  int kv_heads, group, head_dim;  // group: query heads of a kv head
+  float scale;
+  bool causal;
+  int32_t *diag;
+  // TMA descriptors of K and V, {head_dim, kv_heads, num_k_tokens} with box
+  // {64, 1, prompt_attn_box_rows()}
+  const void *k_map;
+  const void *v_map;
+};
+int prompt_attn_box_rows();
+// head_dim a multiple of 8 up to 256, rows of 16-byte aligned heads.
+cudaError_t prompt_attn(const PromptAttnArgs &a, cudaStream_t stream);
+
+// --- rotation and append (kernels/rope.cu) ---
+constexpr int kRopeMaxAxes = 4;
+struct RopeAppendArgs {
+  Dtype dtype;
+  const void *q;  // [num_tokens][num_q_heads][head_dim], strides in elements
+  void *q_out;
+  int64_t q_stride_token, q_stride_head, q_out_stride_token, q_out_stride_head;
+  int num_q_heads;  // 0 for none
+  const void *k;    // [num_tokens] rows of kv_heads * head_dim values
+  const void *v;
+  void *k_out;  // null for none
+  int64_t k_stride, v_stride, k_out_stride;
+  bool neox;  // pairs (i, i + rotary_dim / 2), else (2i, 2i + 1)
+  int rotary_dim;
+  const float *inv_freq;     // [rotary_dim / 2]
+  const int32_t *positions;  // [axes] rows
+  int64_t positions_stride;
+  int axes;
+  bool interleaved;  // pair i: axis i % axes where i < axes * sections[i % axes], else 0
+  int sections[kRopeMaxAxes];
+  // the cache: pages of 16-bit rows
+  void *va_k;
+  void *va_v;
+  uint64_t region_elems;
+  const int64_t *slot_mapping;
+  const uint64_t *block_offsets;  // 2-byte units
+  const uint8_t *valid;           // may be null
+  int offsets_len;
+  int num_tokens;
+  int kv_heads, head_dim, block_size;
+  int32_t *status;  // may be null
+  bool kv4;         // a 4-bit cache
+};
+cudaError_t rope_append(const RopeAppendArgs &a, cudaStream_t stream);
+
 // --- 4-bit KV cache (kernels/kv4.cu) ---
 // Rows of K and V to (append) or from (read) the slots of a 4-bit cache.
 struct Kv4RowsArgs {

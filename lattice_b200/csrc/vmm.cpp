@@ -225,6 +225,26 @@ bool encode_kv_page_tensor_map(void *out, uint64_t base, uint64_t tokens, int kv
   return r == CUDA_SUCCESS;
 }
 
+bool encode_rows_tensor_map(void *out, uint64_t base, uint64_t rows, int heads, int head_dim,
+                            int64_t row_stride, int64_t head_stride, int box_rows) {
+  cuuint64_t dims[3] = {cuuint64_t(head_dim), cuuint64_t(heads), cuuint64_t(rows)};
+  cuuint64_t strides[2] = {cuuint64_t(head_stride) * 2, cuuint64_t(row_stride) * 2};
+  cuuint32_t box[3] = {64, 1, cuuint32_t(box_rows)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const DriverApi *api = nullptr;
+  try {
+    api = &driver();
+  } catch (const Error &) {
+    return false;
+  }
+  CUresult r = api->encode_tiled(
+      static_cast<CUtensorMap *>(out), CU_TENSOR_MAP_DATA_TYPE_UINT16, 3,
+      reinterpret_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
 std::unique_ptr<Vmm> make_host_vmm() { return std::make_unique<HostVmm>(); }
 
 }  // namespace kcmm

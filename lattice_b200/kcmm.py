@@ -261,6 +261,14 @@ SIGNATURES: dict[str, tuple] = {
         (i32, [P, u32, u32, u32, u64, i64, u64, u64, u32, u32, u32, u32, u32, u64, u64, u64, u64,
                i64, u64, u64, u64, u64]),
     "kcmm_truncate_sequence": (i32, [P, u32, u32]),
+    **{f"kcmm_rope_append_{dt}_on_stream":
+       (i32, [P, u32, u32, u32, ctypes.c_void_p, u64, i64, i64, u64, i64, i64, u32, u64, i64, u64,
+              i64, u64, i64, u64, u64, u64, u32, u32, u64, u64])
+       for dt in ("bf16", "f16")},
+    **{f"kcmm_prompt_attn_{dt}_on_stream":
+       (i32, [P, u64, i64, i64, u64, i64, i64, u64, i64, i64, u64, i64, i64, u64, u64, u32, u32,
+              u32, u32, u32, u32, f32, u32, u64])
+       for dt in ("bf16", "f16")},
     "kcmm_beam_select_on_stream":
         (i32, [P, u64, u32, i64, u64, u64, u32, u32, u32, u32, u32, u64, u64, u64, u64]),
     "kcmm_beam_gather_on_stream":
@@ -311,6 +319,28 @@ SIGNATURES: dict[str, tuple] = {
     "kcmm_step_tables_stats": (i32, [P, ctypes.c_void_p]),
     "kcmm_build_info": (ctypes.c_char_p, []),
 }
+
+
+class KcmmRope(ctypes.Structure):
+    """The rotation of a model's q and k rows (`kcmm_rope_t`)."""
+    _fields_ = [("mode", ctypes.c_uint32), ("rotary_dim", ctypes.c_uint32),
+                ("inv_freq_ptr", ctypes.c_uint64), ("positions_ptr", ctypes.c_uint64),
+                ("positions_row_stride", ctypes.c_int64), ("axes", ctypes.c_uint32),
+                ("layout", ctypes.c_uint32), ("sections", ctypes.c_uint32 * 4)]
+
+
+def make_rope(*, rotary_dim: int, inv_freq_ptr: int, positions_ptr: int,
+              positions_row_stride: int = 0, sections=None, mode: str = "neox",
+              layout: str = "sections") -> KcmmRope:
+    """A `KcmmRope`: `sections` are the pairs of each axis (None: one axis), `mode` "neox" or
+    "gptj", `layout` "sections" or "interleaved"."""
+    sections = [rotary_dim // 2] if sections is None else [int(s) for s in sections]
+    if not 1 <= len(sections) <= 4:
+        raise ValueError(f"1 to 4 axes, not {len(sections)}")
+    return KcmmRope({"gptj": RopeMode.GPTJ, "neox": RopeMode.NEOX}[mode], rotary_dim,
+                    inv_freq_ptr, positions_ptr, positions_row_stride, len(sections),
+                    {"sections": 0, "interleaved": 1}[layout],
+                    (ctypes.c_uint32 * 4)(*sections))
 
 
 class KcmmStepTablesStats(ctypes.Structure):
@@ -735,6 +765,40 @@ class KcmmPool:
     def truncate_sequence(self, seq_idx: int, length: int) -> None:
         self._check(self.lib.kcmm_truncate_sequence(self.handle, seq_idx, length),
                     "kcmm_truncate_sequence")
+
+    # --- rotation and append, attention over packed prompts --------------------
+    def rope_append(self, layer: int, *, rope: KcmmRope, head_dim: int, k_ptr: int, v_ptr: int,
+                    slot_mapping_ptr: int, block_offsets_f16_ptr: int,
+                    block_offsets_f16_len: int, num_tokens: int, num_q_heads: int = 0,
+                    q_ptr: int = 0, q_out_ptr: int = 0, k_out_ptr: int = 0,
+                    q_stride_token: int = 0, q_stride_head: int = 0,
+                    q_out_stride_token: int = 0, q_out_stride_head: int = 0,
+                    k_row_stride: int = 0, v_row_stride: int = 0, k_out_row_stride: int = 0,
+                    cache_format: int = CacheFormat.BITS16, valid_blocks_ptr: int = 0,
+                    status_ptr: int = 0, dtype: str = "bf16", stream_ptr: int = 0) -> None:
+        """Rotate q and k by `rope` (`make_rope`) and append k and v to the cache."""
+        op = f"kcmm_rope_append_{dtype}_on_stream"
+        self._check(getattr(self.lib, op)(
+            self.handle, layer, cache_format, head_dim, ctypes.byref(rope), q_ptr, q_stride_token,
+            q_stride_head, q_out_ptr, q_out_stride_token, q_out_stride_head, num_q_heads, k_ptr,
+            k_row_stride, v_ptr, v_row_stride, k_out_ptr, k_out_row_stride, slot_mapping_ptr,
+            block_offsets_f16_ptr, valid_blocks_ptr, block_offsets_f16_len, num_tokens,
+            status_ptr, stream_ptr), op)
+
+    def prompt_attn(self, *, query_ptr: int, key_ptr: int, value_ptr: int, out_ptr: int,
+                    q_start_ptr: int, k_start_ptr: int, batch: int, num_q_tokens: int,
+                    num_k_tokens: int, num_q_heads: int, kv_heads: int, head_dim: int,
+                    scale: float, causal: bool = True, q_stride_token: int = 0,
+                    q_stride_head: int = 0, k_stride_token: int = 0, k_stride_head: int = 0,
+                    v_stride_token: int = 0, v_stride_head: int = 0, out_stride_token: int = 0,
+                    out_stride_head: int = 0, dtype: str = "bf16", stream_ptr: int = 0) -> None:
+        """Attention of packed sequences over packed K and V rows."""
+        op = f"kcmm_prompt_attn_{dtype}_on_stream"
+        self._check(getattr(self.lib, op)(
+            self.handle, query_ptr, q_stride_token, q_stride_head, key_ptr, k_stride_token,
+            k_stride_head, value_ptr, v_stride_token, v_stride_head, out_ptr, out_stride_token,
+            out_stride_head, q_start_ptr, k_start_ptr, batch, num_q_tokens, num_k_tokens,
+            num_q_heads, kv_heads, head_dim, scale, int(causal), stream_ptr), op)
 
     # --- beam search -----------------------------------------------------------
     def beam_select(self, *, logits_ptr: int, dtype: str, scores_in_ptr: int, batch: int,
