@@ -1209,7 +1209,7 @@ static int prompt_attn_impl(kcmm_pool_t *h, const char *op, kcmm::dev::Dtype dty
   p->use_device();
   alignas(64) unsigned char k_map[128], v_map[128];
   const int64_t head = int64_t(hd);
-  const int rows = kcmm::dev::prompt_attn_box_rows();
+  const int rows = kcmm::dev::prompt_attn_box_rows(int(hd));
   if (!kcmm::encode_rows_tensor_map(k_map, k, num_k, int(hkv), int(hd),
                                     k_token ? k_token : head * hkv, k_head ? k_head : head,
                                     rows) ||

@@ -39,39 +39,66 @@ namespace dev {
 namespace {
 
 constexpr uint64_t kWaitNs = 1000000000ull;
-constexpr int kKeys = 64;           // keys of a step
 constexpr float kShift = 7.f;       // log2 of P where a score is the maximum
 constexpr float kRaise = 8.f;       // log2 by which a step has to exceed the maximum to raise it
+// Which of every 8 pairs of exponentials go to the FMA pipe instead of the MUFU unit.
+constexpr uint32_t kPolyOf8 = 0x88;
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kBlk = 128 * 128;         // 64 values of 128 rows
-constexpr uint32_t kKvBlk = kKeys * 128;     // 64 values of a step's keys
+constexpr uint32_t kQBlk = 128 * 128;  // 64 values of 128 rows
 constexpr size_t kMaxSmem = 227 * 1024;
+constexpr int kItemSlots = 2;
+
+// How a tile's scores and P share the TMEM columns that O leaves.
+enum class Scores {
+  kInPlace,   // P over the scores: QK(j+1) after P.V(j)
+  kSeparate,  // P beside the scores: QK(j+1) once the scores are in registers
+  kDouble,    // two score buffers, P over each: QK(j+1) before P.V(j)
+};
 
 template <int DP>
 struct Shape {
   static constexpr int NT = DP <= 128 ? 2 : 1;  // tiles of 128 rows: O takes DP columns each
+  static constexpr Scores kScores = DP <= 64    ? Scores::kSeparate
+                                    : DP <= 128 ? Scores::kInPlace
+                                                : Scores::kDouble;
+  static constexpr bool kAhead = kScores != Scores::kInPlace;  // QK(j+1) comes before P.V(j)
+  static constexpr int kBufs = kScores == Scores::kDouble ? 2 : 1;
+  static constexpr int kKeys = DP <= 128 ? 128 : 64;  // keys of a step
   static constexpr int kRows = 128 * NT;
   static constexpr int kBlocks = DP / 64;
-  static constexpr uint32_t kTileQ = kBlocks * kBlk;
+  static constexpr uint32_t kKvBlk = kKeys * 128;  // 64 values of a step's keys
+  static constexpr uint32_t kTileQ = kBlocks * kQBlk;
   static constexpr uint32_t kTileKv = kBlocks * kKvBlk;
-  static constexpr uint32_t kFixed = NT * kTileQ + 1024 + 512;  // alignment, barriers
-  static constexpr int kFit = int((kMaxSmem - kFixed) / (2 * kTileKv));
-  static constexpr int kStages = kFit > 6 ? 6 : kFit;
-  static_assert(kStages >= 2, "two K and V tiles have to fit");
-  static constexpr uint32_t kOffK = NT * kTileQ;
-  static constexpr uint32_t kOffV = kOffK + kStages * kTileKv;
-  static constexpr uint32_t kOffBar = kOffV + kStages * kTileKv;
+  static constexpr uint32_t kFixed = NT * kTileQ + 1024 + 512 + 256;  // alignment, barriers
+  static constexpr int kFit = int((kMaxSmem - kFixed) / kTileKv);
+  static constexpr int kSlots = kFit > 10 ? 10 : kFit;  // K and V tiles in flight
+  static_assert(kSlots >= 4, "K and V of two steps have to fit");
+  static constexpr uint32_t kOffKv = NT * kTileQ;
+  static constexpr uint32_t kOffBar = kOffKv + kSlots * kTileKv;
   static constexpr size_t kSmem = kOffBar + 512 + 1024;
   static constexpr int kSoftmaxWarps = 4 * NT;
-  static constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
-  static constexpr uint32_t kO = 128 * NT;  // TMEM column of O
-  // barriers
-  static constexpr int kQFull = 0, kKFull = 1, kKEmpty = kKFull + kStages,
-                       kVFull = kKEmpty + kStages, kVEmpty = kVFull + kStages,
-                       kVLast = kVEmpty + kStages, kSFull = kVLast + 1, kPFull = kSFull + 2 * NT,
-                       kODone = kPFull + 2 * NT, kDrain = kODone + 2 * NT, kSlot = kDrain + 1;
-  static_assert((kSlot + 1) * 8 <= 512, "barrier space");
+  static constexpr int kThreads = (kSoftmaxWarps + 4) * 32;
+  // TMEM columns: scores, P where it is separate, O
+  static constexpr uint32_t kS = 0;
+  static constexpr uint32_t kP = kScores == Scores::kSeparate ? NT * kKeys : 0;
+  static constexpr uint32_t kO = NT * kBufs * kKeys +
+                                 (kScores == Scores::kSeparate ? NT * kKeys / 2 : 0);
   static_assert(kO + NT * DP <= kTmemCols, "TMEM");
+  // barriers; those of a tile by [x][buffer]
+  static constexpr int kQFull = 0, kQFree = 1, kKvFull = 2, kKvEmpty = kKvFull + kSlots,
+                       kVLast = kKvEmpty + kSlots, kSFull = kVLast + 1,
+                       kSFree = kSFull + NT * kBufs, kPFull = kSFree + NT,  // halves of P: + 1
+                       kODone = kPFull + 2 * NT, kItemFull = kODone + NT,
+                       kItemEmpty = kItemFull + kItemSlots, kDrain = kItemEmpty + kItemSlots,
+                       kSlot = kDrain + 1;
+  static_assert((kSlot + 1) * 8 <= 512, "barrier space");
+  // Register split: the launch gives every thread kLaunchRegs; two softmax warpgroups then take
+  // kSoftmaxRegs and the other one keeps kOtherRegs.  setmaxnreg.inc waits until the registers
+  // are free in the CTA's pool, so that the split must not exceed it; the launcher checks the
+  // compiled kernel's count too.
+  static constexpr bool kSplitRegs = NT == 2;
+  static constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
+  static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= 384 * kLaunchRegs, "register pool");
 };
 
 struct Params {
@@ -79,6 +106,8 @@ struct Params {
   PromptAttnArgs a;
   float scale_log2;
   uint32_t idesc_qk, idesc_pv;
+  uint32_t group_magic;  // ceil(2^32 / group), 0 for a group of 1
+  int32_t *next_item;    // zero, and zero again after the call
 };
 
 template <typename T>
@@ -101,6 +130,57 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
   }
 }
 
+// Pairs of 32-bit values and their operations, one instruction a pair.
+struct Pair {
+  uint64_t b;
+};
+__device__ __forceinline__ Pair pair(float x, float y) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.b) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(Pair p, float &x, float &y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p.b));
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.b) : "l"(a.b), "l"(b.b), "l"(c.b));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.b) : "l"(a.b), "l"(b.b));
+  return r;
+}
+// Three-input maximum that keeps a NaN.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x of a pair on the FMA and integer pipes, for finite x <= 127 and -inf: x = n + f with n
+// from adding 1.5 2^23, 2^f on [-1/2, 1/2] as a polynomial of degree 4 with 2^0 exactly 1 (fitted
+// for the least largest relative error, 3e-6), n added to its exponent.  Below -127: 0.
+__device__ __forceinline__ void exp2_poly(Pair x, float &e0, float &e1) {
+  constexpr float kMagic = 12582912.f;
+  float a, b;
+  unpair(x, a, b);
+  x = pair(fmaxf(a, -127.f), fmaxf(b, -127.f));
+  const Pair t = add2(x, pair(kMagic, kMagic));
+  const Pair n = add2(t, pair(-kMagic, -kMagic));
+  const Pair f = fma2(n, pair(-1.f, -1.f), x);
+  Pair r = fma2(f, pair(0x1.39f3a6p-7f, 0x1.39f3a6p-7f), pair(0x1.c9fb52p-5f, 0x1.c9fb52p-5f));
+  r = fma2(r, f, pair(0x1.ec03b6p-3f, 0x1.ec03b6p-3f));
+  r = fma2(r, f, pair(0x1.62e132p-1f, 0x1.62e132p-1f));
+  r = fma2(r, f, pair(1.f, 1.f));
+  float t0, t1, r0, r1;
+  unpair(t, t0, t1);
+  unpair(r, r0, r1);
+  e0 = __int_as_float(__float_as_int(r0) + (__float_as_int(t0) << 23));
+  e1 = __int_as_float(__float_as_int(r1) + (__float_as_int(t1) << 23));
+}
+
 struct Seq {
   int q0, nq, k0, nk;
 };
@@ -116,18 +196,23 @@ __device__ __forceinline__ Seq load_seq(const PromptAttnArgs &a, int b, bool *ba
 }
 
 struct Item {
-  int b, h, t;  // sequence, kv head, row tile (from its start)
+  int b, h, t;         // sequence, kv head, row tile (from its start); b < 0: no more
+  int q0, nq, k0, nk;  // the sequence's rows
 };
 // Work item `i` of the list (sequence, kv head, row tiles from the last, which sees the most
-// keys, to the first); false past the list's end.  One warp: lane l looks at sequence 32 n + l.
+// keys, to the first); b = -1 past the list's end, and *total then its length.  One warp: lane l
+// looks at sequence 32 n + l.
 template <int ROWS>
-__device__ __forceinline__ bool find_item(const PromptAttnArgs &a, int64_t i, Item *it) {
+__device__ __forceinline__ Item find_item(const PromptAttnArgs &a, int64_t i, int64_t *total) {
   const int lane = threadIdx.x & 31, G = a.group;
-  bool bad = false, found = false;
-  for (int b0 = 0; b0 < a.batch && !found; b0 += 32) {
+  const int64_t asked = i;
+  bool bad = false;
+  Item it = {-1, 0, 0, 0, 0, 0, 0};
+  for (int b0 = 0; b0 < a.batch && it.b < 0; b0 += 32) {
     const int b = b0 + lane;
-    int64_t nt = 0;
-    if (b < a.batch) nt = (int64_t(load_seq(a, b, &bad).nq) * G + ROWS - 1) / ROWS;
+    Seq s = {0, 0, 0, 0};
+    if (b < a.batch) s = load_seq(a, b, &bad);
+    const int64_t nt = (int64_t(s.nq) * G + ROWS - 1) / ROWS;
     int64_t end = nt * a.kv_heads;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -137,65 +222,76 @@ __device__ __forceinline__ bool find_item(const PromptAttnArgs &a, int64_t i, It
     const uint32_t after = __ballot_sync(0xffffffffu, i < end);
     if (after) {
       const int l = __ffs(after) - 1;
-      const int64_t rel = i - (__shfl_sync(0xffffffffu, end, l) -
-                               __shfl_sync(0xffffffffu, nt, l) * a.kv_heads);
       const int64_t n = __shfl_sync(0xffffffffu, nt, l);
-      it->b = b0 + l;
-      it->h = int(rel / n);
-      it->t = int(n - 1 - rel % n);
-      found = true;
+      const int64_t rel = i - (__shfl_sync(0xffffffffu, end, l) - n * a.kv_heads);
+      it.b = b0 + l;
+      it.h = int(rel / n);
+      it.t = int(n - 1 - rel % n);
+      it.q0 = __shfl_sync(0xffffffffu, s.q0, l);
+      it.nq = __shfl_sync(0xffffffffu, s.nq, l);
+      it.k0 = __shfl_sync(0xffffffffu, s.k0, l);
+      it.nk = __shfl_sync(0xffffffffu, s.nk, l);
     } else {
       i -= __shfl_sync(0xffffffffu, end, 31);
     }
   }
   if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(a.diag, int32_t(kDiagBadLaunch));
-  return found;
+  *total = asked - i;
+  return it;
+}
+
+// Keys that tile x of an item looks at: those that its last row sees.
+template <int ROWS>
+__device__ __forceinline__ int tile_keys(const PromptAttnArgs &a, const Item &it, int x) {
+  const int64_t rows = int64_t(it.nq) * a.group, first = int64_t(it.t) * ROWS + 128 * x;
+  if (first >= rows) return 0;
+  if (!a.causal) return it.nk;
+  const int64_t last = min(first + 128, rows) - 1;
+  return int(max(int64_t(0), min(int64_t(it.nk), last / a.group + it.nk - it.nq + 1)));
 }
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     prompt_attn_kernel(const __grid_constant__ Params P) {
   using S = Shape<DP>;
-  constexpr int NT = S::NT;
+  constexpr int NT = S::NT, KEYS = S::kKeys;
   const PromptAttnArgs &a = P.a;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t raw = ptx::smem_u32(smem_raw);
   const uint32_t sb = (raw + 1023u) & ~1023u;
   unsigned char *smem = smem_raw + (sb - raw);
   __shared__ int s_fail;
-  __shared__ Item s_item;
-  __shared__ int s_found;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int kMmaWarp = S::kSoftmaxWarps, kTmaWarp = kMmaWarp + 1;
+  __shared__ Item s_items[kItemSlots];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  constexpr int kMmaWarp = S::kSoftmaxWarps, kTmaWarp = kMmaWarp + 1, kQWarp = kMmaWarp + 2;
   auto bar = [&](int i) { return sb + S::kOffBar + uint32_t(i) * 8; };
 
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
-  if (warp == 0) {
-    Item it = {0, 0, 0};
-    const bool found = find_item<S::kRows>(a, int64_t(blockIdx.x), &it);
-    if (lane == 0) {
-      s_item = it;
-      s_found = found;
-      s_fail = 0;
-    }
-  } else if (warp == kTmaWarp) {
+  if (warp == kTmaWarp) {
     if (lane == 0) {
       ptx::prefetch_tensormap(&P.tmk);
       ptx::prefetch_tensormap(&P.tmv);
-      ptx::mbar_init(bar(S::kQFull), S::kSoftmaxWarps * 32);
-      for (int i = 0; i < S::kStages; ++i) {
-        ptx::mbar_init(bar(S::kKFull + i), 1);
-        ptx::mbar_init(bar(S::kKEmpty + i), 1);
-        ptx::mbar_init(bar(S::kVFull + i), 1);
-        ptx::mbar_init(bar(S::kVEmpty + i), 1);
+      s_fail = 0;
+      ptx::mbar_init(bar(S::kQFull), 2);
+      ptx::mbar_init(bar(S::kQFree), 1);
+      for (int i = 0; i < S::kSlots; ++i) {
+        ptx::mbar_init(bar(S::kKvFull + i), 1);
+        ptx::mbar_init(bar(S::kKvEmpty + i), 1);
       }
       ptx::mbar_init(bar(S::kVLast), 1);
       ptx::mbar_init(bar(S::kDrain), 1);
-      for (int i = 0; i < 2 * NT; ++i) {
-        ptx::mbar_init(bar(S::kSFull + i), 1);
-        ptx::mbar_init(bar(S::kPFull + i), 128);
-        ptx::mbar_init(bar(S::kODone + i), 1);
+      for (int i = 0; i < NT * S::kBufs; ++i) ptx::mbar_init(bar(S::kSFull + i), 1);
+      for (int x = 0; x < NT; ++x) {
+        ptx::mbar_init(bar(S::kSFree + x), 128);
+        ptx::mbar_init(bar(S::kPFull + 2 * x), 128);
+        ptx::mbar_init(bar(S::kPFull + 2 * x + 1), 128);
+        ptx::mbar_init(bar(S::kODone + x), 1);
+      }
+      for (int i = 0; i < kItemSlots; ++i) {
+        ptx::mbar_init(bar(S::kItemFull + i), 1);
+        ptx::mbar_init(bar(S::kItemEmpty + i), S::kSoftmaxWarps + 3);
       }
       ptx::fence_mbarrier_init();
     }
@@ -209,277 +305,415 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + S::kOffBar + S::kSlot * 8);
   volatile int *fail = &s_fail;
 
-  if (s_found) {
-    const Item it = s_item;
-    bool bad = false;
-    const Seq s = load_seq(a, it.b, &bad);
-    const int G = a.group;
-    const int64_t rows = int64_t(s.nq) * G, row0 = int64_t(it.t) * S::kRows;
-    const int past = s.nk - s.nq;  // keys before the first query
-    // keys that tile x's last row sees, in steps
-    auto steps = [&](int x) {
-      const int64_t last = min(row0 + 128 * (x + 1), rows) - 1;
-      if (last < row0 + 128 * x) return 0;
-      const int64_t n = a.causal ? min(int64_t(s.nk), last / G + past + 1) : int64_t(s.nk);
-      return n <= 0 ? 0 : int((n + kKeys - 1) / kKeys);
-    };
-    int n_steps[NT];
-#pragma unroll
-    for (int x = 0; x < NT; ++x) n_steps[x] = steps(x);
-    int n_max = n_steps[0];
-    if constexpr (NT == 2) n_max = max(n_steps[0], n_steps[1]);
+  // The CTA's k-th item, from the warp that hands them out; b < 0 ends the role.
+  auto next_item = [&](int k) {
+    Item it = {-1, 0, 0, 0, 0, 0, 0};
+    const int slot = k % kItemSlots;
+    if (!wait(bar(S::kItemFull + slot), uint32_t((k / kItemSlots) & 1), fail)) return it;
+    it = s_items[slot];
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(bar(S::kItemEmpty + slot));
+    return it;
+  };
+  auto steps_of = [&](int keys) { return (keys + KEYS - 1) / KEYS; };
+  // K and V tiles pass through the slots in the order in which the products need them:
+  // K0 V0 K1 V1 .., or K0 K1 V0 K2 V1 .. where QK runs ahead.
+  auto pos_k = [&](int j) { return S::kAhead ? (j == 0 ? 0 : 2 * j - 1) : 2 * j; };
+  auto pos_v = [&](int j, int n) { return S::kAhead ? min(2 * j + 2, 2 * n - 1) : 2 * j + 1; };
 
-    if (warp == kTmaWarp) {
-      int issued_k = 0, issued_v = 0;  // steps whose copies have begun
-      for (int j = 0; j < n_max; ++j) {
-        const int st = j % S::kStages;
-        const uint32_t ph = uint32_t((j / S::kStages - 1) & 1);
-        const int key = s.k0 + j * kKeys;
-        if (j >= S::kStages && !wait(bar(S::kKEmpty + st), ph, fail)) break;
+  if (warp >= S::kSoftmaxWarps) {
+  if constexpr (S::kSplitRegs)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegs));
+  if (warp >= kQWarp) {
+    // ---------------- Q, and the first of the two warps hands out the items ----------------
+    // The next item of the list.  Every CTA asks once past the end, and the last to do so leaves
+    // the counter at zero.
+    auto take = [&] {
+      int32_t i = 0;
+      if (lane == 0) i = atomicAdd(P.next_item, 1);
+      i = __shfl_sync(0xffffffffu, i, 0);
+      int64_t total = 0;
+      const Item it = find_item<S::kRows>(a, i, &total);
+      if (it.b < 0 && lane == 0 && i == total + int64_t(gridDim.x) - 1) atomicExch(P.next_item, 0);
+      return it;
+    };
+    bool ended = warp != kQWarp;
+    for (int k = 0;; ++k) {
+      Item it;
+      if (warp == kQWarp) {
+        const int slot = k % kItemSlots;
+        if (k >= kItemSlots &&
+            !wait(bar(S::kItemEmpty + slot), uint32_t((k / kItemSlots - 1) & 1), fail))
+          break;
+        it = take();
+        ended = it.b < 0;
         if (lane == 0) {
-          ptx::mbar_arrive_expect_tx(bar(S::kKFull + st), S::kTileKv);
-#pragma unroll
-          for (int c = 0; c < S::kBlocks; ++c)
-            ptx::tma_load_3d(sb + S::kOffK + st * S::kTileKv + c * kKvBlk, &P.tmk, c * 64, it.h,
-                             key, bar(S::kKFull + st));
+          s_items[slot] = it;
+          ptx::mbar_arrive(bar(S::kItemFull + slot));
         }
         __syncwarp();
-        issued_k = j + 1;
-        if (j >= S::kStages && !wait(bar(S::kVEmpty + st), ph, fail)) break;
-        // Rows past the sequence are another's: P is 0 there, and V has to be finite.
-        const int live = min(kKeys, s.nk - j * kKeys);
-        const uint32_t full = bar(live < kKeys ? S::kVLast : S::kVFull + st);
-        const uint32_t dst = sb + S::kOffV + st * S::kTileKv;
-        if (lane == 0) {
-          ptx::mbar_arrive_expect_tx(full, S::kTileKv);
-#pragma unroll
-          for (int c = 0; c < S::kBlocks; ++c)
-            ptx::tma_load_3d(dst + c * kKvBlk, &P.tmv, c * 64, it.h, key, full);
-        }
-        __syncwarp();
-        if (live < kKeys) {  // the sequence's last step, once
-          if (!wait(full, 0, fail)) break;
-          const int words = (kKeys - live) * 8;  // 16-byte words of a block's rows
-          for (int i = lane; i < words * S::kBlocks; i += 32) {
-            const uint32_t at = dst + (i / words) * kKvBlk + live * 128 + (i % words) * 16;
-            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0) : "memory");
-          }
-          ptx::fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(bar(S::kVFull + st));
-          __syncwarp();
-        } else {
-          issued_v = j + 1;
-        }
+      } else {
+        it = next_item(k);
       }
-      if (*fail) {  // no copy may land after the CTA has gone
-        for (int j = max(0, issued_k - S::kStages); j < issued_k; ++j)
-          ptx::mbar_wait_bounded(bar(S::kKFull + j % S::kStages),
-                                 uint32_t((j / S::kStages) & 1), kWaitNs);
-        for (int j = max(0, issued_v - S::kStages); j < issued_v; ++j)
-          ptx::mbar_wait_bounded(bar(S::kVFull + j % S::kStages),
-                                 uint32_t((j / S::kStages) & 1), kWaitNs);
-      }
-    } else if (warp == kMmaWarp) {
-      auto issue_qk = [&](int x, int j) {
-        if (lane == 0) {
-          const uint32_t qa = sb + uint32_t(x) * S::kTileQ;
-          const uint32_t ka = sb + S::kOffK + (j % S::kStages) * S::kTileKv;
-          const uint32_t tS = tmem + uint32_t(2 * x + (j & 1)) * kKeys;
-          tc::fence_after_sync();
-#pragma unroll
-          for (int k = 0; k < DP / 16; ++k)
-            tc::mma_ss(tS, tc::sw128_desc(qa + (k >> 2) * kBlk + (k & 3) * 32, 16, 1024),
-                       tc::sw128_desc(ka + (k >> 2) * kKvBlk + (k & 3) * 32, 16, 1024),
-                       P.idesc_qk, k > 0);
-          tc::commit(bar(S::kSFull + 2 * x + (j & 1)));
-        }
-        __syncwarp();
-      };
-      auto issue_pv = [&](int x, int j) {
-        if (lane == 0) {
-          const uint32_t va = sb + S::kOffV + (j % S::kStages) * S::kTileKv;
-          const uint32_t tP = tmem + uint32_t(2 * x + (j & 1)) * kKeys;
-          const uint32_t tO = tmem + S::kO + uint32_t(x) * DP;
-          tc::fence_after_sync();
-#pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            tc::mma_ts(tO, tP + k * 8, tc::sw128_desc(va + k * 2048, kKvBlk, 1024), P.idesc_pv,
-                       j > 0 || k > 0);
-          tc::commit(bar(S::kODone + 2 * x + (j & 1)));
-        }
-        __syncwarp();
-      };
-      auto release = [&](int b) {
-        if (lane == 0) tc::commit(bar(b));
-        __syncwarp();
-      };
-      bool ok = n_max == 0 || wait(bar(S::kQFull), 0, fail);
-      for (int j = 0; ok && j < min(2, n_max); ++j) {
-        ok = wait(bar(S::kKFull + j % S::kStages), 0, fail);
-        if (!ok) break;
-#pragma unroll
-        for (int x = 0; x < NT; ++x)
-          if (j < n_steps[x]) issue_qk(x, j);
-        release(S::kKEmpty + j % S::kStages);
-      }
-      for (int j = 0; ok && j < n_max; ++j) {
-        const int st = j % S::kStages, jn = j + 2, sn = jn % S::kStages;
-        ok = wait(bar(S::kVFull + st), uint32_t((j / S::kStages) & 1), fail);
-        if (ok && jn < n_max)
-          ok = wait(bar(S::kKFull + sn), uint32_t((jn / S::kStages) & 1), fail);
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          if (!ok || j >= n_steps[x]) continue;
-          ok = wait(bar(S::kPFull + 2 * x + (j & 1)), uint32_t((j >> 1) & 1), fail);
-          if (!ok) continue;
-          issue_pv(x, j);
-          if (jn < n_steps[x]) issue_qk(x, jn);
-        }
-        if (!ok) break;
-        release(S::kVEmpty + st);
-        if (jn < n_max) release(S::kKEmpty + sn);
-      }
-      if (!ok) {  // no product may run on after the CTA has gone
-        release(S::kDrain);
-        ptx::mbar_wait_bounded(bar(S::kDrain), 0, kWaitNs);
-      }
-    } else {
-      // Q: 16 bytes a lane; rows and values past the end are zeros
+      if (it.b < 0) break;
+      if (k > 0 && !wait(bar(S::kQFree), uint32_t((k - 1) & 1), fail)) break;
+      // 16 bytes a lane; rows and values past the end are zeros
       constexpr int kChunks = DP / 8;
-      for (int i = tid; i < S::kRows * kChunks; i += S::kSoftmaxWarps * 32) {
+      const int G = a.group;
+      const int64_t row0 = int64_t(it.t) * S::kRows;
+      const int tok0 = int(row0 / G), in0 = int(row0 % G);
+      const int left = int(min(int64_t(S::kRows), int64_t(it.nq) * G - row0));
+      const uint16_t *base = static_cast<const uint16_t *>(a.q) +
+                             (int64_t(it.q0) + tok0) * a.q_stride_token +
+                             int64_t(it.h) * G * a.q_stride_head;
+#pragma unroll 4
+      for (int i = (warp - kQWarp) * 32 + lane; i < S::kRows * kChunks; i += 64) {
         const int r = i / kChunks, c = i % kChunks;
-        const int64_t row = row0 + r;
-        const bool in = row < rows && c * 8 < a.head_dim;
-        const int64_t tok = in ? row / G : 0;
-        const int head = in ? it.h * G + int(row % G) : 0;
-        const uint16_t *src = static_cast<const uint16_t *>(a.q) +
-                              (in ? (s.q0 + tok) * a.q_stride_token +
-                                        int64_t(head) * a.q_stride_head + c * 8
-                                  : 0);
-        const uint32_t dst = sb + uint32_t(r >> 7) * S::kTileQ + uint32_t(c >> 3) * kBlk +
+        const bool in = r < left && c * 8 < a.head_dim;
+        const uint32_t at = uint32_t(in0 + r);
+        const uint32_t tok = P.group_magic ? __umulhi(at, P.group_magic) : at;
+        const uint16_t *src = base + int64_t(tok) * a.q_stride_token +
+                              int64_t(at - tok * G) * a.q_stride_head + c * 8;
+        const uint32_t dst = sb + uint32_t(r >> 7) * S::kTileQ + uint32_t(c >> 3) * kQBlk +
                              uint32_t(r & 127) * 128 + uint32_t(((c & 7) ^ (r & 7)) * 16);
-        ptx::cp_async16(dst, src, in ? 16u : 0u);
+        ptx::cp_async16(dst, in ? src : static_cast<const uint16_t *>(a.q), in ? 16u : 0u);
       }
       ptx::cp_async_commit();
       ptx::cp_async_wait<0>();
       ptx::fence_proxy_async_smem();
-      ptx::mbar_arrive(bar(S::kQFull));
-
-      const int x = warp >> 2, q4 = warp & 3;
-      const int n = NT == 2 && x == 1 ? n_steps[NT - 1] : n_steps[0];
-      const int64_t row = row0 + 128 * x + q4 * 32 + lane;
-      const bool row_ok = row < rows;
-      // last key that the row sees; rows past the end go as far as the last one
-      const int tok = int(min(row, rows - 1) / G);
-      const int lim = a.causal ? tok + past : s.nk - 1;
-      const int lim0 = __shfl_sync(0xffffffffu, lim, 0);
-      const uint32_t lanes = uint32_t(q4 * 32) << 16;
-      const uint32_t tO = tmem + S::kO + uint32_t(x) * DP + lanes;
-      float m = -INFINITY, l = 0.f;
-      bool ok = true;
-      for (int j = 0; j < n; ++j) {
-        const uint32_t tS = tmem + uint32_t(2 * x + (j & 1)) * kKeys + lanes;
-        if (!wait(bar(S::kSFull + 2 * x + (j & 1)), uint32_t((j >> 1) & 1), fail)) {
-          ok = false;
-          break;
-        }
-        // S(j) came after P.V(j-2), whose barrier is thus the one before P.V(j)'s
-        if (j >= 2 &&
-            !wait(bar(S::kODone + 2 * x + (j & 1)), uint32_t(((j - 2) >> 1) & 1), fail)) {
-          ok = false;
-          break;
-        }
-        tc::fence_after_sync();
-        float v[kKeys];
-        tc::ld32(tS, v);
-        tc::ld32(tS + 32, v + 32);
-        tc::wait_ld();
-        const int k0 = j * kKeys;
-        if (k0 + kKeys - 1 > lim0) {
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(S::kQFull));
+    }
+    while (!ended) ended = take().b < 0;  // after a failure: the counter has to end at zero
+  } else if (warp == kTmaWarp) {
+    // ---------------- K and V ----------------
+    int pos = 0, lasts = 0;  // tiles of the items before; sequences' last tiles among them
+    int begun = 0;           // tiles whose copies have begun on their slots' barriers
+    bool ok = true, last_begun = false;
+    for (int k = 0; ok; ++k) {
+      const Item it = next_item(k);
+      if (it.b < 0) break;
+      int keys = tile_keys<S::kRows>(a, it, NT - 1);
+      if (NT == 2) keys = max(keys, tile_keys<S::kRows>(a, it, 0));
+      const int n = steps_of(keys);
+      auto slot_of = [&](int p) { return (pos + p) % S::kSlots; };
+      auto free_slot = [&](int p) {
+        const int q = pos + p;
+        return q < S::kSlots ||
+               wait(bar(S::kKvEmpty + q % S::kSlots), uint32_t((q / S::kSlots - 1) & 1), fail);
+      };
+      auto load = [&](const CUtensorMap *map, int p, int j, uint32_t full) {
+        if (lane == 0) {
+          const uint32_t dst = sb + S::kOffKv + uint32_t(slot_of(p)) * S::kTileKv;
+          ptx::mbar_arrive_expect_tx(full, S::kTileKv);
 #pragma unroll
-          for (int c = 0; c < kKeys; ++c) v[c] = k0 + c > lim ? -INFINITY : v[c];
+          for (int c = 0; c < S::kBlocks; ++c)
+            ptx::tma_load_3d(dst + c * S::kKvBlk, map, c * 64, it.h, it.k0 + j * KEYS, full);
+        }
+        __syncwarp();
+      };
+      auto load_k = [&](int j) {
+        const int p = pos_k(j);
+        if (!free_slot(p)) return false;
+        load(&P.tmk, p, j, bar(S::kKvFull + slot_of(p)));
+        begun = pos + p + 1;
+        return true;
+      };
+      auto load_v = [&](int j) {
+        const int p = pos_v(j, n);
+        if (!free_slot(p)) return false;
+        // Rows past the sequence are another's.  P is 0 there, but V has to be finite: those of
+        // the last 16 keys that a product reads are cleared.
+        const int live = min(KEYS, it.nk - j * KEYS), end = min(KEYS, (live + 15) / 16 * 16);
+        if (live == end) {
+          load(&P.tmv, p, j, bar(S::kKvFull + slot_of(p)));
+          begun = pos + p + 1;
+          return true;
+        }
+        load(&P.tmv, p, j, bar(S::kVLast));
+        last_begun = true;
+        if (!wait(bar(S::kVLast), uint32_t(lasts & 1), fail)) return false;
+        last_begun = false;
+        ++lasts;
+        const uint32_t dst = sb + S::kOffKv + uint32_t(slot_of(p)) * S::kTileKv;
+        const int words = (end - live) * 8;  // 16-byte words of a block's rows
+        for (int i = lane; i < words * S::kBlocks; i += 32) {
+          const uint32_t at = dst + (i / words) * S::kKvBlk + live * 128 + (i % words) * 16;
+          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0) : "memory");
+        }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(S::kKvFull + slot_of(p)));
+        __syncwarp();
+        begun = pos + p + 1;
+        return true;
+      };
+      if (S::kAhead && n > 0) ok = load_k(0);
+      for (int j = 0; ok && j < n; ++j) {
+        if (S::kAhead) {
+          ok = (j + 1 >= n || load_k(j + 1)) && load_v(j);
+        } else {
+          ok = load_k(j) && load_v(j);
+        }
+      }
+      pos += 2 * n;
+    }
+    if (*fail) {  // no copy may land after the CTA has gone
+      for (int q = max(0, begun - S::kSlots); q < begun; ++q)
+        ptx::mbar_wait_bounded(bar(S::kKvFull + q % S::kSlots), uint32_t((q / S::kSlots) & 1),
+                               kWaitNs);
+      if (last_begun) ptx::mbar_wait_bounded(bar(S::kVLast), uint32_t(lasts & 1), kWaitNs);
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------- MMA issue ----------------
+    // Warp-uniform in the compiler's eyes too: see mma_ss_warp.
+    const uint32_t base = __shfl_sync(0xffffffffu, sb, 0);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    constexpr uint32_t kHi = tc::kDescHigh;
+    int pos = 0, step[NT] = {};  // of the items before
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      const Item it = next_item(k);
+      if (it.b < 0) break;
+      int keys[NT], n[NT], n_max = 0;
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        keys[x] = __shfl_sync(0xffffffffu, tile_keys<S::kRows>(a, it, x), 0);
+        n[x] = steps_of(keys[x]);
+        n_max = max(n_max, n[x]);
+      }
+      // Slot of a tile, once it is there.
+      auto tile_at = [&](int p, uint32_t *at) {
+        const int q = pos + p;
+        *at = base + S::kOffKv + uint32_t(q % S::kSlots) * S::kTileKv;
+        return wait(bar(S::kKvFull + q % S::kSlots), uint32_t((q / S::kSlots) & 1), fail);
+      };
+      auto release = [&](int p) { tc::commit_warp(bar(S::kKvEmpty + (pos + p) % S::kSlots)); };
+      auto issue_qk = [&](int x, int j, uint32_t at) {
+        const int g = step[x] + j;
+        const uint32_t qa = tc::desc_low(base + uint32_t(x) * S::kTileQ, 16);
+        const uint32_t ka = tc::desc_low(at, 16);
+        const uint32_t tS = tm + S::kS + uint32_t(x * S::kBufs + g % S::kBufs) * KEYS;
+        tc::fence_after_sync();
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+          tc::mma_ss_warp(tS, qa + ((c >> 2) * kQBlk + (c & 3) * 32) / 16,
+                          ka + ((c >> 2) * S::kKvBlk + (c & 3) * 32) / 16, kHi, P.idesc_qk, c > 0);
+        tc::commit_warp(bar(S::kSFull + x * S::kBufs + g % S::kBufs));
+      };
+      // P.V of one half of a step's keys: the 16-key products that hold a key.
+      auto issue_pv = [&](int x, int j, int half, uint32_t at) {
+        const int g = step[x] + j;
+        const uint32_t va = tc::desc_low(at, S::kKvBlk);
+        const uint32_t tP = tm + (S::kScores == Scores::kSeparate
+                                      ? S::kP + uint32_t(x) * (KEYS / 2)
+                                      : S::kS + uint32_t(x * S::kBufs + g % S::kBufs) * KEYS);
+        const uint32_t tO = tm + S::kO + uint32_t(x) * DP;
+        const int live = keys[x] - j * KEYS;
+        tc::fence_after_sync();
+#pragma unroll
+        for (int c = 0; c < KEYS / 32; ++c) {
+          const int i = half * (KEYS / 32) + c;
+          if (i * 16 < live)
+            tc::mma_ts_warp(tO, tP + i * 8, va + i * 2048 / 16, kHi, P.idesc_pv, j > 0 || i > 0);
+        }
+      };
+      ok = wait(bar(S::kQFull), uint32_t(k & 1), fail);
+      uint32_t at_k = 0, at_v = 0;
+      if (ok && n_max > 0) {
+        ok = tile_at(pos_k(0), &at_k);
+        if (!ok) break;
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+          if (n[x] > 0) issue_qk(x, 0, at_k);
+        release(pos_k(0));
+      }
+      for (int j = 0; ok && j < n_max; ++j) {
+        const bool more = j + 1 < n_max;
+        if (S::kAhead && more) {
+          ok = tile_at(pos_k(j + 1), &at_k);
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+            if (!ok || j + 1 >= n[x]) continue;
+            // the scores of step j (two buffers: P of step j - 1) have left their columns
+            if (S::kScores == Scores::kSeparate)
+              ok = wait(bar(S::kSFree + x), uint32_t((step[x] + j) & 1), fail);
+            if (ok) issue_qk(x, j + 1, at_k);
+          }
+          if (!ok) break;
+          release(pos_k(j + 1));
+        }
+        ok = tile_at(pos_v(j, n_max), &at_v);
+        if (ok && !S::kAhead && more) ok = tile_at(pos_k(j + 1), &at_k);
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          if (!ok || j >= n[x]) continue;
+          const uint32_t ph = uint32_t((step[x] + j) & 1);
+          ok = wait(bar(S::kPFull + 2 * x), ph, fail);
+          if (!ok) continue;
+          issue_pv(x, j, 0, at_v);
+          ok = wait(bar(S::kPFull + 2 * x + 1), ph, fail);
+          if (!ok) continue;
+          issue_pv(x, j, 1, at_v);
+          tc::commit_warp(bar(S::kODone + x));
+          if (!S::kAhead && j + 1 < n[x]) issue_qk(x, j + 1, at_k);
+        }
+        if (!ok) break;
+        release(pos_v(j, n_max));
+        if (!S::kAhead && more) release(pos_k(j + 1));
+      }
+      tc::commit_warp(bar(S::kQFree));
+      pos += 2 * n_max;
+#pragma unroll
+      for (int x = 0; x < NT; ++x) step[x] += n[x];
+    }
+    if (*fail) {  // no product may run on after the CTA has gone
+      tc::commit_warp(bar(S::kDrain));
+      ptx::mbar_wait_bounded(bar(S::kDrain), 0, kWaitNs);
+    }
+  }
+  } else {
+    // ---------------- softmax: thread = row of tile x ----------------
+    if constexpr (S::kSplitRegs)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmaxRegs));
+    const int x = warp >> 2, q4 = warp & 3;
+    const uint32_t lanes = uint32_t(q4 * 32) << 16;
+    const uint32_t tO = tmem + S::kO + uint32_t(x) * DP + lanes;
+    int step = 0;  // of the items before
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      const Item it = next_item(k);
+      if (it.b < 0) break;
+      const int G = a.group;
+      const int64_t rows = int64_t(it.nq) * G;
+      const int64_t row = int64_t(it.t) * S::kRows + 128 * x + q4 * 32 + lane;
+      const bool row_ok = row < rows;
+      const int64_t tok = min(row, rows - 1) / G;
+      // last key that the row sees; rows past the end go as far as the last one
+      const int lim = a.causal ? int(tok) + it.nk - it.nq : it.nk - 1;
+      const int lim0 = __shfl_sync(0xffffffffu, lim, 0);
+      const int n = steps_of(tile_keys<S::kRows>(a, it, x));
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; ok && j < n; ++j) {
+        const int g = step + j, buf = g % S::kBufs;
+        const uint32_t tS = tmem + S::kS + uint32_t(x * S::kBufs + buf) * KEYS + lanes;
+        const uint32_t tP =
+            S::kScores == Scores::kSeparate ? tmem + S::kP + uint32_t(x) * (KEYS / 2) + lanes : tS;
+        ok = wait(bar(S::kSFull + x * S::kBufs + buf), uint32_t((g / S::kBufs) & 1), fail);
+        if (!ok) break;
+        tc::fence_after_sync();
+        float v[KEYS];
+#pragma unroll
+        for (int c = 0; c < KEYS; c += 32) tc::ld32(tS + c, v + c);
+        tc::wait_ld();
+        if constexpr (S::kScores == Scores::kSeparate) {
+          tc::fence_before_sync();
+          ptx::mbar_arrive(bar(S::kSFree + x));
+        }
+        const int k0 = j * KEYS;
+        if (k0 + KEYS - 1 > lim0) {
+#pragma unroll
+          for (int c = 0; c < KEYS; ++c) v[c] = k0 + c > lim ? -INFINITY : v[c];
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < kKeys; c += 8) {
+        for (int c = 0; c < KEYS; c += 8) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = ptx::max3(mx[i], v[c + 2 * i], v[c + 2 * i + 1]);
+          for (int i = 0; i < 4; ++i) mx[i] = max3_nan(mx[i], v[c + 2 * i], v[c + 2 * i + 1]);
         }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * P.scale_log2;
-        const bool raise = top > m + kRaise;  // the first step's m is -inf
+        const float top =
+            max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * P.scale_log2;
+        // a NaN or infinite maximum makes the row NaN, as its softmax is
+        const bool raise = !(top <= m + kRaise);  // the first step's m is -inf
         float f = 1.f;
         if (raise) {
           f = ptx::fast_exp2(m - top);  // 0 before the first key
-          m = top;
+          m = top + (top - top);
           l *= f;
         }
-        if (j > 0 && __any_sync(0xffffffffu, raise)) {
-          // P.V(j-1) has to have added to O; P.V(j) has not begun
-          if (!wait(bar(S::kODone + 2 * x + ((j - 1) & 1)), uint32_t(((j - 1) >> 1) & 1), fail)) {
-            ok = false;
-            break;
-          }
-          tc::fence_after_sync();
+        // P.V of the step before has added to O and read P
+        if (j > 0) {
+          ok = wait(bar(S::kODone + x), uint32_t((g - 1) & 1), fail);
+          if (!ok) break;
+          if (__any_sync(0xffffffffu, raise)) {
+            tc::fence_after_sync();
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+              float o[32];
+              tc::ld32(tO + c, o);
+              tc::wait_ld();
 #pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
-            float o[32];
-            tc::ld32(tO + c * 32, o);
-            tc::wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= f;
-            tc::st32(tO + c * 32, o);
+              for (int e = 0; e < 32; ++e) o[e] *= f;
+              tc::st32(tO + c, o);
+            }
+            tc::wait_st();
           }
-          tc::wait_st();
         }
         const float sub = m == -INFINITY ? 0.f : m - kShift;  // nothing seen yet: P is 0
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t w[kKeys / 2];
+        const Pair scale2 = pair(P.scale_log2, P.scale_log2), sub2 = pair(-sub, -sub);
+        Pair sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
-        for (int c = 0; c < kKeys; c += 2) {
-          const float e0 = ptx::fast_exp2(fmaf(v[c], P.scale_log2, -sub));
-          const float e1 = ptx::fast_exp2(fmaf(v[c + 1], P.scale_log2, -sub));
-          sum[c & 2] += e0;
-          sum[(c & 2) + 1] += e1;
-          w[c / 2] = pack2<T>(e0, e1);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tc::st32u(tS, w);
-        tc::wait_st();
-        tc::fence_before_sync();
-        ptx::mbar_arrive(bar(S::kPFull + 2 * x + (j & 1)));
-      }
-      if (ok && n > 0)
-        ok = wait(bar(S::kODone + 2 * x + ((n - 1) & 1)), uint32_t(((n - 1) >> 1) & 1), fail);
-      if (ok) {
-        tc::fence_after_sync();
-        const float inv = l > 0.f ? 1.f / l : l;  // l is 0, or a NaN that stays one
-        const bool none = n == 0 || l == 0.f;
-        uint16_t *dst = static_cast<uint16_t *>(a.out) +
-                        (row_ok ? (s.q0 + row / G) * a.out_stride_token +
-                                      (int64_t(it.h) * G + row % G) * a.out_stride_head
-                                : 0);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t w[KEYS / 4];
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-          float o[32];
-          if (n > 0) {
-            tc::ld32(tO + c * 32, o);
-            tc::wait_ld();
+          for (int i = 0; i < KEYS / 4; ++i) {
+            const int c = half * (KEYS / 4) + i;
+            const Pair e = fma2(pair(v[2 * c], v[2 * c + 1]), scale2, sub2);
+            float e0, e1;
+            if (kPolyOf8 >> (c & 7) & 1) {
+              exp2_poly(e, e0, e1);
+            } else {
+              unpair(e, e0, e1);
+              e0 = ptx::fast_exp2(e0);
+              e1 = ptx::fast_exp2(e1);
+            }
+            sum[c & 1] = add2(sum[c & 1], pair(e0, e1));
+            w[i] = pack2<T>(e0, e1);
           }
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : o[e] * inv;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (!row_ok || c * 32 + q * 8 >= a.head_dim) continue;
-            uint4 u;
-            u.x = pack2<T>(o[q * 8], o[q * 8 + 1]);
-            u.y = pack2<T>(o[q * 8 + 2], o[q * 8 + 3]);
-            u.z = pack2<T>(o[q * 8 + 4], o[q * 8 + 5]);
-            u.w = pack2<T>(o[q * 8 + 6], o[q * 8 + 7]);
-            *reinterpret_cast<uint4 *>(dst + c * 32 + q * 8) = u;
+          if constexpr (KEYS == 128) {
+            tc::st32u(tP + half * 32, w);
+          } else {
+            tc::st16u(tP + half * 16, w);
           }
+          tc::wait_st();
+          tc::fence_before_sync();
+          ptx::mbar_arrive(bar(S::kPFull + 2 * x + half));
+        }
+        float s0, s1;
+        unpair(add2(sum[0], sum[1]), s0, s1);
+        l += s0 + s1;
+      }
+      if (ok && n > 0) ok = wait(bar(S::kODone + x), uint32_t((step + n - 1) & 1), fail);
+      if (!ok) break;
+      step += n;
+      tc::fence_after_sync();
+      const bool none = n == 0 || l == 0.f;
+      const float inv = none ? 0.f : 1.f / l;
+      uint16_t *dst = static_cast<uint16_t *>(a.out) +
+                      (row_ok ? (it.q0 + tok) * a.out_stride_token +
+                                    (int64_t(it.h) * G + (row - tok * G)) * a.out_stride_head
+                              : 0);
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        float o[32];
+        if (n > 0) {
+          tc::ld32(tO + c, o);
+          tc::wait_ld();
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : o[e] * inv;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (!row_ok || c + q * 8 >= a.head_dim) continue;
+          uint4 u;
+          u.x = pack2<T>(o[q * 8], o[q * 8 + 1]);
+          u.y = pack2<T>(o[q * 8 + 2], o[q * 8 + 3]);
+          u.z = pack2<T>(o[q * 8 + 4], o[q * 8 + 5]);
+          u.w = pack2<T>(o[q * 8 + 6], o[q * 8 + 7]);
+          *reinterpret_cast<uint4 *>(dst + c + q * 8) = u;
         }
       }
+      tc::fence_before_sync();  // before the next item's first P says that O may be overwritten
     }
   }
 
@@ -502,21 +736,41 @@ cudaError_t launch(const PromptAttnArgs &a, cudaStream_t stream) {
   p.a = a;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-  p.idesc_qk = tc::idesc_f16(bf16, 128, kKeys, false, false);
+  p.idesc_qk = tc::idesc_f16(bf16, 128, S::kKeys, false, false);
   p.idesc_pv = tc::idesc_f16(bf16, 128, DP, false, true);
+  p.group_magic = a.group == 1 ? 0 : uint32_t(((uint64_t(1) << 32) + a.group - 1) / a.group);
   auto fn = prompt_attn_kernel<T, DP>;
+  if (S::kSplitRegs) {
+    // with fewer registers at launch than the split was made for, setmaxnreg.inc would wait
+    cudaFuncAttributes fa;
+    const cudaError_t e = cudaFuncGetAttributes(&fa, fn);
+    if (e != cudaSuccess) return e;
+    if (fa.numRegs * S::kThreads < 256 * S::kSoftmaxRegs + 128 * S::kOtherRegs)
+      return cudaErrorInvalidConfiguration;
+  }
   cudaError_t e =
       cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmem));
   if (e != cudaSuccess) return e;
+  CallScratch scratch;
+  e = scratch.acquire(stream, 16);  // for its counters
+  if (e != cudaSuccess) return e;
+  p.next_item = scratch.counters;
   // every sequence has at most one partly filled tile a kv head
-  const int64_t tiles = int64_t(a.num_q_tokens) * a.group / S::kRows + a.batch;
-  return launch_pdl(fn, dim3(uint32_t(tiles * a.kv_heads)), dim3(S::kThreads), S::kSmem, stream,
-                    p);
+  const int64_t items = (int64_t(a.num_q_tokens) * a.group / S::kRows + a.batch) * a.kv_heads;
+  const int ctas = int(std::min<int64_t>(items, device_sm_count()));
+  e = launch_pdl(fn, dim3(uint32_t(ctas)), dim3(S::kThreads), S::kSmem, stream, p);
+  const cudaError_t r = scratch.release(stream);
+  return e != cudaSuccess ? e : r;
 }
 
 }  // namespace
 
-int prompt_attn_box_rows() { return kKeys; }
+int prompt_attn_box_rows(int head_dim) {
+  return head_dim <= 64    ? Shape<64>::kKeys
+         : head_dim <= 128 ? Shape<128>::kKeys
+         : head_dim <= 192 ? Shape<192>::kKeys
+                           : Shape<256>::kKeys;
+}
 
 cudaError_t prompt_attn(const PromptAttnArgs &a, cudaStream_t stream) {
   const bool bf16 = a.dtype == Dtype::BF16;

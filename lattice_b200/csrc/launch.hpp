@@ -111,11 +111,11 @@ struct PromptAttnArgs {
   bool causal;
   int32_t *diag;
   // TMA descriptors of K and V, {head_dim, kv_heads, num_k_tokens} with box
-  // {64, 1, prompt_attn_box_rows()}
+  // {64, 1, prompt_attn_box_rows(head_dim)}
   const void *k_map;
   const void *v_map;
 };
-int prompt_attn_box_rows();
+int prompt_attn_box_rows(int head_dim);
 // head_dim a multiple of 8 up to 256, rows of 16-byte aligned heads.
 cudaError_t prompt_attn(const PromptAttnArgs &a, cudaStream_t stream);
 
