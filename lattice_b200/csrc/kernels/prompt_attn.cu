@@ -41,8 +41,6 @@ namespace {
 constexpr uint64_t kWaitNs = 1000000000ull;
 constexpr float kShift = 7.f;       // log2 of P where a score is the maximum
 constexpr float kRaise = 8.f;       // log2 by which a step has to exceed the maximum to raise it
-// Which of every 8 pairs of exponentials go to the FMA pipe instead of the MUFU unit.
-constexpr uint32_t kPolyOf8 = 0x88;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kQBlk = 128 * 128;  // 64 values of 128 rows
 constexpr size_t kMaxSmem = 227 * 1024;
@@ -88,7 +86,7 @@ struct Shape {
   static constexpr int kQFull = 0, kQFree = 1, kKvFull = 2, kKvEmpty = kKvFull + kSlots,
                        kVLast = kKvEmpty + kSlots, kSFull = kVLast + 1,
                        kSFree = kSFull + NT * kBufs, kPFull = kSFree + NT,  // halves of P: + 1
-                       kODone = kPFull + 2 * NT, kItemFull = kODone + NT,
+                       kODone = kPFull + 2 * NT, kItemFull = kODone + 2 * NT,
                        kItemEmpty = kItemFull + kItemSlots, kDrain = kItemEmpty + kItemSlots,
                        kSlot = kDrain + 1;
   static_assert((kSlot + 1) * 8 <= 512, "barrier space");
@@ -116,21 +114,25 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 // Bounded wait of a whole warp, which gives up as soon as another role has failed; every lane
-// gets the same answer.
+// gets the same answer.  Short, since the roles' loops share the SM's instruction cache: the limit
+// is 2^31 clock cycles, about a second.
+__device__ __forceinline__ uint32_t clock32() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%clock;" : "=r"(t));
+  return t;
+}
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *fail) {
   if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
-  const uint64_t t0 = ptx::globaltimer_ns();
-  for (uint32_t n = 1;; ++n) {
+  const uint32_t t0 = clock32();
+  do {
     if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
-    if ((n & 63) == 0) {
-      const bool late = ptx::globaltimer_ns() - t0 > kWaitNs;
-      if (late) *fail = 1;
-      if (__any_sync(0xffffffffu, late || *fail)) return false;
-    }
-  }
+  } while (!__any_sync(0xffffffffu, *fail != 0 || clock32() - t0 > 0x7fffffffu));
+  *fail = 1;
+  return false;
 }
 
-// Pairs of 32-bit values and their operations, one instruction a pair.
+// Pairs of 32-bit values and their operations, one instruction a pair.  Volatile like all of the
+// softmax's arithmetic: exp_half says why.
 struct Pair {
   uint64_t b;
 };
@@ -144,41 +146,148 @@ __device__ __forceinline__ void unpair(Pair p, float &x, float &y) {
 }
 __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
   Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.b) : "l"(a.b), "l"(b.b), "l"(c.b));
+  asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.b) : "l"(a.b), "l"(b.b), "l"(c.b));
   return r;
 }
 __device__ __forceinline__ Pair add2(Pair a, Pair b) {
   Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.b) : "l"(a.b), "l"(b.b));
+  asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(r.b) : "l"(a.b), "l"(b.b));
   return r;
+}
+__device__ __forceinline__ float exp2_mufu(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 // Three-input maximum that keeps a NaN.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm volatile("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_v(float a, float b) {
+  float r;
+  asm volatile("max.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// r's bits + (t << 23): a value of exponent 0 times 2^t, t in the low bits of a float.
+__device__ __forceinline__ float scale_by(float r, float t) {
+  int32_t y;
+  asm volatile("mad.lo.s32 %0, %1, 8388608, %2;"
+               : "=r"(y)
+               : "r"(__float_as_int(t)), "r"(__float_as_int(r)));
+  return __int_as_float(y);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack_v(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) {
+    asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  } else {
+    asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  }
   return r;
 }
 
-// 2^x of a pair on the FMA and integer pipes, for finite x <= 127 and -inf: x = n + f with n
-// from adding 1.5 2^23, 2^f on [-1/2, 1/2] as a polynomial of degree 4 with 2^0 exactly 1 (fitted
-// for the least largest relative error, 3e-6), n added to its exponent.  Below -127: 0.
-__device__ __forceinline__ void exp2_poly(Pair x, float &e0, float &e1) {
+// P of 8 G keys: w = pairs of 16-bit 2^(v scale + sub), their sums added to `sum`.  With MAX the
+// maxima of v and of `more` (8 G values each) go to mx; more_ready waits for `more`, halfway.
+//
+// A warp issues in order, and the MUFU unit takes one of its exponentials every 8 cycles: the other
+// instructions have to stand between those for the unit not to idle.  So by groups of 4 pairs (6
+// exponentials; the next group's arguments, the sums and roundings of the one before, maxima), an
+// order that volatile operations keep.  One pair of four is done on the FMA and integer pipes:
+// 2^x with x = n + f, n from adding 1.5 2^23, 2^f on [-1/2, 1/2] as a polynomial of degree 4 with
+// 2^0 exactly 1 (fitted for the least largest relative error, 3e-6, where f16 rounds to 2^-12), n
+// added to its exponent.  Arguments below -127 give 0; those up to 127 are exact in n.
+template <typename T, int G, bool MAX, typename Ready>
+__device__ __forceinline__ void exp_half(const float *v, const float *more, uint32_t *w, Pair *sum,
+                                         Pair scale, Pair sub, float *mx, Ready more_ready) {
   constexpr float kMagic = 12582912.f;
-  float a, b;
-  unpair(x, a, b);
-  x = pair(fmaxf(a, -127.f), fmaxf(b, -127.f));
-  const Pair t = add2(x, pair(kMagic, kMagic));
-  const Pair n = add2(t, pair(-kMagic, -kMagic));
-  const Pair f = fma2(n, pair(-1.f, -1.f), x);
-  Pair r = fma2(f, pair(0x1.39f3a6p-7f, 0x1.39f3a6p-7f), pair(0x1.c9fb52p-5f, 0x1.c9fb52p-5f));
-  r = fma2(r, f, pair(0x1.ec03b6p-3f, 0x1.ec03b6p-3f));
-  r = fma2(r, f, pair(0x1.62e132p-1f, 0x1.62e132p-1f));
-  r = fma2(r, f, pair(1.f, 1.f));
-  float t0, t1, r0, r1;
-  unpair(t, t0, t1);
-  unpair(r, r0, r1);
-  e0 = __int_as_float(__float_as_int(r0) + (__float_as_int(t0) << 23));
-  e1 = __int_as_float(__float_as_int(r1) + (__float_as_int(t1) << 23));
+  const Pair magic = pair(kMagic, kMagic), unmagic = pair(-kMagic, -kMagic);
+  const Pair minus = pair(-1.f, -1.f), one = pair(1.f, 1.f);
+  const Pair c4 = pair(0x1.39f3a6p-7f, 0x1.39f3a6p-7f), c3 = pair(0x1.c9fb52p-5f, 0x1.c9fb52p-5f);
+  const Pair c2 = pair(0x1.ec03b6p-3f, 0x1.ec03b6p-3f), c1 = pair(0x1.62e132p-1f, 0x1.62e132p-1f);
+  Pair x[4];
+  float e[2][8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = fma2(pair(v[2 * i], v[2 * i + 1]), scale, sub);
+#pragma unroll
+  for (int g = 0; g <= G; ++g) {
+    float *E = e[g & 1], *D = e[(g & 1) ^ 1];  // this group's results, and the last one's
+    const bool cur = g < G, next = g + 1 < G, prev = g > 0;
+    if (MAX && g == G / 2) more_ready();
+    Pair y[4], t, n, f, r;
+    float a, b, x0, x1;
+    // maxima: those of v in the first half of the groups, those of `more` in the second
+    auto max_at = [&](int k) {
+      if (!MAX || !cur) return;
+      const int i = (g % (G / 2)) * 16 + 2 * k;
+      const float *z = g < G / 2 ? v : more;
+      mx[k & 3] = max3_nan(mx[k & 3], z[i], z[i + 1]);
+    };
+    auto arg = [&](int i) {
+      if (next)
+        y[i] = fma2(pair(v[8 * (g + 1) + 2 * i], v[8 * (g + 1) + 2 * i + 1]), scale, sub);
+    };
+    auto add = [&](int i) {
+      if (prev) sum[i & 1] = add2(sum[i & 1], pair(D[2 * i], D[2 * i + 1]));
+    };
+    auto cvt = [&](int i) {
+      if (prev) w[4 * (g - 1) + i] = pack_v<T>(D[2 * i], D[2 * i + 1]);
+    };
+    auto mufu = [&](int i) {
+      if (!cur) return;
+      unpair(x[i / 2], x0, x1);
+      E[i] = exp2_mufu(i & 1 ? x1 : x0);
+    };
+    mufu(0);
+    if (cur) {
+      unpair(x[3], a, b);
+      a = max_v(a, -127.f);
+    }
+    max_at(0);
+    arg(0);
+    add(0);
+    mufu(1);
+    if (cur) b = max_v(b, -127.f);
+    max_at(1);
+    cvt(0);
+    if (cur) t = add2(pair(a, b), magic);
+    mufu(2);
+    max_at(2);
+    arg(1);
+    add(1);
+    if (cur) n = add2(t, unmagic);
+    max_at(3);
+    cvt(1);
+    mufu(3);
+    if (cur) f = fma2(n, minus, pair(a, b));
+    max_at(4);
+    arg(2);
+    add(2);
+    if (cur) r = fma2(f, c4, c3);
+    mufu(4);
+    max_at(5);
+    cvt(2);
+    if (cur) r = fma2(r, f, c2);
+    max_at(6);
+    arg(3);
+    add(3);
+    mufu(5);
+    if (cur) r = fma2(r, f, c1);
+    max_at(7);
+    cvt(3);
+    if (cur) {
+      r = fma2(r, f, one);
+      float r0, r1, t0, t1;
+      unpair(t, t0, t1);
+      unpair(r, r0, r1);
+      E[6] = scale_by(r0, t0);
+      E[7] = scale_by(r1, t1);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = y[i];
+  }
 }
 
 struct Seq {
@@ -254,7 +363,7 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     prompt_attn_kernel(const __grid_constant__ Params P) {
   using S = Shape<DP>;
-  constexpr int NT = S::NT, KEYS = S::kKeys;
+  constexpr int NT = S::NT, KEYS = S::kKeys, H = KEYS / 2;
   const PromptAttnArgs &a = P.a;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t raw = ptx::smem_u32(smem_raw);
@@ -284,10 +393,11 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       ptx::mbar_init(bar(S::kDrain), 1);
       for (int i = 0; i < NT * S::kBufs; ++i) ptx::mbar_init(bar(S::kSFull + i), 1);
       for (int x = 0; x < NT; ++x) {
-        ptx::mbar_init(bar(S::kSFree + x), 128);
-        ptx::mbar_init(bar(S::kPFull + 2 * x), 128);
-        ptx::mbar_init(bar(S::kPFull + 2 * x + 1), 128);
-        ptx::mbar_init(bar(S::kODone + x), 1);
+        ptx::mbar_init(bar(S::kSFree + x), 4);
+        ptx::mbar_init(bar(S::kPFull + 2 * x), 4);
+        ptx::mbar_init(bar(S::kPFull + 2 * x + 1), 4);
+        ptx::mbar_init(bar(S::kODone + 2 * x), 1);
+        ptx::mbar_init(bar(S::kODone + 2 * x + 1), 1);
       }
       for (int i = 0; i < kItemSlots; ++i) {
         ptx::mbar_init(bar(S::kItemFull + i), 1);
@@ -482,6 +592,9 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
         n[x] = steps_of(keys[x]);
         n_max = max(n_max, n[x]);
       }
+      auto n_of = [&](int x) { return NT == 2 && x == 1 ? n[NT - 1] : n[0]; };
+      auto keys_of = [&](int x) { return NT == 2 && x == 1 ? keys[NT - 1] : keys[0]; };
+      auto step_of = [&](int x) { return NT == 2 && x == 1 ? step[NT - 1] : step[0]; };
       // Slot of a tile, once it is there.
       auto tile_at = [&](int p, uint32_t *at) {
         const int q = pos + p;
@@ -490,7 +603,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       };
       auto release = [&](int p) { tc::commit_warp(bar(S::kKvEmpty + (pos + p) % S::kSlots)); };
       auto issue_qk = [&](int x, int j, uint32_t at) {
-        const int g = step[x] + j;
+        const int g = step_of(x) + j;
         const uint32_t qa = tc::desc_low(base + uint32_t(x) * S::kTileQ, 16);
         const uint32_t ka = tc::desc_low(at, 16);
         const uint32_t tS = tm + S::kS + uint32_t(x * S::kBufs + g % S::kBufs) * KEYS;
@@ -503,13 +616,13 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       };
       // P.V of one half of a step's keys: the 16-key products that hold a key.
       auto issue_pv = [&](int x, int j, int half, uint32_t at) {
-        const int g = step[x] + j;
+        const int g = step_of(x) + j;
         const uint32_t va = tc::desc_low(at, S::kKvBlk);
         const uint32_t tP = tm + (S::kScores == Scores::kSeparate
                                       ? S::kP + uint32_t(x) * (KEYS / 2)
                                       : S::kS + uint32_t(x * S::kBufs + g % S::kBufs) * KEYS);
         const uint32_t tO = tm + S::kO + uint32_t(x) * DP;
-        const int live = keys[x] - j * KEYS;
+        const int live = keys_of(x) - j * KEYS;
         tc::fence_after_sync();
 #pragma unroll
         for (int c = 0; c < KEYS / 32; ++c) {
@@ -523,21 +636,21 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       if (ok && n_max > 0) {
         ok = tile_at(pos_k(0), &at_k);
         if (!ok) break;
-#pragma unroll
+#pragma unroll 1
         for (int x = 0; x < NT; ++x)
-          if (n[x] > 0) issue_qk(x, 0, at_k);
+          if (n_of(x) > 0) issue_qk(x, 0, at_k);
         release(pos_k(0));
       }
       for (int j = 0; ok && j < n_max; ++j) {
         const bool more = j + 1 < n_max;
         if (S::kAhead && more) {
           ok = tile_at(pos_k(j + 1), &at_k);
-#pragma unroll
+#pragma unroll 1
           for (int x = 0; x < NT; ++x) {
-            if (!ok || j + 1 >= n[x]) continue;
+            if (!ok || j + 1 >= n_of(x)) continue;
             // the scores of step j (two buffers: P of step j - 1) have left their columns
             if (S::kScores == Scores::kSeparate)
-              ok = wait(bar(S::kSFree + x), uint32_t((step[x] + j) & 1), fail);
+              ok = wait(bar(S::kSFree + x), uint32_t((step_of(x) + j) & 1), fail);
             if (ok) issue_qk(x, j + 1, at_k);
           }
           if (!ok) break;
@@ -545,18 +658,19 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
         }
         ok = tile_at(pos_v(j, n_max), &at_v);
         if (ok && !S::kAhead && more) ok = tile_at(pos_k(j + 1), &at_k);
-#pragma unroll
+#pragma unroll 1
         for (int x = 0; x < NT; ++x) {
-          if (!ok || j >= n[x]) continue;
-          const uint32_t ph = uint32_t((step[x] + j) & 1);
-          ok = wait(bar(S::kPFull + 2 * x), ph, fail);
+          if (!ok || j >= n_of(x)) continue;
+          const uint32_t ph = uint32_t((step_of(x) + j) & 1);
+#pragma unroll 1
+          for (int half = 0; ok && half < 2; ++half) {
+            ok = wait(bar(S::kPFull + 2 * x + half), ph, fail);
+            if (!ok) break;
+            issue_pv(x, j, half, at_v);
+          }
           if (!ok) continue;
-          issue_pv(x, j, 0, at_v);
-          ok = wait(bar(S::kPFull + 2 * x + 1), ph, fail);
-          if (!ok) continue;
-          issue_pv(x, j, 1, at_v);
-          tc::commit_warp(bar(S::kODone + x));
-          if (!S::kAhead && j + 1 < n[x]) issue_qk(x, j + 1, at_k);
+          tc::commit_warp(bar(S::kODone + 2 * x + ((step_of(x) + j) & 1)));
+          if (!S::kAhead && j + 1 < n_of(x)) issue_qk(x, j + 1, at_k);
         }
         if (!ok) break;
         release(pos_v(j, n_max));
@@ -581,6 +695,9 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     const uint32_t tO = tmem + S::kO + uint32_t(x) * DP + lanes;
     int step = 0;  // of the items before
     bool ok = true;
+    auto o_done = [&](int g) {
+      return wait(bar(S::kODone + 2 * x + (g & 1)), uint32_t((g >> 1) & 1), fail);
+    };
     for (int k = 0; ok; ++k) {
       const Item it = next_item(k);
       if (it.b < 0) break;
@@ -602,88 +719,106 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
         ok = wait(bar(S::kSFull + x * S::kBufs + buf), uint32_t((g / S::kBufs) & 1), fail);
         if (!ok) break;
         tc::fence_after_sync();
-        float v[KEYS];
+        const int k0 = j * KEYS;
+        const bool masked = k0 + KEYS - 1 > lim0;
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto row_max = [&] {
+          return max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * P.scale_log2;
+        };
+        if (j == 0) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < KEYS; c0 += 32) {
+            float u[32];
+            tc::ld32(tS + c0, u);
+            tc::wait_ld();
+            const int left = lim - k0 - c0;
 #pragma unroll
-        for (int c = 0; c < KEYS; c += 32) tc::ld32(tS + c, v + c);
-        tc::wait_ld();
+            for (int c = 0; c < 32; c += 2)
+              mx[c / 2 & 3] = max3_nan(mx[c / 2 & 3], c > left ? -INFINITY : u[c],
+                                       c + 1 > left ? -INFINITY : u[c + 1]);
+          }
+          const float top = row_max();
+          m = top == -INFINITY ? top : top + (top - top);  // NaN where it is infinite
+        }
+        // The first half's exponentials run on the maximum so far while the step's own is found;
+        // where that exceeds it (seldom) they run again.
+        float v[KEYS];
+        uint32_t w[KEYS / 4];
+        Pair sum[2];
+        float sub;
+        auto settle_half = [&](int half) {
+          tc::wait_ld();
+          if (masked) {
+#pragma unroll
+            for (int c = half * H; c < half * H + H; ++c) v[c] = k0 + c > lim ? -INFINITY : v[c];
+          }
+        };
+        for (bool again = false;;) {
+#pragma unroll
+          for (int c = 0; c < H; c += 32) tc::ld32(tS + c, v + c);
+          settle_half(0);
+#pragma unroll
+          for (int c = H; c < KEYS; c += 32) tc::ld32(tS + c, v + c);
+          sub = m == -INFINITY ? 0.f : kShift - m;  // nothing seen yet: P is 0
+          sum[0] = sum[1] = pair(0.f, 0.f);
+          exp_half<T, KEYS / 16, true>(v, v + H, w, sum, pair(P.scale_log2, P.scale_log2),
+                                       pair(sub, sub), mx, [&] { settle_half(1); });
+          const float top = row_max();
+          // a NaN or infinite maximum makes the row NaN, as its softmax is
+          const bool raise = !(top <= m + kRaise);
+          if (S::kAhead && j > 0 && !again)  // P.V of the step before has added to O and read P
+            ok = o_done(g - 1);
+          if (!ok || j == 0 || again || !__any_sync(0xffffffffu, raise)) break;
+          again = true;
+          float f = 1.f;
+          if (raise) {
+            f = ptx::fast_exp2(m - top);  // 0 before the first key
+            m = top + (top - top);
+            l *= f;
+          }
+          tc::fence_after_sync();
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 32) {
+            float o[32];
+            tc::ld32(tO + c, o);
+            tc::wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= f;
+            tc::st32(tO + c, o);
+          }
+          tc::wait_st();
+        }
+        if (!ok) break;
         if constexpr (S::kScores == Scores::kSeparate) {
           tc::fence_before_sync();
-          ptx::mbar_arrive(bar(S::kSFree + x));
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(S::kSFree + x));
         }
-        const int k0 = j * KEYS;
-        if (k0 + KEYS - 1 > lim0) {
-#pragma unroll
-          for (int c = 0; c < KEYS; ++c) v[c] = k0 + c > lim ? -INFINITY : v[c];
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < KEYS; c += 8) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = max3_nan(mx[i], v[c + 2 * i], v[c + 2 * i + 1]);
-        }
-        const float top =
-            max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * P.scale_log2;
-        // a NaN or infinite maximum makes the row NaN, as its softmax is
-        const bool raise = !(top <= m + kRaise);  // the first step's m is -inf
-        float f = 1.f;
-        if (raise) {
-          f = ptx::fast_exp2(m - top);  // 0 before the first key
-          m = top + (top - top);
-          l *= f;
-        }
-        // P.V of the step before has added to O and read P
-        if (j > 0) {
-          ok = wait(bar(S::kODone + x), uint32_t((g - 1) & 1), fail);
-          if (!ok) break;
-          if (__any_sync(0xffffffffu, raise)) {
-            tc::fence_after_sync();
-#pragma unroll 1
-            for (int c = 0; c < DP; c += 32) {
-              float o[32];
-              tc::ld32(tO + c, o);
-              tc::wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] *= f;
-              tc::st32(tO + c, o);
-            }
-            tc::wait_st();
-          }
-        }
-        const float sub = m == -INFINITY ? 0.f : m - kShift;  // nothing seen yet: P is 0
-        const Pair scale2 = pair(P.scale_log2, P.scale_log2), sub2 = pair(-sub, -sub);
-        Pair sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t w[KEYS / 4];
-#pragma unroll
-          for (int i = 0; i < KEYS / 4; ++i) {
-            const int c = half * (KEYS / 4) + i;
-            const Pair e = fma2(pair(v[2 * c], v[2 * c + 1]), scale2, sub2);
-            float e0, e1;
-            if (kPolyOf8 >> (c & 7) & 1) {
-              exp2_poly(e, e0, e1);
-            } else {
-              unpair(e, e0, e1);
-              e0 = ptx::fast_exp2(e0);
-              e1 = ptx::fast_exp2(e1);
-            }
-            sum[c & 1] = add2(sum[c & 1], pair(e0, e1));
-            w[i] = pack2<T>(e0, e1);
-          }
-          if constexpr (KEYS == 128) {
+        auto store_half = [&](int half) {
+          if constexpr (H == 64) {
             tc::st32u(tP + half * 32, w);
           } else {
             tc::st16u(tP + half * 16, w);
           }
           tc::wait_st();
           tc::fence_before_sync();
-          ptx::mbar_arrive(bar(S::kPFull + 2 * x + half));
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(S::kPFull + 2 * x + half));
+        };
+        store_half(0);
+        exp_half<T, KEYS / 16, false>(v + H, v, w, sum, pair(P.scale_log2, P.scale_log2),
+                                      pair(sub, sub), mx, [] {});
+        store_half(1);
+        // In place: S(j) came after P.V(j-1), whose phase has to be passed before P.V(j+1)'s.
+        if (!S::kAhead && j > 0) {
+          ok = o_done(g - 1);
+          if (!ok) break;
         }
         float s0, s1;
         unpair(add2(sum[0], sum[1]), s0, s1);
         l += s0 + s1;
       }
-      if (ok && n > 0) ok = wait(bar(S::kODone + x), uint32_t((step + n - 1) & 1), fail);
+      if (ok && n > 0) ok = o_done(step + n - 1);
       if (!ok) break;
       step += n;
       tc::fence_after_sync();
