@@ -393,9 +393,9 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       ptx::mbar_init(bar(S::kDrain), 1);
       for (int i = 0; i < NT * S::kBufs; ++i) ptx::mbar_init(bar(S::kSFull + i), 1);
       for (int x = 0; x < NT; ++x) {
-        ptx::mbar_init(bar(S::kSFree + x), 4);
-        ptx::mbar_init(bar(S::kPFull + 2 * x), 4);
-        ptx::mbar_init(bar(S::kPFull + 2 * x + 1), 4);
+        ptx::mbar_init(bar(S::kSFree + x), 128);
+        ptx::mbar_init(bar(S::kPFull + 2 * x), 128);
+        ptx::mbar_init(bar(S::kPFull + 2 * x + 1), 128);
         ptx::mbar_init(bar(S::kODone + 2 * x), 1);
         ptx::mbar_init(bar(S::kODone + 2 * x + 1), 1);
       }
@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
         for (int x = 0; x < NT; ++x) {
           if (!ok || j >= n_of(x)) continue;
           const uint32_t ph = uint32_t((step_of(x) + j) & 1);
-#pragma unroll 1
+#pragma unroll
           for (int half = 0; ok && half < 2; ++half) {
             ok = wait(bar(S::kPFull + 2 * x + half), ph, fail);
             if (!ok) break;
@@ -755,10 +755,8 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
         };
         for (bool again = false;;) {
 #pragma unroll
-          for (int c = 0; c < H; c += 32) tc::ld32(tS + c, v + c);
+          for (int c = 0; c < KEYS; c += 32) tc::ld32(tS + c, v + c);
           settle_half(0);
-#pragma unroll
-          for (int c = H; c < KEYS; c += 32) tc::ld32(tS + c, v + c);
           sub = m == -INFINITY ? 0.f : kShift - m;  // nothing seen yet: P is 0
           sum[0] = sum[1] = pair(0.f, 0.f);
           exp_half<T, KEYS / 16, true>(v, v + H, w, sum, pair(P.scale_log2, P.scale_log2),
@@ -791,8 +789,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
         if (!ok) break;
         if constexpr (S::kScores == Scores::kSeparate) {
           tc::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(bar(S::kSFree + x));
+          ptx::mbar_arrive(bar(S::kSFree + x));
         }
         auto store_half = [&](int half) {
           if constexpr (H == 64) {
@@ -802,8 +799,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
           }
           tc::wait_st();
           tc::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(bar(S::kPFull + 2 * x + half));
+          ptx::mbar_arrive(bar(S::kPFull + 2 * x + half));
         };
         store_half(0);
         exp_half<T, KEYS / 16, false>(v + H, v, w, sum, pair(P.scale_log2, P.scale_log2),
