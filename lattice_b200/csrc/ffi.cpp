@@ -1207,15 +1207,15 @@ static int prompt_attn_impl(kcmm_pool_t *h, const char *op, kcmm::dev::Dtype dty
   Pool *p = P(h);
   if (guarded(h, op, [&] { p->require_device(op); })) return -1;
   p->use_device();
-  alignas(64) unsigned char k_map[128], v_map[128];
+  alignas(64) unsigned char k_map[128], v_map[128], q_map[128];
   const int64_t head = int64_t(hd);
   const int rows = kcmm::dev::prompt_attn_box_rows(int(hd));
   if (!kcmm::encode_rows_tensor_map(k_map, k, num_k, int(hkv), int(hd),
-                                    k_token ? k_token : head * hkv, k_head ? k_head : head,
-                                    rows) ||
+                                    k_token ? k_token : head * hkv, k_head ? k_head : head, rows,
+                                    1) ||
       !kcmm::encode_rows_tensor_map(v_map, v, num_k, int(hkv), int(hd),
-                                    v_token ? v_token : head * hkv, v_head ? v_head : head,
-                                    rows)) {
+                                    v_token ? v_token : head * hkv, v_head ? v_head : head, rows,
+                                    1)) {
     set_error(h, std::string(op) + ": k and v cannot be described to the copy engine");
     return -1;
   }
@@ -1240,6 +1240,11 @@ static int prompt_attn_impl(kcmm_pool_t *h, const char *op, kcmm::dev::Dtype dty
   a.diag = p->diag_word();
   a.k_map = k_map;
   a.v_map = v_map;
+  // 128 rows of a group's heads as one box, where the group divides them
+  if (128 % a.group == 0 &&
+      kcmm::encode_rows_tensor_map(q_map, q, num_q, int(hq), int(hd), a.q_stride_token,
+                                   a.q_stride_head, 128 / a.group, a.group))
+    a.q_map = q_map;
   return check_launch(h, op, kcmm::dev::prompt_attn(a, S(stream)));
 }
 

@@ -71,10 +71,10 @@ bool encode_kv_tensor_map(void *out, uint64_t base, uint64_t tokens, int kv_head
 bool encode_kv_page_tensor_map(void *out, uint64_t base, uint64_t tokens, int kv_heads,
                                int head_dim);
 // {head_dim, heads, rows} view of packed 16-bit rows (strides in elements) whose box is 64 values
-// of one head of box_rows rows, with the 128-byte swizzle; head_dim a multiple of 8, zeros past
+// of box_heads heads of box_rows rows, with the 128-byte swizzle; head_dim a multiple of 8, zeros past
 // it and past the rows.
 bool encode_rows_tensor_map(void *out, uint64_t base, uint64_t rows, int heads, int head_dim,
-                            int64_t row_stride, int64_t head_stride, int box_rows);
+                            int64_t row_stride, int64_t head_stride, int box_rows, int box_heads);
 
 // ---------------------------------------------------------------------------
 // Allocator

@@ -100,10 +100,11 @@ struct Shape {
 };
 
 struct Params {
-  CUtensorMap tmk, tmv;
+  CUtensorMap tmk, tmv, tmq;
   PromptAttnArgs a;
   float scale_log2;
   uint32_t idesc_qk, idesc_pv;
+  bool q_boxes;          // tmq holds: Q's tiles are boxes
   uint32_t group_magic;  // ceil(2^32 / group), 0 for a group of 1
   int32_t *next_item;    // zero, and zero again after the call
 };
@@ -383,7 +384,8 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       ptx::prefetch_tensormap(&P.tmk);
       ptx::prefetch_tensormap(&P.tmv);
       s_fail = 0;
-      ptx::mbar_init(bar(S::kQFull), 2);
+      ptx::mbar_init(bar(S::kQFull), P.q_boxes ? 1 : 2);
+      if (P.q_boxes) ptx::prefetch_tensormap(&P.tmq);
       ptx::mbar_init(bar(S::kQFree), 1);
       for (int i = 0; i < S::kSlots; ++i) {
         ptx::mbar_init(bar(S::kKvFull + i), 1);
@@ -448,6 +450,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       return it;
     };
     bool ended = warp != kQWarp;
+    int q_begun = 0;  // items whose Q is copied as boxes
     for (int k = 0;; ++k) {
       Item it;
       if (warp == kQWarp) {
@@ -467,12 +470,29 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       }
       if (it.b < 0) break;
       if (k > 0 && !wait(bar(S::kQFree), uint32_t((k - 1) & 1), fail)) break;
-      // 16 bytes a lane; rows and values past the end are zeros
-      constexpr int kChunks = DP / 8;
       const int G = a.group;
       const int64_t row0 = int64_t(it.t) * S::kRows;
-      const int tok0 = int(row0 / G), in0 = int(row0 % G);
       const int left = int(min(int64_t(S::kRows), int64_t(it.nq) * G - row0));
+      if (P.q_boxes) {
+        // rows past the sequence are the next one's: their results are not stored
+        if (warp == kQWarp && lane == 0) {
+          const int tiles = NT == 2 && left > 128 ? 2 : 1;
+          ptx::mbar_arrive_expect_tx(bar(S::kQFull), uint32_t(tiles) * S::kTileQ);
+          for (int x = 0; x < tiles; ++x) {
+            const int tok = it.q0 + int(row0 / G) + x * (128 / G);
+#pragma unroll
+            for (int c = 0; c < S::kBlocks; ++c)
+              ptx::tma_load_3d(sb + uint32_t(x) * S::kTileQ + c * kQBlk, &P.tmq, c * 64, it.h * G,
+                               tok, bar(S::kQFull));
+          }
+        }
+        __syncwarp();
+        q_begun = k + 1;
+        continue;
+      }
+      // 16 bytes a lane; rows and values past the end are zeros
+      constexpr int kChunks = DP / 8;
+      const int tok0 = int(row0 / G), in0 = int(row0 % G);
       const uint16_t *base = static_cast<const uint16_t *>(a.q) +
                              (int64_t(it.q0) + tok0) * a.q_stride_token +
                              int64_t(it.h) * G * a.q_stride_head;
@@ -494,6 +514,8 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar(S::kQFull));
     }
+    if (*fail && q_begun)  // no copy may land after the CTA has gone
+      ptx::mbar_wait_bounded(bar(S::kQFull), uint32_t((q_begun - 1) & 1), kWaitNs);
     while (!ended) ended = take().b < 0;  // after a failure: the counter has to end at zero
   } else if (warp == kTmaWarp) {
     // ---------------- K and V ----------------
@@ -864,6 +886,8 @@ cudaError_t launch(const PromptAttnArgs &a, cudaStream_t stream) {
   std::memset(static_cast<void *>(&p), 0, sizeof(p));
   std::memcpy(&p.tmk, a.k_map, sizeof(CUtensorMap));
   std::memcpy(&p.tmv, a.v_map, sizeof(CUtensorMap));
+  p.q_boxes = a.q_map != nullptr;
+  if (p.q_boxes) std::memcpy(&p.tmq, a.q_map, sizeof(CUtensorMap));
   p.a = a;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;

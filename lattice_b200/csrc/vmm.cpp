@@ -226,10 +226,11 @@ bool encode_kv_page_tensor_map(void *out, uint64_t base, uint64_t tokens, int kv
 }
 
 bool encode_rows_tensor_map(void *out, uint64_t base, uint64_t rows, int heads, int head_dim,
-                            int64_t row_stride, int64_t head_stride, int box_rows) {
+                            int64_t row_stride, int64_t head_stride, int box_rows,
+                            int box_heads) {
   cuuint64_t dims[3] = {cuuint64_t(head_dim), cuuint64_t(heads), cuuint64_t(rows)};
   cuuint64_t strides[2] = {cuuint64_t(head_stride) * 2, cuuint64_t(row_stride) * 2};
-  cuuint32_t box[3] = {64, 1, cuuint32_t(box_rows)};
+  cuuint32_t box[3] = {64, cuuint32_t(box_heads), cuuint32_t(box_rows)};
   cuuint32_t estr[3] = {1, 1, 1};
   const DriverApi *api = nullptr;
   try {
