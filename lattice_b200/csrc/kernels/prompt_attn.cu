@@ -305,20 +305,28 @@ __device__ __forceinline__ Seq load_seq(const PromptAttnArgs &a, int b, bool *ba
   return s;
 }
 
+// A work item: the rows of one CTA, row = (token - tok0) * G + head in the group - in0.
 struct Item {
-  int b, h, t;         // sequence, kv head, row tile (from its start); b < 0: no more
-  int q0, nq, k0, nk;  // the sequence's rows
+  int rows;     // 1 to 128 NT; -1: no more items
+  int h;        // kv head
+  int tok0;     // token of the first row, within its sequence
+  int in0;      // head in the group of the first row
+  int q0;       // row of q and out that tok0 is
+  int k0, nk;   // the sequence's keys
+  int past;     // keys in front of its first query
+  int keys[2];  // keys that each tile looks at: those that its last row sees
 };
 // Work item `i` of the list (sequence, kv head, row tiles from the last, which sees the most
-// keys, to the first); b = -1 past the list's end, and *total then its length.  One warp: lane l
-// looks at sequence 32 n + l.
+// keys, to the first); rows = -1 past the list's end, and *total then its length.  One warp: lane
+// l looks at sequence 32 n + l.
 template <int ROWS>
 __device__ __forceinline__ Item find_item(const PromptAttnArgs &a, int64_t i, int64_t *total) {
   const int lane = threadIdx.x & 31, G = a.group;
   const int64_t asked = i;
   bool bad = false;
-  Item it = {-1, 0, 0, 0, 0, 0, 0};
-  for (int b0 = 0; b0 < a.batch && it.b < 0; b0 += 32) {
+  Item it;
+  it.rows = -1;
+  for (int b0 = 0; b0 < a.batch && it.rows < 0; b0 += 32) {
     const int b = b0 + lane;
     Seq s = {0, 0, 0, 0};
     if (b < a.batch) s = load_seq(a, b, &bad);
@@ -334,13 +342,23 @@ __device__ __forceinline__ Item find_item(const PromptAttnArgs &a, int64_t i, in
       const int l = __ffs(after) - 1;
       const int64_t n = __shfl_sync(0xffffffffu, nt, l);
       const int64_t rel = i - (__shfl_sync(0xffffffffu, end, l) - n * a.kv_heads);
-      it.b = b0 + l;
+      const int nq = __shfl_sync(0xffffffffu, s.nq, l);
+      const int64_t rows = int64_t(nq) * G, row0 = (n - 1 - rel % n) * ROWS;
       it.h = int(rel / n);
-      it.t = int(n - 1 - rel % n);
-      it.q0 = __shfl_sync(0xffffffffu, s.q0, l);
-      it.nq = __shfl_sync(0xffffffffu, s.nq, l);
+      it.rows = int(min(int64_t(ROWS), rows - row0));
+      it.tok0 = int(row0 / G);
+      it.in0 = int(row0 % G);
+      it.q0 = __shfl_sync(0xffffffffu, s.q0, l) + it.tok0;
       it.k0 = __shfl_sync(0xffffffffu, s.k0, l);
       it.nk = __shfl_sync(0xffffffffu, s.nk, l);
+      it.past = it.nk - nq;
+      for (int x = 0; x < 2; ++x) {
+        const int last = min(128 * (x + 1), it.rows) - 1;  // the tile's last row
+        it.keys[x] = last < 128 * x ? 0
+                     : a.causal
+                         ? max(0, min(it.nk, it.tok0 + (it.in0 + last) / G + it.past + 1))
+                         : it.nk;
+      }
     } else {
       i -= __shfl_sync(0xffffffffu, end, 31);
     }
@@ -348,16 +366,6 @@ __device__ __forceinline__ Item find_item(const PromptAttnArgs &a, int64_t i, in
   if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(a.diag, int32_t(kDiagBadLaunch));
   *total = asked - i;
   return it;
-}
-
-// Keys that tile x of an item looks at: those that its last row sees.
-template <int ROWS>
-__device__ __forceinline__ int tile_keys(const PromptAttnArgs &a, const Item &it, int x) {
-  const int64_t rows = int64_t(it.nq) * a.group, first = int64_t(it.t) * ROWS + 128 * x;
-  if (first >= rows) return 0;
-  if (!a.causal) return it.nk;
-  const int64_t last = min(first + 128, rows) - 1;
-  return int(max(int64_t(0), min(int64_t(it.nk), last / a.group + it.nk - it.nq + 1)));
 }
 
 template <typename T, int DP>
@@ -417,15 +425,20 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + S::kOffBar + S::kSlot * 8);
   volatile int *fail = &s_fail;
 
-  // The CTA's k-th item, from the warp that hands them out; b < 0 ends the role.
+  // The CTA's k-th item, from the warp that hands them out; without rows it ends the role.
   auto next_item = [&](int k) {
-    Item it = {-1, 0, 0, 0, 0, 0, 0};
+    Item it;
+    it.rows = -1;
     const int slot = k % kItemSlots;
     if (!wait(bar(S::kItemFull + slot), uint32_t((k / kItemSlots) & 1), fail)) return it;
     it = s_items[slot];
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(bar(S::kItemEmpty + slot));
     return it;
+  };
+  // Row of an item, counted from its first token's first head -> token; below 2^16.
+  auto token_of = [&](uint32_t at) {
+    return P.group_magic ? __umulhi(at, P.group_magic) : at;
   };
   auto steps_of = [&](int keys) { return (keys + KEYS - 1) / KEYS; };
   // K and V tiles pass through the slots in the order in which the products need them:
@@ -446,7 +459,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       i = __shfl_sync(0xffffffffu, i, 0);
       int64_t total = 0;
       const Item it = find_item<S::kRows>(a, i, &total);
-      if (it.b < 0 && lane == 0 && i == total + int64_t(gridDim.x) - 1) atomicExch(P.next_item, 0);
+      if (it.rows < 0 && lane == 0 && i == total + int64_t(gridDim.x) - 1) atomicExch(P.next_item, 0);
       return it;
     };
     bool ended = warp != kQWarp;
@@ -459,7 +472,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
             !wait(bar(S::kItemEmpty + slot), uint32_t((k / kItemSlots - 1) & 1), fail))
           break;
         it = take();
-        ended = it.b < 0;
+        ended = it.rows < 0;
         if (lane == 0) {
           s_items[slot] = it;
           ptx::mbar_arrive(bar(S::kItemFull + slot));
@@ -468,22 +481,19 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       } else {
         it = next_item(k);
       }
-      if (it.b < 0) break;
+      if (it.rows < 0) break;
       if (k > 0 && !wait(bar(S::kQFree), uint32_t((k - 1) & 1), fail)) break;
       const int G = a.group;
-      const int64_t row0 = int64_t(it.t) * S::kRows;
-      const int left = int(min(int64_t(S::kRows), int64_t(it.nq) * G - row0));
       if (P.q_boxes) {
         // rows past the sequence are the next one's: their results are not stored
         if (warp == kQWarp && lane == 0) {
-          const int tiles = NT == 2 && left > 128 ? 2 : 1;
+          const int tiles = NT == 2 && it.rows > 128 ? 2 : 1;
           ptx::mbar_arrive_expect_tx(bar(S::kQFull), uint32_t(tiles) * S::kTileQ);
           for (int x = 0; x < tiles; ++x) {
-            const int tok = it.q0 + int(row0 / G) + x * (128 / G);
 #pragma unroll
             for (int c = 0; c < S::kBlocks; ++c)
               ptx::tma_load_3d(sb + uint32_t(x) * S::kTileQ + c * kQBlk, &P.tmq, c * 64, it.h * G,
-                               tok, bar(S::kQFull));
+                               it.q0 + x * (128 / G), bar(S::kQFull));
           }
         }
         __syncwarp();
@@ -492,16 +502,13 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       }
       // 16 bytes a lane; rows and values past the end are zeros
       constexpr int kChunks = DP / 8;
-      const int tok0 = int(row0 / G), in0 = int(row0 % G);
-      const uint16_t *base = static_cast<const uint16_t *>(a.q) +
-                             (int64_t(it.q0) + tok0) * a.q_stride_token +
+      const uint16_t *base = static_cast<const uint16_t *>(a.q) + int64_t(it.q0) * a.q_stride_token +
                              int64_t(it.h) * G * a.q_stride_head;
 #pragma unroll 4
       for (int i = (warp - kQWarp) * 32 + lane; i < S::kRows * kChunks; i += 64) {
         const int r = i / kChunks, c = i % kChunks;
-        const bool in = r < left && c * 8 < a.head_dim;
-        const uint32_t at = uint32_t(in0 + r);
-        const uint32_t tok = P.group_magic ? __umulhi(at, P.group_magic) : at;
+        const bool in = r < it.rows && c * 8 < a.head_dim;
+        const uint32_t at = uint32_t(it.in0 + r), tok = token_of(at);
         const uint16_t *src = base + int64_t(tok) * a.q_stride_token +
                               int64_t(at - tok * G) * a.q_stride_head + c * 8;
         const uint32_t dst = sb + uint32_t(r >> 7) * S::kTileQ + uint32_t(c >> 3) * kQBlk +
@@ -516,7 +523,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     }
     if (*fail && q_begun)  // no copy may land after the CTA has gone
       ptx::mbar_wait_bounded(bar(S::kQFull), uint32_t((q_begun - 1) & 1), kWaitNs);
-    while (!ended) ended = take().b < 0;  // after a failure: the counter has to end at zero
+    while (!ended) ended = take().rows < 0;  // after a failure: the counter has to end at zero
   } else if (warp == kTmaWarp) {
     // ---------------- K and V ----------------
     int pos = 0, lasts = 0;  // tiles of the items before; sequences' last tiles among them
@@ -524,10 +531,8 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     bool ok = true, last_begun = false;
     for (int k = 0; ok; ++k) {
       const Item it = next_item(k);
-      if (it.b < 0) break;
-      int keys = tile_keys<S::kRows>(a, it, NT - 1);
-      if (NT == 2) keys = max(keys, tile_keys<S::kRows>(a, it, 0));
-      const int n = steps_of(keys);
+      if (it.rows < 0) break;
+      const int n = steps_of(max(it.keys[0], it.keys[1]));
       auto slot_of = [&](int p) { return (pos + p) % S::kSlots; };
       auto free_slot = [&](int p) {
         const int q = pos + p;
@@ -606,11 +611,11 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     bool ok = true;
     for (int k = 0; ok; ++k) {
       const Item it = next_item(k);
-      if (it.b < 0) break;
+      if (it.rows < 0) break;
       int keys[NT], n[NT], n_max = 0;
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
-        keys[x] = __shfl_sync(0xffffffffu, tile_keys<S::kRows>(a, it, x), 0);
+        keys[x] = __shfl_sync(0xffffffffu, it.keys[x], 0);
         n[x] = steps_of(keys[x]);
         n_max = max(n_max, n[x]);
       }
@@ -722,16 +727,13 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     };
     for (int k = 0; ok; ++k) {
       const Item it = next_item(k);
-      if (it.b < 0) break;
-      const int G = a.group;
-      const int64_t rows = int64_t(it.nq) * G;
-      const int64_t row = int64_t(it.t) * S::kRows + 128 * x + q4 * 32 + lane;
-      const bool row_ok = row < rows;
-      const int64_t tok = min(row, rows - 1) / G;
+      if (it.rows < 0) break;
+      const int r = 128 * x + q4 * 32 + lane;
       // last key that the row sees; rows past the end go as far as the last one
-      const int lim = a.causal ? int(tok) + it.nk - it.nq : it.nk - 1;
+      const int tok = int(token_of(uint32_t(it.in0 + min(r, it.rows - 1))));
+      const int lim = a.causal ? it.tok0 + tok + it.past : it.nk - 1;
       const int lim0 = __shfl_sync(0xffffffffu, lim, 0);
-      const int n = steps_of(tile_keys<S::kRows>(a, it, x));
+      const int n = steps_of(x == 0 ? it.keys[0] : it.keys[1]);
       float m = -INFINITY, l = 0.f;
       for (int j = 0; ok && j < n; ++j) {
         const int g = step + j, buf = g % S::kBufs;
@@ -840,30 +842,59 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       if (!ok) break;
       step += n;
       tc::fence_after_sync();
+      // The output, 8 rows of 64 bytes a store: rows g + 8 i lie with the four lanes of g, which
+      // trade 8-column groups so that each stores 16 bytes.  (A row a lane would touch 32 lines a
+      // store: 5000 cycles an item where this takes a third.)
       const bool none = n == 0 || l == 0.f;
       const float inv = none ? 0.f : 1.f / l;
-      uint16_t *dst = static_cast<uint16_t *>(a.out) +
-                      (row_ok ? (it.q0 + tok) * a.out_stride_token +
-                                    (int64_t(it.h) * G + (row - tok * G)) * a.out_stride_head
-                              : 0);
+      const int g8 = lane >> 2, c4 = lane & 3;
 #pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
-        float o[32];
-        if (n > 0) {
-          tc::ld32(tO + c, o);
-          tc::wait_ld();
+      for (int i = 0; i < 4; i += 2) {
+        float scale[2];
+        uint16_t *dst[2];
+        bool empty[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int from = g8 + 8 * (i + e), rr = 128 * x + q4 * 32 + from;
+          scale[e] = __shfl_sync(0xffffffffu, inv, from);
+          empty[e] = __shfl_sync(0xffffffffu, int(none), from);
+          const uint32_t at = uint32_t(it.in0 + rr), t = token_of(at);
+          dst[e] = rr < it.rows
+                       ? static_cast<uint16_t *>(a.out) + (int64_t(it.q0) + t) * a.out_stride_token +
+                             int64_t(it.h * a.group + int(at - t * a.group)) * a.out_stride_head
+                       : nullptr;
         }
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          float o[16];
+          if (n > 0) {
+            tc::ld16x256b_x4(tO + (uint32_t(i * 8) << 16) + c, o);
+            tc::wait_ld();
+          }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : o[e] * inv;
+          for (int e = 0; e < 2; ++e) {
+            uint32_t u[4];  // columns 8 q + 2 c4, + 1 of the row
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (!row_ok || c + q * 8 >= a.head_dim) continue;
-          uint4 u;
-          u.x = pack2<T>(o[q * 8], o[q * 8 + 1]);
-          u.y = pack2<T>(o[q * 8 + 2], o[q * 8 + 3]);
-          u.z = pack2<T>(o[q * 8 + 4], o[q * 8 + 5]);
-          u.w = pack2<T>(o[q * 8 + 6], o[q * 8 + 7]);
-          *reinterpret_cast<uint4 *>(dst + c + q * 8) = u;
+            for (int q = 0; q < 4; ++q) {
+              const float y0 = o[4 * q + 2 * e] * scale[e], y1 = o[4 * q + 2 * e + 1] * scale[e];
+              u[q] = empty[e] ? 0u : pack2<T>(y0, y1);
+            }
+            // lane c4 gets the words of columns 8 c4 ..: a 4 x 4 transposition in two exchanges
+#pragma unroll
+            for (int d = 1; d < 4; d *= 2) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                if (q & d) continue;
+                const bool up = c4 & d;
+                const uint32_t give = up ? u[q] : u[q | d];
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, give, d);
+                u[q] = up ? got : u[q];
+                u[q | d] = up ? u[q | d] : got;
+              }
+            }
+            if (dst[e] && c + 8 * c4 < a.head_dim)
+              *reinterpret_cast<uint4 *>(dst[e] + c + 8 * c4) = make_uint4(u[0], u[1], u[2], u[3]);
+          }
         }
       }
       tc::fence_before_sync();  // before the next item's first P says that O may be overwritten
