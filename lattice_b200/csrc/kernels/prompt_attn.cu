@@ -67,13 +67,15 @@ struct Shape {
   static constexpr uint32_t kKvBlk = kKeys * 128;  // 64 values of a step's keys
   static constexpr uint32_t kTileQ = kBlocks * kQBlk;
   static constexpr uint32_t kTileKv = kBlocks * kKvBlk;
-  static constexpr uint32_t kFixed = NT * kTileQ + 1024 + 512 + 256;  // alignment, barriers
+  static constexpr uint32_t kBars = 512, kMisc = 256, kPatch = 3 * DP * 2;
+  static constexpr uint32_t kFixed = NT * kTileQ + kBars + kMisc + kPatch;
   static constexpr int kFit = int((kMaxSmem - kFixed) / kTileKv);
   static constexpr int kSlots = kFit > 10 ? 10 : kFit;  // K and V tiles in flight
   static_assert(kSlots >= 4, "K and V of two steps have to fit");
   static constexpr uint32_t kOffKv = NT * kTileQ;
   static constexpr uint32_t kOffBar = kOffKv + kSlots * kTileKv;
-  static constexpr size_t kSmem = kOffBar + 512 + 1024;
+  static constexpr uint32_t kOffMisc = kOffBar + kBars, kOffPatch = kOffMisc + kMisc;
+  static constexpr size_t kSmem = kOffPatch + kPatch;
   static constexpr int kSoftmaxWarps = 4 * NT;
   static constexpr int kThreads = (kSoftmaxWarps + 4) * 32;
   // TMEM columns: scores, P where it is separate, O
@@ -84,12 +86,12 @@ struct Shape {
   static_assert(kO + NT * DP <= kTmemCols, "TMEM");
   // barriers; those of a tile by [x][buffer]
   static constexpr int kQFull = 0, kQFree = 1, kKvFull = 2, kKvEmpty = kKvFull + kSlots,
-                       kVLast = kKvEmpty + kSlots, kSFull = kVLast + 1,
+                       kRaw = kKvEmpty + kSlots, kSFull = kRaw + kSlots,
                        kSFree = kSFull + NT * kBufs, kPFull = kSFree + NT,  // halves of P: + 1
                        kODone = kPFull + 2 * NT, kItemFull = kODone + 2 * NT,
-                       kItemEmpty = kItemFull + kItemSlots, kDrain = kItemEmpty + kItemSlots,
-                       kSlot = kDrain + 1;
-  static_assert((kSlot + 1) * 8 <= 512, "barrier space");
+                       kItemEmpty = kItemFull + kItemSlots, kChecked = kItemEmpty + kItemSlots,
+                       kRead = kChecked + 2, kDrain = kRead + 2, kSlot = kDrain + 1;
+  static_assert((kSlot + 1) * 8 <= kBars, "barrier space");
   // Register split: the launch gives every thread kLaunchRegs; two softmax warpgroups then take
   // kSoftmaxRegs and the other one keeps kOtherRegs.  setmaxnreg.inc waits until the registers
   // are free in the CTA's pool, so that the split must not exceed it; the launcher checks the
@@ -388,15 +390,23 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
   using S = Shape<DP>;
   constexpr int NT = S::NT, KEYS = S::kKeys, H = KEYS / 2;
   const PromptAttnArgs &a = P.a;
-  extern __shared__ __align__(1024) unsigned char smem_raw[];
-  const uint32_t raw = ptx::smem_u32(smem_raw);
-  const uint32_t sb = (raw + 1023u) & ~1023u;
-  unsigned char *smem = smem_raw + (sb - raw);
-  __shared__ int s_fail;
-  __shared__ Item s_items[kItemSlots];
+  extern __shared__ __align__(1024) unsigned char smem[];  // the swizzle goes by 1024 bytes
+  const uint32_t sb = ptx::smem_u32(smem);
+  if (sb & 1023u) {
+    if (threadIdx.x == 0) atomicOr(a.diag, int32_t(kDiagBadLaunch));
+    return;
+  }
+  Item *s_items = reinterpret_cast<Item *>(smem + S::kOffMisc);
+  // by item parity: V held values that some rows must not see (see the checking warp)
+  volatile int *s_patched = reinterpret_cast<volatile int *>(s_items + kItemSlots);
+  int *s_fail = const_cast<int *>(s_patched) + 2;
+  static_assert(kItemSlots * sizeof(Item) + 12 <= S::kMisc, "space");
+  // first such key of each column, from the first key that a row does not see: NaN, inf, -inf
+  volatile uint16_t *s_patch = reinterpret_cast<volatile uint16_t *>(smem + S::kOffPatch);
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  constexpr int kMmaWarp = S::kSoftmaxWarps, kTmaWarp = kMmaWarp + 1, kQWarp = kMmaWarp + 2;
+  constexpr int kMmaWarp = S::kSoftmaxWarps, kTmaWarp = kMmaWarp + 1, kQWarp = kMmaWarp + 2,
+                kCheckWarp = kMmaWarp + 3;
   auto bar = [&](int i) { return sb + S::kOffBar + uint32_t(i) * 8; };
 
   ptx::grid_dependency_wait();
@@ -405,15 +415,19 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     if (lane == 0) {
       ptx::prefetch_tensormap(&P.tmk);
       ptx::prefetch_tensormap(&P.tmv);
-      s_fail = 0;
-      ptx::mbar_init(bar(S::kQFull), P.q_boxes ? 1 : 2);
+      *s_fail = 0;
+      ptx::mbar_init(bar(S::kQFull), 1);
       if (P.q_boxes) ptx::prefetch_tensormap(&P.tmq);
       ptx::mbar_init(bar(S::kQFree), 1);
       for (int i = 0; i < S::kSlots; ++i) {
         ptx::mbar_init(bar(S::kKvFull + i), 1);
         ptx::mbar_init(bar(S::kKvEmpty + i), 1);
+        ptx::mbar_init(bar(S::kRaw + i), 1);
       }
-      ptx::mbar_init(bar(S::kVLast), 1);
+      for (int i = 0; i < 2; ++i) {  // even and odd items: either side may be an item ahead
+        ptx::mbar_init(bar(S::kChecked + i), 1);
+        ptx::mbar_init(bar(S::kRead + i), S::kSoftmaxWarps);
+      }
       ptx::mbar_init(bar(S::kDrain), 1);
       for (int i = 0; i < NT * S::kBufs; ++i) ptx::mbar_init(bar(S::kSFull + i), 1);
       for (int x = 0; x < NT; ++x) {
@@ -437,7 +451,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + S::kOffBar + S::kSlot * 8);
-  volatile int *fail = &s_fail;
+  volatile int *fail = s_fail;
 
   // The CTA's k-th item, from the warp that hands them out; without rows it ends the role.
   auto next_item = [&](int k) {
@@ -460,11 +474,22 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
   auto pos_k = [&](int j) { return S::kAhead ? (j == 0 ? 0 : 2 * j - 1) : 2 * j; };
   auto pos_v = [&](int j, int n) { return S::kAhead ? min(2 * j + 2, 2 * n - 1) : 2 * j + 1; };
 
+  // Keys of an item from this one on are hidden from its first row, at least.
+  auto hidden_from = [&](const Item &it) {
+    return a.causal ? max(0, it.tok0 + it.past + 1) : it.nk;
+  };
+  // Whether V's tile j holds such keys, or rows past the sequence that a product reads: then it
+  // goes through the checking warp.
+  auto to_check = [&](const Item &it, int j) {
+    const int end = (j + 1) * KEYS;
+    return hidden_from(it) < min(end, it.nk) || (it.nk < end && it.nk % 16 != 0);
+  };
+
   if (warp >= S::kSoftmaxWarps) {
   if constexpr (S::kSplitRegs)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegs));
-  if (warp >= kQWarp) {
-    // ---------------- Q, and the first of the two warps hands out the items ----------------
+  if (warp == kQWarp) {
+    // ---------------- Q, and the items ----------------
     // The next item of the list.  Every CTA asks once past the end, and the last to do so leaves
     // the counter at zero.
     auto take = [&] {
@@ -476,31 +501,26 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       if (it.rows < 0 && lane == 0 && i == total + int64_t(gridDim.x) - 1) atomicExch(P.next_item, 0);
       return it;
     };
-    bool ended = warp != kQWarp;
+    bool ended = false;
     int q_begun = 0;  // items whose Q is copied as boxes
     for (int k = 0;; ++k) {
-      Item it;
-      if (warp == kQWarp) {
-        const int slot = k % kItemSlots;
-        if (k >= kItemSlots &&
-            !wait(bar(S::kItemEmpty + slot), uint32_t((k / kItemSlots - 1) & 1), fail))
-          break;
-        it = take();
-        ended = it.rows < 0;
-        if (lane == 0) {
-          s_items[slot] = it;
-          ptx::mbar_arrive(bar(S::kItemFull + slot));
-        }
-        __syncwarp();
-      } else {
-        it = next_item(k);
+      const int slot = k % kItemSlots;
+      if (k >= kItemSlots &&
+          !wait(bar(S::kItemEmpty + slot), uint32_t((k / kItemSlots - 1) & 1), fail))
+        break;
+      const Item it = take();
+      ended = it.rows < 0;
+      if (lane == 0) {
+        s_items[slot] = it;
+        ptx::mbar_arrive(bar(S::kItemFull + slot));
       }
+      __syncwarp();
       if (it.rows < 0) break;
       if (k > 0 && !wait(bar(S::kQFree), uint32_t((k - 1) & 1), fail)) break;
       const int G = a.group;
       if (P.q_boxes) {
         // rows past the sequence are the next one's: their results are not stored
-        if (warp == kQWarp && lane == 0) {
+        if (lane == 0) {
           const int tiles = NT == 2 && it.rows > 128 ? 2 : 1;
           ptx::mbar_arrive_expect_tx(bar(S::kQFull), uint32_t(tiles) * S::kTileQ);
           for (int x = 0; x < tiles; ++x) {
@@ -519,7 +539,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       const uint16_t *base = static_cast<const uint16_t *>(a.q) + int64_t(it.q0) * a.q_stride_token +
                              int64_t(it.h) * G * a.q_stride_head;
 #pragma unroll 4
-      for (int i = (warp - kQWarp) * 32 + lane; i < S::kRows * kChunks; i += 64) {
+      for (int i = lane; i < S::kRows * kChunks; i += 32) {
         const int r = i / kChunks, c = i % kChunks;
         const bool in = r < it.rows && c * 8 < a.head_dim;
         const uint32_t at = uint32_t(it.in0 + r), tok = token_of(at);
@@ -540,9 +560,10 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     while (!ended) ended = take().rows < 0;  // after a failure: the counter has to end at zero
   } else if (warp == kTmaWarp) {
     // ---------------- K and V ----------------
-    int pos = 0, lasts = 0;  // tiles of the items before; sequences' last tiles among them
-    int begun = 0;           // tiles whose copies have begun on their slots' barriers
-    bool ok = true, last_begun = false;
+    int pos = 0;                   // tiles of the items before
+    int begun = 0;                 // tiles whose copies have begun
+    uint32_t raw_phase = 0, raw = 0;  // by slot: parity of its next unchecked tile; it holds one
+    bool ok = true;
     for (int k = 0; ok; ++k) {
       const Item it = next_item(k);
       if (it.rows < 0) break;
@@ -553,52 +574,25 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
         return q < S::kSlots ||
                wait(bar(S::kKvEmpty + q % S::kSlots), uint32_t((q / S::kSlots - 1) & 1), fail);
       };
-      auto load = [&](const CUtensorMap *map, int p, int j, uint32_t full) {
+      auto load = [&](const CUtensorMap *map, int p, int j, bool check) {
+        if (!free_slot(p)) return false;
+        const int slot = slot_of(p);
         if (lane == 0) {
-          const uint32_t dst = sb + S::kOffKv + uint32_t(slot_of(p)) * S::kTileKv;
+          const uint32_t dst = sb + S::kOffKv + uint32_t(slot) * S::kTileKv;
+          const uint32_t full = bar((check ? S::kRaw : S::kKvFull) + slot);
           ptx::mbar_arrive_expect_tx(full, S::kTileKv);
 #pragma unroll
           for (int c = 0; c < S::kBlocks; ++c)
             ptx::tma_load_3d(dst + c * S::kKvBlk, map, c * 64, it.h, it.k0 + j * KEYS, full);
         }
         __syncwarp();
-      };
-      auto load_k = [&](int j) {
-        const int p = pos_k(j);
-        if (!free_slot(p)) return false;
-        load(&P.tmk, p, j, bar(S::kKvFull + slot_of(p)));
         begun = pos + p + 1;
+        raw = check ? raw | 1u << slot : raw & ~(1u << slot);
+        if (check) raw_phase ^= 1u << slot;
         return true;
       };
-      auto load_v = [&](int j) {
-        const int p = pos_v(j, n);
-        if (!free_slot(p)) return false;
-        // Rows past the sequence are another's.  P is 0 there, but V has to be finite: those of
-        // the last 16 keys that a product reads are cleared.
-        const int live = min(KEYS, it.nk - j * KEYS), end = min(KEYS, (live + 15) / 16 * 16);
-        if (live == end) {
-          load(&P.tmv, p, j, bar(S::kKvFull + slot_of(p)));
-          begun = pos + p + 1;
-          return true;
-        }
-        load(&P.tmv, p, j, bar(S::kVLast));
-        last_begun = true;
-        if (!wait(bar(S::kVLast), uint32_t(lasts & 1), fail)) return false;
-        last_begun = false;
-        ++lasts;
-        const uint32_t dst = sb + S::kOffKv + uint32_t(slot_of(p)) * S::kTileKv;
-        const int words = (end - live) * 8;  // 16-byte words of a block's rows
-        for (int i = lane; i < words * S::kBlocks; i += 32) {
-          const uint32_t at = dst + (i / words) * S::kKvBlk + live * 128 + (i % words) * 16;
-          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0) : "memory");
-        }
-        ptx::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar(S::kKvFull + slot_of(p)));
-        __syncwarp();
-        begun = pos + p + 1;
-        return true;
-      };
+      auto load_k = [&](int j) { return load(&P.tmk, pos_k(j), j, false); };
+      auto load_v = [&](int j) { return load(&P.tmv, pos_v(j, n), j, to_check(it, j)); };
       if (S::kAhead && n > 0) ok = load_k(0);
       for (int j = 0; ok && j < n; ++j) {
         if (S::kAhead) {
@@ -610,10 +604,105 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       pos += 2 * n;
     }
     if (*fail) {  // no copy may land after the CTA has gone
-      for (int q = max(0, begun - S::kSlots); q < begun; ++q)
-        ptx::mbar_wait_bounded(bar(S::kKvFull + q % S::kSlots), uint32_t((q / S::kSlots) & 1),
-                               kWaitNs);
-      if (last_begun) ptx::mbar_wait_bounded(bar(S::kVLast), uint32_t(lasts & 1), kWaitNs);
+      for (int q = max(0, begun - S::kSlots); q < begun; ++q) {
+        const int slot = q % S::kSlots;
+        if (raw >> slot & 1) {
+          ptx::mbar_wait_bounded(bar(S::kRaw + slot), raw_phase >> slot & 1 ^ 1, kWaitNs);
+        } else {
+          ptx::mbar_wait_bounded(bar(S::kKvFull + slot), uint32_t((q / S::kSlots) & 1), kWaitNs);
+        }
+      }
+    }
+  } else if (warp == kCheckWarp) {
+    // ---------------- V's tiles at the causal border ----------------
+    // A product multiplies a key that a row does not see by P = 0, which an infinity or NaN in V
+    // turns into NaN.  So where some row of the item does not see a key, the tile is looked
+    // through before the products read it; what is not finite there becomes 0 and is noted by
+    // column, and the rows that do see it get their infinity or NaN at the end.  Rows past the
+    // sequence that a product reads (its last 16 keys) are another's, or nothing, and are cleared.
+    constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t kOne = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+    int pos = 0;
+    uint32_t raw_phase = 0;
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      const Item it = next_item(k);
+      if (it.rows < 0) break;
+      const int n = steps_of(max(it.keys[0], it.keys[1])), hidden = hidden_from(it);
+      // the flag of the item before last has been read
+      if (k >= 2) ok = wait(bar(S::kRead + (k & 1)), uint32_t((k / 2 - 1) & 1), fail);
+      if (!ok) break;
+      if (lane == 0) s_patched[k & 1] = 0;
+      __syncwarp();
+      bool dirty = false;
+      for (int j = 0; ok && j < n; ++j) {
+        if (!to_check(it, j)) continue;
+        const int slot = (pos + pos_v(j, n)) % S::kSlots;
+        ok = wait(bar(S::kRaw + slot), raw_phase >> slot & 1, fail);
+        raw_phase ^= 1u << slot;
+        if (!ok) break;
+        const uint32_t tile = sb + S::kOffKv + uint32_t(slot) * S::kTileKv;
+        // rows that a product reads (whole 16s of the keys that the item sees), and of these the
+        // sequence's own
+        const int seen = max(it.keys[0], it.keys[1]) - j * KEYS;
+        const int end = min(KEYS, (seen + 15) / 16 * 16), live = min(end, it.nk - j * KEYS);
+        const int from = max(0, hidden - j * KEYS);
+        const auto at = [&](int row, int chunk) {  // 16 bytes of 8 columns
+          return tile + (chunk >> 3) * S::kKvBlk + row * 128 + (((chunk & 7) ^ (row & 7)) * 16);
+        };
+        // kLanes lanes a row
+        constexpr int kChunks = DP / 8, kLanes = kChunks > 16 ? 32 : kChunks;
+        const int chunk = lane % kLanes, first_row = lane / kLanes;
+        uint32_t odd = 0;
+        if (chunk < kChunks) {
+          for (int row = live + first_row; row < end; row += 32 / kLanes)
+            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at(row, chunk)), "r"(0)
+                         : "memory");
+#pragma unroll 8
+          for (int row = from + first_row; row < live; row += 32 / kLanes) {
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(at(row, chunk)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= (w[e] & kExp) + kOne;
+          }
+        }
+        __syncwarp();
+        if (__any_sync(0xffffffffu, odd & 0x80008000u)) {
+          if (!dirty) {
+            // the notes of the item before have been read
+            if (k > 0) ok = wait(bar(S::kRead + ((k - 1) & 1)), uint32_t((k - 1) / 2 & 1), fail);
+            if (!ok) break;
+            for (int i = lane; i < 3 * DP; i += 32) s_patch[i] = 0xffffu;
+            if (lane == 0) s_patched[k & 1] = 1;
+            __syncwarp();
+            dirty = true;
+          }
+          // a lane has 8 columns to itself
+          for (int row = from; row < live && lane < kChunks; ++row) {
+            uint16_t h[8];
+            uint4 *p = reinterpret_cast<uint4 *>(smem + (at(row, lane) - sb));
+            *reinterpret_cast<uint4 *>(h) = *p;
+            for (int e = 0; e < 8; ++e) {
+              if ((h[e] & (kExp & 0xffffu)) != (kExp & 0xffffu)) continue;
+              const int kind = (h[e] & 0x7fffu) > (kExp & 0xffffu) ? 0 : h[e] & 0x8000u ? 2 : 1;
+              volatile uint16_t *first = s_patch + kind * DP + lane * 8 + e;
+              if (*first == 0xffffu) *first = uint16_t(j * KEYS + row - hidden);
+              h[e] = 0;
+            }
+            *p = *reinterpret_cast<uint4 *>(h);
+          }
+        }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(S::kKvFull + slot));
+        __syncwarp();
+      }
+      if (!ok) break;
+      if (lane == 0) ptx::mbar_arrive(bar(S::kChecked + (k & 1)));
+      __syncwarp();
+      pos += 2 * n;
     }
   } else if (warp == kMmaWarp) {
     // ---------------- MMA issue ----------------
@@ -853,7 +942,9 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
         l += s0 + s1;
       }
       if (ok && n > 0) ok = o_done(step + n - 1);
+      if (ok) ok = wait(bar(S::kChecked + (k & 1)), uint32_t((k / 2) & 1), fail);
       if (!ok) break;
+      const bool patched = s_patched[k & 1];
       step += n;
       tc::fence_after_sync();
       // The output, 8 rows of 64 bytes a store: rows g + 8 i lie with the four lanes of g, which
@@ -867,12 +958,14 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
         float scale[2];
         uint16_t *dst[2];
         bool empty[2];
+        int sees[2];  // keys that the row sees of those hidden from the item's first
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int from = g8 + 8 * (i + e), rr = 128 * x + q4 * 32 + from;
           scale[e] = __shfl_sync(0xffffffffu, inv, from);
           empty[e] = __shfl_sync(0xffffffffu, int(none), from);
           const uint32_t at = uint32_t(it.in0 + rr), t = token_of(at);
+          sees[e] = it.tok0 + int(t) + it.past + 1 - hidden_from(it);
           dst[e] = rr < it.rows
                        ? static_cast<uint16_t *>(a.out) + (int64_t(it.q0) + t) * a.out_stride_token +
                              int64_t(it.h * a.group + int(at - t * a.group)) * a.out_stride_head
@@ -906,18 +999,35 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
                 u[q | d] = up ? u[q | d] : got;
               }
             }
+            if (patched && !empty[e] && sees[e] > 0) {
+              constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+              for (int q = 0; q < 8; ++q) {
+                const volatile uint16_t *first = s_patch + c + 8 * c4 + q;
+                const bool nan = first[0] < sees[e], up = first[DP] < sees[e],
+                           down = first[2 * DP] < sees[e];
+                if (!nan && !up && !down) continue;
+                const uint32_t v = nan || (up && down) ? kInf | 0x40u : up ? kInf : kInf | 0x8000u;
+                // what is not finite already (a NaN of the row, an infinity seen by all) adds up
+                const uint32_t had = u[q / 2] >> (16 * (q & 1)) & 0xffffu;
+                const bool odd = (had & kInf) == kInf && had != v;
+                u[q / 2] = (u[q / 2] & ~(0xffffu << (16 * (q & 1)))) |
+                           ((odd ? kInf | 0x40u : v) << (16 * (q & 1)));
+              }
+            }
             if (dst[e] && c + 8 * c4 < a.head_dim)
               *reinterpret_cast<uint4 *>(dst[e] + c + 8 * c4) = make_uint4(u[0], u[1], u[2], u[3]);
           }
         }
       }
       tc::fence_before_sync();  // before the next item's first P says that O may be overwritten
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(S::kRead + (k & 1)));
     }
   }
 
   tc::fence_before_sync();
   __syncthreads();
-  if (s_fail && tid == 0) atomicOr(a.diag, int32_t(kDiagWaitTimeout));
+  if (*s_fail && tid == 0) atomicOr(a.diag, int32_t(kDiagWaitTimeout));
   if (warp == kMmaWarp) {
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, kTmemCols);

@@ -167,6 +167,71 @@ def test_a_sequence_of_nan_leaves_its_neighbours(pool, dtype, d):
     check(q, k, v, out, qs, qs, True, dtype, d ** -0.5)
 
 
+@pytest.mark.parametrize("dtype,d,hq,hkv", [("bf16", 128, 8, 2), ("f16", 64, 4, 4),
+                                            ("bf16", 256, 2, 1), ("f16", 80, 7, 1)])
+@pytest.mark.parametrize("past", [0, 150])
+def test_infinities_and_nan_reach_only_the_rows_that_see_them(pool, dtype, d, hq, hkv, past):
+    """V with infinities and NaN, K with NaN, at tokens in the middle: no row in front of them
+    changes by a bit; a row that sees an infinity of V has it in that column, one that sees both
+    signs or a NaN has NaN there, one that sees a NaN of K is NaN."""
+    torch = torch_cuda()
+    nq = [300, 61, 520]
+    nk = [n + past for n in nq]
+    qs, ks = starts(nq), starts(nk)
+    q, k, v = inputs(sum(nq), sum(nk), hq, hkv, d, dtype, 12)
+    clean = call(pool, q, k, v, torch.zeros_like(q), qs, ks, True, dtype, d ** -0.5)
+    bad = v.clone()
+    marks = []  # sequence, key, kv head, column, value
+    r = np.random.default_rng(13)
+    for b in range(3):
+        for _ in range(12):
+            marks.append((b, int(r.integers(0, nk[b])), int(r.integers(hkv)), int(r.integers(d)),
+                          [np.inf, -np.inf, np.nan][r.integers(3)]))
+    marks += [(2, nk[2] - 1, 0, 3, np.nan), (2, nk[2] - 2, 0, 3, np.inf), (0, 0, 0, 1, np.inf)]
+    want, odd = clean.clone(), torch.zeros(clean.shape, dtype=torch.bool, device="cuda")
+    group = hq // hkv
+    for b, j, h, c, x in marks:
+        bad[ks[b] + j, h, c] = x
+    for b, j, h, c, _ in set(marks):
+        x = float(bad[ks[b] + j, h, c])
+        first = max(0, j - (nk[b] - nq[b]))
+        rows = want[qs[b] + first:qs[b + 1], h * group:(h + 1) * group, c]
+        before = torch.isfinite(rows)
+        rows.copy_(torch.where(before, torch.full_like(rows, x), rows + x))
+        odd[qs[b] + first:qs[b + 1], h * group:(h + 1) * group, c] = True
+    got = call(pool, q, k, bad, torch.zeros_like(q), qs, ks, True, dtype, d ** -0.5)
+    assert torch.equal(got[~odd].view(torch.int16), clean[~odd].view(torch.int16))
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf], want[inf])
+    # K: the whole row
+    for b, j in ((0, 200 + past), (1, 60 + past), (2, 300 + past)):
+        k[ks[b] + j] = float("nan")
+    got = call(pool, q, k, v, torch.zeros_like(q), qs, ks, True, dtype, d ** -0.5)
+    for b, j in ((0, 200), (1, 60), (2, 300)):
+        assert torch.equal(got[qs[b]:qs[b] + j].view(torch.int16),
+                           clean[qs[b]:qs[b] + j].view(torch.int16))
+        assert torch.isnan(got[qs[b] + j:qs[b + 1]]).all()
+    assert pool.kernel_status() == 0
+
+
+def test_infinite_rows_of_a_bidirectional_batch_stay_in_their_sequence(pool):
+    torch = torch_cuda()
+    lens = [100, 40, 77]
+    q, k, v = inputs(sum(lens), sum(lens), 4, 4, 64, "bf16", 14)
+    qs = starts(lens)
+    v[qs[1] + 3, :, 5] = float("inf")
+    out = call(pool, q, k, v, torch.zeros_like(q), qs, qs, False, "bf16", 0.125)
+    assert torch.isinf(out[qs[1]:qs[2], :, 5]).all()
+    v[qs[1] + 3, :, 5] = 0
+    out[qs[1]:qs[2], :, 5] = 0
+    keep = torch.ones(64, dtype=torch.bool)
+    keep[5] = False
+    for b in (0, 2):
+        assert torch.isfinite(out[qs[b]:qs[b + 1]]).all()
+    assert torch.isfinite(out[qs[1]:qs[2]][:, :, keep]).all()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_peaked_rising_and_falling_scores(pool, dtype):
     """Rows whose maximum keeps rising (O is rescaled every step), falls, or sits on one key."""
