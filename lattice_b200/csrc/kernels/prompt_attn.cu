@@ -109,8 +109,17 @@ struct Params {
   bool q_boxes;          // tmq holds: Q's tiles are boxes
   uint32_t group_magic;  // ceil(2^32 / group), 0 for a group of 1
   int32_t *next_item;    // zero, and zero again after the call
+  int parts;             // that an item is cut into, at most
+  int32_t *merged;       // [item][softmax warp]: parts that are done, as next_item
+  float *part_o;         // [part][row of q][head][DP]: sums of P V
+  float2 *part_ml;       // [part][row of q][head]: maximum (log2 units) and sum of P
 };
 
+template <typename T>
+__device__ __forceinline__ float widen(uint32_t bits) {
+  if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(uint16_t(bits)));
+  return __uint_as_float(bits << 16);
+}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return ptx::Mma<T>::pack(lo, hi);
@@ -317,7 +326,12 @@ struct Item {
   int k0, nk;   // the sequence's keys
   int past;     // keys in front of its first query
   int keys[2];  // keys that each tile looks at: those that its last row sees
+  int parts;    // of the item's keys, merged by the last to finish; 1: the output itself
+  int part;     // k0, nk, past and keys are from this part's first key on
+  int id;       // of the item, where it has parts
 };
+constexpr int kMinSteps = 4;  // of a part
+constexpr int kMaxParts = 16;
 // Work item `i` of the list (sequences, of every 32 the longest first; kv heads; row tiles from the
 // last, which sees the most keys, to the first: the short items fill the end); rows = -1 past the
 // list's end, and *total then its length.  One warp: lane l looks at sequence 32 n + l.  (In the
@@ -384,7 +398,40 @@ __device__ __forceinline__ Item find_item(const PromptAttnArgs &a, int64_t i, in
   return it;
 }
 
+// Cut an item down to one of its parts: whole steps of keys; false where it has fewer parts.
+template <int KEYS>
+__device__ __forceinline__ bool take_part(Item *it, int part, int parts) {
+  const int steps = (max(it->keys[0], it->keys[1]) + KEYS - 1) / KEYS;
+  it->parts = max(1, min(parts, steps / kMinSteps));
+  it->part = part;
+  if (part >= it->parts) return false;
+  const int lo = part * steps / it->parts * KEYS, n = (part + 1) * steps / it->parts * KEYS - lo;
+  it->k0 += lo;
+  it->nk -= lo;
+  it->past -= lo;
+  for (int x = 0; x < 2; ++x) it->keys[x] = max(0, min(it->keys[x] - lo, n));
+  return true;
+}
+
+// The outputs of a row that sees infinities or NaN which the products did not (`sees` keys from the
+// first hidden one).  Out of line: beside the loops its few instructions cost them 4 %.
 template <typename T, int DP>
+__device__ __noinline__ void patch_row(uint16_t *dst, const volatile uint16_t *patch, int sees,
+                                       int head_dim) {
+  __syncwarp();  // the row's other lanes have stored theirs
+  if (!dst || sees <= 0) return;
+  for (int c = 0; c < head_dim; ++c) {
+    float y = widen<T>(__ldcg(reinterpret_cast<const unsigned short *>(dst) + c));
+    if (patch[c] < sees) y = NAN;
+    if (patch[DP + c] < sees) y += INFINITY;
+    if (patch[2 * DP + c] < sees) y -= INFINITY;
+    dst[c] = uint16_t(pack2<T>(y, 0.f));
+  }
+}
+
+// PARTS: items are cut into P.parts.  A kernel of its own, since the merge's instructions beside
+// the others cost calls without parts up to a third (the SM's instruction cache).
+template <typename T, int DP, bool PARTS>
 __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     prompt_attn_kernel(const __grid_constant__ Params P) {
   using S = Shape<DP>;
@@ -492,13 +539,25 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     // ---------------- Q, and the items ----------------
     // The next item of the list.  Every CTA asks once past the end, and the last to do so leaves
     // the counter at zero.
-    auto take = [&] {
+    auto take = [&](bool *whole) {
       int32_t i = 0;
       if (lane == 0) i = atomicAdd(P.next_item, 1);
       i = __shfl_sync(0xffffffffu, i, 0);
       int64_t total = 0;
-      const Item it = find_item<S::kRows>(a, i, &total);
-      if (it.rows < 0 && lane == 0 && i == total + int64_t(gridDim.x) - 1) atomicExch(P.next_item, 0);
+      const int parts = PARTS ? P.parts : 1;
+      Item it = find_item<S::kRows>(a, i / parts, &total);
+      if (it.rows < 0 && lane == 0 && i == total * parts + int64_t(gridDim.x) - 1)
+        atomicExch(P.next_item, 0);
+      it.id = i / parts;
+      it.parts = 1;
+      *whole = !PARTS || it.rows < 0 || take_part<KEYS>(&it, i % parts, parts);
+      return it;
+    };
+    // Parts that an item does not have are passed over.
+    auto take_next = [&] {
+      Item it;
+      bool whole = false;
+      while (!whole) it = take(&whole);
       return it;
     };
     bool ended = false;
@@ -508,7 +567,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       if (k >= kItemSlots &&
           !wait(bar(S::kItemEmpty + slot), uint32_t((k / kItemSlots - 1) & 1), fail))
         break;
-      const Item it = take();
+      const Item it = take_next();
       ended = it.rows < 0;
       if (lane == 0) {
         s_items[slot] = it;
@@ -557,7 +616,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     }
     if (*fail && q_begun)  // no copy may land after the CTA has gone
       ptx::mbar_wait_bounded(bar(S::kQFull), uint32_t((q_begun - 1) & 1), kWaitNs);
-    while (!ended) ended = take().rows < 0;  // after a failure: the counter has to end at zero
+    while (!ended) ended = take_next().rows < 0;  // after a failure: the counter has to end at zero
   } else if (warp == kTmaWarp) {
     // ---------------- K and V ----------------
     int pos = 0;                   // tiles of the items before
@@ -825,6 +884,14 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     const uint32_t tO = tmem + S::kO + uint32_t(x) * DP + lanes;
     int step = 0;  // of the items before
     bool ok = true;
+    // An output whose row sees infinities or NaN that the products did not.
+    auto patch_of = [&](float y, int col, int sees) {
+      const volatile uint16_t *first = s_patch + col;
+      if (first[0] < sees) y = NAN;
+      if (first[DP] < sees) y += INFINITY;
+      if (first[2 * DP] < sees) y -= INFINITY;
+      return y;
+    };
     auto o_done = [&](int g) {
       return wait(bar(S::kODone + 2 * x + (g & 1)), uint32_t((g >> 1) & 1), fail);
     };
@@ -950,26 +1017,51 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       // The output, 8 rows of 64 bytes a store: rows g + 8 i lie with the four lanes of g, which
       // trade 8-column groups so that each stores 16 bytes.  (A row a lane would touch 32 lines a
       // store: 5000 cycles an item where this takes a third.)
-      const bool none = n == 0 || l == 0.f;
-      const float inv = none ? 0.f : 1.f / l;
-      const int g8 = lane >> 2, c4 = lane & 3;
+      // The output, 8 rows of 64 bytes a store: rows g + 8 i lie with the four lanes of g, which
+      // trade 8-column groups so that each stores 16 bytes.  (A row a lane would touch 32 lines a
+      // store: 5000 cycles an item where this takes a third.)
+      const int g8 = lane >> 2, c4 = lane & 3, warp_row = 128 * x + q4 * 32;
+      // Four words of each of a row's lanes (u[q]: columns 8 q + 2 c4, + 1) -> lane c4 stores the
+      // words of columns 8 c4 ..: a 4 x 4 transposition in two exchanges.
+      auto store_row = [&](uint16_t *dst, uint32_t *u, int c) {
+#pragma unroll
+        for (int d = 1; d < 4; d *= 2) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (q & d) continue;
+            const bool up = c4 & d;
+            const uint32_t give = up ? u[q] : u[q | d];
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, give, d);
+            u[q] = up ? got : u[q];
+            u[q | d] = up ? u[q | d] : got;
+          }
+        }
+        if (dst && c + 8 * c4 < a.head_dim)
+          *reinterpret_cast<uint4 *>(dst + c + 8 * c4) = make_uint4(u[0], u[1], u[2], u[3]);
+      };
+      auto out_of = [&](int rr) {  // null past the item
+        const uint32_t at = uint32_t(it.in0 + rr), t = token_of(at);
+        return rr < it.rows
+                   ? static_cast<uint16_t *>(a.out) + (int64_t(it.q0) + t) * a.out_stride_token +
+                         int64_t(it.h * a.group + int(at - t * a.group)) * a.out_stride_head
+                   : nullptr;
+      };
+      // keys that a row sees of those hidden from the item's first
+      auto sees_of = [&](int rr) {
+        return it.tok0 + int(token_of(uint32_t(it.in0 + rr))) + it.past + 1 - hidden_from(it);
+      };
+      const float sum = n == 0 ? 0.f : l;
+      const bool split = PARTS && it.parts > 1;
 #pragma unroll 1
-      for (int i = 0; i < 4; i += 2) {
+      for (int i = 0; !split && i < 4 && warp_row + 8 * i < it.rows; i += 2) {
         float scale[2];
         uint16_t *dst[2];
-        bool empty[2];
-        int sees[2];  // keys that the row sees of those hidden from the item's first
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int from = g8 + 8 * (i + e), rr = 128 * x + q4 * 32 + from;
-          scale[e] = __shfl_sync(0xffffffffu, inv, from);
-          empty[e] = __shfl_sync(0xffffffffu, int(none), from);
-          const uint32_t at = uint32_t(it.in0 + rr), t = token_of(at);
-          sees[e] = it.tok0 + int(t) + it.past + 1 - hidden_from(it);
-          dst[e] = rr < it.rows
-                       ? static_cast<uint16_t *>(a.out) + (int64_t(it.q0) + t) * a.out_stride_token +
-                             int64_t(it.h * a.group + int(at - t * a.group)) * a.out_stride_head
-                       : nullptr;
+          const int from = g8 + 8 * (i + e);
+          scale[e] = __shfl_sync(0xffffffffu, inv, from);  // 0: nothing seen
+          dst[e] = out_of(warp_row + from);
         }
 #pragma unroll 2
         for (int c = 0; c < DP; c += 32) {
@@ -980,42 +1072,126 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
           }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            uint32_t u[4];  // columns 8 q + 2 c4, + 1 of the row
+            uint32_t u[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               const float y0 = o[4 * q + 2 * e] * scale[e], y1 = o[4 * q + 2 * e + 1] * scale[e];
-              u[q] = empty[e] ? 0u : pack2<T>(y0, y1);
+              u[q] = scale[e] == 0.f ? 0u : pack2<T>(y0, y1);
             }
-            // lane c4 gets the words of columns 8 c4 ..: a 4 x 4 transposition in two exchanges
+            store_row(dst[e], u, c);
+          }
+        }
+      }
+      if (patched && !split)
+        patch_row<T, DP>(out_of(warp_row + lane), s_patch, sum == 0.f ? 0 : sees_of(warp_row + lane),
+                         a.head_dim);
+      if constexpr (PARTS) {
+        // row of q * heads + head of a row of the CTA
+        auto row_of = [&](int rr) {
+          const uint32_t at = uint32_t(it.in0 + rr), t = token_of(at);
+          return (int64_t(it.q0) + t) * (a.kv_heads * a.group) + it.h * a.group +
+                 int(at - t * a.group);
+        };
+        const int64_t all_rows = int64_t(a.num_q_tokens) * a.kv_heads * a.group;
+        if (split && warp_row < it.rows) {
+          // the part's sums as they are
+          if (warp_row + lane < it.rows)
+            __stcg(P.part_ml + it.part * all_rows + row_of(warp_row + lane), make_float2(m, sum));
+#pragma unroll 1
+          for (int i = 0; n > 0 && i < 4 && warp_row + 8 * i < it.rows; i += 2) {
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+              float o[16];
+              tc::ld16x256b_x4(tO + (uint32_t(i * 8) << 16) + c, o);
+              tc::wait_ld();
 #pragma unroll
-            for (int d = 1; d < 4; d *= 2) {
+              for (int e = 0; e < 2; ++e) {
+                const int rr = warp_row + g8 + 8 * (i + e);
+                if (rr >= it.rows) continue;
+                float *y = P.part_o + (it.part * all_rows + row_of(rr)) * DP + c + 2 * c4;
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                if (q & d) continue;
-                const bool up = c4 & d;
-                const uint32_t give = up ? u[q] : u[q | d];
-                const uint32_t got = __shfl_xor_sync(0xffffffffu, give, d);
-                u[q] = up ? got : u[q];
-                u[q | d] = up ? u[q | d] : got;
+                for (int q = 0; q < 4; ++q)
+                  __stcg(reinterpret_cast<float2 *>(y + 8 * q),
+                         make_float2(o[4 * q + 2 * e], o[4 * q + 2 * e + 1]));
               }
             }
-            if (patched && !empty[e] && sees[e] > 0) {
-              constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-              for (int q = 0; q < 8; ++q) {
-                const volatile uint16_t *first = s_patch + c + 8 * c4 + q;
-                const bool nan = first[0] < sees[e], up = first[DP] < sees[e],
-                           down = first[2 * DP] < sees[e];
-                if (!nan && !up && !down) continue;
-                const uint32_t v = nan || (up && down) ? kInf | 0x40u : up ? kInf : kInf | 0x8000u;
-                // what is not finite already (a NaN of the row, an infinity seen by all) adds up
-                const uint32_t had = u[q / 2] >> (16 * (q & 1)) & 0xffffu;
-                const bool odd = (had & kInf) == kInf && had != v;
-                u[q / 2] = (u[q / 2] & ~(0xffffu << (16 * (q & 1)))) |
-                           ((odd ? kInf | 0x40u : v) << (16 * (q & 1)));
+          }
+          if (patched && n > 0) {
+            __syncwarp();
+            const int rr = warp_row + lane, sees = rr < it.rows && sum != 0.f ? sees_of(rr) : 0;
+            float *y = P.part_o + (it.part * all_rows + row_of(min(rr, it.rows - 1))) * DP;
+#pragma unroll 1
+            for (int c = 0; sees > 0 && c < a.head_dim; ++c) y[c] = patch_of(__ldcg(y + c), c, sees);
+          }
+          // the last warp to have these rows' sums of a part merges all of them
+          __threadfence();
+          __syncwarp();
+          uint32_t before = 0;
+          if (lane == 0)
+            before = atomicInc(reinterpret_cast<unsigned *>(P.merged) + it.id * S::kSoftmaxWarps +
+                                   warp,
+                               unsigned(it.parts - 1));
+          before = __shfl_sync(0xffffffffu, before, 0);
+          __threadfence();
+          if (before == uint32_t(it.parts - 1)) {
+#pragma unroll 1
+            for (int i = 0; i < 4 && warp_row + 8 * i < it.rows; ++i) {
+              const int rr = warp_row + g8 + 8 * i;
+              const int64_t row = row_of(min(rr, it.rows - 1));
+              // all loads of a step before the first is used
+              float2 ml[kMaxParts];
+#pragma unroll
+              for (int p = 0; p < kMaxParts; ++p)
+                ml[p] = p < it.parts ? __ldcg(P.part_ml + p * all_rows + row)
+                                     : make_float2(-INFINITY, 0.f);
+              float top = -INFINITY, all = 0.f;
+#pragma unroll
+              for (int p = 0; p < kMaxParts; ++p)
+                if (ml[p].y != 0.f) top = max3_nan(top, ml[p].x, ml[p].x);
+#pragma unroll
+              for (int p = 0; p < kMaxParts; ++p) {
+                ml[p].x = ml[p].y == 0.f ? 0.f : ptx::fast_exp2(ml[p].x - top);
+                all += ml[p].x * ml[p].y;
+              }
+              const float inv = all == 0.f ? 0.f : 1.f / all;
+#pragma unroll 1
+              for (int c = 0; c < DP; c += 32) {
+                float2 o[4] = {};
+                const float *y = P.part_o + row * DP + c + 2 * c4;
+#pragma unroll
+                for (int p0 = 0; p0 < kMaxParts; p0 += 4) {
+                  if (p0 >= it.parts) break;
+                  float2 v[4][4];
+#pragma unroll
+                  for (int p = 0; p < 4; ++p) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                      v[p][q] = ml[p0 + p].y == 0.f
+                                    ? make_float2(0.f, 0.f)
+                                    : __ldcg(reinterpret_cast<const float2 *>(
+                                          y + (p0 + p) * all_rows * DP + 8 * q));
+                  }
+#pragma unroll
+                  for (int p = 0; p < 4; ++p) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                      o[q].x += ml[p0 + p].x * v[p][q].x;
+                      o[q].y += ml[p0 + p].x * v[p][q].y;
+                    }
+                  }
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  o[q].x *= inv;
+                  o[q].y *= inv;
+                }
+                uint32_t u[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) u[q] = pack2<T>(o[q].x, o[q].y);
+                __syncwarp();
+                store_row(out_of(rr), u, c);
               }
             }
-            if (dst[e] && c + 8 * c4 < a.head_dim)
-              *reinterpret_cast<uint4 *>(dst[e] + c + 8 * c4) = make_uint4(u[0], u[1], u[2], u[3]);
           }
         }
       }
@@ -1049,26 +1225,40 @@ cudaError_t launch(const PromptAttnArgs &a, cudaStream_t stream) {
   p.idesc_qk = tc::idesc_f16(bf16, 128, S::kKeys, false, false);
   p.idesc_pv = tc::idesc_f16(bf16, 128, DP, false, true);
   p.group_magic = a.group == 1 ? 0 : uint32_t(((uint64_t(1) << 32) + a.group - 1) / a.group);
-  auto fn = prompt_attn_kernel<T, DP>;
+  // every sequence has at most one partly filled tile a kv head
+  const int64_t items = (int64_t(a.num_q_tokens) * a.group / S::kRows + a.batch) * a.kv_heads;
+  const int sms = device_sm_count();
+  // Two SMs or more an item: its keys in parts, as many as run at once.
+  p.parts = 1;
+  if (a.num_k_tokens >= 2 * kMinSteps * S::kKeys)
+    p.parts = int(std::max<int64_t>(1, std::min<int64_t>(kMaxParts, sms / items)));
+  const int64_t rows = int64_t(a.num_q_tokens) * a.group * a.kv_heads;
+  CallScratch scratch;
+  cudaError_t e = scratch.acquire(stream, p.parts > 1 ? size_t(rows) * p.parts * (DP + 2) * 4 : 16);
+  if (e != cudaSuccess && p.parts > 1) {  // no room for the parts' sums
+    cudaGetLastError();
+    p.parts = 1;
+    e = scratch.acquire(stream, 16);
+  }
+  if (e != cudaSuccess) return e;
+  auto fn = p.parts > 1 ? prompt_attn_kernel<T, DP, true> : prompt_attn_kernel<T, DP, false>;
   if (S::kSplitRegs) {
     // with fewer registers at launch than the split was made for, setmaxnreg.inc would wait
     cudaFuncAttributes fa;
-    const cudaError_t e = cudaFuncGetAttributes(&fa, fn);
-    if (e != cudaSuccess) return e;
-    if (fa.numRegs * S::kThreads < 256 * S::kSoftmaxRegs + 128 * S::kOtherRegs)
-      return cudaErrorInvalidConfiguration;
+    e = cudaFuncGetAttributes(&fa, fn);
+    if (e == cudaSuccess &&
+        fa.numRegs * S::kThreads < 256 * S::kSoftmaxRegs + 128 * S::kOtherRegs)
+      e = cudaErrorInvalidConfiguration;
   }
-  cudaError_t e =
-      cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmem));
-  if (e != cudaSuccess) return e;
-  CallScratch scratch;
-  e = scratch.acquire(stream, 16);  // for its counters
-  if (e != cudaSuccess) return e;
-  p.next_item = scratch.counters;
-  // every sequence has at most one partly filled tile a kv head
-  const int64_t items = (int64_t(a.num_q_tokens) * a.group / S::kRows + a.batch) * a.kv_heads;
-  const int ctas = int(std::min<int64_t>(items, device_sm_count()));
-  e = launch_pdl(fn, dim3(uint32_t(ctas)), dim3(S::kThreads), S::kSmem, stream, p);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmem));
+  p.next_item = scratch.counters + kZeroedCounters / 2 - 1;
+  p.merged = scratch.counters + kZeroedCounters / 2;  // 8 an item at most
+  p.part_o = static_cast<float *>(scratch.ptr);
+  p.part_ml = reinterpret_cast<float2 *>(p.part_o + rows * p.parts * DP);
+  const int ctas = int(std::min<int64_t>(items * p.parts, sms));
+  if (e == cudaSuccess)
+    e = launch_pdl(fn, dim3(uint32_t(ctas)), dim3(S::kThreads), S::kSmem, stream, p);
   const cudaError_t r = scratch.release(stream);
   return e != cudaSuccess ? e : r;
 }

@@ -128,6 +128,36 @@ def test_pasts_and_rows_without_keys(pool, dtype, d, hq, hkv):
     assert pool.kernel_status() == 0
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,d,hq,hkv", [("bf16", 128, 8, 2), ("f16", 64, 4, 4),
+                                            ("bf16", 256, 5, 1), ("f16", 136, 4, 2)])
+def test_few_queries_over_many_keys(pool, dtype, d, hq, hkv, causal):
+    """So few items that their keys are cut into parts, whose sums are merged."""
+    torch = torch_cuda()
+    nq = [1, 7, 64, 0, 200, 1, 130]
+    nk = [5000, 3001, 2100, 900, 4096, 1023, 8191]
+    qs, ks = starts(nq), starts(nk)
+    for seed, q_amp in ((15, 1.5), (16, 8.0)):  # flat rows, and peaked ones
+        q, k, v = inputs(sum(nq), sum(nk), hq, hkv, d, dtype, seed, q_amp)
+        out = call(pool, q, k, v, torch.full_like(q, 9.0), qs, ks, causal, dtype, d ** -0.5)
+        check(q, k, v, out, qs, ks, causal, dtype, d ** -0.5)
+        again = call(pool, q, k, v, torch.full_like(q, 9.0), qs, ks, causal, dtype, d ** -0.5)
+        assert torch.equal(out.view(torch.int16), again.view(torch.int16))
+    assert pool.kernel_status() == 0
+
+
+def test_parts_that_see_nothing(pool):
+    """One sequence whose first queries see no key and the last many: of its tile's parts some
+    give some rows nothing."""
+    torch = torch_cuda()
+    nq, nk = [1500, 40], [1400, 2000]
+    qs, ks = starts(nq), starts(nk)
+    q, k, v = inputs(sum(nq), sum(nk), 1, 1, 128, "bf16", 17)
+    out = call(pool, q, k, v, torch.full_like(q, 9.0), qs, ks, True, "bf16", 0.09)
+    check(q, k, v, out, qs, ks, True, "bf16", 0.09)
+    assert (out[:100] == 0).all()
+
+
 @pytest.mark.parametrize("dtype,d", [("bf16", 128), ("f16", 64), ("bf16", 256)])
 def test_strided_views_and_rows_outside(pool, dtype, d):
     """Views of a fused projection, heads outermost for k, out inside a larger tensor; rows in
@@ -169,7 +199,7 @@ def test_a_sequence_of_nan_leaves_its_neighbours(pool, dtype, d):
 
 @pytest.mark.parametrize("dtype,d,hq,hkv", [("bf16", 128, 8, 2), ("f16", 64, 4, 4),
                                             ("bf16", 256, 2, 1), ("f16", 80, 7, 1)])
-@pytest.mark.parametrize("past", [0, 150])
+@pytest.mark.parametrize("past", [0, 150, 2600])
 def test_infinities_and_nan_reach_only_the_rows_that_see_them(pool, dtype, d, hq, hkv, past):
     """V with infinities and NaN, K with NaN, at tokens in the middle: no row in front of them
     changes by a bit; a row that sees an infinity of V has it in that column, one that sees both
@@ -278,7 +308,7 @@ def test_malformed_starts_are_reported(pool, which, bad):
 def test_other_stream_and_graph(pool):
     """On a side stream, and captured into a graph that is replayed on new inputs."""
     torch = torch_cuda()
-    lens = [200, 3, 511]
+    lens = [200, 3, 1511]  # in parts
     qs = starts(lens)
     q, k, v = inputs(sum(lens), sum(lens), 8, 2, 128, "bf16", 8)
     out = torch.zeros_like(q)
