@@ -34,6 +34,7 @@ CU_SOURCES = ["kernels/decode.cu", "kernels/decode_noalloc.cu", "kernels/append.
 CPP_SOURCES = ["pool.cpp", "vmm.cpp", "ffi.cpp", "step_tables.cpp", "policy.cpp"]
 HEADERS = ["kcmm_internal.hpp", "launch.hpp", "kernels/ptx.cuh",
            "kernels/tcgen05.cuh", "kernels/pdl.cuh", "kernels/finish.cuh", "kernels/kv4_layout.cuh",
+           "kernels/rope.cuh",
            "step_tables.hpp", "policy.hpp"]
 
 

@@ -15,23 +15,13 @@
 #include "../launch.hpp"
 #include "pdl.cuh"
 #include "ptx.cuh"
+#include "rope.cuh"
 
 namespace kcmm {
 namespace dev {
 namespace {
 
-constexpr int kThreads = 128;
-
-__device__ __forceinline__ int pair_axis(const RopeAppendArgs &a, int i) {
-  if (a.axes == 1) return 0;
-  if (a.interleaved) {
-    const int x = i % a.axes;
-    return i < a.axes * a.sections[x] ? x : 0;
-  }
-  int x = 0;
-  for (int end = a.sections[0]; i >= end && x + 1 < a.axes; end += a.sections[x]) ++x;
-  return x;
-}
+constexpr int kFewCtas = 4;  // an SM, up to which a token is cut into parts
 
 // Element offset of the token's row in its page, or -1 (nothing to write; a status as for the
 // slot write where the slot is no row of the cache).
@@ -56,122 +46,54 @@ __device__ __forceinline__ int64_t page_row(const RopeAppendArgs &a, int token) 
   return -1;
 }
 
+// The cosines of the CTA's token and its row in the pages, seen by all threads afterwards.
 template <int V>
-struct Chunk {
-  uint16_t e[V];
-};
-template <int V>
-__device__ __forceinline__ Chunk<V> load(const uint16_t *p) {
-  Chunk<V> c;
-  if constexpr (V == 8) {
-    *reinterpret_cast<uint4 *>(c.e) = *reinterpret_cast<const uint4 *>(p);
-  } else if constexpr (V == 4) {
-    *reinterpret_cast<uint2 *>(c.e) = *reinterpret_cast<const uint2 *>(p);
-  } else {
-    c.e[0] = p[0];
-  }
-  return c;
-}
-template <int V>
-__device__ __forceinline__ void store(uint16_t *p, const Chunk<V> &c) {
-  if constexpr (V == 8) {
-    *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(c.e);
-  } else if constexpr (V == 4) {
-    *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(c.e);
-  } else {
-    p[0] = c.e[0];
-  }
+__device__ __forceinline__ void token_setup(const RopeAppendArgs &a, float2 *s_cs,
+                                            int64_t *s_dst) {
+  const int token = int(blockIdx.x), tid = int(threadIdx.x);
+  if (tid < a.rotary_dim / 2) s_cs[tid] = cos_sin(a, token, tid);
+  if (tid == kRopeThreads - 1) *s_dst = a.va_k ? page_row<V>(a, token) : -1;
+  __syncthreads();
 }
 
-template <typename T>
-__device__ __forceinline__ float widen(uint16_t v) {
-  return ptx::to_f32<T>(*reinterpret_cast<T *>(&v));
-}
-template <typename T>
-__device__ __forceinline__ uint16_t narrow(float v) {
-  const T t = ptx::from_f32<T>(v);
-  return *reinterpret_cast<const uint16_t *>(&t);
-}
-template <typename T>
-__device__ __forceinline__ void turn(uint16_t &x1, uint16_t &x2, float2 cs) {
-  const float a = widen<T>(x1), b = widen<T>(x2);
-  x1 = narrow<T>(__fsub_rn(__fmul_rn(a, cs.x), __fmul_rn(b, cs.y)));
-  x2 = narrow<T>(__fadd_rn(__fmul_rn(b, cs.x), __fmul_rn(a, cs.y)));
-}
-
-// One CTA a token.  A unit of work is V pairs of a head (two chunks of V values), V values
-// past rotary_dim, or V values of the v row.
+// Many tokens, a CTA each: bound by HBM, for which the loads of many small CTAs suffice.
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const RopeAppendArgs a) {
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeAppendArgs a) {
   __shared__ float2 s_cs[128];
   __shared__ int64_t s_dst;
-  const int token = int(blockIdx.x), tid = int(threadIdx.x);
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
-  const int half = a.rotary_dim / 2;
-  if (tid < half) {
-    const int64_t at = pair_axis(a, tid) * a.positions_stride + token;
-    double s, c;
-    sincos(double(a.positions[at]) * double(a.inv_freq[tid]), &s, &c);
-    s_cs[tid] = make_float2(float(c), float(s));
+  token_setup<V>(a, s_cs, &s_dst);
+  rotate_token<T, V, true>(a, int(blockIdx.x), s_cs, s_dst);
+}
+
+// A few tokens are bound by the latency of a CTA's steps (slot -> page; positions -> cosines;
+// rows).  So CTAs (tokens, parts), a part of the token's units each, and a thread's first loads
+// under way before the cosines: 64 tokens of 32 + 8 heads of 128 take 5.4 us, with the kernel above
+// 7.0.  (Many tokens take longer so, since the loads' registers cost CTAs an SM: 16,384 take 84 us
+// against 69.)
+template <typename T, int V>
+__global__ void __launch_bounds__(kRopeThreads) rope_few_kernel(const RopeAppendArgs a) {
+  __shared__ float2 s_cs[128];
+  __shared__ int64_t s_dst;
+  const int token = int(blockIdx.x);
+  ptx::grid_dependency_wait();
+  ptx::launch_dependents();
+  const TokenUnits t = token_units<V>(a);
+  const int end = int(int64_t(t.all) * (blockIdx.y + 1) / gridDim.y);
+  int u = int(int64_t(t.all) * blockIdx.y / gridDim.y) + int(threadIdx.x);
+  Unit<V> w;
+  if (u < end) fetch<V>(a, t, token, u, &w);
+  token_setup<V>(a, s_cs, &s_dst);
+  uint16_t *page_k = nullptr, *page_v = nullptr;
+  if (s_dst >= 0) {
+    page_k = static_cast<uint16_t *>(a.va_k) + s_dst;
+    page_v = static_cast<uint16_t *>(a.va_v) + s_dst;
   }
-  if (tid == kThreads - 1) s_dst = a.va_k ? page_row<V>(a, token) : -1;
-  __syncthreads();
-  const int64_t dst = s_dst;
-  const int D = a.head_dim;
-  const int turned = half / V, per_head = turned + (D - a.rotary_dim) / V;
-  const int rows = (a.num_q_heads + a.kv_heads) * per_head;
-  const int units = rows + (dst >= 0 ? a.kv_heads * D / V : 0);
-  for (int u = tid; u < units; u += kThreads) {
-    if (u >= rows) {
-      const int e = (u - rows) * V;
-      store<V>(static_cast<uint16_t *>(a.va_v) + dst + e,
-               load<V>(static_cast<const uint16_t *>(a.v) + token * a.v_stride + e));
-      continue;
-    }
-    const int r = u / per_head, i = u % per_head;
-    const bool is_k = r >= a.num_q_heads;
-    const int h = is_k ? r - a.num_q_heads : r;
-    const uint16_t *src =
-        is_k ? static_cast<const uint16_t *>(a.k) + token * a.k_stride + int64_t(h) * D
-             : static_cast<const uint16_t *>(a.q) + token * a.q_stride_token +
-                   h * a.q_stride_head;
-    uint16_t *out = is_k ? a.k_out ? static_cast<uint16_t *>(a.k_out) + token * a.k_out_stride +
-                                         int64_t(h) * D
-                                   : nullptr
-                         : static_cast<uint16_t *>(a.q_out) + token * a.q_out_stride_token +
-                               h * a.q_out_stride_head;
-    uint16_t *page = is_k && dst >= 0
-                         ? static_cast<uint16_t *>(a.va_k) + dst + int64_t(h) * D : nullptr;
-    if (i >= turned) {  // past rotary_dim: as they are
-      const int e = a.rotary_dim + (i - turned) * V;
-      const Chunk<V> x = load<V>(src + e);
-      if (out) store<V>(out + e, x);
-      if (page) store<V>(page + e, x);
-      continue;
-    }
-    const int e0 = a.neox ? i * V : 2 * i * V, e1 = e0 + (a.neox ? half : V);
-    Chunk<V> x = load<V>(src + e0), y = load<V>(src + e1);
-    if (a.neox) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) turn<T>(x.e[j], y.e[j], s_cs[i * V + j]);
-    } else if constexpr (V == 1) {
-      turn<T>(x.e[0], y.e[0], s_cs[i]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V / 2; ++j) {
-        turn<T>(x.e[2 * j], x.e[2 * j + 1], s_cs[i * V + j]);
-        turn<T>(y.e[2 * j], y.e[2 * j + 1], s_cs[i * V + V / 2 + j]);
-      }
-    }
-    if (out) {
-      store<V>(out + e0, x);
-      store<V>(out + e1, y);
-    }
-    if (page) {
-      store<V>(page + e0, x);
-      store<V>(page + e1, y);
-    }
+  while (u < end) {
+    finish<T, V>(a, s_cs, w, page_k, page_v);
+    u += kRopeThreads;
+    if (u < end) fetch<V>(a, t, token, u, &w);
   }
 }
 
@@ -195,8 +117,15 @@ int vector_width(const RopeAppendArgs &a) {
 template <typename T>
 cudaError_t launch(const RopeAppendArgs &a, cudaStream_t stream) {
   const int v = vector_width(a);
-  auto fn = v == 8 ? rope_kernel<T, 8> : v == 4 ? rope_kernel<T, 4> : rope_kernel<T, 1>;
-  return launch_pdl(fn, dim3(uint32_t(a.num_tokens)), dim3(kThreads), 0, stream, a);
+  const int units = (a.num_q_heads + 2 * a.kv_heads) * a.head_dim / (2 * v);  // about
+  const int parts = std::max(1, std::min(kFewCtas * device_sm_count() / a.num_tokens,
+                                         (units + kRopeThreads - 1) / kRopeThreads));
+  auto many = v == 8 ? rope_kernel<T, 8> : v == 4 ? rope_kernel<T, 4> : rope_kernel<T, 1>;
+  auto few = v == 8   ? rope_few_kernel<T, 8>
+             : v == 4 ? rope_few_kernel<T, 4>
+                      : rope_few_kernel<T, 1>;
+  return launch_pdl(parts > 1 ? few : many, dim3(uint32_t(a.num_tokens), uint32_t(parts)), dim3(kRopeThreads), 0,
+                    stream, a);
 }
 
 }  // namespace
