@@ -28,6 +28,7 @@
 #include "kv4_layout.cuh"
 #include "pdl.cuh"
 #include "ptx.cuh"
+#include "rope.cuh"
 
 namespace kcmm {
 namespace dev {
@@ -171,13 +172,13 @@ struct Tile {
   int t;
 };
 template <int ROWS>
-__device__ __forceinline__ bool find_tile(const Kv4RowsArgs &a, Tile *tile) {
+__device__ __forceinline__ bool find_tile(const Kv4RowsArgs &a, int bx, int by, Tile *tile) {
   const int lane = threadIdx.x & 31;
-  const int w = int(blockIdx.y) * (kRowsThreads / 32) + int(threadIdx.x >> 5);
+  const int w = by * (kRowsThreads / 32) + int(threadIdx.x >> 5);
   if (w >= 2 * a.kv_heads) return false;
   tile->is_v = w >= a.kv_heads;
   tile->head = tile->is_v ? w - a.kv_heads : w;
-  tile->row0 = int(blockIdx.x) * ROWS;
+  tile->row0 = bx * ROWS;
   tile->rows = min(ROWS, a.num_tokens - tile->row0);
   tile->chunk = -1;
   tile->t = 0;
@@ -233,20 +234,26 @@ __device__ __forceinline__ uint32_t magnitudes(const uint32_t *w) {
 }
 __device__ __forceinline__ uint32_t larger_half(uint32_t m) { return max(m & 0xffffu, m >> 16); }
 
-template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kRowsThreads) kv4_append_kernel(const Kv4RowsArgs a) {
+// K's words of rows outside whole units, as they are in memory.
+struct PlainK {
+  // piece `piece` of row r of the tile (in_tile), which has a slot (live)
+  __device__ __forceinline__ void row(uint32_t *x, const uint16_t *src, int64_t stride, int r,
+                                      int piece, bool, bool live, bool vec) {
+    if (live) load_row<4>(x, src + r * stride + piece * 8, vec);
+  }
+};
+
+// Codes and scales of a warp's tile; `kw` gives K's words of rows outside whole units.
+template <typename T, int D, int ROWS, typename Words>
+__device__ __forceinline__ void append_tile(const Kv4RowsArgs &a, const Tile &tile, Words &kw) {
   constexpr int NG = D / kGroup, PAIR = NG % 2 == 0 ? 2 : 1;  // groups of a code vector
-  ptx::grid_dependency_wait();
-  ptx::launch_dependents();
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  Tile tile;
-  if (!find_tile<ROWS>(a, &tile)) return;
   const uint16_t *src = static_cast<const uint16_t *>(tile.is_v ? a.v : a.k) + tile.head * D;
   const int64_t stride = tile.is_v ? a.v_stride : a.k_stride;
   uint8_t *region = static_cast<uint8_t *>(tile.is_v ? a.va_v : a.va_k);
   src += int64_t(tile.row0) * stride;
 
-  if (tile.unit) {
+  if (ROWS == kUnit && tile.unit) {
     uint8_t *chunk = region + __shfl_sync(0xffffffffu, tile.chunk, 0);
     alignas(16) uint32_t scales[2 * NG];
 #pragma unroll
@@ -323,7 +330,11 @@ __global__ void __launch_bounds__(kRowsThreads) kv4_append_kernel(const Kv4RowsA
     const int t = __shfl_sync(0xffffffffu, tile.t, r);
     const bool live = i < tile.rows * P && at >= 0;
     alignas(16) uint32_t x[4] = {0u, 0u, 0u, 0u};
-    if (live) load_row<4>(x, src + r * stride + piece * 8, a.vec);
+    if (!tile.is_v) {
+      kw.row(x, src, stride, r, piece, i < tile.rows * P, live, a.vec);
+    } else if (live) {
+      load_row<4>(x, src + r * stride + piece * 8, a.vec);
+    }
     uint32_t m = magnitudes<4>(x);  // P is a multiple of 4: the lanes of a group are one row's
     m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
@@ -351,6 +362,112 @@ __global__ void __launch_bounds__(kRowsThreads) kv4_append_kernel(const Kv4RowsA
   }
 }
 
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kRowsThreads) kv4_append_kernel(const Kv4RowsArgs a) {
+  ptx::grid_dependency_wait();
+  ptx::launch_dependents();
+  Tile tile;
+  if (!find_tile<ROWS>(a, int(blockIdx.x), int(blockIdx.y), &tile)) return;
+  PlainK words;
+  append_tile<T, D, ROWS>(a, tile, words);
+}
+
+// K's words turned by their positions (kernels/rope.cu has the arithmetic), and stored to k_out.
+// A row belongs to one warp, which loads all of it before it stores any (k_out may be k).
+template <typename T, int D>
+struct TurnedK {
+  const RopeAppendArgs &r;
+  const float2 *cs;  // [row of the tile][D / 2]
+  uint16_t *out;     // the tile's first row at this head, or null
+
+  // x: dims d0 .. d0 + 7 of row t, p: the dims that NEOX pairs them with
+  __device__ __forceinline__ void turn(uint32_t *o, const uint32_t *w, const uint32_t *p, int d0,
+                                       int t) const {
+    const int half = r.rotary_dim / 2;
+    if (d0 >= r.rotary_dim) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = w[e];
+      return;
+    }
+    const bool second = r.neox && d0 >= half;
+    const float2 *c = cs + t * (D / 2) + (!r.neox ? d0 / 2 : second ? d0 - half : d0);
+    float f[8], q[8], z[8];
+    widen_all<T, 8>(w, f);
+    if (r.neox) {
+      widen_all<T, 8>(p, q);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float own = __fmul_rn(f[e], c[e].x), other = __fmul_rn(q[e], c[e].y);
+        z[e] = second ? __fadd_rn(own, other) : __fsub_rn(own, other);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float2 k = c[e / 2];
+        z[e] = __fsub_rn(__fmul_rn(f[e], k.x), __fmul_rn(f[e + 1], k.y));
+        z[e + 1] = __fadd_rn(__fmul_rn(f[e + 1], k.x), __fmul_rn(f[e], k.y));
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = ptx::Mma<T>::pack(z[2 * e], z[2 * e + 1]);
+  }
+  __device__ __forceinline__ int partner(int d0) const {
+    const int half = r.rotary_dim / 2;
+    return d0 >= r.rotary_dim ? d0 : d0 < half ? d0 + half : d0 - half;
+  }
+  // The lanes of a warp have whole rows where D / 8 divides 32; otherwise k_out is not k.
+  __device__ __forceinline__ void row(uint32_t *o, const uint16_t *src, int64_t stride, int t,
+                                      int piece, bool in_tile, bool, bool vec) {
+    alignas(16) uint32_t w[4] = {}, p[4] = {};
+    if (in_tile) {
+      load_row<4>(w, src + t * stride + piece * 8, vec);
+      if (r.neox) load_row<4>(p, src + t * stride + partner(piece * 8), vec);
+      turn(o, w, p, piece * 8, t);
+    }
+    __syncwarp();
+    if (in_tile && out) store_row<4>(out + t * r.k_out_stride + piece * 8, o, vec);
+  }
+};
+
+// Append of kFewRows tiles with the rotation on the way, and the queries' rotation, in one launch:
+// the first tiles * ky CTAs are those of the append, one a token the queries'.  With 32 + 8 heads
+// of 128 and k_out 64, 512 and 1400 tokens take 6.0, 8.3 and 14.9 us, where the rotation and the
+// append one after the other take 9.4, 11.5 and 16.9.  More tokens, whose append goes by whole
+// units, take them one after the other: as one kernel its registers leave the queries too few
+// CTAs an SM (4099 tokens 42 us against 33).
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowsThreads)
+    kv4_rope_append_kernel(const Kv4RowsArgs a, const RopeAppendArgs r, const int tiles,
+                           const int ky) {
+  __shared__ float2 s_cs[kFewRows * (D / 2)];
+  static_assert(kRowsThreads == kRopeThreads, "rotate_token's CTA");
+  ptx::grid_dependency_wait();
+  ptx::launch_dependents();
+  const int half = r.rotary_dim / 2, tid = int(threadIdx.x);
+  if (int(blockIdx.x) >= tiles * ky) {
+    const int token = int(blockIdx.x) - tiles * ky;
+    if (tid < half) s_cs[tid] = cos_sin(r, token, tid);
+    __syncthreads();
+    rotate_token<T, 8, false>(r, token, s_cs, -1);
+    return;
+  }
+  const int bx = int(blockIdx.x) / ky, by = int(blockIdx.x) % ky;
+  if (by * (kRowsThreads / 32) < a.kv_heads) {
+    for (int i = tid; i < kFewRows * half; i += kRowsThreads) {
+      const int t = i / half, p = i - t * half, token = bx * kFewRows + t;
+      if (token < a.num_tokens) s_cs[t * (D / 2) + p] = cos_sin(r, token, p);
+    }
+  }
+  __syncthreads();
+  Tile tile;
+  if (!find_tile<kFewRows>(a, bx, by, &tile)) return;
+  TurnedK<T, D> words = {r, s_cs,
+                         r.k_out ? static_cast<uint16_t *>(r.k_out) +
+                                       int64_t(tile.row0) * r.k_out_stride + tile.head * D
+                                 : nullptr};
+  append_tile<T, D, kFewRows>(a, tile, words);
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   return ptx::Mma<T>::pack(lo, hi);
@@ -363,7 +480,7 @@ __global__ void __launch_bounds__(kRowsThreads) kv4_read_kernel(const Kv4RowsArg
   ptx::launch_dependents();
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   Tile tile;
-  if (!find_tile<ROWS>(a, &tile)) return;
+  if (!find_tile<ROWS>(a, int(blockIdx.x), int(blockIdx.y), &tile)) return;
   uint16_t *dst = static_cast<uint16_t *>(tile.is_v ? a.v : a.k) + tile.head * D;
   const int64_t stride = tile.is_v ? a.v_stride : a.k_stride;
   const uint8_t *region = static_cast<const uint8_t *>(tile.is_v ? a.va_v : a.va_k);
@@ -1146,9 +1263,29 @@ Kv4RowsFn pick_rows(int D, bool append, bool tiles) {
   }
 }
 
+// Tiles of whole units, not of a few rows.
+bool unit_tiles(const Kv4RowsArgs &a) {
+  return int64_t(a.num_tokens / kUnit) * 2 * a.kv_heads >= int64_t(kTileWarps) * device_sm_count();
+}
+
+using Kv4RopeFn = void (*)(const Kv4RowsArgs, const RopeAppendArgs, const int, const int);
+template <typename T>
+Kv4RopeFn pick_rope(int D) {
+  switch (D) {
+    case 32: return kv4_rope_append_kernel<T, 32>;
+    case 64: return kv4_rope_append_kernel<T, 64>;
+    case 96: return kv4_rope_append_kernel<T, 96>;
+    case 128: return kv4_rope_append_kernel<T, 128>;
+    case 160: return kv4_rope_append_kernel<T, 160>;
+    case 192: return kv4_rope_append_kernel<T, 192>;
+    case 224: return kv4_rope_append_kernel<T, 224>;
+    case 256: return kv4_rope_append_kernel<T, 256>;
+    default: return nullptr;
+  }
+}
+
 cudaError_t launch_rows(const Kv4RowsArgs &a, bool append, cudaStream_t stream) {
-  const bool tiles =
-      int64_t(a.num_tokens / kUnit) * 2 * a.kv_heads >= int64_t(kTileWarps) * device_sm_count();
+  const bool tiles = unit_tiles(a);
   const Kv4RowsFn fn = a.dtype == Dtype::BF16
                            ? pick_rows<__nv_bfloat16>(a.head_dim, append, tiles)
                            : pick_rows<__half>(a.head_dim, append, tiles);
@@ -1162,6 +1299,16 @@ cudaError_t launch_rows(const Kv4RowsArgs &a, bool append, cudaStream_t stream) 
 
 cudaError_t kv4_append(const Kv4RowsArgs &a, cudaStream_t stream) {
   return launch_rows(a, true, stream);
+}
+
+cudaError_t kv4_rope_append(const Kv4RowsArgs &a, const RopeAppendArgs &r, cudaStream_t stream) {
+  const Kv4RopeFn fn = a.dtype == Dtype::BF16 ? pick_rope<__nv_bfloat16>(a.head_dim)
+                                              : pick_rope<__half>(a.head_dim);
+  if (!fn || unit_tiles(a)) return cudaErrorNotSupported;
+  const int per = kRowsThreads / 32;
+  const int tiles = (a.num_tokens + kFewRows - 1) / kFewRows, ky = (2 * a.kv_heads + per - 1) / per;
+  const int ctas = tiles * ky + (r.num_q_heads ? a.num_tokens : 0);
+  return launch_pdl(fn, dim3(uint32_t(ctas)), dim3(kRowsThreads), 0, stream, a, r, tiles, ky);
 }
 
 cudaError_t kv4_read(const Kv4RowsArgs &a, cudaStream_t stream) {

@@ -137,15 +137,7 @@ cudaError_t rope_append(const RopeAppendArgs &args, cudaStream_t stream) {
     return bf16 ? launch<__nv_bfloat16>(a, stream) : launch<__half>(a, stream);
   };
   if (!a.kv4) return rotate();
-  // the 4-bit cache takes the rotated rows from k_out, or from scratch
   const int64_t row = int64_t(a.kv_heads) * a.head_dim;
-  CallScratch scratch;
-  if (!a.k_out) {
-    const cudaError_t e = scratch.acquire(stream, size_t(a.num_tokens) * row * 2);
-    if (e != cudaSuccess) return e;
-    a.k_out = scratch.ptr;
-    a.k_out_stride = row;
-  }
   Kv4RowsArgs c = {};
   c.dtype = a.dtype;
   c.va_k = a.va_k;
@@ -159,11 +151,26 @@ cudaError_t rope_append(const RopeAppendArgs &args, cudaStream_t stream) {
   c.kv_heads = a.kv_heads;
   c.head_dim = a.head_dim;
   c.block_size = a.block_size;
-  c.k = a.k_out;
+  c.k = const_cast<void *>(a.k);
   c.v = const_cast<void *>(a.v);
-  c.k_stride = a.k_out_stride;
+  c.k_stride = a.k_stride;
   c.v_stride = a.v_stride;
   c.status = a.status;
+  c.vec = true;
+  if (vector_width(a) == 8 && (a.k_out != a.k || 32 % (a.head_dim / 8) == 0)) {
+    const cudaError_t e = kv4_rope_append(c, a, stream);
+    if (e != cudaErrorNotSupported) return e;
+  }
+  // Many tokens, and rows off their alignment: rotated first, to k_out or scratch, then appended.
+  CallScratch scratch;
+  if (!a.k_out) {
+    const cudaError_t e = scratch.acquire(stream, size_t(a.num_tokens) * row * 2);
+    if (e != cudaSuccess) return e;
+    a.k_out = scratch.ptr;
+    a.k_out_stride = row;
+  }
+  c.k = a.k_out;
+  c.k_stride = a.k_out_stride;
   c.vec = ((reinterpret_cast<uint64_t>(a.k_out) | reinterpret_cast<uint64_t>(a.v)) & 15) == 0 &&
           a.k_out_stride % 8 == 0 && a.v_stride % 8 == 0;
   a.va_k = a.va_v = nullptr;

@@ -177,6 +177,10 @@ struct Kv4RowsArgs {
   bool vec;         // every row starts on 16 bytes
 };
 cudaError_t kv4_append(const Kv4RowsArgs &a, cudaStream_t stream);
+// kv4_append of a.k turned by `r`, the turned rows to r.k_out where that is set, and r's queries,
+// in one launch.  Accesses of 8 values (see kernels/rope.cu); where r.k_out is a.k, D / 8 divides
+// 32.  cudaErrorNotSupported for more tokens than it is the faster way for.
+cudaError_t kv4_rope_append(const Kv4RowsArgs &a, const RopeAppendArgs &r, cudaStream_t stream);
 cudaError_t kv4_read(const Kv4RowsArgs &a, cudaStream_t stream);
 
 // Accumulated attention weights of a decode: w_out = w_in + this step's weights, rows

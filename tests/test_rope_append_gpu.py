@@ -157,6 +157,49 @@ def test_rotates_and_appends(shape, kv4):
     c.cache.close()
 
 
+# enough tokens for the append's tiles of whole units; the ends of the chunk go row by row
+LONG = [
+    # tokens, hq, hkv, d, rot, mode, layout, sections, dtype
+    (1613, 2, 8, 128, 128, "neox", "sections", [22, 21, 21], "bf16"),
+    (1613, 1, 8, 128, 64, "neox", "interleaved", [12, 10, 10], "f16"),
+    (1600, 1, 8, 64, 64, "gptj", "sections", None, "bf16"),
+    (1505, 0, 8, 96, 96, "neox", "sections", [16, 16, 16], "f16"),
+    (1505, 1, 8, 256, 256, "neox", "sections", None, "bf16"),
+    (1490, 1, 8, 160, 128, "neox", "sections", [32, 32], "bf16"),
+    (3100, 1, 4, 32, 32, "neox", "sections", None, "f16"),
+]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("shape", LONG)
+def test_long_prompts_into_four_bits(shape, in_place):
+    torch = torch_cuda()
+    tokens, hq, hkv, d, rot, mode, layout, sections, dtype = shape
+    c = Case(tokens, hq, hkv, d, rot, mode=mode, layout=layout, sections=sections, dtype=dtype,
+             kv4=True, seed=12)
+    q, k, v = c.views(c.dev)
+    q_out = q if in_place else torch.zeros(tokens, hq, d, dtype=k.dtype, device="cuda")
+    k_out = k if in_place else torch.zeros(tokens, hkv, d, dtype=k.dtype, device="cuda")
+    kw = {} if hq else dict(q_ptr=0, q_out_ptr=0)
+    c.run(q, k, v, q_out, k_out, **kw)
+    assert same(q_out.cpu(), c.want_q) and same(k_out.cpu(), c.want_k) and same(v.cpu(), c.v)
+    c.check_cache()
+    assert int(c.cache.status.item()) == 0
+    c.cache.close()
+
+
+@pytest.mark.parametrize("d", [32, 96, 160, 192, 224, 256])
+def test_in_place_of_every_row_size(d):
+    """Rows of which a warp's lanes hold whole ones, and rows that they do not."""
+    for tokens in (5, 64):
+        c = Case(tokens, 2, 3, d, d, kv4=True, seed=13)
+        q, k, v = c.views(c.dev)
+        c.run(q, k, v, q, k)
+        assert same(q.cpu(), c.want_q) and same(k.cpu(), c.want_k)
+        c.check_cache()
+        c.cache.close()
+
+
 @pytest.mark.parametrize("shape", SHAPES16)
 def test_odd_shapes(shape):
     torch = torch_cuda()
