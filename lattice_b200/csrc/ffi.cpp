@@ -1240,8 +1240,10 @@ static int prompt_attn_impl(kcmm_pool_t *h, const char *op, kcmm::dev::Dtype dty
   a.diag = p->diag_word();
   a.k_map = k_map;
   a.v_map = v_map;
-  // 128 rows of a group's heads as one box, where the group divides them
-  if (128 % a.group == 0 &&
+  // The whole tokens that 128 rows of a group's heads hold as one box, where they are seven eighths
+  // of the rows at least.  (28 query heads on 4, 8 prompts of 2048 tokens: 269 us, where plain
+  // copies of all 128 rows take 301.)
+  if (a.group <= 128 && 128 / a.group * a.group >= 112 &&
       kcmm::encode_rows_tensor_map(q_map, q, num_q, int(hq), int(hd), a.q_stride_token,
                                    a.q_stride_head, 128 / a.group, a.group))
     a.q_map = q_map;

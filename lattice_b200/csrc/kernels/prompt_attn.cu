@@ -6,17 +6,31 @@
 // with the running maximum m_i and sum of p in 32 bits over one pass of the keys.  A row that
 // sees no key gives zeros.
 //
-// A CTA owns 128 NT consecutive rows of one sequence and kv head, row = query * G + head in
-// the group of G, so that every K and V tile feeds the query heads of its group; groups need
-// not divide the rows.  Keys go by in steps of 64.  Two score buffers a tile: QK(j+2) is
-// issued as soon as P.V(j) has read the buffer, so that the softmax of a step never waits for
-// the products of the step before it, and the tensor pipe not for the softmax.
-//   warps 0 .. 4NT-1  softmax: thread = row.  S from TMEM, P back over it, output at the end
-//   then one warp     MMA issue and TMEM
-//   then one warp     K and V tiles by TMA: boxes of 64 values x 64 tokens, 128-byte swizzle,
-//                     values past head_dim and tokens past the tensor zero-filled
-// TMEM columns: score buffer (tile x, step parity) at 64 (2x + parity), P in its first 32;
-// O of tile x at 128 NT + x DP.
+// A work item is NT tiles of up to 128 rows of one sequence and kv head (row = query * G + head in
+// the group of G, so that every K and V tile feeds the query heads of its group) over the keys
+// that they see.  Persistent CTAs, one an SM, take items from a list; K and V go by in steps of 128
+// keys (64 above head_dim 128) through a ring of shared memory tiles.
+//   8 or 4 warps  softmax, thread = row of a tile: S from TMEM, P back to it, the output at the end
+//   MMA warp      issue of QK and P.V, a whole warp in uniform control flow
+//   TMA warp      K and V tiles: boxes of 64 values x a step's tokens, 128-byte swizzle, values past
+//                 head_dim and tokens past the tensor zero-filled
+//   Q warp        hands out the items and loads their Q tiles
+//   checking warp V's tiles at the causal border
+// TMEM holds O of both tiles and, in what is left, scores and P (enum Scores).  Two tiles take
+// turns: the products of one run while the other's softmax does.  The scores stand in registers
+// while P is computed, the maximum of a step is found beside its exponentials, which run on the
+// maximum so far, and the first half of P goes to its product before the second is computed.
+//
+// What bounds it, by the clock in a CTA at head_dim 128 (a step of both tiles: 3000 cycles): the
+// softmax, 2 x 128 keys for each of 128 threads, whose exponentials alone are 1536 cycles of the
+// MUFU unit with a quarter of them computed otherwise; the products are 2200 (64 an MMA, Q's rows
+// from shared memory).  At 64 the same softmax stands beside half the products.  The loops of all
+// roles have to fit the SM's instruction cache: with some thousand instructions more they missed
+// it and took up to a third longer.  Calls of few short items are bound by an item's chain of
+// steps, some 10,000 cycles.
+// Measured (device, bf16): 32,768 tokens of 8 heads on 1 of 128: 1.63 ms, 1350 TFLOP/s; 16 prompts
+// of 1 to 2048 tokens, 32 heads on 8: 224 us, 845; 16,384 tokens at head dims of 64, 256: 760 and
+// 1240 TFLOP/s.
 //
 // P is rounded to V's 16-bit type (both operands of a product have one type): an output is off
 // by at most half a unit of that type times sum(p |v|) / sum(p) more than its own rounding.
@@ -62,7 +76,6 @@ struct Shape {
   static constexpr bool kAhead = kScores != Scores::kInPlace;  // QK(j+1) comes before P.V(j)
   static constexpr int kBufs = kScores == Scores::kDouble ? 2 : 1;
   static constexpr int kKeys = DP <= 128 ? 128 : 64;  // keys of a step
-  static constexpr int kRows = 128 * NT;
   static constexpr int kBlocks = DP / 64;
   static constexpr uint32_t kKvBlk = kKeys * 128;  // 64 values of a step's keys
   static constexpr uint32_t kTileQ = kBlocks * kQBlk;
@@ -107,6 +120,7 @@ struct Params {
   float scale_log2;
   uint32_t idesc_qk, idesc_pv;
   bool q_boxes;          // tmq holds: Q's tiles are boxes
+  int tile_rows;         // of a tile's 128: whole tokens where Q's tiles are boxes
   uint32_t group_magic;  // ceil(2^32 / group), 0 for a group of 1
   int32_t *next_item;    // zero, and zero again after the call
   int parts;             // that an item is cut into, at most
@@ -318,7 +332,7 @@ __device__ __forceinline__ Seq load_seq(const PromptAttnArgs &a, int b, bool *ba
 
 // A work item: the rows of one CTA, row = (token - tok0) * G + head in the group - in0.
 struct Item {
-  int rows;     // 1 to 128 NT; -1: no more items
+  int rows;     // 1 to tile_rows NT; -1: no more items
   int h;        // kv head
   int tok0;     // token of the first row, within its sequence
   int in0;      // head in the group of the first row
@@ -336,9 +350,10 @@ constexpr int kMaxParts = 16;
 // last, which sees the most keys, to the first: the short items fill the end); rows = -1 past the
 // list's end, and *total then its length.  One warp: lane l looks at sequence 32 n + l.  (In the
 // order of the sequences 32 tokens over pasts of up to 4095 keys took 92 us, longest first 62.)
-template <int ROWS>
-__device__ __forceinline__ Item find_item(const PromptAttnArgs &a, int64_t i, int64_t *total) {
-  const int lane = threadIdx.x & 31, G = a.group;
+template <int NT>
+__device__ __forceinline__ Item find_item(const PromptAttnArgs &a, int tile_rows, int64_t i,
+                                          int64_t *total) {
+  const int lane = threadIdx.x & 31, G = a.group, ROWS = NT * tile_rows;
   const int64_t asked = i;
   bool bad = false;
   Item it;
@@ -383,8 +398,8 @@ __device__ __forceinline__ Item find_item(const PromptAttnArgs &a, int64_t i, in
       it.nk = __shfl_sync(0xffffffffu, s.nk, l);
       it.past = it.nk - nq;
       for (int x = 0; x < 2; ++x) {
-        const int last = min(128 * (x + 1), it.rows) - 1;  // the tile's last row
-        it.keys[x] = last < 128 * x ? 0
+        const int last = min(tile_rows * (x + 1), it.rows) - 1;  // the tile's last row
+        it.keys[x] = last < tile_rows * x ? 0
                      : a.causal
                          ? max(0, min(it.nk, it.tok0 + (it.in0 + last) / G + it.past + 1))
                          : it.nk;
@@ -545,7 +560,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       i = __shfl_sync(0xffffffffu, i, 0);
       int64_t total = 0;
       const int parts = PARTS ? P.parts : 1;
-      Item it = find_item<S::kRows>(a, i / parts, &total);
+      Item it = find_item<NT>(a, P.tile_rows, i / parts, &total);
       if (it.rows < 0 && lane == 0 && i == total * parts + int64_t(gridDim.x) - 1)
         atomicExch(P.next_item, 0);
       it.id = i / parts;
@@ -580,8 +595,9 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       if (P.q_boxes) {
         // rows past the sequence are the next one's: their results are not stored
         if (lane == 0) {
-          const int tiles = NT == 2 && it.rows > 128 ? 2 : 1;
-          ptx::mbar_arrive_expect_tx(bar(S::kQFull), uint32_t(tiles) * S::kTileQ);
+          const int tiles = NT == 2 && it.rows > P.tile_rows ? 2 : 1;
+          ptx::mbar_arrive_expect_tx(bar(S::kQFull),
+                                     uint32_t(tiles * S::kBlocks * P.tile_rows) * 128);
           for (int x = 0; x < tiles; ++x) {
 #pragma unroll
             for (int c = 0; c < S::kBlocks; ++c)
@@ -598,7 +614,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       const uint16_t *base = static_cast<const uint16_t *>(a.q) + int64_t(it.q0) * a.q_stride_token +
                              int64_t(it.h) * G * a.q_stride_head;
 #pragma unroll 4
-      for (int i = lane; i < S::kRows * kChunks; i += 32) {
+      for (int i = lane; i < NT * 128 * kChunks; i += 32) {
         const int r = i / kChunks, c = i % kChunks;
         const bool in = r < it.rows && c * 8 < a.head_dim;
         const uint32_t at = uint32_t(it.in0 + r), tok = token_of(at);
@@ -898,9 +914,10 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     for (int k = 0; ok; ++k) {
       const Item it = next_item(k);
       if (it.rows < 0) break;
-      const int r = 128 * x + q4 * 32 + lane;
+      const int warp_row = P.tile_rows * x + q4 * 32, r = warp_row + lane;
+      const int rows_end = min(it.rows, P.tile_rows * (x + 1));  // of the tile
       // last key that the row sees; rows past the end go as far as the last one
-      const int tok = int(token_of(uint32_t(it.in0 + min(r, it.rows - 1))));
+      const int tok = int(token_of(uint32_t(it.in0 + min(r, rows_end - 1))));
       const int lim = a.causal ? it.tok0 + tok + it.past : it.nk - 1;
       const int lim0 = __shfl_sync(0xffffffffu, lim, 0);
       const int n = steps_of(x == 0 ? it.keys[0] : it.keys[1]);
@@ -956,8 +973,9 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
           exp_half<T, KEYS / 16, true>(v, v + H, w, sum, pair(P.scale_log2, P.scale_log2),
                                        pair(sub, sub), mx, [&] { settle_half(1); });
           const float top = row_max();
-          // a NaN or infinite maximum makes the row NaN, as its softmax is
-          const bool raise = !(top <= m + kRaise);
+          // a NaN or infinite maximum makes the row NaN, as its softmax is (what stands in rows
+          // past the tile's is nobody's)
+          const bool raise = !(top <= m + kRaise) && r < rows_end;
           if (S::kAhead && j > 0 && !again)  // P.V of the step before has added to O and read P
             ok = o_done(g - 1);
           if (!ok || j == 0 || again || !__any_sync(0xffffffffu, raise)) break;
@@ -1020,7 +1038,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       // The output, 8 rows of 64 bytes a store: rows g + 8 i lie with the four lanes of g, which
       // trade 8-column groups so that each stores 16 bytes.  (A row a lane would touch 32 lines a
       // store: 5000 cycles an item where this takes a third.)
-      const int g8 = lane >> 2, c4 = lane & 3, warp_row = 128 * x + q4 * 32;
+      const int g8 = lane >> 2, c4 = lane & 3;
       // Four words of each of a row's lanes (u[q]: columns 8 q + 2 c4, + 1) -> lane c4 stores the
       // words of columns 8 c4 ..: a 4 x 4 transposition in two exchanges.
       auto store_row = [&](uint16_t *dst, uint32_t *u, int c) {
@@ -1039,9 +1057,9 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
         if (dst && c + 8 * c4 < a.head_dim)
           *reinterpret_cast<uint4 *>(dst + c + 8 * c4) = make_uint4(u[0], u[1], u[2], u[3]);
       };
-      auto out_of = [&](int rr) {  // null past the item
+      auto out_of = [&](int rr) {  // null past the tile
         const uint32_t at = uint32_t(it.in0 + rr), t = token_of(at);
-        return rr < it.rows
+        return rr < rows_end
                    ? static_cast<uint16_t *>(a.out) + (int64_t(it.q0) + t) * a.out_stride_token +
                          int64_t(it.h * a.group + int(at - t * a.group)) * a.out_stride_head
                    : nullptr;
@@ -1053,7 +1071,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       const float sum = n == 0 ? 0.f : l;
       const bool split = PARTS && it.parts > 1;
 #pragma unroll 1
-      for (int i = 0; !split && i < 4 && warp_row + 8 * i < it.rows; i += 2) {
+      for (int i = 0; !split && i < 4 && warp_row + 8 * i < rows_end; i += 2) {
         float scale[2];
         uint16_t *dst[2];
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -1093,12 +1111,12 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
                  int(at - t * a.group);
         };
         const int64_t all_rows = int64_t(a.num_q_tokens) * a.kv_heads * a.group;
-        if (split && warp_row < it.rows) {
+        if (split && warp_row < rows_end) {
           // the part's sums as they are
-          if (warp_row + lane < it.rows)
+          if (warp_row + lane < rows_end)
             __stcg(P.part_ml + it.part * all_rows + row_of(warp_row + lane), make_float2(m, sum));
 #pragma unroll 1
-          for (int i = 0; n > 0 && i < 4 && warp_row + 8 * i < it.rows; i += 2) {
+          for (int i = 0; n > 0 && i < 4 && warp_row + 8 * i < rows_end; i += 2) {
 #pragma unroll 1
             for (int c = 0; c < DP; c += 32) {
               float o[16];
@@ -1107,7 +1125,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const int rr = warp_row + g8 + 8 * (i + e);
-                if (rr >= it.rows) continue;
+                if (rr >= rows_end) continue;
                 float *y = P.part_o + (it.part * all_rows + row_of(rr)) * DP + c + 2 * c4;
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
@@ -1118,8 +1136,8 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
           }
           if (patched && n > 0) {
             __syncwarp();
-            const int rr = warp_row + lane, sees = rr < it.rows && sum != 0.f ? sees_of(rr) : 0;
-            float *y = P.part_o + (it.part * all_rows + row_of(min(rr, it.rows - 1))) * DP;
+            const int rr = warp_row + lane, sees = rr < rows_end && sum != 0.f ? sees_of(rr) : 0;
+            float *y = P.part_o + (it.part * all_rows + row_of(min(rr, rows_end - 1))) * DP;
 #pragma unroll 1
             for (int c = 0; sees > 0 && c < a.head_dim; ++c) y[c] = patch_of(__ldcg(y + c), c, sees);
           }
@@ -1135,9 +1153,9 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
           __threadfence();
           if (before == uint32_t(it.parts - 1)) {
 #pragma unroll 1
-            for (int i = 0; i < 4 && warp_row + 8 * i < it.rows; ++i) {
+            for (int i = 0; i < 4 && warp_row + 8 * i < rows_end; ++i) {
               const int rr = warp_row + g8 + 8 * i;
-              const int64_t row = row_of(min(rr, it.rows - 1));
+              const int64_t row = row_of(min(rr, rows_end - 1));
               // all loads of a step before the first is used
               float2 ml[kMaxParts];
 #pragma unroll
@@ -1219,6 +1237,7 @@ cudaError_t launch(const PromptAttnArgs &a, cudaStream_t stream) {
   std::memcpy(&p.tmv, a.v_map, sizeof(CUtensorMap));
   p.q_boxes = a.q_map != nullptr;
   if (p.q_boxes) std::memcpy(&p.tmq, a.q_map, sizeof(CUtensorMap));
+  p.tile_rows = p.q_boxes ? 128 / a.group * a.group : 128;
   p.a = a;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -1226,7 +1245,8 @@ cudaError_t launch(const PromptAttnArgs &a, cudaStream_t stream) {
   p.idesc_pv = tc::idesc_f16(bf16, 128, DP, false, true);
   p.group_magic = a.group == 1 ? 0 : uint32_t(((uint64_t(1) << 32) + a.group - 1) / a.group);
   // every sequence has at most one partly filled tile a kv head
-  const int64_t items = (int64_t(a.num_q_tokens) * a.group / S::kRows + a.batch) * a.kv_heads;
+  const int64_t items =
+      (int64_t(a.num_q_tokens) * a.group / (S::NT * p.tile_rows) + a.batch) * a.kv_heads;
   const int sms = device_sm_count();
   // Two SMs or more an item: its keys in parts, as many as run at once.
   p.parts = 1;

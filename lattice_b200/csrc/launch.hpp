@@ -114,8 +114,7 @@ struct PromptAttnArgs {
   // {64, 1, prompt_attn_box_rows(head_dim)}
   const void *k_map;
   const void *v_map;
-  // Q's, {head_dim, heads, num_q_tokens} with box {64, group, 128 / group}; null where the group
-  // does not divide 128
+  // Q's, {head_dim, heads, num_q_tokens} with box {64, group, 128 / group}, or null
   const void *q_map;
 };
 int prompt_attn_box_rows(int head_dim);

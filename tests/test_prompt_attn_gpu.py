@@ -111,6 +111,21 @@ def test_ragged(pool, dtype, d, hq, hkv, causal):
     assert pool.kernel_status() == 0
 
 
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("group", [3, 5, 9, 12, 20, 28, 65, 96, 128, 130, 200])
+def test_groups_that_do_not_divide_a_tile(pool, group, d):
+    """Tiles of whole tokens with idle rows, groups whose tokens lie across tiles, and groups of
+    more than a tile."""
+    torch = torch_cuda()
+    lens, past = [1, 43, 90, 0, 131], [0, 70, 3, 5, 200]
+    total = [n + p for n, p in zip(lens, past)]
+    q, k, v = inputs(sum(lens), sum(total), group, 1, d, "bf16", 18)
+    qs, ks = starts(lens), starts(total)
+    out = call(pool, q, k, v, torch.full_like(q, 9.0), qs, ks, True, "bf16", d ** -0.5)
+    check(q, k, v, out, qs, ks, True, "bf16", d ** -0.5)
+    assert pool.kernel_status() == 0
+
+
 @pytest.mark.parametrize("dtype,d,hq,hkv", [("bf16", 128, 8, 2), ("f16", 64, 4, 4),
                                             ("bf16", 256, 5, 1), ("f16", 192, 4, 2)])
 def test_pasts_and_rows_without_keys(pool, dtype, d, hq, hkv):
