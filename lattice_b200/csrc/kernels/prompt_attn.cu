@@ -319,14 +319,11 @@ __device__ __forceinline__ void exp_half(const float *v, const float *more, uint
 struct Seq {
   int q0, nq, k0, nk;
 };
-// A sequence's rows, empty (and *bad set) where its starts are no ascending part of the rows.
+// A sequence's rows; *bad set where its starts are no ascending part of the rows.
 __device__ __forceinline__ Seq load_seq(const PromptAttnArgs &a, int b, bool *bad) {
   const int q0 = a.q_start[b], q1 = a.q_start[b + 1], k0 = a.k_start[b], k1 = a.k_start[b + 1];
   Seq s = {q0, q1 - q0, k0, k1 - k0};
-  if (q0 < 0 || q1 < q0 || q1 > a.num_q_tokens || k0 < 0 || k1 < k0 || k1 > a.num_k_tokens) {
-    s.nq = 0;
-    *bad = true;
-  }
+  *bad = q0 < 0 || q1 < q0 || q1 > a.num_q_tokens || k0 < 0 || k1 < k0 || k1 > a.num_k_tokens;
   return s;
 }
 
@@ -349,7 +346,9 @@ constexpr int kMaxParts = 16;
 // Work item `i` of the list (sequences, of every 32 the longest first; kv heads; row tiles from the
 // last, which sees the most keys, to the first: the short items fill the end); rows = -1 past the
 // list's end, and *total then its length.  One warp: lane l looks at sequence 32 n + l.  (In the
-// order of the sequences 32 tokens over pasts of up to 4095 keys took 92 us, longest first 62.)
+// order of the sequences 32 tokens over pasts of up to 4095 keys took 92 us, longest first 73.)
+// The list ends at the first 32 that hold malformed starts: it is then no longer than the launch
+// assumed, whatever the starts are.
 template <int NT>
 __device__ __forceinline__ Item find_item(const PromptAttnArgs &a, int tile_rows, int64_t i,
                                           int64_t *total) {
@@ -362,6 +361,7 @@ __device__ __forceinline__ Item find_item(const PromptAttnArgs &a, int tile_rows
     const int b = b0 + lane;
     Seq s = {0, 0, 0, 0};
     if (b < a.batch) s = load_seq(a, b, &bad);
+    if (__any_sync(0xffffffffu, bad)) break;
     if (a.batch > 1) {  // lane l takes the l-th longest of the 32
       int rank = 0, from = 0;
       for (int o = 0; o < 32; ++o) {
@@ -1040,11 +1040,8 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       step += n;
       tc::fence_after_sync();
       // The output, 8 rows of 64 bytes a store: rows g + 8 i lie with the four lanes of g, which
-      // trade 8-column groups so that each stores 16 bytes.  (A row a lane would touch 32 lines a
-      // store: 5000 cycles an item where this takes a third.)
-      // The output, 8 rows of 64 bytes a store: rows g + 8 i lie with the four lanes of g, which
-      // trade 8-column groups so that each stores 16 bytes.  (A row a lane would touch 32 lines a
-      // store: 5000 cycles an item where this takes a third.)
+      // trade 8-column groups so that each stores 16 bytes.  (A row a lane touches 32 lines a store:
+      // 5000 cycles an item where this takes 3400.)
       const int g8 = lane >> 2, c4 = lane & 3;
       // Four words of each of a row's lanes (u[q]: columns 8 q + 2 c4, + 1) -> lane c4 stores the
       // words of columns 8 c4 ..: a 4 x 4 transposition in two exchanges.

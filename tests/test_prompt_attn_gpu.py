@@ -320,6 +320,20 @@ def test_malformed_starts_are_reported(pool, which, bad):
     assert (big[:32] == 9.0).all() and (big[32 + 90:] == 9.0).all()
 
 
+def test_malformed_starts_among_many(pool):
+    """Sequences in front of the 32 that hold a malformed one are answered; those behind it, which
+    overlap it here, are not."""
+    torch = torch_cuda()
+    lens = np.full(32, 5)
+    q, k, v = inputs(260, 260, 4, 2, 64, "bf16", 8)
+    good = starts(lens)
+    bad = np.concatenate([good, np.tile([260, 160], 24)])
+    out = call(pool, q, k, v, torch.full_like(q, 9.0), bad, bad, True, "bf16", 0.125)
+    assert pool.kernel_status() == 4
+    check(q[:160], k[:160], v[:160], out[:160], good, good, True, "bf16", 0.125)
+    assert (out[160:] == 9.0).all()
+
+
 def test_other_stream_and_graph(pool):
     """On a side stream, and captured into a graph that is replayed on new inputs."""
     torch = torch_cuda()
