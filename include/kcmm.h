@@ -712,8 +712,8 @@ int kcmm_rope_append_f16_on_stream(
  * zeros where a query sees no key (or only scores of -inf).  Any number of queries from 0, any
  * nk from 0; rows of out that belong to no sequence are left as they were.  Strides are in
  * elements (0 = dense); pointers and strides are multiples of 16 bytes, head_dim is a multiple
- * of 8 up to 256, num_q_heads a multiple of kv_heads.  Keys and values past a sequence may hold
- * anything.  Starts that do not ascend, or pass num_q_tokens or num_k_tokens, set bit 2 of
+ * of 8 up to 256, num_q_heads a multiple of kv_heads, scale positive.  Keys and values past a
+ * sequence may hold anything.  Starts that do not ascend, or pass num_q_tokens or num_k_tokens, set bit 2 of
  * kcmm_get_kernel_status; what the call writes within out is then undefined.  No page of the
  * pool is touched: it gives the device and the status word.
  */

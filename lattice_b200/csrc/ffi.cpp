@@ -5,6 +5,7 @@
 // sm_100a and linked in; the reference's lazy NVRTC step
 // (ref src/kcmm/ffi.rs:103-171) has no counterpart, so the precompile entry
 // points only force the CUDA module to load.
+#include <cmath>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -1166,9 +1167,15 @@ static int prompt_attn_impl(kcmm_pool_t *h, const char *op, kcmm::dev::Dtype dty
     set_error(h, std::string(op) + ": shape arguments must be positive");
     return -1;
   }
-  if (batch > 0xFFFF || hq > 0xFFFF || num_q > 0x7fffffffu || num_k > 0x7fffffffu ||
-      (uint64_t(num_q) * hq / 128 + uint64_t(batch) * hkv) > 0x7fffffffull) {
+  // tokens: the end of a step of keys behind them fits 31 bits; the work items do as well
+  if (batch > 0xFFFF || hq > 0xFFFF || num_q > 0x7fffff00u || num_k > 0x7fffff00u ||
+      (uint64_t(num_q) * hq / 64 + uint64_t(batch) * hkv) > 0x7fffff00ull) {
     set_error(h, std::string(op) + ": shape argument exceeds its limit");
+    return -1;
+  }
+  // a masked score is -inf * scale
+  if (!(scale > 0.f) || !std::isfinite(scale * 1.4426950408889634f)) {
+    set_error(h, std::string(op) + ": scale must be positive and finite");
     return -1;
   }
   if (hq % hkv != 0) {

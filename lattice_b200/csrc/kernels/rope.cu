@@ -124,8 +124,8 @@ cudaError_t launch(const RopeAppendArgs &a, cudaStream_t stream) {
   auto few = v == 8   ? rope_few_kernel<T, 8>
              : v == 4 ? rope_few_kernel<T, 4>
                       : rope_few_kernel<T, 1>;
-  return launch_pdl(parts > 1 ? few : many, dim3(uint32_t(a.num_tokens), uint32_t(parts)), dim3(kRopeThreads), 0,
-                    stream, a);
+  return launch_pdl(parts > 1 ? few : many, dim3(uint32_t(a.num_tokens), uint32_t(parts)),
+                    dim3(kRopeThreads), 0, stream, a);
 }
 
 }  // namespace

@@ -100,6 +100,9 @@ def test_rope_append_into_a_four_bit_pool(host_pool_factory):
     (dict(q_stride_head=68), "multiples of 8"), (dict(v_stride_token=2 ** 39), "multiples of 8"),
     (dict(query_ptr=8), "16-byte"), (dict(value_ptr=18), "16-byte"), (dict(out_ptr=24), "16-byte"),
     (dict(q_start_ptr=18), "4-byte"), (dict(k_start_ptr=17), "4-byte"),
+    *((dict(scale=x), "scale must be positive")
+      for x in (0.0, -0.125, float("nan"), float("inf"), 3e38)),
+    (dict(num_k_tokens=2 ** 31 - 1), "limit"),
     ({}, "no device memory")])
 def test_prompt_attn_checks(host_pool_factory, kw, msg, dtype):
     pool = make_pool(host_pool_factory)
