@@ -28,9 +28,10 @@
 // roles have to fit the SM's instruction cache: with some thousand instructions more they missed
 // it and took up to a third longer.  Calls of few short items are bound by an item's chain of
 // steps, some 10,000 cycles.
-// Measured (device, bf16): 32,768 tokens of 8 heads on 1 of 128: 1.63 ms, 1350 TFLOP/s; 16 prompts
-// of 1 to 2048 tokens, 32 heads on 8: 224 us, 845; 16,384 tokens at head dims of 64, 256: 760 and
-// 1240 TFLOP/s.
+// Measured (device, one call after the other): 32,768 tokens of 8 heads on 1 of 128: 1.63 ms, 1350
+// TFLOP/s; 16 prompts of 1 to 2048 tokens, 32 heads on 8: 229 us, 830; 4 chunks of 300 to 512 behind
+// 2000 to 8192: 129 us, 1110; 8 prompts of 511 to 4001, 16 heads on 4 of 64: 174 us, 600; 3 of 1025
+// to 5000, 8 on 2 of 256: 136 us, 1060; 32 single tokens over up to 4095: 55 us, 4.9 TB/s.
 //
 // P is rounded to V's 16-bit type (both operands of a product have one type): an output is off
 // by at most half a unit of that type times sum(p |v|) / sum(p) more than its own rounding.
@@ -584,7 +585,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
           !wait(bar(S::kItemEmpty + slot), uint32_t((k / kItemSlots - 1) & 1), fail))
         break;
       // Taken when all copies of the last one have begun, not before: an SM with a long item leaves
-      // the next to others (64 single tokens over pasts of 64 to 4096 keys: 77 us -> 61).  Up to four
+      // the next to others (32 single tokens over pasts of up to 4095 keys: 77 us -> 61).  Up to four
       // steps earlier measures the same.
       if (k > 0 && !wait(bar(S::kWant), uint32_t((k - 1) & 1), fail)) break;
       const Item it = take_next();
