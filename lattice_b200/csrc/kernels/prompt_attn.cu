@@ -29,9 +29,9 @@
 // it and took up to a third longer.  Calls of few short items are bound by an item's chain of
 // steps, some 10,000 cycles.
 // Measured (device, one call after the other): 32,768 tokens of 8 heads on 1 of 128: 1.63 ms, 1350
-// TFLOP/s; 16 prompts of 1 to 2048 tokens, 32 heads on 8: 229 us, 830; 4 chunks of 300 to 512 behind
-// 2000 to 8192: 129 us, 1110; 8 prompts of 511 to 4001, 16 heads on 4 of 64: 174 us, 600; 3 of 1025
-// to 5000, 8 on 2 of 256: 136 us, 1060; 32 single tokens over up to 4095: 55 us, 4.9 TB/s.
+// TFLOP/s; 16 prompts of 1 to 2048 tokens, 32 heads on 8: 221 us, 860; 4 chunks of 300 to 512 behind
+// 2000 to 8192: 127 us, 1130; 8 prompts of 511 to 4001, 16 heads on 4 of 64: 171 us, 610; 3 of 1025
+// to 5000, 8 on 2 of 256: 136 us, 1060; 32 single tokens over up to 4095: 53 us, 5.1 TB/s.
 //
 // P is rounded to V's 16-bit type (both operands of a product have one type): an output is off
 // by at most half a unit of that type times sum(p |v|) / sum(p) more than its own rounding.
@@ -916,6 +916,11 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       if (first[2 * DP] < sees) y -= INFINITY;
       return y;
     };
+    // The first `last` + 1 of 32 columns, as bits: they become predicates several at a time, where
+    // a comparison a column took 2 % of a call of short prompts.
+    auto seen_of = [](int last) {
+      return last < 0 ? 0u : last > 30 ? ~0u : (2u << last) - 1;
+    };
     auto o_done = [&](int g) {
       return wait(bar(S::kODone + 2 * x + (g & 1)), uint32_t((g >> 1) & 1), fail);
     };
@@ -950,11 +955,11 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
             float u[32];
             tc::ld32(tS + c0, u);
             tc::wait_ld();
-            const int left = lim - k0 - c0;
+            const uint32_t seen = seen_of(lim - k0 - c0);
 #pragma unroll
             for (int c = 0; c < 32; c += 2)
-              mx[c / 2 & 3] = max3_nan(mx[c / 2 & 3], c > left ? -INFINITY : u[c],
-                                       c + 1 > left ? -INFINITY : u[c + 1]);
+              mx[c / 2 & 3] = max3_nan(mx[c / 2 & 3], seen >> c & 1 ? u[c] : -INFINITY,
+                                       seen >> (c + 1) & 1 ? u[c + 1] : -INFINITY);
           }
           const float top = row_max();
           m = top == -INFINITY ? top : top + (top - top);  // NaN where it is infinite
@@ -969,7 +974,11 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
           tc::wait_ld();
           if (masked) {
 #pragma unroll
-            for (int c = half * H; c < half * H + H; ++c) v[c] = k0 + c > lim ? -INFINITY : v[c];
+            for (int c0 = half * H; c0 < half * H + H; c0 += 32) {
+              const uint32_t seen = seen_of(lim - k0 - c0);
+#pragma unroll
+              for (int c = 0; c < 32; ++c) v[c0 + c] = seen >> c & 1 ? v[c0 + c] : -INFINITY;
+            }
           }
         };
         for (bool again = false;;) {
@@ -1086,7 +1095,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
           scale[e] = __shfl_sync(0xffffffffu, inv, from);  // 0: nothing seen
           dst[e] = out_of(warp_row + from);
         }
-#pragma unroll 2
+#pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
           float o[16];
           if (n > 0) {
