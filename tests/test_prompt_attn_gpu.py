@@ -364,6 +364,37 @@ def test_other_stream_and_graph(pool):
         check(q, k, v, out, qs, qs, True, "bf16", 0.1)
 
 
+def test_two_graphs_at_once(pool):
+    """Two captured calls with keys in parts, replayed side by side: neither has the other's sums."""
+    torch = torch_cuda()
+    lens = [64, 5]
+    qs, ks = starts(lens), starts([3000, 2500])
+    sets, graphs, streams = [], [], []
+    d_q, d_k = (torch.from_numpy(x.astype(np.int32)).cuda() for x in (qs, ks))
+    for seed in (12, 13):
+        q, k, v = inputs(69, 5500, 8, 1, 128, "bf16", seed)
+        out = torch.zeros_like(q)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            pool.prompt_attn(
+                query_ptr=q.data_ptr(), key_ptr=k.data_ptr(), value_ptr=v.data_ptr(),
+                out_ptr=out.data_ptr(), q_start_ptr=d_q.data_ptr(), k_start_ptr=d_k.data_ptr(),
+                batch=2, num_q_tokens=69, num_k_tokens=5500, num_q_heads=8, kv_heads=1,
+                head_dim=128, scale=0.1, stream_ptr=torch.cuda.current_stream().cuda_stream)
+        sets.append((q, k, v, out))
+        graphs.append(g)
+        streams.append(torch.cuda.Stream())
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for q, k, v, out in sets:
+        check(q, k, v, out, qs, ks, True, "bf16", 0.1)
+    assert pool.kernel_status() == 0
+
+
 def test_same_bits_twice(pool):
     torch = torch_cuda()
     lens = [900, 40, 1300]
