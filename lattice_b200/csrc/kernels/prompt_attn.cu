@@ -2,7 +2,7 @@
 //
 // Sequence b has queries [q_start[b], q_start[b+1]) and keys [k_start[b], k_start[b+1]) in
 // packed rows; query i of nq attends to the keys j <= i + nk - nq (all nk where not causal):
-//   out_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = 2^(scale log2(e) q_i.k_j - m_i + kShift),
+//   out_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = 2^(scale log2(e) q_i.k_j - m_i + shift),
 // with the running maximum m_i and sum of p in 32 bits over one pass of the keys.  A row that
 // sees no key gives zeros.
 //
@@ -35,8 +35,12 @@
 //
 // P is rounded to V's 16-bit type (both operands of a product have one type): an output is off
 // by at most half a unit of that type times sum(p |v|) / sum(p) more than its own rounding.
-// kShift places P in [2^-24, 2^15]: the maximum is raised when a step exceeds it by more than
-// 2^8, and f16 then still holds weights of 2^-31 of the largest.
+// m_i is raised when a step exceeds it by more than 2^8, so that P is at most 2^(shift + 8).  For
+// f16 the shift is 7: P up to 2^15, and weights of 2^-31 of the largest are still held.  bf16's
+// values reach 2^128, as 32 bits do, and the sum of P v must not pass that: there the shift lies so
+// far below zero that the P of a row's keys add up to less than 1.  It goes by the item's keys and
+// no further than they need, for the small end's sake: values near bf16's least keep their products
+// as well.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -54,7 +58,7 @@ namespace dev {
 namespace {
 
 constexpr uint64_t kWaitNs = 1000000000ull;
-constexpr float kShift = 7.f;       // log2 of P where a score is the maximum
+constexpr float kShiftF16 = 7.f;    // log2 of P where a score is the maximum
 constexpr float kRaise = 8.f;       // log2 by which a step has to exceed the maximum to raise it
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kQBlk = 128 * 128;  // 64 values of 128 rows
@@ -338,6 +342,7 @@ struct Item {
   int k0, nk;   // the sequence's keys
   int past;     // keys in front of its first query
   int keys[2];  // keys that each tile looks at: those that its last row sees
+  int log_keys;  // the item's keys (all parts) are fewer than 2^log_keys
   int parts;    // of the item's keys, merged by the last to finish; 1: the output itself
   int part;     // k0, nk, past and keys are from this part's first key on
   int id;       // of the item, where it has parts
@@ -405,6 +410,7 @@ __device__ __forceinline__ Item find_item(const PromptAttnArgs &a, int tile_rows
                          ? max(0, min(it.nk, it.tok0 + (it.in0 + last) / G + it.past + 1))
                          : it.nk;
       }
+      it.log_keys = 32 - __clz(max(it.keys[0], it.keys[1]));
     } else {
       i -= __shfl_sync(0xffffffffu, end, 31);
     }
@@ -935,6 +941,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       const int lim0 = __shfl_sync(0xffffffffu, lim, 0);
       const int n = steps_of(x == 0 ? it.keys[0] : it.keys[1]);
       float m = -INFINITY, l = 0.f;
+      const float shift = std::is_same<T, __half>::value ? kShiftF16 : -kRaise - float(it.log_keys);
       for (int j = 0; ok && j < n; ++j) {
         const int g = step + j, buf = g % S::kBufs;
         const uint32_t tS = tmem + S::kS + uint32_t(x * S::kBufs + buf) * KEYS + lanes;
@@ -985,7 +992,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
 #pragma unroll
           for (int c = 0; c < KEYS; c += 32) tc::ld32(tS + c, v + c);
           settle_half(0);
-          sub = m == -INFINITY ? 0.f : kShift - m;  // nothing seen yet: P is 0
+          sub = m == -INFINITY ? 0.f : shift - m;  // nothing seen yet: P is 0
           sum[0] = sum[1] = pair(0.f, 0.f);
           exp_half<T, KEYS / 16, true>(v, v + H, w, sum, pair(P.scale_log2, P.scale_log2),
                                        pair(sub, sub), mx, [&] { settle_half(1); });

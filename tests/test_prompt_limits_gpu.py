@@ -1,0 +1,55 @@
+"""Packed prompt attention at the ends of its ranges: values near the type's largest and smallest,
+against the definition in 64 bits with the bound of `test_prompt_attn_gpu.py`."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from kv_cases import torch_cuda
+from test_prompt_attn_gpu import HALF, call, inputs, pool, reference, starts  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def check_sequences(q, k, v, out, qs, ks, causal, dtype, scale):
+    """As `check` there, without its absolute term: the values are of any size."""
+    for b in range(len(qs) - 1):
+        got = out[qs[b]:qs[b + 1]].double()
+        ref, mass = reference(q[qs[b]:qs[b + 1]].double(), k[ks[b]:ks[b + 1]].double(),
+                              v[ks[b]:ks[b + 1]].double(), scale, causal)
+        bound = HALF[dtype] * (ref.abs() + mass) + 2.0 ** -12 * mass
+        assert (got.isfinite() & ((got - ref).abs() <= bound)).all(), b
+
+
+@pytest.mark.parametrize("size", [2e38, 1e-26])
+@pytest.mark.parametrize("scores", ["equal", "flat", "peaked", "rising"])
+@pytest.mark.parametrize("d,hq,hkv", [(64, 4, 4), (128, 8, 2), (80, 7, 1), (256, 3, 1)])
+def test_large_and_small_values(pool, d, hq, hkv, scores, size):  # noqa: F811
+    """bf16 values near the largest, of one sign by column or of both: the weighted mean is finite,
+    the sum of the values is not.  Over one key, some and many, the last ones in parts."""
+    torch = torch_cuda()
+    nq, nk = [1, 3, 300, 130, 5], [1, 2, 300, 4000, 9000]
+    qs, ks = starts(nq), starts(nk)
+    q, k, v = inputs(sum(nq), sum(nk), hq, hkv, d, "bf16", 31, 12.0 if scores == "peaked" else 1.5)
+    if scores == "equal":
+        k.zero_()
+    if scores == "rising":  # the running maximum lags behind every step's
+        u = torch.ones(d, device="cuda") / d ** 0.5
+        t = torch.cat([torch.linspace(0, 25 * n / 4000, n, device="cuda") for n in nk])
+        k = (0.1 * k.float() + t[:, None, None] * u).to(k.dtype)
+        q = (0.1 * q.float() + u * d ** 0.5).to(q.dtype)
+    g = torch.Generator(device="cuda").manual_seed(32)
+    v = size * (1 + 0.6 * torch.rand(v.shape, device="cuda", generator=g).double())
+    v[..., d // 4:d // 2] *= -1
+    v[..., 3 * d // 4:] *= torch.where(torch.arange(sum(nk), device="cuda") % 2 == 0, 1, -1)[
+        :, None, None]
+    v = v.to(q.dtype)
+    for causal in (True, False):
+        out = call(pool, q, k, v, torch.zeros_like(q), qs, ks, causal, "bf16", d ** -0.5)
+        check_sequences(q, k, v, out, qs, ks, causal, "bf16", d ** -0.5)
+    # few items: keys in parts
+    out = call(pool, q[:1], k[:9000], v[:9000], torch.zeros_like(q[:1]), np.array([0, 1]),
+               np.array([0, 9000]), True, "bf16", d ** -0.5)
+    check_sequences(q[:1], k[:9000], v[:9000], out, np.array([0, 1]), np.array([0, 9000]), True,
+                    "bf16", d ** -0.5)
+    assert pool.kernel_status() == 0
