@@ -28,6 +28,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -1142,8 +1143,10 @@ size_t decode_scratch_bytes(const DecodeArgs &a) { return make_plan(a).scratch_b
 // caller then allocates for the call alone.
 constexpr size_t kMaxCachedStreams = 16;
 
-// Every buffer starts with kZeroedCounters zeroed words that the bytes asked for follow.
-constexpr size_t kCounterBytes = size_t(kZeroedCounters) * sizeof(int32_t);
+// Every buffer starts with kZeroedCounters and kTickets zeroed words that the bytes asked for
+// follow.
+constexpr size_t kTicketsAt = size_t(kZeroedCounters) * sizeof(int32_t);
+constexpr size_t kCounterBytes = kTicketsAt + size_t(kTickets) * sizeof(unsigned long long);
 
 void *stream_scratch(cudaStream_t stream, size_t bytes, std::unique_lock<std::mutex> *hold) {
   cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
@@ -1219,7 +1222,11 @@ cudaError_t CallScratch::acquire(cudaStream_t stream, size_t bytes) {
       return e;
     }
   }
+  // numbered with the buffer held: ascending in the order in which a stream runs its calls
+  static std::atomic<unsigned long long> calls{0};
   counters = reinterpret_cast<int32_t *>(base);
+  tickets = reinterpret_cast<unsigned long long *>(base + kTicketsAt);
+  ticket_base = ++calls * kTicketRange;
   ptr = base + kCounterBytes;
   return cudaSuccess;
 }

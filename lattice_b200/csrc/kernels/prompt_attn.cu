@@ -129,7 +129,8 @@ struct Params {
   uint32_t group_magic;  // ceil(2^32 / group), 0 for a group of 1
   int32_t *next_item;    // zero, and zero again after the call
   int parts;             // that an item is cut into, at most
-  int32_t *merged;       // [item][softmax warp]: parts that are done, as next_item
+  unsigned long long *merged;  // [item][softmax warp]: tickets that count the parts that are done
+  unsigned long long ticket_base;
   float *part_o;         // [part][row of q][head][DP]: sums of P V
   float2 *part_ml;       // [part][row of q][head]: maximum (log2 units) and sum of P
 };
@@ -1166,10 +1167,11 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
           __threadfence();
           __syncwarp();
           uint32_t before = 0;
-          if (lane == 0)
-            before = atomicInc(reinterpret_cast<unsigned *>(P.merged) + it.id * S::kSoftmaxWarps +
-                                   warp,
-                               unsigned(it.parts - 1));
+          if (lane == 0) {
+            unsigned long long *done = P.merged + it.id * S::kSoftmaxWarps + warp;
+            atomicMax(done, P.ticket_base);
+            before = uint32_t(atomicAdd(done, 1ull) - P.ticket_base);
+          }
           before = __shfl_sync(0xffffffffu, before, 0);
           __threadfence();
           if (before == uint32_t(it.parts - 1)) {
@@ -1273,6 +1275,8 @@ cudaError_t launch(const PromptAttnArgs &a, cudaStream_t stream) {
   p.parts = 1;
   if (a.num_k_tokens >= 2 * kMinSteps * S::kKeys)
     p.parts = int(std::max<int64_t>(1, std::min<int64_t>(kMaxParts, sms / items)));
+  if (items * S::kSoftmaxWarps > kTickets) p.parts = 1;
+  static_assert(kMaxParts < kTicketRange, "parts of an item are counted by a ticket");
   const int64_t rows = int64_t(a.num_q_tokens) * a.group * a.kv_heads;
   CallScratch scratch;
   cudaError_t e = scratch.acquire(stream, p.parts > 1 ? size_t(rows) * p.parts * (DP + 2) * 4 : 16);
@@ -1294,7 +1298,8 @@ cudaError_t launch(const PromptAttnArgs &a, cudaStream_t stream) {
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmem));
   p.next_item = scratch.counters + kZeroedCounters / 2 - 1;
-  p.merged = scratch.counters + kZeroedCounters / 2;  // 8 an item at most
+  p.merged = scratch.tickets;
+  p.ticket_base = scratch.ticket_base;
   p.part_o = static_cast<float *>(scratch.ptr);
   p.part_ml = reinterpret_cast<float2 *>(p.part_o + rows * p.parts * DP);
   const int ctas = int(std::min<int64_t>(items * p.parts, sms));

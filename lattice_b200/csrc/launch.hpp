@@ -267,10 +267,17 @@ cudaError_t beam_gather(const BeamGatherArgs &a, cudaStream_t stream);
 // buffer between acquire() and release() (or this object's end): launches in between may hand
 // results to each other through it, whatever other threads queue on the stream.
 // `counters` are kZeroedCounters 32-bit zeros: a kernel that raises some leaves them zero.
+// `tickets` are kTickets words for counts that have to be right however an earlier call ended (one
+// whose wait ran out leaves its counts where they were): a count first raises its word to
+// ticket_base, which lies above all that earlier calls on the buffer can have left there, and then
+// adds at most kTicketRange - 1.  They need no reset.
 constexpr int kZeroedCounters = 65536;
+constexpr int kTickets = 2048, kTicketRange = 32;
 struct CallScratch {
   void *ptr = nullptr;
   int32_t *counters = nullptr;
+  unsigned long long *tickets = nullptr;
+  unsigned long long ticket_base = 0;
   bool owned = false;
   std::unique_lock<std::mutex> hold;
   cudaError_t acquire(cudaStream_t stream, size_t bytes);

@@ -1,6 +1,9 @@
 """Packed prompt attention at the ends of its ranges: values near the type's largest and smallest,
-against the definition in 64 bits with the bound of `test_prompt_attn_gpu.py`."""
+and what an earlier call that failed leaves in the stream's scratch; against the definition in 64
+bits with the bound of `test_prompt_attn_gpu.py`."""
 from __future__ import annotations
+
+import ctypes
 
 import numpy as np
 import pytest
@@ -52,4 +55,64 @@ def test_large_and_small_values(pool, d, hq, hkv, scores, size):  # noqa: F811
                np.array([0, 9000]), True, "bf16", d ** -0.5)
     check_sequences(q[:1], k[:9000], v[:9000], out, np.array([0, 1]), np.array([0, 9000]), True,
                     "bf16", d ** -0.5)
+    assert pool.kernel_status() == 0
+
+
+class Scratch(ctypes.Structure):
+    """`CallScratch` of `csrc/launch.hpp`: what a call holds of its stream's buffer."""
+    _fields_ = [("ptr", ctypes.c_uint64), ("counters", ctypes.c_uint64),
+                ("tickets", ctypes.c_uint64), ("ticket_base", ctypes.c_uint64),
+                ("owned", ctypes.c_bool), ("mutex", ctypes.c_uint64), ("owns", ctypes.c_bool)]
+    COUNTERS, TICKETS, RANGE = 65536, 2048, 32
+
+    def __init__(self, lib, stream, nbytes):
+        super().__init__()
+        self.acquire = lib["_ZN4kcmm3dev11CallScratch7acquireEP11CUstream_stm"]
+        self.release = lib["_ZN4kcmm3dev11CallScratch7releaseEP11CUstream_st"]
+        for fn in (self.acquire, self.release):
+            fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p] + [ctypes.c_size_t] * (
+                fn is self.acquire)
+        self.stream, self.nbytes = stream, nbytes
+
+    def __enter__(self):
+        assert self.acquire(ctypes.addressof(self), self.stream, self.nbytes) == 0
+        assert not self.owned  # the stream's kept buffer
+        return self
+
+    def __exit__(self, *exc):
+        assert self.release(ctypes.addressof(self), self.stream) == 0
+
+    def words(self, at, count, dtype):
+        """Device words as a tensor."""
+        import torch
+
+        class View:
+            __cuda_array_interface__ = dict(shape=(count,), typestr=dtype, data=(at, False),
+                                            version=2)
+
+        return torch.as_tensor(View(), device="cuda")
+
+
+def test_scratch_counts_start_anew_after_a_call_that_failed(pool):  # noqa: F811
+    """Keys in parts, behind counts that an earlier call left where they stood when its waits ran
+    out: every part is merged, whatever they were.  The earlier sums are NaN, so that one taken
+    too early shows."""
+    torch = torch_cuda()
+    nq, nk, hq, hkv, d = [40, 1], [3000, 2500], 8, 1, 128
+    qs, ks = starts(nq), starts(nk)
+    stream = torch.cuda.current_stream().cuda_stream
+    for left in (0, 1, 2, 7, 15, 16, Scratch.RANGE - 1):
+        q, k, v = inputs(sum(nq), sum(nk), hq, hkv, d, "bf16", 40 + left)
+        call(pool, q, k, v, torch.zeros_like(q), qs, ks, True, "bf16", 0.1)
+        nbytes = sum(nq) * hq * 16 * (d + 2) * 4
+        with Scratch(pool.lib, stream, nbytes) as held:
+            assert not held.words(held.counters, held.COUNTERS, "<i4").any()
+            tickets = held.words(held.tickets, held.TICKETS, "<i8")
+            assert int(tickets.max()) < held.ticket_base
+            tickets.fill_(held.ticket_base + left)
+            held.words(held.ptr, nbytes // 4, "<i4").fill_(-1)
+            torch.cuda.synchronize()
+        for _ in range(2):
+            out = call(pool, q, k, v, torch.zeros_like(q), qs, ks, True, "bf16", 0.1)
+            check_sequences(q, k, v, out, qs, ks, True, "bf16", 0.1)
     assert pool.kernel_status() == 0
