@@ -148,17 +148,28 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // Bounded wait of a whole warp, which gives up as soon as another role has failed; every lane
 // gets the same answer.  Short, since the roles' loops share the SM's instruction cache: the limit
 // is 2^31 clock cycles, about a second.
-__device__ __forceinline__ uint32_t clock32() {
+// A wait that may SPAN an item, which takes some 60 cycles a key at most, has 2^38: more than the
+// longest item.  A stall does not last that long: the copies and products of an item that does not
+// go on are always waited for within a step too.  (A limit that starts anew with every step, tried
+// instead, cost short prompts 2 to 4 %.)
+template <bool SPAN>
+__device__ __forceinline__ uint32_t wait_clock() {
   uint32_t t;
-  asm volatile("mov.u32 %0, %%clock;" : "=r"(t));
+  if constexpr (SPAN) {
+    asm volatile("mov.u32 %0, %%clock_hi;" : "=r"(t));
+  } else {
+    asm volatile("mov.u32 %0, %%clock;" : "=r"(t));
+  }
   return t;
 }
+template <bool SPAN = false>
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *fail) {
+  constexpr uint32_t kLimit = SPAN ? 64 : 0x7fffffffu;
   if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
-  const uint32_t t0 = clock32();
+  const uint32_t t0 = wait_clock<SPAN>();
   do {
     if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
-  } while (!__any_sync(0xffffffffu, *fail != 0 || clock32() - t0 > 0x7fffffffu));
+  } while (!__any_sync(0xffffffffu, *fail != 0 || wait_clock<SPAN>() - t0 > kLimit));
   *fail = 1;
   return false;
 }
@@ -529,7 +540,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     Item it;
     it.rows = -1;
     const int slot = k % kItemSlots;
-    if (!wait(bar(S::kItemFull + slot), uint32_t((k / kItemSlots) & 1), fail)) return it;
+    if (!wait<true>(bar(S::kItemFull + slot), uint32_t((k / kItemSlots) & 1), fail)) return it;
     it = s_items[slot];
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(bar(S::kItemEmpty + slot));
@@ -594,7 +605,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       // Taken when all copies of the last one have begun, not before: an SM with a long item leaves
       // the next to others (32 single tokens over pasts of up to 4095 keys: 77 us -> 61).  Up to four
       // steps earlier measures the same.
-      if (k > 0 && !wait(bar(S::kWant), uint32_t((k - 1) & 1), fail)) break;
+      if (k > 0 && !wait<true>(bar(S::kWant), uint32_t((k - 1) & 1), fail)) break;
       const Item it = take_next();
       ended = it.rows < 0;
       if (lane == 0) {
@@ -728,7 +739,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
       for (int j = 0; ok && j < n; ++j) {
         if (!to_check(it, j)) continue;
         const int slot = (pos + pos_v(j, n)) % S::kSlots;
-        ok = wait(bar(S::kRaw + slot), raw_phase >> slot & 1, fail);
+        ok = wait<true>(bar(S::kRaw + slot), raw_phase >> slot & 1, fail);
         raw_phase ^= 1u << slot;
         if (!ok) break;
         const uint32_t tile = sb + S::kOffKv + uint32_t(slot) * S::kTileKv;
@@ -1052,7 +1063,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
         l += s0 + s1;
       }
       if (ok && n > 0) ok = o_done(step + n - 1);
-      if (ok) ok = wait(bar(S::kChecked + (k & 1)), uint32_t((k / 2) & 1), fail);
+      if (ok) ok = wait<true>(bar(S::kChecked + (k & 1)), uint32_t((k / 2) & 1), fail);
       if (!ok) break;
       const bool patched = s_patched[k & 1];
       step += n;

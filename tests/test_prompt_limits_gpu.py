@@ -1,6 +1,6 @@
 """Packed prompt attention at the ends of its ranges: values near the type's largest and smallest,
-and what an earlier call that failed leaves in the stream's scratch; against the definition in 64
-bits with the bound of `test_prompt_attn_gpu.py`."""
+what an earlier call that failed leaves in the stream's scratch, and long items; against the
+definition in 64 bits with the bound of `test_prompt_attn_gpu.py`."""
 from __future__ import annotations
 
 import ctypes
@@ -116,3 +116,25 @@ def test_scratch_counts_start_anew_after_a_call_that_failed(pool):  # noqa: F811
             out = call(pool, q, k, v, torch.zeros_like(q), qs, ks, True, "bf16", 0.1)
             check_sequences(q, k, v, out, qs, ks, True, "bf16", 0.1)
     assert pool.kernel_status() == 0
+
+
+def test_an_item_that_takes_seconds(pool):  # noqa: F811
+    """More items than are cut into parts, each over 200 million keys: some 1.5 million steps, of
+    2000 to 3000 cycles.  The roles that wait for an item's end wait for longer than 2^31 cycles
+    and do not give up.  The last keys outweigh all others by e^60."""
+    torch = torch_cuda()
+    nq, nk, last, d = 20480, 200_000_000, 100, 8
+    q = torch.zeros(nq, 1, d, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 1
+    k = torch.zeros(nk, 1, d, dtype=torch.bfloat16, device="cuda")
+    k[:-last, :, 0] = -60
+    v = torch.ones_like(k)
+    g = torch.Generator(device="cuda").manual_seed(51)
+    v[-last:] = torch.randn(last, 1, d, device="cuda", generator=g).to(v.dtype)
+    out = call(pool, q, k, v, torch.zeros_like(q), np.array([0, nq]), np.array([0, nk]), False,
+               "bf16", 1.0)
+    assert pool.kernel_status() == 0
+    rows = v[-last:].double()
+    ref, mass = rows.mean(0, keepdim=True), rows.abs().mean(0, keepdim=True)
+    assert ((out.double() - ref).abs() <= HALF["bf16"] * (ref.abs() + mass)
+            + 2.0 ** -12 * mass).all()
