@@ -812,6 +812,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     constexpr uint32_t kHi = tc::kDescHigh;
     int pos = 0, step[NT] = {};  // of the items before
+    int issued = 0;              // items whose last commit is issued
     bool ok = true;
     for (int k = 0; ok; ++k) {
       const Item it = next_item(k);
@@ -908,13 +909,18 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
         if (!S::kAhead && more) release(pos_k(j + 1));
       }
       tc::commit_warp(bar(S::kQFree));
+      issued = k + 1;
       pos += 2 * n_max;
 #pragma unroll
       for (int x = 0; x < NT; ++x) step[x] += n[x];
     }
-    if (*fail) {  // no product may run on after the CTA has gone
+    // No product may run on, and no arrival of a commit land, after the CTA has gone: the last
+    // commits come after those that the softmax waits for.
+    if (*fail) {
       tc::commit_warp(bar(S::kDrain));
       ptx::mbar_wait_bounded(bar(S::kDrain), 0, kWaitNs);
+    } else if (issued > 0) {
+      ptx::mbar_wait_bounded(bar(S::kQFree), uint32_t((issued - 1) & 1), kWaitNs);
     }
   }
   } else {
