@@ -675,8 +675,8 @@ typedef struct {
  * q and q_out [num_tokens][num_q_heads][head_dim] with element strides (0 = dense), q_out may be
  * q with its strides; num_q_heads 0: neither is touched.  k, v and k_out are rows of kv_heads *
  * head_dim values (row strides 0 = dense), k_out may be k with its stride, or 0 for none.
- * cache_format (kcmm_cache_format_t) and head_dim (the model's, even) say what the pool's pages
- * hold; a 4-bit cache quantises the rounded k' as kcmm_kv4_append_* does.  Slots, offsets, valid
+ * cache_format (kcmm_cache_format_t) and head_dim (the model's, even, at most 256) say what the
+ * pool's pages hold; a 4-bit cache quantises the rounded k' as kcmm_kv4_append_* does.  Slots, offsets, valid
  * flags and status word as for kcmm_append_kv_device_slots_on_stream: a slot below 0 or with a
  * status is not written, its q_out and k_out rows are.  Slots within a call must differ.
  */
@@ -709,13 +709,16 @@ int kcmm_rope_append_f16_on_stream(
  * same.  With nq and nk of them, query i attends to the keys j <= i + nk - nq where causal is 1,
  * to all nk where it is 0:
  *   out[i] = sum_j softmax_j(scale * q[i].k[j]) v[j],
- * zeros where a query sees no key (or only scores of -inf).  Any number of queries from 0, any
- * nk from 0; rows of out that belong to no sequence are left as they were.  Strides are in
- * elements (0 = dense); pointers and strides are multiples of 16 bytes, head_dim is a multiple
- * of 8 up to 256, num_q_heads a multiple of kv_heads, scale positive.  Keys and values past a
- * sequence may hold anything.  Starts that do not ascend, or pass num_q_tokens or num_k_tokens, set bit 2 of
- * kcmm_get_kernel_status; what the call writes within out is then undefined.  No page of the
- * pool is touched: it gives the device and the status word.
+ * zeros where a query sees no key (or only scores of -inf).  A sequence may have any number of
+ * queries and of keys from 0, but batch, num_q_tokens and num_k_tokens are at least 1 and no
+ * pointer is null: a call without any query or without any key is refused.  Rows of out that
+ * belong to no sequence are left as they were.  Strides are in elements (0 = dense); pointers and
+ * strides are multiples of 16 bytes, head_dim is a multiple of 8 up to 256, num_q_heads a multiple
+ * of kv_heads, scale positive.  Scores and sums are held in 32 bits and a key's weight is rounded
+ * to the 16-bit type before it multiplies v; finite scores and values, the largest too, give finite
+ * results.  Keys and values past a sequence may hold anything.  Starts that do not ascend, or pass
+ * num_q_tokens or num_k_tokens, set bit 2 of kcmm_get_kernel_status; what the call writes within
+ * out is then undefined.  No page of the pool is touched: it gives the device and the status word.
  */
 int kcmm_prompt_attn_bf16_on_stream(
     kcmm_pool_t *pool, uint64_t query_ptr, int64_t q_stride_token, int64_t q_stride_head,

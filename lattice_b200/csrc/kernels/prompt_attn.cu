@@ -28,19 +28,23 @@
 // roles have to fit the SM's instruction cache: with some thousand instructions more they missed
 // it and took up to a third longer.  Calls of few short items are bound by an item's chain of
 // steps, some 10,000 cycles.
-// Measured (device, one call after the other): 32,768 tokens of 8 heads on 1 of 128: 1.63 ms, 1350
-// TFLOP/s; 16 prompts of 1 to 2048 tokens, 32 heads on 8: 221 us, 860; 4 chunks of 300 to 512 behind
-// 2000 to 8192: 127 us, 1130; 8 prompts of 511 to 4001, 16 heads on 4 of 64: 171 us, 610; 3 of 1025
-// to 5000, 8 on 2 of 256: 136 us, 1060; 32 single tokens over up to 4095: 53 us, 5.1 TB/s.
+// Measured (device; one call after the other, inputs in L2 as far as they fit | L2 flushed, other
+// kernels between the calls): 32,768 tokens of 8 heads on 1 of 128: 1.63 | 1.87 ms, 1350 | 1170
+// TFLOP/s; 16 prompts of 1 to 2048 tokens, 32 heads on 8: 221 | 259 us, 860 | 730; 4
+// chunks of 300 to 512 behind 2000 to 8192: 128 | 150 us, 1120 | 960; 8 prompts of 511 to 4001, 16
+// heads on 4 of 64: 174 | 178 us, 600 | 590; 3 of 1025 to 5000, 8 on 2 of 256: 135 | 157 us, 1070 |
+// 920; 32 single tokens over up to 4095: 54 | 63 us, and from HBM 4.3 TB/s.
 //
 // P is rounded to V's 16-bit type (both operands of a product have one type): an output is off
-// by at most half a unit of that type times sum(p |v|) / sum(p) more than its own rounding.
+// by at most half a unit of that type times sum(p |v|) / sum(p) more than its own rounding.  (The
+// remainder of P as a second product would add half of the products' 2200 cycles a step, which is
+// 3300 beside the softmax's 3000.)
 // m_i is raised when a step exceeds it by more than 2^8, so that P is at most 2^(shift + 8).  For
 // f16 the shift is 7: P up to 2^15, and weights of 2^-31 of the largest are still held.  bf16's
 // values reach 2^128, as 32 bits do, and the sum of P v must not pass that: there the shift lies so
 // far below zero that the P of a row's keys add up to less than 1.  It goes by the item's keys and
-// no further than they need, for the small end's sake: values near bf16's least keep their products
-// as well.
+// no further than they need, so that products of small values stay what they are as long as can be
+// (down to 2^-93 in full for the largest weights of 32,768 keys).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
